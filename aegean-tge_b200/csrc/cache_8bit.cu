@@ -1,0 +1,286 @@
+// A paged key/value cache held in 8 bits: rotation, quantisation and store of a step's keys and values; reading entries back.
+//
+// A block is `block` consecutive positions of one request and kv head (a power of two that divides the page; keys and values have
+// blocks of their own).  Its scale s is the largest magnitude in it, a code c = rint(127 x / s), ties to even, and c stands for
+// c s / 127.  Pages: codes int8 [pages, kv_heads, page, head_dim], scales float32 [pages, kv_heads, page / block].  Appending to a
+// block that is partly filled makes its scale the larger of its own and the new rows' one; codes of a scale s that grows to s'
+// become rint(c s / s').  A block that begins in this step forgets what the page held.  A value that is not finite makes its block's
+// scale NaN: the block reads as NaN until it is begun anew.  With blocks of one position an entry is a function of its own row alone,
+// whatever step brought it; larger blocks cost less memory (4 / block bytes beside head_dim) and depend on what shares the block.
+//
+// Rotation (rotate-half over the first `rotary` numbers of a head, float32), as in elementwise.cu:
+//   lo' = lo cos - hi sin ; hi' = lo sin + hi cos
+// keys are quantised from these float32 numbers, with no rounding to the run's type in between.  127 x is exact for a bfloat16 x and
+// the division is rounded once, so x = s (k + 1/2) / 127 meets its tie exactly and goes to even wherever it is computed.
+#include "common.cuh"
+
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int MAX_PER_LANE = 8;                // head_dim <= 256
+
+// Codes of a block of scale s: rint(127 x / s).  Scales beyond 1e30 (where 127 x may pass float32's largest number) are divided
+// out in two steps that are exact powers of two apart.
+struct Coder {
+  float over, shrink;
+  bool any;
+  __device__ __forceinline__ explicit Coder(float scale) {
+    shrink = scale > 1e30f ? 9.5367431640625e-7f : 1.0f;
+    over = scale * shrink;
+    any = scale > 0.0f;                        // false for a block of zeros and for NaN
+  }
+  __device__ __forceinline__ int code(float x) const {
+    return any ? min(max(__float2int_rn(__fdiv_rn(127.0f * (x * shrink), over)), -127), 127) : 0;
+  }
+};
+
+// max that keeps NaN, and turns an infinity into one
+__device__ __forceinline__ float magnitude(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ float larger(float a, float b) { return a > b || !(a == a) ? a : b; }
+
+__device__ __forceinline__ float warp_larger(float v) {
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, offset));
+  return v;
+}
+
+struct StoreParams {
+  const void* qkv;
+  void* q_out;
+  long long row_stride, q_stride;
+  const float *cos_table, *sin_table;
+  int table_rows;
+  const int *positions, *seq_of_token, *q_start, *block_table;
+  int max_pages;
+  int8_t *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  int num_pages, page_size, block, tokens, num_seqs, heads, kv_heads, head_dim, rotary;
+  int* status;
+};
+
+// Number i of this lane (d = lane + 32 i) of a head's row at `src`, rotated for position `pos`.
+template <typename T>
+__device__ __forceinline__ float rotated(const StoreParams& p, const T* src, int d, int pos, bool rotate) {
+  const float own = to_float<T>(src[d]);
+  if (!rotate || d >= p.rotary) return own;
+  const int half = p.rotary >> 1, j = d < half ? d : d - half;
+  const float other = to_float<T>(src[d < half ? d + half : d - half]);
+  const float c = p.cos_table[(size_t)pos * half + j], s = p.sin_table[(size_t)pos * half + j];
+  return d < half ? own * c - other * s : other * s + own * c;
+}
+
+// One warp per (token, head): a query head is rotated into q_out; a key or value head is quantised by the warp of the block's first
+// token in this step, which walks the tokens of its block.
+template <typename T>
+__global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParams p) {
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x;
+  const int h = blockIdx.y * WARPS + (threadIdx.x >> 5);
+  const int pos = p.positions[t], seq = p.seq_of_token[t];
+  if (h >= p.heads + 2 * p.kv_heads) return;
+  const bool rotate = p.rotary > 0;
+  if (pos < 0 || (rotate && pos >= p.table_rows) || seq < 0 || seq >= p.num_seqs) {
+    if (lane == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    return;
+  }
+  pdl_wait();
+  const T* rows = static_cast<const T*>(p.qkv) + (size_t)h * p.head_dim;
+  if (h < p.heads) {
+    const T* src = rows + (size_t)t * p.row_stride;
+    T* dst = static_cast<T*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * p.head_dim;
+    for (int d = lane; d < p.head_dim; d += 32) dst[d] = from_float<T>(rotated<T>(p, src, d, pos, rotate));
+    return;
+  }
+  const bool is_key = h < p.heads + p.kv_heads;
+  const int kvh = h - p.heads - (is_key ? 0 : p.kv_heads);
+  const int first = p.q_start[seq], last = p.q_start[seq + 1];
+  const int inside = pos & (p.block - 1);
+  if (t != first && inside != 0) return;                         // an earlier token of the step leads this block
+  const int count = min(p.block - inside, last - t);
+  const int page_index = pos / p.page_size;
+  const int page = page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+  if (page < 0 || page >= p.num_pages || count <= 0 || t + count > p.tokens) {
+    if (lane == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+    return;
+  }
+  if (rotate && is_key && pos + count > p.table_rows) {
+    if (lane == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    return;
+  }
+  const int slot = pos % p.page_size;
+  const size_t entry = ((size_t)page * p.kv_heads + kvh) * p.page_size;
+  int8_t* codes = (is_key ? p.k_pages : p.v_pages) + (entry + slot) * p.head_dim;
+  float* scale_at = (is_key ? p.k_scale : p.v_scale) + (entry + slot) / p.block;
+  const bool turn = rotate && is_key;
+
+  float most = 0.0f;
+  for (int j = 0; j < count; ++j) {
+    const T* src = rows + (size_t)(t + j) * p.row_stride;
+    for (int d = lane; d < p.head_dim; d += 32) most = larger(most, magnitude(rotated<T>(p, src, d, pos + j, turn)));
+  }
+  most = warp_larger(most);
+  const float before = inside != 0 ? *scale_at : 0.0f;
+  const float scale = larger(before, most);
+  if (inside != 0 && !(before >= scale)) {                       // the scale grew: what the block held is rounded again
+    const Coder again(scale);
+    int8_t* old = codes - (size_t)inside * p.head_dim;
+    for (int i = lane; i < inside * p.head_dim; i += 32) {
+      const float stands = (float)old[i] * (before * again.shrink);
+      old[i] = (int8_t)(again.any ? __float2int_rn(__fdiv_rn(stands, again.over)) : 0);
+    }
+  }
+  const Coder coder(scale);
+  for (int j = 0; j < count; ++j) {
+    const T* src = rows + (size_t)(t + j) * p.row_stride;
+    for (int d = lane; d < p.head_dim; d += 32) codes[(size_t)j * p.head_dim + d] = (int8_t)coder.code(rotated<T>(p, src, d, pos + j, turn));
+  }
+  __syncwarp();
+  if (lane == 0) *scale_at = scale;
+}
+
+// ---------------------------------------------------------------------------
+// Entries read back: the positions that a step's queries may see, request after request, in runs of 64 positions
+// [runs, kv_heads, 64, head_dim] (zeros behind a request's last), and a block table over those runs.
+// ---------------------------------------------------------------------------
+struct ReadParams {
+  const int8_t *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  const int *block_table, *q_start, *start_pos;
+  int max_pages, num_pages, page_size, block, first_seq, num_seqs, kv_heads, head_dim, window;
+  void *k_out, *v_out;
+  int* table;
+  int runs, width;
+  int* status;
+};
+
+struct Span { int first, count; };             // a request's runs: from position 64 first on
+__device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
+  const int start = p.start_pos[seq], held = start + p.q_start[seq + 1] - p.q_start[seq];
+  const int lo = p.window > 0 ? max(start - p.window + 1, 0) : 0;
+  Span s;
+  s.first = lo >> 6;
+  s.count = max((held + 63) / 64 - s.first, 0);
+  return s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
+  __shared__ int found[3];
+  pdl_trigger();
+  const int run = blockIdx.x, kvh = blockIdx.y;
+  if (run == p.runs) {                         // the last block: table entries that name no run, and a look at the sum of all
+    if (kvh != 0) return;
+    int total = 0;
+    for (int seq = p.first_seq; seq < p.num_seqs; ++seq) {
+      const Span s = span_of(p, seq);
+      for (int i = threadIdx.x; i < p.width; i += blockDim.x)
+        if (i < s.first || i >= s.first + s.count) p.table[(size_t)(seq - p.first_seq) * p.width + i] = -1;
+      if (s.first + s.count > p.width && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+      total += s.count;
+    }
+    if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    return;
+  }
+  if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
+    int before = 0, seq_found = -1, first_run = 0, index = 0;
+    for (int base = p.first_seq; base < p.num_seqs && seq_found < 0; base += 32) {
+      const int seq = base + threadIdx.x;
+      Span s{0, 0};
+      if (seq < p.num_seqs) s = span_of(p, seq);
+      int upto = s.count;
+#pragma unroll
+      for (int offset = 1; offset < 32; offset <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, offset);
+        if ((int)threadIdx.x >= offset) upto += v;
+      }
+      const unsigned mine = __ballot_sync(0xffffffffu, run < before + upto);
+      if (mine != 0) {
+        const int who = __ffs(mine) - 1;
+        seq_found = base + who;
+        index = run - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, s.count, who));
+        first_run = __shfl_sync(0xffffffffu, s.first, who);
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (threadIdx.x == 0) { found[0] = seq_found; found[1] = first_run + index; }
+  }
+  __syncthreads();
+  const int seq = found[0], tile = found[1];
+  T* k_dst = static_cast<T*>(p.k_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
+  T* v_dst = static_cast<T*>(p.v_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
+  pdl_wait();
+  if (seq < 0) {                               // the caller counted more runs than there are
+    for (int i = threadIdx.x; i < 64 * p.head_dim; i += blockDim.x) k_dst[i] = v_dst[i] = from_float<T>(0.0f);
+    return;
+  }
+  const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
+  if (kvh == 0 && threadIdx.x == 0 && tile < p.width) p.table[(size_t)(seq - p.first_seq) * p.width + tile] = run;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int j = warp; j < 64; j += 8) {
+    const int pos = tile * 64 + j;
+    const int page_index = pos / p.page_size;
+    const int page = pos < held && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+    const bool here = page >= 0 && page < p.num_pages;
+    if (!here && pos < held && lane == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+    const size_t entry = here ? ((size_t)page * p.kv_heads + kvh) * p.page_size + pos % p.page_size : 0;
+    const float ks = here ? __fdiv_rn(p.k_scale[entry / p.block], 127.0f) : 0.0f;
+    const float vs = here ? __fdiv_rn(p.v_scale[entry / p.block], 127.0f) : 0.0f;
+    for (int d = lane; d < p.head_dim; d += 32) {
+      k_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.k_pages[entry * p.head_dim + d] * ks : 0.0f);
+      v_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.v_pages[entry * p.head_dim + d] * vs : 0.0f);
+    }
+  }
+}
+
+int cache_shape(const char* what, int num_pages, int page_size, int block, int kv_heads, int head_dim, int max_pages) {
+  TGE_REQUIRE(num_pages > 0 && page_size > 0 && kv_heads > 0 && max_pages > 0, "%s: bad page geometry", what);
+  TGE_REQUIRE(head_dim > 0 && head_dim <= 32 * MAX_PER_LANE, "%s: head size %d, at most %d", what, head_dim, 32 * MAX_PER_LANE);
+  TGE_REQUIRE(block > 0 && (block & (block - 1)) == 0 && page_size % block == 0, "%s: blocks of %d positions in pages of %d", what, block, page_size);
+  return 0;
+}
+
+}  // namespace
+
+TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, void* q_out, long long q_stride, const float* cos_table,
+                           const float* sin_table, int table_rows, int rotary, const int* positions, const int* seq_of_token,
+                           const int* q_start, int num_seqs, const int* block_table, int max_pages, void* k_pages, void* v_pages,
+                           float* k_scale, float* v_scale, int num_pages, int page_size, int block, int tokens, int heads, int kv_heads,
+                           int head_dim, int* status, cudaStream_t stream) {
+  const int rc = cache_shape("store_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
+  if (rc != 0) return rc;
+  TGE_REQUIRE(tokens >= 0 && heads > 0 && num_seqs >= 0, "store_8bit: bad sizes");
+  TGE_REQUIRE(rotary >= 0 && rotary <= head_dim && rotary % 2 == 0, "store_8bit: rotary width %d must be even and at most head_dim %d", rotary, head_dim);
+  TGE_REQUIRE(row_stride >= (long long)(heads + 2 * kv_heads) * head_dim && q_stride >= (long long)heads * head_dim, "store_8bit: rows too short");
+  if (tokens == 0) return 0;
+  const StoreParams p{qkv, q_out, row_stride, q_stride, cos_table, sin_table, table_rows, positions, seq_of_token, q_start, block_table,
+                      max_pages, (int8_t*)k_pages, (int8_t*)v_pages, k_scale, v_scale, num_pages, page_size, block, tokens, num_seqs,
+                      heads, kv_heads, head_dim, rotary, status};
+  const dim3 grid(tokens, (heads + 2 * kv_heads + WARPS - 1) / WARPS);
+  if (is_bf16)
+    tge_launch(store_8bit_kernel<__nv_bfloat16>, grid, WARPS * 32, 0, stream, p);
+  else
+    tge_launch(store_8bit_kernel<float>, grid, WARPS * 32, 0, stream, p);
+  return tge_launched("store_8bit", 1);
+}
+
+TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int num_pages, int page_size,
+                          int block, const int* block_table, int max_pages, const int* q_start, const int* start_pos, int first_seq,
+                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int is_bf16, int* table, int runs,
+                          int width, int* status, cudaStream_t stream) {
+  const int rc = cache_shape("read_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
+  if (rc != 0) return rc;
+  TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
+  if (num_seqs == first_seq || width == 0) return 0;
+  const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
+                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, runs, width, status};
+  const dim3 grid(runs + 1, kv_heads);
+  if (is_bf16)
+    tge_launch(read_8bit_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);
+  else
+    tge_launch(read_8bit_kernel<float>, grid, 256, 0, stream, p);
+  return tge_launched("read_8bit", 1);
+}

@@ -202,6 +202,17 @@ def core() -> ctypes.CDLL:
                                               _c_float, _c_ptr])
         _declare(lib, "tge_concat_rows", [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr])
         lib.tge_device_sm_count.argtypes = []
+        _declare(lib, "tge_store_8bit", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr,
+                                         _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                         _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr])
+        _declare(lib, "tge_read_8bit", [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
+                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int,
+                                        _c_ptr, _c_ptr])
+        _declare(lib, "tge_attention_8bit_simple", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                                    _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ll, _c_int, _c_int,
+                                                    _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_ptr])
+        _declare(lib, "tge_token_logprobs", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                             _c_ptr, _c_ptr, _c_ptr])
         lib.tge_device_sm_count.restype = _c_int
         lib.tge_sample_cuts_padded.argtypes = [_c_int]
         lib.tge_sample_cuts_padded.restype = _c_ll
@@ -1068,6 +1079,157 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
     return out
 
 
+# ----------------------------------------------------------------------------
+# a cache held in 8 bits
+# ----------------------------------------------------------------------------
+def _cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+                num_seqs: int, kv_heads: int, head_dim: int) -> Tuple[int, int, int]:
+    """(pages, positions in a page, positions in a block) of a cache held in 8 bits."""
+    for name, t, dtype in (("k pages", k_pages, torch.int8), ("v pages", v_pages, torch.int8), ("k scales", k_scale, torch.float32),
+                           ("v scales", v_scale, torch.float32), ("block table", block_table, torch.int32)):
+        _want(t, name, dtype)
+    if k_pages.dim() != 4 or k_pages.shape[1] != kv_heads or k_pages.shape[3] != head_dim or v_pages.shape != k_pages.shape:
+        raise KernelError(f"8-bit pages must be [pages, {kv_heads}, page_size, {head_dim}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    num_pages, _, page_size, _ = k_pages.shape
+    blocks = k_scale.shape[2] if k_scale.dim() == 3 else 0
+    if tuple(k_scale.shape) != (num_pages, kv_heads, blocks) or v_scale.shape != k_scale.shape or blocks <= 0 or page_size % blocks:
+        raise KernelError(f"scales must be [{num_pages}, {kv_heads}, blocks of a page], got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+    block = page_size // blocks
+    if block & (block - 1):
+        raise KernelError(f"a block of {block} positions: blocks are a power of two")
+    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or block_table.shape[1] == 0:
+        raise KernelError(f"the block table must be [{num_seqs}, pages], got {tuple(block_table.shape)}")
+    return num_pages, page_size, block
+
+
+def _portions(q_start: torch.Tensor, start_pos: torch.Tensor, num_seqs: int) -> None:
+    _want(q_start, "q_start", torch.int32)
+    _want(start_pos, "start_pos", torch.int32)
+    if q_start.numel() < num_seqs + 1 or start_pos.numel() < num_seqs:
+        raise KernelError(f"{num_seqs} portions with {q_start.numel()} q_start and {start_pos.numel()} start_pos entries")
+
+
+def _per_token(positions: torch.Tensor, seq_of_token: torch.Tensor, tokens: int) -> None:
+    _want(positions, "positions", torch.int32)
+    _want(seq_of_token, "seq_of_token", torch.int32)
+    if positions.numel() < tokens or seq_of_token.numel() < tokens:
+        raise KernelError(f"{tokens} tokens with {positions.numel()} positions and {seq_of_token.numel()} portions")
+
+
+def rope_kv_store_8bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary: int, positions: torch.Tensor,
+                       seq_of_token: torch.Tensor, q_start: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
+                       v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates q and k and appends k and v to a paged cache of 8-bit codes; returns the rotated queries [T, heads * head_dim].
+
+    qkv: [T, >= (heads + 2*kv_heads) * head_dim], unchanged; cos/sin as for :func:`rope_kv_store`.  Pages: int8 [num_pages, kv_heads,
+    page_size, head_dim]; scales: float32 [num_pages, kv_heads, page_size / block], one per ``block`` (a power of two) consecutive
+    positions and head, the block's largest magnitude: a code c of a block of scale s stands for c * s / 127.  A step that
+    appends to a block that is partly filled may raise its scale; the codes already there are then rounded again.  With blocks of
+    one position a position's entry does not depend on how its request was cut into steps.  A block with a value that is not
+    finite reads as NaN.
+    """
+    _want(qkv, "qkv", _FLOAT, contiguous=False)
+    stride = _rows_2d(qkv, "qkv")
+    tokens = qkv.shape[0]
+    if qkv.shape[1] < (heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"qkv rows of {qkv.shape[1]} numbers for {heads} + 2 * {kv_heads} heads of {head_dim}")
+    if rotary > 0:
+        _want(cos, "cos table", torch.float32)
+        _want(sin, "sin table", torch.float32)
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rotary // 2:
+            raise KernelError(f"rotary tables must be [positions, {rotary // 2}], got {tuple(cos.shape)}")
+    _per_token(positions, seq_of_token, tokens)
+    _want(q_start, "q_start", torch.int32)
+    num_seqs = q_start.numel() - 1
+    num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
+    if out is None:
+        out = torch.empty((tokens, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+    _want(out, "rotated queries", qkv.dtype, contiguous=False)
+    if tuple(out.shape) != (tokens, heads * head_dim):
+        raise KernelError(f"rotated queries must be [{tokens}, {heads * head_dim}], got {tuple(out.shape)}")
+    lib = core()
+    _check(lib.tge_store_8bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), _rows_2d(out, "rotated queries"),
+                              _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0], rotary, positions.data_ptr(),
+                              seq_of_token.data_ptr(), q_start.data_ptr(), num_seqs, block_table.data_ptr(), block_table.shape[1],
+                              k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size,
+                              block, tokens, heads, kv_heads, head_dim, status_word().data_ptr(), _stream()), lib)
+    return out
+
+
+def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+                    q_start: torch.Tensor, start_pos: torch.Tensor, ctx_lens, dtype: torch.dtype, window: int = 0,
+                    first_seq: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What the requests of a step hold in a cache of 8-bit codes, as values: (k, v, table).
+
+    ``ctx_lens``: for every request how many positions it holds after the step (host numbers; the device has them as
+    start_pos + q_start's differences).  k and v [runs, kv_heads, 64, head_dim] in ``dtype`` (float32 or bfloat16): the requests' positions one request after the
+    other in runs of 64, zeros behind a request's last position; table [requests, runs of the longest]: run i of a request, -1
+    where there is none.  With a ``window`` only runs that the step's queries may see.  ``first_seq``: leave out the requests before.
+    """
+    if k_pages.dim() != 4:
+        raise KernelError(f"8-bit pages must be [pages, kv_heads, page_size, head_dim], got {tuple(k_pages.shape)}")
+    if dtype not in _FLOAT:
+        raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
+    num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
+    num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
+    _portions(q_start, start_pos, num_seqs)
+    # a window may leave out runs in front: the sum is then a bound
+    mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
+    runs, width = sum(mine), max(mine, default=0)
+    k = torch.empty((runs, kv_heads, 64, head_dim), dtype=dtype, device=k_pages.device)
+    v = torch.empty_like(k)
+    table = torch.empty((len(mine), width), dtype=torch.int32, device=k_pages.device)
+    lib = core()
+    _check(lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
+                             block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
+                             kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), int(dtype == torch.bfloat16), table.data_ptr(),
+                             runs, width, status_word().data_ptr(), _stream()), lib)
+    return k, v, table
+
+
+def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                   block_table: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, positions: torch.Tensor,
+                   seq_of_token: torch.Tensor, num_seqs: int, max_q_len: int, max_ctx_len: int, heads: int, kv_heads: int, head_dim: int,
+                   scale: float, window: int = 0, out: Optional[torch.Tensor] = None, decode_prefix: int = 0,
+                   sink: Optional[torch.Tensor] = None, ctx_lens=None) -> torch.Tensor:
+    """:func:`attention` over a cache of 8-bit codes (see :func:`rope_kv_store_8bit`): [T, heads * head_dim].
+
+    q: [T, >= heads*head_dim] (dense rows, any row stride), rotated; the cache already holds every position up to each portion's
+    last token.  ``window``: how many of the latest positions a query sees (0: all); ``sink`` (float32 [heads]): a score per head
+    that joins the softmax's denominator once, with no key or value.  ``decode_prefix``: how many requests at the head of the batch
+    are known to bring one token each while others bring more.  ``ctx_lens`` (host numbers): what every request holds after the
+    step (None: ``max_ctx_len``, a bound).
+    """
+    _want(q, "queries", _FLOAT, contiguous=False)
+    q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or q.shape[1] < heads * head_dim:
+        raise KernelError(f"attention: rows of {q.shape[1]} numbers for {heads} heads of {head_dim} over {kv_heads}")
+    num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
+    _portions(q_start, start_pos, num_seqs)
+    _per_token(positions, seq_of_token, tokens)
+    if ctx_lens is not None and len(ctx_lens) != num_seqs:
+        raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
+    if not 0 <= decode_prefix <= num_seqs or window < 0:
+        raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
+    if sink is not None:
+        _want(sink, "attention sinks", torch.float32)
+        if sink.numel() != heads:
+            raise KernelError(f"attention: {sink.numel()} sinks for {heads} heads")
+    if out is None:
+        out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=q.device)
+    _want(out, "attention output", q.dtype, contiguous=False)
+    if tuple(out.shape) != (tokens, heads * head_dim):
+        raise KernelError(f"attention: the output must be [{tokens}, {heads * head_dim}], got {tuple(out.shape)}")
+    lib = core()
+    _check(lib.tge_attention_8bit_simple(q.data_ptr(), int(q.dtype == torch.bfloat16), q_stride, k_pages.data_ptr(), v_pages.data_ptr(),
+                                         k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block, block_table.data_ptr(),
+                                         block_table.shape[1], positions.data_ptr(), seq_of_token.data_ptr(), num_seqs, tokens,
+                                         out.data_ptr(), _rows_2d(out, "attention output"), heads, kv_heads, head_dim, float(scale),
+                                         int(window), _ptr(sink), status_word().data_ptr(), _stream()), lib)
+    return out
+
+
 def to_run_dtype(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The float32 rows ``x`` in the format the products read (``x`` itself when that is float32)."""
     _want(x, "rows", torch.float32)
@@ -1419,6 +1581,34 @@ def sample_cuts(scores: torch.Tensor, temperature: torch.Tensor, top_k: torch.Te
                                min_p.data_ptr(), uniform.data_ptr(), sort_prob.data_ptr(), sort_index.data_ptr(),
                                out.data_ptr(), rows, vocab, int(skip_uncut), _stream()), lib)
     return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """Log probabilities of given tokens: (logprob, entropy, rank, top_ids, top_logprobs).
+
+    logits: float32 or bfloat16 [R, V] (dense rows, any row stride); tokens: int32 [R], one per row.  logprob, entropy float32 [R]: the
+    token's log probability and the entropy of its row in nats; rank int32 [R]: how many tokens come before it in the order of
+    falling logits, the lower index first among equals; top_ids int32, top_logprobs float32 [R, top]: the first ``top`` (at most 32) in that order.
+    A logit of -inf is a token that cannot come.  Rows with NaN, with +inf or without a finite logit give NaN.  A token outside the
+    vocabulary is reported through the status word; its log probability is NaN, its rank -1.
+    """
+    _want(logits, "logits", _FLOAT, contiguous=False)
+    stride = _rows_2d(logits, "logits")
+    rows, vocab = logits.shape
+    _want(tokens, "tokens", torch.int32)
+    if tokens.numel() != rows:
+        raise KernelError(f"token_logprobs: {tokens.numel()} tokens for {rows} rows")
+    device = logits.device
+    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    rank = torch.empty(rows, dtype=torch.int32, device=device)
+    top_ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=device)
+    top_logprobs = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=device)
+    lib = core()
+    _check(lib.tge_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride, tokens.data_ptr(), rows, vocab, int(top),
+                                  logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(),
+                                  status_word().data_ptr(), _stream()), lib)
+    return logprob, entropy, rank, top_ids, top_logprobs
 
 
 # ----------------------------------------------------------------------------

@@ -1,0 +1,434 @@
+"""The 8-bit cache on the device against its definition in float64: store, reading back, attention, refusals."""
+import math
+import random
+
+import pytest
+import torch
+
+from helpers import TOL, batch_index, rel_error
+from plain import cache_8bit_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from aegean_tge_b200 import ops as module
+    module.core()
+    return module
+
+
+class Cache:
+    """Random codes and scales of requests that hold ``held`` positions, on shuffled pages; what no request holds reads as NaN."""
+
+    def __init__(self, held, kv_heads, dim, page, block, seed=0):
+        gen = torch.Generator().manual_seed(seed)
+        self.held, self.kv_heads, self.dim, self.page, self.block = held, kv_heads, dim, page, block
+        need = [-(-n // page) for n in held]
+        order = list(range(sum(need) + 3))
+        random.Random(seed).shuffle(order)
+        self.table = torch.full((len(held), max(max(need), 1)), -1, dtype=torch.int32)
+        at = 0
+        for r, n in enumerate(need):
+            self.table[r, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+            at += n
+        pages = len(order)
+        self.codes = {n: (torch.randn(pages, kv_heads, page, dim, generator=gen) * 40).round().clamp(-127, 127).to(torch.int8) for n in "kv"}
+        self.scales = {n: torch.full((pages, kv_heads, page // block), math.nan) for n in "kv"}
+        for n in "kv":
+            for r, count in enumerate(held):
+                for b in range(-(-count // block)):
+                    where = self.table[r, b * block // page]
+                    self.scales[n][where, :, b * block % page // block] = 2.0 + torch.rand(kv_heads, generator=gen)
+
+    def of(self, name, request, codes=None, scales=None):
+        """(codes [held, kv, dim], scales [blocks, kv]) of one request."""
+        codes, scales = (self.codes if codes is None else codes)[name].cpu(), (self.scales if scales is None else scales)[name].cpu()
+        pos = torch.arange(self.held[request])
+        where = self.table[request, pos // self.page].long()
+        lead = pos[::self.block]
+        return (codes[where, :, pos % self.page],
+                scales[self.table[request, lead // self.page].long(), :, lead % self.page // self.block])
+
+    def values(self, name, request, codes=None, scales=None):
+        c, s = self.of(name, request, codes, scales)
+        if not len(c):
+            return torch.zeros(0, self.kv_heads, self.dim, dtype=torch.float64)
+        return torch.stack([plain.values(c[:, h], s[:, h], self.block) for h in range(self.kv_heads)], 1)
+
+    def device(self):
+        return (self.codes["k"].to(DEV), self.codes["v"].to(DEV), self.scales["k"].to(DEV), self.scales["v"].to(DEV))
+
+
+def tables(positions, rotary):
+    angles = torch.arange(positions)[:, None].float() * (10000.0 ** (-torch.arange(0, rotary, 2).float() / max(rotary, 1)))
+    return angles.cos(), angles.sin()
+
+
+def store(ops, cache, qkv, starts, heads, rotary, cos, sin, lens, out=None):
+    """Appends and compares scales, codes and rotated queries with the definition; returns the device's cache."""
+    positions, seq, q_start, start_pos = batch_index(lens, starts, DEV)
+    device = cache.device()
+    kv, dim, block = cache.kv_heads, cache.dim, cache.block
+    q = ops.rope_kv_store_8bit(qkv.to(DEV), cos.to(DEV) if rotary else None, sin.to(DEV) if rotary else None, rotary, positions, seq, q_start,
+                               cache.table.to(DEV), *device, heads, kv, dim, out=out)
+    after = {"k": device[0].cpu(), "v": device[1].cpu()}, {"k": device[2].cpu(), "v": device[3].cpu()}
+    rows = qkv[:, :(heads + 2 * kv) * dim].double().view(len(qkv), heads + 2 * kv, dim)
+    turned = torch.stack([plain.rotated(rows[t, :heads + kv], cos, sin, rotary, int(positions[t])) for t in range(len(qkv))])
+    # one rounding to the output's type behind two products and a sum in float32
+    assert rel_error(q, turned[:, :heads].flatten(1)) < (2 ** -8 if qkv.dtype == torch.bfloat16 else 3e-7)
+    at = 0
+    for r, (n, start) in enumerate(zip(lens, starts)):
+        for name, new in (("k", turned[at:at + n, heads:]), ("v", rows[at:at + n, heads + kv:])):
+            codes, scales = cache.of(name, r)
+            got_codes, got_scales = cache.of(name, r, *after)
+            for h in range(kv):
+                want, wanted_scales = plain.append(codes[:, h].double(), scales[:, h].double(), new[:, h], start, block)
+                s = got_scales[:, h].double()
+                assert torch.equal(torch.isnan(s), torch.isnan(wanted_scales))
+                fine = ~torch.isnan(s)
+                # keys: products and a sum rounded in float32; values as they are
+                assert ((s - wanted_scales).abs()[fine] <= 4e-7 * wanted_scales[fine]).all()
+                off = (got_codes[:, h].double() - want).abs()
+                # a code is the nearest whole number of a quotient that float32 knows to 127 * 2e-6 (a rotation that cancels
+                # leaves an error relative to the block's largest, not to the number)
+                assert float(off.max()) <= 0.5 + 127 * 2e-6, (name, r, h, float(off.max()))
+        at += n
+    ops.check_status()
+    return device, after
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,rotary,page,block", [
+    (28, 4, 128, 128, 64, 1), (40, 8, 128, 128, 16, 16), (12, 2, 128, 128, 32, 4), (4, 2, 64, 64, 64, 64), (3, 1, 16, 16, 8, 2),
+    (5, 1, 256, 128, 64, 8), (6, 3, 80, 40, 16, 1), (2, 2, 10, 6, 4, 4), (2, 1, 33, 0, 64, 16)])
+def test_store(ops, dtype, heads, kv, dim, rotary, page, block):
+    lens, starts = [1, 1, 37, 5, 130, 64], [0, 77, 9, 3, 0, 64]
+    cache = Cache([a + b for a, b in zip(lens, starts)], kv, dim, page, block)
+    cos, sin = tables(300, rotary)
+    gen = torch.Generator().manual_seed(3)
+    qkv = torch.randn(sum(lens), (heads + 2 * kv) * dim + 16, generator=gen)          # the row goes on behind the values
+    qkv[:, heads * dim] *= 20.0                                                       # scales that old blocks have to grow to
+    qkv[7, (heads + kv) * dim:(heads + 2 * kv) * dim] = 0.0                           # a position of zeros
+    store(ops, cache, qkv.to(dtype), starts, heads, rotary, cos, sin, lens)
+
+
+@pytest.mark.parametrize("size", [1e-42, 1e-38, 1e-30, 1e30, 3e38])
+@pytest.mark.parametrize("block", [1, 8])
+def test_store_at_the_ends_of_the_range(ops, size, block):
+    lens, starts = [3, 9], [5, 0]
+    cache = Cache([8, 9], 2, 64, 16, block)
+    cache.scales["k"] = torch.full_like(cache.scales["k"], size / 4)
+    cache.scales["v"] = torch.full_like(cache.scales["v"], size * 0.3)
+    gen = torch.Generator().manual_seed(4)
+    qkv = ((torch.rand(12, 6 * 64, generator=gen).double() * 2 - 1) * size).float()
+    store(ops, cache, qkv, starts, 2, 0, None, None, lens)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("block", [1, 4])
+def test_store_of_values_that_are_not_finite(ops, bad, block):
+    """Their block reads as NaN, its neighbours do not; begun anew, the block forgets it."""
+    lens, starts = [6, 7], [2, 0]
+    cache = Cache([8, 7], 2, 64, 8, block)
+    qkv = torch.randn(13, 6 * 64, generator=torch.Generator().manual_seed(5))
+    qkv[3, 2 * 64 + 5] = bad              # a key of head 0 at position 5 of request 0
+    qkv[8, 5 * 64 + 9] = bad              # a value of head 1 at position 2 of request 1
+    device, _ = store(ops, cache, qkv, starts, 2, 0, None, None, lens)
+    assert int(torch.isnan(device[2][cache.table[0, 0].item()]).sum()) == 1
+    clean = torch.randn(7, 6 * 64, generator=torch.Generator().manual_seed(6))
+    positions, seq, q_start, _ = batch_index([7], [0], DEV)
+    ops.rope_kv_store_8bit(clean.to(DEV), None, None, 0, positions, seq, q_start, cache.table[1:].to(DEV), *device, 2, 2, 64)
+    assert torch.isfinite(device[3][cache.table[1, 0].item(), :, :-(-7 // block)]).all()
+
+
+def test_store_rows_of_an_inner_buffer(ops):
+    """Odd row strides, starts that are no multiple of 16 bytes, an output inside a wider buffer; neighbours stay as they are."""
+    heads, kv, dim = 4, 2, 64
+    cache = Cache([40, 3], kv, dim, 16, 1)
+    cos, sin = tables(64, dim)
+    gen = torch.Generator().manual_seed(8)
+    for dtype in (torch.bfloat16, torch.float32):
+        for lead, width in ((1, 8 * 64 + 3), (8, 8 * 64 + 8), (0, 8 * 64 + 1)):
+            rows = torch.randn(43, width, generator=gen).to(dtype).to(DEV)
+            before = rows.clone()
+            wide = torch.full((43, heads * dim + 5), 7.0, dtype=dtype, device=DEV)
+            view = rows[:, lead:lead + 8 * 64] if width - lead >= 8 * 64 else rows
+            store(ops, cache, view.cpu(), [0, 0], heads, dim, cos, sin, [40, 3], out=wide[:, 3:3 + heads * dim])
+            assert (wide[:, :3] == 7).all() and (wide[:, 3 + heads * dim:] == 7).all()
+            positions, seq, q_start, _ = batch_index([40, 3], [0, 0], DEV)
+            d1, d2 = cache.device(), cache.device()
+            a = ops.rope_kv_store_8bit(view, cos.to(DEV), sin.to(DEV), dim, positions, seq, q_start, cache.table.to(DEV), *d1, heads, kv, dim)
+            b = ops.rope_kv_store_8bit(view.contiguous(), cos.to(DEV), sin.to(DEV), dim, positions, seq, q_start, cache.table.to(DEV), *d2, heads, kv, dim)
+            assert torch.equal(a, b) and torch.equal(d1[0], d2[0]) and torch.equal(d1[1], d2[1])
+            assert torch.equal(rows, before)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_entries_do_not_depend_on_the_cut_with_blocks_of_one(ops, dtype):
+    heads, kv, dim, n = 4, 2, 128, 150
+    cos, sin = tables(n, dim)
+    qkv = torch.randn(n, 8 * dim, generator=torch.Generator().manual_seed(9)).to(dtype).to(DEV)
+    found = []
+    for cuts in ([150], [1] * 150, [64, 1, 85], [7, 63, 80]):
+        cache = Cache([n], kv, dim, 16, 1)
+        device, at, q = cache.device(), 0, []
+        for count in cuts:
+            positions, seq, q_start, _ = batch_index([count], [at], DEV)
+            q.append(ops.rope_kv_store_8bit(qkv[at:at + count], cos.to(DEV), sin.to(DEV), dim, positions, seq, q_start, cache.table.to(DEV), *device, heads, kv, dim))
+            at += count
+        found.append([torch.cat(q)] + list(device[:2]) + [s.nan_to_num(0.0) for s in device[2:]])
+    for other in found[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(found[0], other))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kv,dim,page,block,window", [(4, 128, 64, 1, 0), (2, 128, 16, 16, 100), (1, 16, 8, 2, 0), (3, 80, 4, 4, 70), (2, 33, 64, 64, 1), (1, 256, 32, 1, 0)])
+def test_read_back(ops, dtype, kv, dim, page, block, window):
+    held, lens = [1, 64, 65, 200, 0, 130] + [3] * 40, [1, 1, 65, 20, 0, 2] + [1] * 40
+    cache = Cache(held, kv, dim, page, block)
+    _, _, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+    for first in (0, 2, 44):
+        k, v, table = ops.read_cache_8bit(*cache.device(), cache.table.to(DEV), q_start, start_pos, held, dtype, window=window, first_seq=first)
+        for got, name in ((k, "k"), (v, "v")):
+            for r in range(first, len(held)):
+                seen = max(held[r] - lens[r] - window + 1, 0) // 64 if window else 0
+                runs = table[r - first].tolist()
+                want = cache.values(name, r)
+                for i, run in enumerate(runs):
+                    if i < seen or i >= -(-held[r] // 64):
+                        assert run == -1
+                        continue
+                    part = got[run].transpose(0, 1).double().cpu()
+                    n = min(64, held[r] - i * 64)
+                    # one rounding to the output's type, two in float32 before it
+                    assert rel_error(part[:n], want[i * 64:i * 64 + n]) < (2 ** -8 if dtype == torch.bfloat16 else 3e-7)
+                    assert (part[n:] == 0).all()
+    ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+def attend(ops, cache, lens, heads, dtype, window=0, sink=False, scale=None, **kw):
+    starts = [h - n for h, n in zip(cache.held, lens)]
+    positions, seq, q_start, start_pos = batch_index(lens, starts, DEV)
+    gen = torch.Generator().manual_seed(11)
+    q = (torch.randn(sum(lens), heads * cache.dim, generator=gen) * 1.5).to(dtype)
+    sinks = torch.randn(heads, generator=gen) if sink else None
+    scale = cache.dim ** -0.5 if scale is None else scale
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, len(lens), max(lens), max(cache.held),
+                             heads, cache.kv_heads, cache.dim, scale, window=window, sink=None if sinks is None else sinks.to(DEV), **kw)
+    want, at = [], 0
+    for r, n in enumerate(lens):
+        want.append(plain.attend(q[at:at + n].view(n, heads, cache.dim), cache.values("k", r), cache.values("v", r), starts[r], scale, window, sinks))
+        at += n
+    ops.check_status()
+    return out, torch.cat(want).flatten(1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(28, 4, 128), (40, 8, 128), (12, 2, 128), (14, 2, 64), (4, 2, 16), (3, 1, 32), (16, 1, 128), (33, 3, 128),
+                                          (40, 2, 64), (6, 2, 80), (2, 2, 256), (4, 1, 33)])
+def test_single_tokens(ops, dtype, heads, kv, dim):
+    cache = Cache([1, 2, 7, 15, 16, 17, 63, 64, 65, 127, 128, 129, 300, 1000], kv, dim, 64, 1)
+    out, want = attend(ops, cache, [1] * 14, heads, dtype)
+    assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page,block", [(64, 64), (64, 4), (32, 1), (16, 16), (16, 2), (8, 8), (4, 1), (1, 1)])
+@pytest.mark.parametrize("window,sink", [(0, False), (0, True), (1, False), (50, True), (128, False)])
+def test_single_tokens_on_pages_blocks_windows(ops, dtype, page, block, window, sink):
+    cache = Cache([1, 33, 64, 100, 513], 2, 128, page, block)
+    out, want = attend(ops, cache, [1] * 5, 14, dtype, window=window, sink=sink)
+    assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,page,block", [(28, 4, 128, 64, 1), (12, 2, 128, 16, 16), (4, 2, 16, 32, 4), (3, 1, 32, 8, 1), (6, 2, 80, 64, 2), (2, 1, 256, 64, 1)])
+@pytest.mark.parametrize("window,sink", [(0, False), (33, True)])
+def test_portions(ops, dtype, heads, kv, dim, page, block, window, sink):
+    cache = Cache([40, 2, 65, 200, 129], kv, dim, page, block)
+    out, want = attend(ops, cache, [40, 2, 64, 5, 1], heads, dtype, window=window, sink=sink)
+    assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("singles,told", [(9, 9), (9, 8), (2, 2), (9, 0)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_single_tokens_beside_portions(ops, dtype, singles, told, window):
+    """However many of the single tokens the caller tells of, and whether it tells the contexts."""
+    held = [1, 5, 64, 65, 200, 17, 128, 90, 400][:singles] + [100, 70]
+    cache = Cache(held, 2, 128, 16, 1)
+    for ctx in (None, held):
+        out, want = attend(ops, cache, [1] * singles + [30, 70], 14, dtype, window=window, decode_prefix=told, ctx_lens=ctx)
+        assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_peaked_and_shifted_scores(ops, dtype):
+    """Scores in the hundreds: sums that start far below their maximum, and rows that are one key."""
+    cache = Cache([700, 64, 1], 2, 128, 64, 1)
+    for scale in (20.0, 1e-8):
+        out, want = attend(ops, cache, [1, 1, 1], 8, dtype, scale=scale)
+        # a score of some thousands is known to 2^-24 of the sum of its products' magnitudes
+        assert rel_error(out, want) < (TOL[dtype] if dtype == torch.bfloat16 or scale < 1 else 2e-3)
+
+
+def test_one_request_among_many_lengths(ops):
+    cache = Cache([1 + 7 * i % 90 for i in range(300)], 2, 64, 16, 1)
+    out, want = attend(ops, cache, [1] * 300, 8, torch.bfloat16)
+    assert rel_error(out, want) < TOL[torch.bfloat16]
+
+
+def test_long_contexts(ops):
+    """Against float64 on the device: 40,000 positions, offsets of entries beyond 2^31 bytes."""
+    kv, dim, heads, page = 2, 128, 8, 64
+    pages = 2 ** 31 // (kv * page * dim) + 700
+    codes = torch.empty(pages, kv, page, dim, dtype=torch.int8, device=DEV).random_(-127, 128)
+    scales = torch.rand(pages, kv, page, device=DEV) + 1.0
+    held = [40000, 39, 3000]
+    table = torch.full((3, 625), -1, dtype=torch.int32)
+    table[0, :625] = torch.arange(pages - 1, pages - 626, -1)
+    table[1, :1] = 5
+    table[2, :47] = torch.arange(pages - 700, pages - 653)
+    q = torch.randn(3, heads * dim, device=DEV).bfloat16()
+    positions, seq, q_start, start_pos = batch_index([1, 1, 1], [n - 1 for n in held], DEV)
+    out = ops.attention_8bit(q, codes, codes, scales, scales, table.to(DEV), q_start, start_pos, positions, seq, 3, 1, 40000, heads, kv, dim, 0.05)
+    for r, n in enumerate(held):
+        pos = torch.arange(n, device=DEV)
+        where = table[r].to(DEV)[pos // page].long()
+        k = codes[where, :, pos % page].double() * scales[where, :, pos % page].double()[..., None] / 127
+        p = torch.softmax(torch.einsum("kgd,ckd->kgc", q[r].double().view(kv, 4, dim), k) * 0.05, -1)
+        assert rel_error(out[r], torch.einsum("kgc,ckd->kgd", p, k).flatten()) < TOL[torch.bfloat16]
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_block_that_reads_as_nan_reaches_only_who_sees_it(ops, dtype):
+    cache = Cache([100, 100, 100], 2, 128, 16, 1)
+    cache.scales["v"][cache.table[0, 2].item(), 1, 3] = math.nan           # position 35 of request 0, head 1
+    cache.scales["k"][cache.table[1, 1].item(), 0, 0] = math.nan           # position 16 of request 1, head 0
+    lens, heads = [1, 1, 1], 8
+    positions, seq, q_start, start_pos = batch_index(lens, [99] * 3, DEV)
+    q = torch.randn(3, heads * 128, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    for window in (0, 64):
+        out = ops.attention_8bit(q, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 3, 1, 100, heads, 2, 128, 0.09, window=window)
+        nan = torch.isnan(out.view(3, heads, 128)).all(-1).cpu()
+        some = torch.isnan(out.view(3, heads, 128)).any(-1).cpu()
+        want = torch.zeros(3, heads, dtype=torch.bool)
+        if not window:
+            want[0, 4:], want[1, :4] = True, True
+        assert torch.equal(nan, want) and torch.equal(some, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[1, 1], [3, 20]])
+def test_pages_outside_the_pool_are_reported_not_read(ops, dtype, lens):
+    cache = Cache([50, 80], 2, 128, 16, 1)
+    table = cache.table.clone()
+    table[0] = torch.tensor([-1, 9999, -7, 10 ** 6, -1])
+    positions, seq, q_start, start_pos = batch_index(lens, [50 - lens[0], 80 - lens[1]], DEV)
+    q = torch.randn(sum(lens), 8 * 128).to(dtype).to(DEV)
+    args = (q_start, start_pos, positions, seq, 2, max(lens), 80, 8, 2, 128, 0.1)
+    good = ops.attention_8bit(q, *cache.device(), cache.table.to(DEV), *args)
+    ops.check_status()
+    out = ops.attention_8bit(q, *cache.device(), table.to(DEV), *args)
+    with pytest.raises(ops.DeviceStatusError):
+        ops.check_status()
+    assert (out[:lens[0]] == 0).all() and torch.equal(out[lens[0]:], good[lens[0]:])
+    device = cache.device()
+    before = [t.clone() for t in device]
+    ops.rope_kv_store_8bit(torch.randn(lens[0], 12 * 128).to(dtype).to(DEV), None, None, 0, positions[:lens[0]], seq[:lens[0]], q_start[:2].clone(), table.to(DEV), *device, 8, 2, 128)
+    with pytest.raises(ops.DeviceStatusError):
+        ops.check_status()
+    assert all(torch.equal(a.nan_to_num(0) if a.is_floating_point() else a, b.nan_to_num(0) if b.is_floating_point() else b) for a, b in zip(before, device))
+
+
+def test_positions_outside_the_tables_are_reported(ops):
+    cache = Cache([70], 2, 64, 16, 1)
+    cos, sin = tables(50, 64)
+    positions, seq, q_start, _ = batch_index([1], [60], DEV)
+    device = cache.device()
+    ops.rope_kv_store_8bit(torch.randn(1, 6 * 64).to(DEV), cos.to(DEV), sin.to(DEV), 64, positions, seq, q_start, cache.table.to(DEV), *device, 2, 2, 64)
+    with pytest.raises(ops.DeviceStatusError):
+        ops.check_status()
+    assert torch.equal(device[0].cpu(), cache.codes["k"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_on_a_stream_of_its_own_and_again(ops, dtype):
+    """On another stream than the default, with rows of an inner buffer: the same bits."""
+    cache = Cache([200, 65, 3, 90], 2, 128, 64, 1)
+    lens = [1, 1, 1, 1]
+    positions, seq, q_start, start_pos = batch_index(lens, [h - 1 for h in cache.held], DEV)
+    wide = torch.randn(4, 8 * 128 + 24, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    device, table = cache.device(), cache.table.to(DEV)
+    args = (*device, table, q_start, start_pos, positions, seq, 4, 1, 200, 8, 2, 128, 0.1)
+    first = ops.attention_8bit(wide[:, 8:8 + 1024].contiguous(), *args)
+    odd = ops.attention_8bit(wide[:, 8:8 + 1024], *args)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = ops.attention_8bit(wide[:, 8:8 + 1024], *args)
+    side.synchronize()
+    assert torch.equal(first, odd) and torch.equal(first, again)
+    into = torch.zeros(4, 1024 + 8, dtype=dtype, device=DEV)
+    ops.attention_8bit(wide[:, 8:8 + 1024], *args, out=into[:, 8:])
+    assert torch.equal(into[:, 8:], first) and (into[:, :8] == 0).all()
+    # rows that start on odd elements
+    odd_rows = torch.zeros(4, 1024 + 1, dtype=dtype, device=DEV)
+    odd_rows[:, 1:] = wide[:, 8:8 + 1024]
+    assert rel_error(ops.attention_8bit(odd_rows[:, 1:], *args), first) < TOL[dtype]
+
+
+def test_nothing_to_do(ops):
+    cache = Cache([5], 2, 64, 16, 1)
+    empty = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    start = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert ops.rope_kv_store_8bit(empty(0, 6 * 64), None, None, 0, none, none, start, cache.table.to(DEV), *cache.device(), 2, 2, 64).shape == (0, 128)
+    assert ops.attention_8bit(empty(0, 128), *cache.device(), cache.table.to(DEV), start, none, none, none, 0, 0, 0, 2, 2, 64, 0.1).shape == (0, 128)
+    k, _v, table = ops.read_cache_8bit(*cache.device(), cache.table.to(DEV), start, none, [], torch.bfloat16)
+    assert k.shape == (0, 2, 64, 64) and table.shape == (0, 0)
+
+
+def test_refusals(ops):
+    cache = Cache([20], 2, 64, 16, 1)
+    kp, vp, ks, vs = cache.device()
+    table = cache.table.to(DEV)
+    positions, seq, q_start, start_pos = batch_index([1], [19], DEV)
+    q = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device=DEV)
+    qkv = torch.zeros(1, 8 * 64, dtype=torch.bfloat16, device=DEV)
+
+    def attention(q=q, kp=kp, vp=vp, ks=ks, vs=vs, table=table, q_start=q_start, positions=positions, seqs=1, heads=4, kv=2, dim=64, **kw):
+        return ops.attention_8bit(q, kp, vp, ks, vs, table, q_start, start_pos, positions, seq, seqs, 1, 20, heads, kv, dim, 0.1, **kw)
+
+    def stored(qkv=qkv, kp=kp, vp=vp, ks=ks, vs=vs, rotary=0, cos=None, sin=None, positions=positions, **kw):
+        return ops.rope_kv_store_8bit(qkv, cos, sin, rotary, positions, seq, q_start, table, kp, vp, ks, vs, 4, 2, 64, **kw)
+
+    attention(), stored()
+    wrong = [
+        lambda: attention(q=q.half()), lambda: attention(q=q.cpu()), lambda: attention(kp=kp.float()), lambda: attention(kp=kp[:, :1]),
+        lambda: attention(vp=vp[:1]), lambda: attention(ks=ks.double()), lambda: attention(ks=ks[:, :, :5].contiguous()),
+        lambda: attention(vs=vs[:, :, :8].contiguous()), lambda: attention(ks=ks[:, :, :0], vs=vs[:, :, :0]), lambda: attention(heads=5), lambda: attention(heads=8),
+        lambda: attention(seqs=2), lambda: attention(positions=positions.long()), lambda: attention(q_start=q_start[:1]), lambda: attention(ctx_lens=[20, 20]),
+        lambda: attention(sink=torch.zeros(3, device=DEV)), lambda: attention(window=-1), lambda: attention(decode_prefix=2),
+        lambda: attention(out=torch.zeros(1, 5, dtype=torch.bfloat16, device=DEV)), lambda: attention(out=torch.zeros(1, 256, device=DEV)),
+        lambda: attention(dim=32), lambda: attention(table=table.long()),
+        lambda: stored(qkv=qkv[:, :7 * 64]), lambda: stored(qkv=qkv.int()), lambda: stored(rotary=64), lambda: stored(rotary=3, cos=torch.zeros(30, 1, device=DEV), sin=torch.zeros(30, 1, device=DEV)),
+        lambda: stored(rotary=66, cos=torch.zeros(30, 33, device=DEV), sin=torch.zeros(30, 33, device=DEV)), lambda: stored(kp=kp.to(torch.uint8)),
+        lambda: stored(positions=positions[:0]), lambda: stored(out=torch.zeros(1, 5, dtype=torch.bfloat16, device=DEV)), lambda: stored(ks=ks.transpose(1, 2)),
+        lambda: ops.read_cache_8bit(kp, vp, ks, vs, table, q_start, start_pos, [20], torch.float16),
+        lambda: ops.read_cache_8bit(kp, vp, ks, vs, table, q_start, start_pos, [20, 20], torch.float32),
+    ]
+    for call in wrong:
+        with pytest.raises((ops.KernelError, AttributeError, TypeError)):
+            call()
+    three = torch.zeros(4, 2, 3, 64, dtype=torch.int8, device=DEV), torch.zeros(4, 2, 1, device=DEV)      # a block of three
+    with pytest.raises(ops.KernelError):
+        attention(kp=three[0], vp=three[0], ks=three[1], vs=three[1])
+    wide = torch.zeros(4, 2, 16, 320, dtype=torch.int8, device=DEV), torch.zeros(4, 2, 16, device=DEV)
+    with pytest.raises(ops.KernelError):
+        attention(q=torch.zeros(1, 4 * 320, device=DEV), kp=wide[0], vp=wide[0], ks=wide[1], vs=wide[1], dim=320)
+    ops.check_status()
