@@ -81,13 +81,13 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
   const int t = blockIdx.x;
   const int h = blockIdx.y * WARPS + (threadIdx.x >> 5);
   const int pos = p.positions[t], seq = p.seq_of_token[t];
+  pdl_wait();
   if (h >= p.heads + 2 * p.kv_heads) return;
   const bool rotate = p.rotary > 0;
   if (pos < 0 || (rotate && pos >= p.table_rows) || seq < 0 || seq >= p.num_seqs) {
     if (lane == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
     return;
   }
-  pdl_wait();
   const T* rows = static_cast<const T*>(p.qkv) + (size_t)h * p.head_dim;
   if (h < p.heads) {
     const T* src = rows + (size_t)t * p.row_stride;
@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 
 // ---------------------------------------------------------------------------
 // Entries read back: the positions that a step's queries may see, request after request, in runs of 64 positions
-// [runs, kv_heads, 64, head_dim] (zeros behind a request's last), and a block table over those runs.
+// [runs, kv_heads, 64, head_dim] (zeros behind a request's last), a block table over those runs and (starts, if wanted) the requests'
+// first tokens counted from the first one's.
 // ---------------------------------------------------------------------------
 struct ReadParams {
   const int8_t *k_pages, *v_pages;
@@ -152,7 +153,7 @@ struct ReadParams {
   const int *block_table, *q_start, *start_pos;
   int max_pages, num_pages, page_size, block, first_seq, num_seqs, kv_heads, head_dim, window;
   void *k_out, *v_out;
-  int* table;
+  int *table, *starts;
   int runs, width;
   int* status;
 };
@@ -173,7 +174,10 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   pdl_trigger();
   const int run = blockIdx.x, kvh = blockIdx.y;
   if (run == p.runs) {                         // the last block: table entries that name no run, and a look at the sum of all
+    pdl_wait();
     if (kvh != 0) return;
+    for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += blockDim.x)
+      p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
     int total = 0;
     for (int seq = p.first_seq; seq < p.num_seqs; ++seq) {
       const Span s = span_of(p, seq);
@@ -269,14 +273,14 @@ TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, v
 
 TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int num_pages, int page_size,
                           int block, const int* block_table, int max_pages, const int* q_start, const int* start_pos, int first_seq,
-                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int is_bf16, int* table, int runs,
+                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int is_bf16, int* table, int* starts, int runs,
                           int width, int* status, cudaStream_t stream) {
   const int rc = cache_shape("read_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
   if (rc != 0) return rc;
   TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
   if (num_seqs == first_seq || width == 0) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
-                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, runs, width, status};
+                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, starts, runs, width, status};
   const dim3 grid(runs + 1, kv_heads);
   if (is_bf16)
     tge_launch(read_8bit_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);

@@ -206,8 +206,13 @@ def core() -> ctypes.CDLL:
                                          _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                          _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr])
         _declare(lib, "tge_read_8bit", [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
-                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int,
+                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int,
                                         _c_ptr, _c_ptr])
+        lib.tge_attention_8bit_decode_floats.argtypes = [_c_int] * 7
+        lib.tge_attention_8bit_decode_floats.restype = _c_ll
+        _declare(lib, "tge_attention_8bit_decode", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                                    _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int,
+                                                    _c_float, _c_int, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr])
         _declare(lib, "tge_attention_8bit_simple", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                                     _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ll, _c_int, _c_int,
                                                     _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_ptr])
@@ -1171,6 +1176,11 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
         raise KernelError(f"8-bit pages must be [pages, kv_heads, page_size, head_dim], got {tuple(k_pages.shape)}")
     if dtype not in _FLOAT:
         raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
+    return _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, None)
+
+
+def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
+    """:func:`read_cache_8bit`, and the requests' q_start counted from ``first_seq``'s into ``starts``."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
     num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
     _portions(q_start, start_pos, num_seqs)
@@ -1184,7 +1194,7 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
     _check(lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                              block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
                              kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), int(dtype == torch.bfloat16), table.data_ptr(),
-                             runs, width, status_word().data_ptr(), _stream()), lib)
+                             _ptr(starts), runs, width, status_word().data_ptr(), _stream()), lib)
     return k, v, table
 
 
@@ -1221,11 +1231,34 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     _want(out, "attention output", q.dtype, contiguous=False)
     if tuple(out.shape) != (tokens, heads * head_dim):
         raise KernelError(f"attention: the output must be [{tokens}, {heads * head_dim}], got {tuple(out.shape)}")
-    lib = core()
-    _check(lib.tge_attention_8bit_simple(q.data_ptr(), int(q.dtype == torch.bfloat16), q_stride, k_pages.data_ptr(), v_pages.data_ptr(),
-                                         k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block, block_table.data_ptr(),
-                                         block_table.shape[1], positions.data_ptr(), seq_of_token.data_ptr(), num_seqs, tokens,
-                                         out.data_ptr(), _rows_2d(out, "attention output"), heads, kv_heads, head_dim, float(scale),
+    out_stride, is_bf16 = _rows_2d(out, "attention output"), int(q.dtype == torch.bfloat16)
+    lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
+                          block_table.data_ptr(), block_table.shape[1])
+    singles = num_seqs if max_q_len <= 1 else decode_prefix
+    done = 0                                            # requests, and so tokens, that are served
+    if singles:
+        need = lib.tge_attention_8bit_decode_floats(is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
+        if need >= 0:
+            parts = torch.empty(need, dtype=torch.float32, device=q.device)
+            rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
+                                               out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
+                                               parts.data_ptr(), need, status_word().data_ptr(), _stream())
+            if _check(rc, lib) != UNSUPPORTED:
+                done = singles
+    if done == num_seqs:
+        return out
+    ctx_lens = [max_ctx_len] * num_seqs if ctx_lens is None else ctx_lens
+    if max_q_len > 1 and done == singles and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
+                                              else head_dim in (16, 32, 64, 128) and sink is None):
+        # portions: their keys and values are read once into run-type pages of 64, which the prefill kernels take; a query tile of
+        # those reads each of them again, so that turning codes into numbers there would be done many times over
+        starts = torch.empty(num_seqs - done + 1, dtype=torch.int32, device=q.device)
+        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, done, starts)
+        attention(q[done:, :heads * head_dim], k, v, table, starts, start_pos[done:], positions[done:], seq_of_token[done:], num_seqs - done,
+                  max_q_len, max(ctx_lens[done:]), heads, kv_heads, head_dim, scale, window=window, out=out[done:], sink=sink)
+        return out
+    _check(lib.tge_attention_8bit_simple(q[done:].data_ptr(), is_bf16, q_stride, *cache, positions[done:].data_ptr(), seq_of_token[done:].data_ptr(),
+                                         num_seqs, tokens - done, out[done:].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale),
                                          int(window), _ptr(sink), status_word().data_ptr(), _stream()), lib)
     return out
 
