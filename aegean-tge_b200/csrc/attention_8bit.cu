@@ -92,22 +92,26 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 }
 
 // ---------------------------------------------------------------------------
-// Single tokens on the tensor cores: head sizes 64, 128 and 256, pages that are multiples of 16 positions.
+// Single tokens on the tensor cores: head sizes 64, 128 and 256, pages of 16, 32, 64, ... positions.
 //
 // What bounds it: the cache's bytes, 2 head_dim + 8 / block of them a position and kv head.  A warp takes slices of 16 positions and
 // nothing of them passes through shared memory: codes go from global memory into the registers that hold them as operands.
-//   scores   S^T [16 positions x 8 heads] = C [16 x d] Q^T [d x 8]   (mma m16n8k16, a position per row): a lane needs, of positions
-//            g and g + 8 (g = lane / 4), a quarter of the row, whole 16-byte chunks, because the order of d is free as long as the
-//            queries come in the same one;
-//   values   O^T [d x 8 heads] += C'^T [d x 16 positions] P^T [16 x 8]: a lane needs, of positions 2t, 2t + 1, 2t + 8, 2t + 9
-//            (t = lane % 4), the numbers that are rows g and g + 8 of every 16-row tile; which 16 numbers of d make a tile is free
-//            too, so they are those of one 16-byte chunk.
+//   scores   S^T [16 positions x 8 heads] = C [16 x d] Q^T [d x 8]   (m16n8k32 of 8-bit whole numbers, a position per row): a lane
+//            needs, of positions g and g + 8 (g = lane / 4), a quarter of the row, whole 16-byte chunks, because the order of d is
+//            free as long as the queries come in the same one.  The codes are operands as they are.  A row of queries is rounded to
+//            whole numbers of 15 bits (float32: 22) of its largest and taken as two (three) digits to the base 128, whose products are
+//            added exactly in 32 bits: 2^-15 of the row's largest number is a 64th of what bfloat16 has rounded that number by;
+//   values   O^T [d x 8 heads] += C'^T [d x 16 positions] P^T [16 x 8]   (m16n8k16 of float16): a lane needs, of positions 2t, 2t + 1,
+//            2t + 8, 2t + 9 (t = lane % 4), the numbers that are rows g and g + 8 of every 16-row tile; which 16 numbers of d make a
+//            tile is free too, so they are those of one 16-byte chunk.  A code becomes a float16 exactly: its byte, the sign bit turned over,
+//            below the exponent of 1,024, less 1,152.  (Whole numbers would need no conversion here either, but a probability's small
+//            numbers matter: a long tail of 2^-16 each must not become zeros.)  p is at most 2^8; with its position's scale over the largest
+//            scale so far it is held times 2^6, at most 2^15, and keeps 11 bits down to 2^-21 of a probability of 1 and some down to
+//            2^-31.  float32 runs add what float16 leaves of it as a second part.
 // Every load of the codes is 16 bytes a lane and whole 128-byte lines a warp.  Probabilities turn from S^T's accumulators into P^T's
 // operand by two 8x8 transposes.  With heads as the narrow side of 8, a group of up to 8 heads wastes no more than its rest.
-// A code becomes a bfloat16 exactly: (0x4300 | low seven bits) - (0x4300 | sign bit), that is 128 + low - (128 or 256), two numbers at a
-// time.  Scales go on scores and probabilities in float32.  The running maximum is raised only when a score passes it by 2^8 (one
-// vote a slice); the sums of probabilities stay in their lanes until the end.
-// float32 queries and probabilities are the sum of three bfloat16 numbers each, products of parts are added in float32.
+// The running maximum is raised only when a score passes it by 2^8, the scales' one when a scale is twice it (one vote a slice); the
+// sums of probabilities stay in their lanes until the end.
 //
 // Work: the slices of all (request, kv head, tile of heads) units in one row, cut into equal runs, one per block, whatever the
 // requests' lengths; the blocks work that out from the lengths on the device, so a captured graph stays right as they grow.  A run
@@ -116,22 +120,26 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // ---------------------------------------------------------------------------
 constexpr int DWARPS = 8;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float HELD = 64.0f;                   // probabilities are held times this
 
 struct Decode8 {
   Attn8 a;
   const int *q_start, *start_pos;
   int units;                                    // per request: kv heads x tiles of heads
   int head_tiles, least;                        // least: slices of a run
-  float* parts;                                 // [2 x blocks][heads of a tile][head_dim + 2]
+  int page_shift, block_shift;                  // pages and blocks are powers of two here: no division in the loop
+  int q_by_eight;                               // queries may be read eight bytes (two words) at a time
+  float *parts, *states;                        // [2 x blocks][heads of a tile][head_dim], [2 x blocks][heads of a tile][2]
 };
 
 // The slices of 16 positions that request `seq` sees: [first, first + count).
-struct Slices { int pos, lo, hi, first, count; };
+struct Slices { int lo, hi, first, count; };
 __device__ __forceinline__ Slices slices_of(const Decode8& p, int seq) {
   Slices s;
-  s.pos = p.start_pos[seq];
-  s.hi = min(max(s.pos + 1, 0), p.a.max_pages * p.a.page_size);
-  s.lo = p.a.window > 0 ? max(s.pos - p.a.window + 1, 0) : 0;
+  const int pos = p.start_pos[seq];
+  s.hi = min(max(pos + 1, 0), p.a.max_pages << p.page_shift);
+  s.lo = p.a.window > 0 ? max(pos - p.a.window + 1, 0) : 0;
   s.first = s.lo >> 4;
   s.count = max((s.hi + 15) / 16 - s.first, 1);
   return s;
@@ -147,97 +155,165 @@ __device__ __forceinline__ int slices_before(const Decode8& p, int upto, int lan
 }
 __device__ __forceinline__ int run_length(const Decode8& p, int total, int blocks) { return max((total + blocks - 1) / blocks, p.least); }
 
-__device__ __forceinline__ uint32_t even_codes(uint32_t x) {      // bytes 0 and 2 as two bfloat16
-  uint32_t low, high, r;
-  asm("lop3.b32 %0, %1, 0x007f007f, 0x43004300, 0xea;\n" : "=r"(low) : "r"(x));
-  asm("lop3.b32 %0, %1, 0x00800080, 0x43004300, 0xea;\n" : "=r"(high) : "r"(x));
-  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(low), "r"(high));
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Codes of bytes `which` of two words as two float16.
+__device__ __forceinline__ uint32_t two_codes(uint32_t a, uint32_t b, uint32_t which) {
+  uint32_t r = __byte_perm(a, b, which), v;
+  asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;\n" : "=r"(v) : "r"(r));       // (r & mask) ^ pattern: 1,024 + (byte ^ 128)
+  asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0xe480e480u));            // - 1,152
   return r;
 }
-__device__ __forceinline__ uint32_t odd_codes(uint32_t x) { return even_codes(x >> 8); }
 
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {      // an 8x8 tile of 16-bit numbers across the warp
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-// What bfloat16 leaves of a pair, as the next pair of parts.
+// What float16 leaves of a pair.
 __device__ __forceinline__ void leave(uint32_t taken, float& lo, float& hi) {
-  const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&taken));
-  lo -= v.x;
-  hi -= v.y;
+  float a, b;
+  asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.f32.f16 %0, x;\ncvt.f32.f16 %1, y;\n}\n" : "=f"(a), "=f"(b) : "r"(taken));
+  lo -= a;
+  hi -= b;
 }
 
 template <int HD>
 struct Codes {
   static constexpr int KC = HD / 64;            // 16-byte chunks of a key that a lane holds
   static constexpr int VB = HD >= 128 ? 16 : HD / 8, VC = HD / 8 / VB;   // bytes of a chunk of a value, chunks
-  uint4 k[2][KC];
+  uint32_t k[2][KC][4];
   uint32_t v[4][VC][VB / 4];
   float ks[2], vs[2];
 };
 
+__device__ __forceinline__ void load16(const void* src, uint32_t (&x)[4]) {
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "l"(src));
+}
+__device__ __forceinline__ void load16(const void* src, uint32_t (&x)[2]) {     // the half of it that heads of 64 numbers have
+  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n" : "=r"(x[0]), "=r"(x[1]) : "l"(src));
+}
+
 template <int HD>
 __device__ __forceinline__ void load_keys(const Decode8& p, Codes<HD>& c, size_t row, int g, int t) {
+  const int8_t* src = p.a.k_pages + (row + g) * HD + 16 * t;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const size_t entry = row + g + 8 * i;
 #pragma unroll
-    for (int j = 0; j < Codes<HD>::KC; ++j)
-      c.k[i][j] = __ldcs(reinterpret_cast<const uint4*>(p.a.k_pages + entry * HD) + t + 4 * j);
-    c.ks[i] = p.a.k_scale[entry / p.a.block];
+    for (int j = 0; j < Codes<HD>::KC; ++j) load16(src + 8 * i * HD + 64 * j, c.k[i][j]);
+    c.ks[i] = p.a.k_scale[(row + g + 8 * i) >> p.block_shift];
   }
 }
 template <int HD>
 __device__ __forceinline__ void load_values(const Decode8& p, Codes<HD>& c, size_t row, int g, int t) {
+  const int8_t* src = p.a.v_pages + (row + 2 * t) * HD + Codes<HD>::VB * g;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int8_t* src = p.a.v_pages + (row + 2 * t + (i & 1) + 8 * (i >> 1)) * HD;
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < Codes<HD>::VC; ++j) {
-      if constexpr (Codes<HD>::VB == 16) {
-        const uint4 x = __ldcs(reinterpret_cast<const uint4*>(src) + g + 8 * j);
-        c.v[i][j][0] = x.x; c.v[i][j][1] = x.y; c.v[i][j][2] = x.z; c.v[i][j][3] = x.w;
-      } else {
-        const uint2 x = __ldcs(reinterpret_cast<const uint2*>(src) + g);
-        c.v[i][j][0] = x.x; c.v[i][j][1] = x.y;
-      }
-    }
-  }
+    for (int j = 0; j < Codes<HD>::VC; ++j) load16(src + ((i & 1) + 8 * (i >> 1)) * HD + 128 * j, c.v[i][j]);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) c.vs[i] = p.a.v_scale[(row + g + 8 * i) / p.a.block];
+  for (int i = 0; i < 2; ++i) c.vs[i] = p.a.v_scale[(row + g + 8 * i) >> p.block_shift];
 }
 
-// The queries' parts as operands: for head `h` the four numbers from d on, in the order (d, d + 2), (d + 1, d + 3).
-template <typename T, int PARTS>
-__device__ __forceinline__ void query_operands(const T* q, bool valid, int d, uint32_t (&b)[PARTS][2]) {
-  float x[4];
+// Four numbers of a row of queries.
+template <typename T>
+__device__ __forceinline__ void four(const T* q, bool vector, float (&x)[4]) {
+  if (vector) {
+    if constexpr (sizeof(T) == 2) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(q);
+      x[0] = __uint_as_float(raw.x << 16); x[1] = __uint_as_float(raw.x & 0xffff0000u);
+      x[2] = __uint_as_float(raw.y << 16); x[3] = __uint_as_float(raw.y & 0xffff0000u);
+    } else {
+      const float2 lo = *reinterpret_cast<const float2*>(q), hi = *reinterpret_cast<const float2*>(q + 2);
+      x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = valid ? to_float<T>(q[d + i]) : 0.0f;
-#pragma unroll
-  for (int part = 0; part < PARTS; ++part) {
-    b[part][0] = two_bf16(x[0], x[2]);
-    b[part][1] = two_bf16(x[1], x[3]);
-    leave(b[part][0], x[0], x[2]);
-    leave(b[part][1], x[1], x[3]);
+    for (int i = 0; i < 4; ++i) x[i] = to_float<T>(q[i]);
   }
+}
+
+// A row of queries as DIGITS whole numbers to the base 128 per number, four numbers to a word, in the order of the codes' words; the lane has
+// a quarter of the row, the four lanes of a row agree on its largest number.  Returns what the whole numbers are to be multiplied with
+// (NaN if a number is not finite).
+template <typename T, int HD, int DIGITS>
+__device__ __forceinline__ float query_digits(const T* q, bool valid, bool vector, int t, uint32_t (&b)[HD / 64][4][DIGITS]) {
+  constexpr float TOP = DIGITS == 2 ? 16256.0f : 2080768.0f;          // 127 x 128^(DIGITS - 1)
+  float most = 0.0f;
+  bool fine = true;
+  auto each = [&](auto use) {
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (valid) four<T>(q + 16 * (t + 4 * j) + 4 * w, vector, x);
+        use(j, w, x);
+      }
+  };
+  each([&](int, int, const float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      most = fmaxf(most, fabsf(x[i]));
+      fine &= fabsf(x[i]) < INFINITY;
+    }
+  });
+  most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const float over = most > 1e-30f ? TOP / most : 0.0f;               // rows below that are zeros
+  each([&](int j, int w, const float (&x)[4]) {
+    int whole[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) whole[i] = __float2int_rn(x[i] * over);
+#pragma unroll
+    for (int digit = DIGITS - 1; digit >= 0; --digit) {
+      int here[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rest = (whole[i] + 64) >> 7;
+        here[i] = digit > 0 ? whole[i] - 128 * rest : whole[i];
+        whole[i] = rest;
+      }
+      b[j][w][digit] = __byte_perm(__byte_perm(here[0], here[1], 0x0040), __byte_perm(here[2], here[3], 0x0040), 0x5410);
+    }
+  });
+  // a number that is not finite in any quarter
+  const unsigned rest = __ballot_sync(0xffffffffu, !fine) >> (threadIdx.x & 28);
+  return (rest & 15u) == 0u ? most * (1.0f / TOP) : __int_as_float(0x7fc00000);
+}
+
+// The first of the two numbers of d that a pair in the accumulators' order is (tile pair / 8, lanes g = pair % 8).
+template <int HD>
+__device__ __forceinline__ int number_of(int pair) {
+  constexpr int VB = Codes<HD>::VB;
+  const int i = pair >> 3, g = pair & 7, j = i / (VB / 2);
+  return VB * (g + 8 * j) + 2 * (i - j * (VB / 2));
 }
 
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 ? 2 : 1) decode_8bit_kernel(const Decode8 p) {
-  constexpr int PARTS = sizeof(T) == 2 ? 1 : 3;
-  constexpr int HEADS = 8 * NT, KSTEPS = HD / 16, MTILES = HD / 16, PITCH = HD + 4;
+  constexpr int DIGITS = sizeof(T) == 2 ? 2 : 3, PARTS = sizeof(T) == 2 ? 1 : 2;
+  constexpr int HEADS = 8 * NT, MTILES = HD / 16, PITCH = HD + 4;
   using C = Codes<HD>;
-  extern __shared__ float merge_o[];                              // [warps][HEADS][PITCH]
-  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS];
+  extern __shared__ float merge_o[];                              // [warps][HEADS][PITCH], a head's numbers in the order of the accumulators
+  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS];
   __shared__ int start_of[4];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = uniform_warp_index();
@@ -285,14 +361,35 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
     const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
     const int token = p.q_start[seq];
     const int* table = p.a.block_table + (size_t)seq * p.a.max_pages;
+    const int first = s.first + skip, last = first + length;
+    bool bad = false;
+    auto page_of = [&](int slice) {
+      const int index = (slice << 4) >> p.page_shift;
+      return slice < last && index < p.a.max_pages ? table[index] : -1;
+    };
+    // the entry at which a slice starts; a page outside the pool reads page 0, unseen
+    auto row_of = [&](int slice, int page) {
+      const bool here = page >= 0 && page < p.a.num_pages;
+      return ((size_t)((here ? page : 0) * p.a.kv_heads + kvh) << p.page_shift) + ((slice << 4) & (p.a.page_size - 1));
+    };
+    C c;
+    int slice = first + warp;
+    int page = page_of(slice), page_next = page_of(slice + DWARPS);
+    if (slice < last) {
+      const size_t row = row_of(slice, page);
+      load_keys<HD>(p, c, row, g, t);
+      load_values<HD>(p, c, row, g, t);
+    }
 
-    uint32_t q[NT][KSTEPS][PARTS][2];
+    uint32_t q[NT][HD / 64][4][DIGITS];
+    float factor[NT][2];                                          // of the scores of heads 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool valid = 8 * nt + g < heads_here;
       const T* src = static_cast<const T*>(p.a.q) + (size_t)token * p.a.q_stride + (size_t)(head0 + (valid ? 8 * nt + g : 0)) * HD;
-#pragma unroll
-      for (int kc = 0; kc < KSTEPS; ++kc) query_operands<T, PARTS>(src, valid, 16 * (t + 4 * (kc >> 2)) + 4 * (kc & 3), q[nt][kc]);
+      const float unit_of = query_digits<T, HD, DIGITS>(src, valid, p.q_by_eight != 0, t, q[nt]) * (p.a.scale * (LOG2E / 127.0f));
+      factor[nt][0] = __shfl_sync(0xffffffffu, unit_of, 8 * t);
+      factor[nt][1] = __shfl_sync(0xffffffffu, unit_of, 8 * t + 4);
     }
     float o[NT][MTILES][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -304,27 +401,8 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
       m[nt][0] = m[nt][1] = NONE;
       l[nt][0] = l[nt][1] = 0.0f;
     }
-    const float factor = p.a.scale * (1.4426950408889634f / 127.0f);
+    float v_most = 1e-30f, v_over = HELD / 1e-30f;                // the largest scale of the values so far, and what scales are multiplied with
 
-    const int first = s.first + skip, last = first + length;
-    bool bad = false;
-    // the entry at which a slice starts; a page outside the pool reads page 0, unseen
-    auto page_of = [&](int slice) {
-      const int index = slice * 16 / p.a.page_size;
-      return slice < last && index < p.a.max_pages ? table[index] : -1;
-    };
-    auto row_of = [&](int slice, int page) {
-      const bool here = page >= 0 && page < p.a.num_pages;
-      return ((size_t)(here ? page : 0) * p.a.kv_heads + kvh) * p.a.page_size + (slice * 16) % p.a.page_size;
-    };
-    C c;
-    int slice = first + warp;
-    int page = page_of(slice), page_next = page_of(slice + DWARPS);
-    if (slice < last) {
-      const size_t row = row_of(slice, page);
-      load_keys<HD>(p, c, row, g, t);
-      load_values<HD>(p, c, row, g, t);
-    }
     for (; slice < last; slice += DWARPS) {
       const int next = slice + DWARPS;
       const size_t row_next = row_of(next, page_next);
@@ -335,51 +413,63 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
 
       float sc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        int acc[DIGITS][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] = 0.0f;
+        for (int digit = 0; digit < DIGITS; ++digit)
 #pragma unroll
-      for (int j = 0; j < C::KC; ++j) {
-        const uint32_t *w0 = reinterpret_cast<const uint32_t*>(&c.k[0][j]), *w1 = reinterpret_cast<const uint32_t*>(&c.k[1][j]);
+          for (int e = 0; e < 4; ++e) acc[digit][e] = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t a0 = even_codes(w0[w]), a1 = even_codes(w1[w]), a2 = odd_codes(w0[w]), a3 = odd_codes(w1[w]);
+        for (int j = 0; j < C::KC; ++j)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int w = 0; w < 4; w += 2)
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part)
-              mma_16x8x16(sc[nt], a0, a1, a2, a3, q[nt][4 * j + w][part][0], q[nt][4 * j + w][part][1]);
+            for (int digit = 0; digit < DIGITS; ++digit)
+              mma_s8(acc[digit], c.k[0][j][w], c.k[1][j][w], c.k[0][j][w + 1], c.k[1][j][w + 1], q[nt][j][w][digit], q[nt][j][w + 1][digit]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // at most 256 x 127 x 127 in a digit's sum: two of them fit 32 bits, the third is added in float32
+          float sum = (float)(128 * acc[DIGITS - 2][e] + acc[DIGITS - 1][e]);
+          if constexpr (DIGITS == 3) sum = fmaf((float)acc[0][e], 16384.0f, sum);
+          sc[nt][e] = sum;
         }
       }
-      const float f0 = c.ks[0] * factor, f1 = c.ks[1] * factor;
-      const float v0 = c.vs[0] * (1.0f / 127.0f), v1 = c.vs[1] * (1.0f / 127.0f);
-      if (next < last) load_keys<HD>(p, c, row_next, g, t);
-
       const int k0 = slice * 16 + g;
       const bool see0 = here && k0 >= s.lo && k0 < s.hi, see1 = here && k0 + 8 >= s.lo && k0 + 8 < s.hi;
-      bool raise = false;
+      const float f0 = c.ks[0], f1 = c.ks[1];
+      // an unseen position's scales may be anything, NaN too
+      const float v0 = see0 ? c.vs[0] : 0.0f, v1 = see1 ? c.vs[1] : 0.0f;
+      if (next < last) load_keys<HD>(p, c, row_next, g, t);
+
+      bool raise = fmaxf(v0, v1) > 2.0f * v_most;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sc[nt][e] = see0 ? sc[nt][e] * f0 : -INFINITY;
-          sc[nt][2 + e] = see1 ? sc[nt][2 + e] * f1 : -INFINITY;
+          sc[nt][e] = see0 ? sc[nt][e] * (f0 * factor[nt][e]) : -INFINITY;
+          sc[nt][2 + e] = see1 ? sc[nt][2 + e] * (f1 * factor[nt][e]) : -INFINITY;
           raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + 8.0f;
         }
       if (__any_sync(0xffffffffu, raise)) {
+        float v_now = fmaxf(fmaxf(v0, v1), v_most);
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) v_now = fmaxf(v_now, __shfl_xor_sync(0xffffffffu, v_now, offset));
+        const float v_down = v_most / v_now;
+        v_most = v_now;
+        v_over = HELD / v_now;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float down[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float most = fmaxf(sc[nt][e], sc[nt][2 + e]);
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+#pragma unroll
+            for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
             most = fmaxf(most, m[nt][e]);
-            down[e] = exp2f(m[nt][e] - most);
+            down[e] = exp2_fast(m[nt][e] - most);
             m[nt][e] = most;
             l[nt][e] *= down[e];
+            down[e] *= v_down;
           }
 #pragma unroll
           for (int i = 0; i < MTILES; ++i) {
@@ -389,18 +479,17 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
         }
       }
       uint32_t pr[NT][PARTS][2];
+      const float w0 = v0 * v_over, w1 = v1 * v_over;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float e0 = exp2f(sc[nt][0] - m[nt][0]), e1 = exp2f(sc[nt][1] - m[nt][1]);
-        float e2 = exp2f(sc[nt][2] - m[nt][0]), e3 = exp2f(sc[nt][3] - m[nt][1]);
+        float e0 = exp2_fast(sc[nt][0] - m[nt][0]), e1 = exp2_fast(sc[nt][1] - m[nt][1]);
+        float e2 = exp2_fast(sc[nt][2] - m[nt][0]), e3 = exp2_fast(sc[nt][3] - m[nt][1]);
         l[nt][0] += e0 + e2;
         l[nt][1] += e1 + e3;
-        // an unseen position's scale may be anything, NaN too
-        e0 = see0 ? e0 * v0 : 0.0f; e1 = see0 ? e1 * v0 : 0.0f;
-        e2 = see1 ? e2 * v1 : 0.0f; e3 = see1 ? e3 * v1 : 0.0f;
+        e0 *= w0; e1 *= w0; e2 *= w1; e3 *= w1;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const uint32_t x = two_bf16(e0, e1), y = two_bf16(e2, e3);
+          const uint32_t x = two_halves(e0, e1), y = two_halves(e2, e3);
           pr[nt][part][0] = transposed(x);
           pr[nt][part][1] = transposed(y);
           if (part + 1 < PARTS) {
@@ -415,71 +504,72 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
         for (int w = 0; w < C::VB / 4; ++w)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            // two bytes of a word of positions 2t and 2t + 1, and of 2t + 8 and 2t + 9: rows g and g + 8 of a tile
-            const uint32_t x = __byte_perm(c.v[0][j][w], c.v[1][j][w], half ? 0x7632 : 0x5410);
-            const uint32_t y = __byte_perm(c.v[2][j][w], c.v[3][j][w], half ? 0x7632 : 0x5410);
-            const uint32_t a0 = even_codes(x), a1 = odd_codes(x), a2 = even_codes(y), a3 = odd_codes(y);
+            // bytes 2 half and 2 half + 1 of a word of positions 2t and 2t + 1, and of 2t + 8 and 2t + 9: rows g and g + 8 of a tile
+            const uint32_t low = half ? 0x6622 : 0x4400, high = half ? 0x7733 : 0x5511;
+            const uint32_t a0 = two_codes(c.v[0][j][w], c.v[1][j][w], low), a1 = two_codes(c.v[0][j][w], c.v[1][j][w], high);
+            const uint32_t a2 = two_codes(c.v[2][j][w], c.v[3][j][w], low), a3 = two_codes(c.v[2][j][w], c.v[3][j][w], high);
             const int i = (j * (C::VB / 4) + w) * 2 + half;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int part = 0; part < PARTS; ++part) mma_16x8x16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
+              for (int part = 0; part < PARTS; ++part) mma_f16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
           }
       if (next < last) load_values<HD>(p, c, row_next, g, t);
     }
     if (bad && lane == 0) atomicOr(p.a.status, TGE_STATUS_BAD_PAGE);
 
-    // the warps' states meet in shared memory
+    // the warps' states meet in shared memory: the two numbers of a lane and a tile side by side, then the lanes g, then the tiles
     __syncthreads();                                              // whoever still reads the unit before
+    if (lane == 0) merge_v[warp] = v_most * (1.0f / (127.0f * HELD));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sum = l[nt][e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
         const int head = 8 * nt + 2 * t + e;
         if (g == 0) {
           merge_m[warp][head] = m[nt][e];
           merge_l[warp][head] = sum;
         }
-        float* dst = merge_o + (warp * HEADS + head) * PITCH;
+        float* dst = merge_o + (warp * HEADS + head) * PITCH + 2 * g;
 #pragma unroll
-        for (int i = 0; i < MTILES; ++i) {
-          const int j = i / (C::VB / 2), inner = i - j * (C::VB / 2);
-          *reinterpret_cast<float2*>(dst + C::VB * (g + 8 * j) + 2 * inner) = make_float2(o[nt][i][e], o[nt][i][2 + e]);
-        }
+        for (int i = 0; i < MTILES; ++i) *reinterpret_cast<float2*>(dst + 16 * i) = make_float2(o[nt][i][e], o[nt][i][2 + e]);
       }
     }
     __syncthreads();
     const bool whole = length == s.count;
-    float* part = p.parts + (size_t)(2 * blockIdx.x + (skip == 0 ? 1 : 0)) * HEADS * (HD + 2);
-    for (int i = threadIdx.x; i < heads_here * HD; i += DWARPS * 32) {
-      const int head = i / HD, d = i - head * HD;
+    const size_t place = (size_t)(2 * blockIdx.x + (skip == 0 ? 1 : 0)) * HEADS;
+    for (int i = threadIdx.x; i < heads_here * (HD / 2); i += DWARPS * 32) {
+      const int head = i / (HD / 2), pair = i - head * (HD / 2);
       float most = NONE;
 #pragma unroll
       for (int w = 0; w < DWARPS; ++w) most = fmaxf(most, merge_m[w][head]);
-      float sum = 0.0f, acc = 0.0f;
+      float sum = 0.0f;
+      float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < DWARPS; ++w) {
-        const float f = exp2f(merge_m[w][head] - most);
+        const float f = exp2_fast(merge_m[w][head] - most), fv = f * merge_v[w];
+        const float2 x = *reinterpret_cast<const float2*>(merge_o + (w * HEADS + head) * PITCH + 2 * pair);
         sum = fmaf(f, merge_l[w][head], sum);
-        acc = fmaf(f, merge_o[(w * HEADS + head) * PITCH + d], acc);
+        acc.x = fmaf(fv, x.x, acc.x);
+        acc.y = fmaf(fv, x.y, acc.y);
       }
       if (whole) {
         if (p.a.sink != nullptr) {
-          const float sink = p.a.sink[head0 + head] * 1.4426950408889634f, top = fmaxf(most, sink), down = exp2f(most - top);
-          sum = fmaf(sum, down, exp2f(sink - top));
-          acc *= down;
+          const float sink = p.a.sink[head0 + head] * LOG2E, top = fmaxf(most, sink), down = exp2_fast(most - top);
+          sum = fmaf(sum, down, exp2_fast(sink - top));
+          acc.x *= down;
+          acc.y *= down;
         }
-        static_cast<T*>(p.a.out)[(size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD + d] = from_float<T>(sum == 0.0f ? 0.0f : acc / sum);
+        const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* dst = static_cast<T*>(p.a.out) + (size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD + number_of<HD>(pair);
+        dst[0] = from_float<T>(acc.x * over);
+        dst[1] = from_float<T>(acc.y * over);
       } else {
-        part[head * (HD + 2) + d] = acc;
-        if (d == 0) {
-          part[head * (HD + 2) + HD] = most;
-          part[head * (HD + 2) + HD + 1] = sum;
-        }
+        *reinterpret_cast<float2*>(p.parts + (place + head) * HD + 2 * pair) = acc;
+        if (pair == 0) *reinterpret_cast<float2*>(p.states + (place + head) * 2) = make_float2(most, sum);
       }
     }
     at += length;
@@ -490,14 +580,18 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
   }
 }
 
-// Joins the parts of the units that more than one block worked on: one block per unit.
+// Joins the parts of the units that more than one block worked on: one block per unit, two warps per head, which take the first and the
+// second half of its parts.
+constexpr int JOIN_WARPS = 16, JOIN_AHEAD = 8;
+
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(256) decode_8bit_join_kernel(const Decode8 p, int blocks) {
-  constexpr int HEADS = 8 * NT;
-  __shared__ int where[3];
+__global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const Decode8 p, int blocks) {
+  constexpr int HEADS = 8 * NT, PAIRS = HD / 64;                   // pairs of numbers of a lane
+  __shared__ int where[2];
+  __shared__ float half_m[8], half_l[8], half_o[8][HD];
   pdl_trigger();
-  const int seq = blockIdx.x, unit = blockIdx.y, lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
+  const int seq = blockIdx.x, unit = blockIdx.y, lane = threadIdx.x & 31, warp = uniform_warp_index();
+  if (warp == 0) {
     const int total = slices_before(p, p.a.num_seqs, lane) * p.units, run = run_length(p, total, blocks);
     const int count = slices_of(p, seq).count, from = slices_before(p, seq, lane) * p.units + unit * count;
     if (lane == 0) {
@@ -512,20 +606,71 @@ __global__ void __launch_bounds__(256) decode_8bit_join_kernel(const Decode8 p, 
   const int kvh = unit / p.head_tiles, tile = unit - kvh * p.head_tiles;
   const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
   const int token = p.q_start[seq];
-  for (int i = threadIdx.x; i < heads_here * HD; i += blockDim.x) {
-    const int head = i / HD, d = i - head * HD;
+  const int middle = first + (last - first + 2) / 2;
+  const bool second = warp >= 8;
+  for (int head = warp & 7; head < (heads_here + 7) / 8 * 8; head += 8) {
+    const bool valid = head < heads_here;
+    const int from = second ? middle : first, to = valid ? (second ? last + 1 : middle) : 0;
     // the block in which the unit begins left its part in its second place, the others in their first
-    auto state = [&](int b) { return p.parts + ((size_t)(2 * b + (b == first ? 1 : 0)) * HEADS + head) * (HD + 2); };
-    float most = p.a.sink != nullptr ? p.a.sink[head0 + head] * 1.4426950408889634f : NONE;
-    float sum = p.a.sink != nullptr ? 1.0f : 0.0f, acc = 0.0f;
-    for (int b = first; b <= last; ++b) {
-      const float* part = state(b);
-      const float m = part[HD], top = fmaxf(most, m), down = exp2f(most - top), f = exp2f(m - top);
-      sum = fmaf(sum, down, f * part[HD + 1]);
-      acc = fmaf(acc, down, f * part[d]);
+    auto place = [&](int b) { return (size_t)(2 * b + (b == first ? 1 : 0)) * HEADS + head; };
+    float most = NONE, sum = 0.0f;
+    float2 acc[PAIRS];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) acc[i] = make_float2(0.0f, 0.0f);
+    for (int b0 = from; b0 < to; b0 += 32) {
+      // 32 parts' states, a lane each, then their numbers, the whole warp each
+      const int count = min(32, to - b0);
+      float2 state = make_float2(NONE, 0.0f);
+      if (lane < count) state = *reinterpret_cast<const float2*>(p.states + place(b0 + lane) * 2);
+      const float top = fmaxf(most, warp_max(state.x));
+      const float weight = exp2_fast(state.x - top), down = exp2_fast(most - top);
+      sum = fmaf(sum, down, warp_sum(weight * state.y));
       most = top;
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) { acc[i].x *= down; acc[i].y *= down; }
+      for (int b = 0; b < count; b += JOIN_AHEAD) {
+        float2 x[JOIN_AHEAD][PAIRS];
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k)
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i)
+            x[k][i] = b + k < count ? *reinterpret_cast<const float2*>(p.parts + place(b0 + b + k) * HD + 2 * (lane + 32 * i)) : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) {
+          const float f = __shfl_sync(0xffffffffu, weight, (b + k) & 31);
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            acc[i].x = b + k < count ? fmaf(f, x[k][i].x, acc[i].x) : acc[i].x;
+            acc[i].y = b + k < count ? fmaf(f, x[k][i].y, acc[i].y) : acc[i].y;
+          }
+        }
+      }
     }
-    static_cast<T*>(p.a.out)[(size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD + d] = from_float<T>(sum == 0.0f ? 0.0f : acc / sum);
+    __syncthreads();
+    if (second) {
+      if (lane == 0) {
+        half_m[head & 7] = most;
+        half_l[head & 7] = sum;
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) *reinterpret_cast<float2*>(&half_o[head & 7][2 * (lane + 32 * i)]) = acc[i];
+    }
+    __syncthreads();
+    if (!second && valid) {
+      const float sink = p.a.sink != nullptr ? p.a.sink[head0 + head] * LOG2E : NONE;
+      const float top = fmaxf(fmaxf(most, half_m[head & 7]), sink);
+      const float f0 = exp2_fast(most - top), f1 = exp2_fast(half_m[head & 7] - top);
+      const float all = fmaf(sum, f0, f1 * half_l[head & 7]) + (p.a.sink != nullptr ? exp2_fast(sink - top) : 0.0f);
+      const float over = all == 0.0f ? 0.0f : 1.0f / all;
+      T* dst = static_cast<T*>(p.a.out) + (size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD;
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 x = *reinterpret_cast<const float2*>(&half_o[head & 7][2 * (lane + 32 * i)]);
+        const int d = number_of<HD>(lane + 32 * i);
+        dst[d] = from_float<T>(fmaf(acc[i].x, f0, f1 * x.x) * over);
+        dst[d + 1] = from_float<T>(fmaf(acc[i].y, f0, f1 * x.y) * over);
+      }
+    }
   }
 }
 
@@ -540,8 +685,9 @@ int launch_decode(Decode8 p, int blocks, cudaStream_t stream) {
     TGE_REQUIRE(rc == cudaSuccess, "attention_8bit: %d bytes of shared memory: %s", smem, cudaGetErrorString(rc));
     if (device < 64) ready[device] = true;
   }
+  p.states = p.parts + (size_t)2 * blocks * 8 * NT * HD;
   tge_launch(decode_8bit_kernel<T, HD, NT>, blocks, DWARPS * 32, smem, stream, p);
-  tge_launch(decode_8bit_join_kernel<T, HD, NT>, dim3(p.a.num_seqs, p.units), 256, 0, stream, p, blocks);
+  tge_launch(decode_8bit_join_kernel<T, HD, NT>, dim3(p.a.num_seqs, p.units), JOIN_WARPS * 32, 0, stream, p, blocks);
   return tge_launched("attention_8bit", 2);
 }
 
@@ -556,7 +702,7 @@ static int decode_tile(int group, int head_dim) { return group <= 8 || head_dim 
 
 // float32 scratch numbers of tge_attention_8bit_decode; -1: sizes that it does not take.
 TGE_API long long tge_attention_8bit_decode_floats(int is_bf16, int num_seqs, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
-  if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size % 16 != 0 || kv_heads <= 0 || heads % kv_heads != 0) return -1;
+  if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size < 16 || (page_size & (page_size - 1)) != 0 || kv_heads <= 0 || heads % kv_heads != 0) return -1;
   const int tile = decode_tile(heads / kv_heads, head_dim);
   const long long units = (long long)kv_heads * ((heads / kv_heads + tile - 1) / tile);
   // places in the row of all slices are counted in 32 bits, units along a grid's second axis
@@ -574,6 +720,7 @@ TGE_API int tge_attention_8bit_decode(const void* q, int is_bf16, long long q_st
   if (need < 0 || ((uintptr_t)k_pages | (uintptr_t)v_pages) % 16 != 0) return TGE_UNSUPPORTED;
   TGE_REQUIRE(part_floats >= need, "attention_8bit: %lld floats of scratch memory, %lld wanted", part_floats, need);
   TGE_REQUIRE(num_pages > 0 && block > 0 && page_size % block == 0 && max_pages > 0 && window >= 0, "attention_8bit: bad page geometry");
+  if ((long long)num_pages * kv_heads > 0x7fffffffll) return TGE_UNSUPPORTED;
   if (num_seqs == 0) return 0;
   const int group = heads / kv_heads, tile = decode_tile(group, head_dim);
   Decode8 p;
@@ -584,6 +731,10 @@ TGE_API int tge_attention_8bit_decode(const void* q, int is_bf16, long long q_st
   p.head_tiles = (group + tile - 1) / tile;
   p.units = kv_heads * p.head_tiles;
   p.least = DWARPS;
+  const int element = is_bf16 ? 2 : 4;
+  p.q_by_eight = (uintptr_t)q % 8 == 0 && q_stride * element % 8 == 0;
+  p.page_shift = __builtin_ctz(page_size);
+  p.block_shift = __builtin_ctz(block);
   p.parts = parts;
   const int blocks = decode_blocks(head_dim, tile, is_bf16 != 0);
   auto run = [&](auto type) {
