@@ -11,6 +11,13 @@ namespace {
 
 constexpr int THREADS = 512;
 constexpr int MOST_TOP = 32;
+constexpr int MINE = 16;                        // logits of a thread and round
+constexpr int ROUND = THREADS * MINE;
+constexpr int ROOM = 4096 + MOST_TOP;           // keys in the list of candidates: what one load of all threads may add to a full choice
+constexpr int SORTED_AT_ONCE = 512;             // more are chosen one after the other
+constexpr int MOST_SPLITS = 128;
+constexpr float LEAST = -3.402823466e38f;       // where a thread's reference starts: finite, so that -inf less it is -inf
+constexpr float LOG2E = 1.4426950408889634f;
 
 // An unsigned number that orders like the logit (-0 as 0, NaN below everything), and with the index below it, so that keys of a row
 // are all different: a larger key comes first.
@@ -27,93 +34,382 @@ __device__ __forceinline__ float logit_of(unsigned long long key) {
   return u == 0u ? __int_as_float(0x7fc00000) : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-__device__ __forceinline__ unsigned long long block_largest(unsigned long long v, unsigned long long* scratch) {
+__device__ __forceinline__ unsigned long long warp_largest(unsigned long long v, int width = 32) {
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) {
     const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, offset);
-    v = o > v ? o : v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = (threadIdx.x & 31) < THREADS / 32 ? scratch[threadIdx.x & 31] : 0ull;
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, offset);
-    v = o > v ? o : v;
+    if (offset < width) v = o > v ? o : v;
   }
   return v;
 }
+__device__ __forceinline__ unsigned long long block_largest(unsigned long long v, unsigned long long* scratch) {
+  v = warp_largest(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_largest((threadIdx.x & 31) < THREADS / 32 ? scratch[threadIdx.x & 31] : 0ull);
+}
 
-// One block per row, which passes over it once for the largest key, once for the sums and once per alternative.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) token_logprobs_simple_kernel(const T* logits, long long stride, const int* tokens, int vocab,
-                                                                        int top, float* logprob, float* entropy, int* rank, int* top_ids,
-                                                                        float* top_logprobs, int* status) {
-  __shared__ unsigned long long keys[32];
-  __shared__ float sums[32];
-  pdl_trigger();
-  pdl_wait();
-  const int r = blockIdx.x;
-  const T* x = logits + (size_t)r * stride;
-  const int token = tokens[r];
-  const bool known = token >= 0 && token < vocab;
-  if (!known && threadIdx.x == 0) atomicOr(status, TGE_STATUS_BAD_TOKEN);
-  unsigned long long best = 0;
-  bool broken = false;
-  for (int i = threadIdx.x; i < vocab; i += THREADS) {
-    const float v = to_float<T>(x[i]);
-    broken |= !(v < INFINITY);
-    best = max(best, key_of(v, i));
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Sums over some of a row's logits: z = sum exp(x - m), w = sum exp(x - m) (x - m), relative to a reference m that no logit passes by more
+// than 16; how many of them come before the given token.
+struct Sums {
+  float m, z, w;
+  int before;
+  // the same relative to `to`
+  __device__ __forceinline__ void move(float to) {
+    const float f = exp2_fast((m - to) * LOG2E);
+    w = z > 0.0f && f > 0.0f ? f * fmaf(z, m - to, w) : 0.0f;      // (0 times a distance that may be infinite)
+    z = z > 0.0f ? f * z : z;                          // NaN stays
+    if (!(z == z)) w = z;
+    m = to;
   }
-  broken = __syncthreads_or(broken);
-  best = block_largest(best, keys);
-  const float m = logit_of(best);
-  broken |= !(m > -INFINITY);
-  const unsigned long long mine = known ? key_of(to_float<T>(x[token]), token) : ~0ull;
-  float z = 0.0f, weighed = 0.0f, before = 0.0f;
-  for (int i = threadIdx.x; i < vocab; i += THREADS) {
-    const float v = to_float<T>(x[i]), d = v - m, e = expf(d);
-    z += e;
-    weighed = e > 0.0f ? fmaf(e, d, weighed) : weighed;
-    before += key_of(v, i) > mine ? 1.0f : 0.0f;
+};
+
+// The sums of a block's threads, in every thread.
+__device__ __forceinline__ Sums block_sums(Sums mine, float* scratch, int* counts) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top = warp_max(mine.m);
+  __syncthreads();
+  if (lane == 0) scratch[warp] = top;
+  __syncthreads();
+  top = warp_max(lane < THREADS / 32 ? scratch[lane] : LEAST);
+  mine.move(top);
+  mine.before = __reduce_add_sync(0xffffffffu, mine.before);
+  if (lane == 0) counts[warp] = mine.before;
+  mine.z = block_sum(mine.z, scratch);
+  mine.w = block_sum(mine.w, scratch);
+  mine.before = __reduce_add_sync(0xffffffffu, lane < THREADS / 32 ? counts[lane] : 0);
+  return mine;
+}
+
+// The `top` largest of the `count` keys at `list`, sorted, to its start; the smallest of them (0 if there are fewer).
+__device__ __forceinline__ unsigned long long choose(unsigned long long* list, int count, int top, unsigned long long* scratch) {
+  __syncthreads();
+  if (count <= SORTED_AT_ONCE) {
+    const unsigned long long mine = (int)threadIdx.x < count ? list[threadIdx.x] : 0ull;
+    int ahead = 0;
+    if ((int)(threadIdx.x & ~31) < count)
+      for (int i = 0; i < count; ++i) ahead += list[i] > mine ? 1 : 0;
+    __syncthreads();
+    if ((int)threadIdx.x < count && ahead < top) list[ahead] = mine;
+  } else {
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < top; ++k) {
+      unsigned long long next = 0;
+      for (int i = threadIdx.x; i < count; i += THREADS) next = list[i] < last ? max(next, list[i]) : next;
+      last = block_largest(next, scratch);
+      if (threadIdx.x == 0) scratch[32 + k] = last;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < top) list[threadIdx.x] = scratch[32 + threadIdx.x];
   }
-  z = block_sum(z, sums);
-  weighed = block_sum(weighed, sums);
-  before = block_sum(before, sums);
-  const float nan = __int_as_float(0x7fc00000), log_z = logf(z);
+  __syncthreads();
+  return count >= top ? list[top - 1] : 0ull;
+}
+
+struct LogprobParams {
+  const void* logits;
+  const int* tokens;
+  long long stride;
+  int rows, vocab, top, splits, chunk;          // a row goes in `splits` chunks of `chunk` logits, one block each
+  float *logprob, *entropy, *top_logprobs;
+  int *rank, *top_ids;
+  float* sums;                                  // [rows, splits, 4]
+  unsigned long long* keys;                     // [rows, splits, top]
+  int* status;
+};
+
+// What a row's answers are, once its sums and its first keys are known.
+__device__ __forceinline__ void answer(const LogprobParams& p, int r, const Sums& all, float own, bool known, const unsigned long long* keys) {
+  const float nan = __int_as_float(0x7fc00000);
+  const bool broken = !(all.z > 0.0f);                                // NaN, or nothing but -inf
+  const float log_z = logf(all.z);
   if (threadIdx.x == 0) {
-    logprob[r] = broken || !known ? nan : logit_of(mine) - m - log_z;
-    entropy[r] = broken ? nan : log_z - weighed / z;
-    rank[r] = known ? (int)before : -1;
+    p.logprob[r] = broken || !known ? nan : own - all.m - log_z;
+    p.entropy[r] = broken ? nan : log_z - all.w / all.z;
+    p.rank[r] = known ? all.before : -1;
   }
-  for (int k = 0; k < top; ++k) {
-    if (threadIdx.x == 0) {
-      top_ids[(size_t)r * top + k] = (int)~(uint32_t)best;
-      top_logprobs[(size_t)r * top + k] = broken ? nan : logit_of(best) - m - log_z;
-    }
-    unsigned long long next = 0;
-    for (int i = threadIdx.x; i < vocab && k + 1 < top; i += THREADS) {
-      const unsigned long long key = key_of(to_float<T>(x[i]), i);
-      if (key < best) next = max(next, key);
-    }
-    best = block_largest(next, keys);
+  if ((int)threadIdx.x < p.top) {
+    const unsigned long long key = keys[threadIdx.x];
+    p.top_ids[(size_t)r * p.top + threadIdx.x] = (int)~(uint32_t)key;
+    p.top_logprobs[(size_t)r * p.top + threadIdx.x] = broken ? nan : logit_of(key) - all.m - log_z;
   }
+}
+
+// Sixteen logits of a thread in loads of 16 bytes, `per` of them each: load k holds those from first + (k THREADS + thread) per on.
+// What lies behind the chunk is -inf (and told apart by its index where that matters).
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[MINE]) {
+  constexpr int per = 16 / sizeof(T);
+#pragma unroll
+  for (int k = 0; k < MINE / per; ++k) {
+    const int at = first + (k * THREADS + threadIdx.x) * per;
+    if (VECTOR && at + per <= end) {
+      uint32_t raw[4];
+      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]) : "l"(x + at));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (per == 4) {
+          v[4 * k + i] = __uint_as_float(raw[i]);
+        } else {
+          v[8 * k + 2 * i] = __uint_as_float(raw[i] << 16);
+          v[8 * k + 2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < per; ++i) v[per * k + i] = at + i < end ? to_float<T>(x[at + i]) : -INFINITY;
+    }
+  }
+}
+
+// One pass over a chunk of a row.  What bounds it is reading the logits: a thread holds its next sixteen on their way while it works on
+// these, keeps sums of its own, and looks at single logits only where its largest reaches the smallest of the best so far.  Those that do are listed
+// with the block's others; a list that grows beyond SORTED_AT_ONCE is cut to the best again.  After the first round the best are a
+// choice among the largest of 32 half warps' logits and whatever passes the n-th of those, so that of random rows some hundred
+// logits are ever listed, and of no row more than there is room for.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const LogprobParams p) {
+  constexpr int per = 16 / sizeof(T);
+  __shared__ unsigned long long list[ROOM], scratch[64];
+  __shared__ float floats[32];
+  __shared__ int counts[32], listed;
+  pdl_trigger();
+  const int r = blockIdx.x / p.splits, split = blockIdx.x - r * p.splits, lane = threadIdx.x & 31;
+  const int begin = split * p.chunk, end = min(begin + p.chunk, p.vocab);
+  if (threadIdx.x == 0) listed = 0;
+  pdl_wait();
+  const T* x = static_cast<const T*>(p.logits) + (size_t)r * p.stride;
+  float v[MINE], ahead[MINE];
+  take<T, VECTOR>(x, begin, end, v);
+  const int token = p.tokens[r];
+  const bool known = token >= 0 && token < p.vocab;
+  if (!known && split == 0 && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_TOKEN);
+  const float own = known ? to_float<T>(x[token]) : 0.0f;
+  // before the token come logits that are larger and, with a lower index, equal ones: those of at least `own` in front of it and
+  // of at least the next float behind it
+  const uint32_t bits = __float_as_uint(own + 0.0f);
+  const float above = own != own ? own : __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
+  const bool token_is_nan = own != own;
+  Sums mine{LEAST, 0.0f, 0.0f, 0};
+  unsigned long long least = 0;                  // the smallest of the best so far (0: not as many yet)
+  __syncthreads();
+
+  for (int first = begin; first < end; first += ROUND) {
+    if (first + ROUND < end) take<T, VECTOR>(x, first + ROUND, end, ahead);
+    float largest = v[0];
+#pragma unroll
+    for (int i = 1; i < MINE; ++i) largest = fmaxf(largest, v[i]);
+    if (largest > mine.m + 16.0f) mine.move(largest);
+    float z = 0.0f, w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const float d = v[i] - mine.m, e = exp2_fast(d * LOG2E);
+      z += e;
+      w = fmaf(e, fmaxf(d, -200.0f), w);        // -inf has no weight (and NaN shows in z)
+    }
+    mine.z += z;
+    mine.w += w;
+    auto index_of = [&](int i) { return first + ((i / per) * THREADS + (int)threadIdx.x) * per + i % per; };
+    if (!token_is_nan) {
+#pragma unroll
+      for (int k = 0; k < MINE / per; ++k) {
+        const int at = index_of(per * k);
+        if (at <= token && token < at + per) {
+#pragma unroll
+          for (int i = 0; i < per; ++i) mine.before += v[per * k + i] >= (at + i < token ? own : above) ? 1 : 0;
+        } else {
+          const float from = at < token ? own : above;
+#pragma unroll
+          for (int i = 0; i < per; ++i) mine.before += v[per * k + i] >= from ? 1 : 0;
+        }
+      }
+    } else {                                     // it comes behind all that are numbers
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) mine.before += index_of(i) < end && (v[i] == v[i] || index_of(i) < token) ? 1 : 0;
+    }
+
+    if (p.top > 0) {
+      if (first == begin) {                      // the n-th of the half warps' largest keys: that many logits are no smaller
+        unsigned long long key = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+          if (index_of(i) < end) key = max(key, key_of(v[i], index_of(i)));
+        key = warp_largest(key, 16);
+        if ((lane & 15) == 0) scratch[threadIdx.x >> 4] = key;
+        __syncthreads();
+        key = scratch[lane];
+        int in_front = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) in_front += __shfl_sync(0xffffffffu, key, i) > key ? 1 : 0;
+        const unsigned nth = __ballot_sync(0xffffffffu, key != 0 && in_front == p.top - 1);
+        // keys of at least the n-th: those above its predecessor
+        least = nth ? __shfl_sync(0xffffffffu, key, __ffs(nth) - 1) - 1 : 0ull;
+      }
+      const float bar = logit_of(least);         // NaN where anything may enter
+      int entering = 0;
+      if (!(largest < bar)) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+          if (!(v[i] < bar)) entering += index_of(i) < end && key_of(v[i], index_of(i)) > least ? 1 : 0;
+      }
+      int place = 0;
+      if (entering > 0) {
+        place = atomicAdd(&listed, entering);
+        int at = place;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+          if (index_of(i) < end && key_of(v[i], index_of(i)) > least) {
+            if (at < ROOM) list[at] = key_of(v[i], index_of(i));
+            ++at;
+          }
+      }
+      const bool full = __syncthreads_or(place + entering > SORTED_AT_ONCE);
+      if (full || first == begin) {
+        const int count = listed;
+        if (count <= ROOM) {
+          least = max(least, choose(list, count, p.top, scratch));
+          if (threadIdx.x == 0) listed = min(count, p.top);
+          __syncthreads();
+        } else {
+          // more than there is room for: again, a load of every thread at a time.  What the list held before this round lies in
+          // front of it no longer (threads wrote in any order): the whole chunk up to here is looked through.
+          __syncthreads();
+          if (threadIdx.x == 0) listed = 0;
+          least = 0;
+          __syncthreads();
+          for (int from = begin; from <= first; from += ROUND)
+            for (int k = 0; k < MINE / per; ++k) {
+              const int at0 = from + (k * THREADS + (int)threadIdx.x) * per;
+              for (int i = 0; i < per; ++i) {
+                const int index = at0 + i;
+                const unsigned long long key = index < end ? key_of(to_float<T>(x[index]), index) : 0ull;
+                if (key > least) list[atomicAdd(&listed, 1)] = key;
+              }
+              __syncthreads();
+              const int so_far = listed;
+              least = max(least, choose(list, so_far, p.top, scratch));
+              if (threadIdx.x == 0) listed = min(so_far, p.top);
+              __syncthreads();
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) v[i] = ahead[i];
+  }
+  if (p.top > 0) {
+    __syncthreads();
+    choose(list, listed, p.top, scratch);
+  }
+  const int found = p.top > 0 ? min(listed, p.top) : 0;
+  mine = block_sums(mine, floats, counts);
+  if (p.splits == 1) {
+    answer(p, r, mine, own, known, list);
+    return;
+  }
+  const size_t place = (size_t)r * p.splits + split;
+  if (threadIdx.x == 0) *reinterpret_cast<float4*>(p.sums + 4 * place) = make_float4(mine.m, mine.z, mine.w, __int_as_float(mine.before));
+  if ((int)threadIdx.x < p.top) p.keys[place * p.top + threadIdx.x] = (int)threadIdx.x < found ? list[threadIdx.x] : 0ull;
+}
+
+// The chunks of a row joined: their sums in order, and the best of their best.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const LogprobParams p) {
+  __shared__ unsigned long long list[ROOM], scratch[64];
+  __shared__ int listed;
+  pdl_trigger();
+  const int r = blockIdx.x, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) listed = 0;
+  pdl_wait();
+  const int token = p.tokens[r];
+  const bool known = token >= 0 && token < p.vocab;
+  const float own = known ? to_float<T>(static_cast<const T*>(p.logits)[(size_t)r * p.stride + token]) : 0.0f;
+  // every warp for itself, splits lane by lane
+  Sums part[MOST_SPLITS / 32], all{LEAST, 0.0f, 0.0f, 0};
+  unsigned long long least = 0;
+#pragma unroll
+  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
+    const int split = lane + 32 * i;
+    part[i] = Sums{LEAST, 0.0f, 0.0f, 0};
+    if (split < p.splits) {
+      const float4 s = *reinterpret_cast<const float4*>(p.sums + 4 * ((size_t)r * p.splits + split));
+      part[i] = Sums{s.x, s.y, s.z, __float_as_int(s.w)};
+      // no key below the last of a chunk's best is among the row's
+      if (p.top > 0) least = max(least, p.keys[((size_t)r * p.splits + split) * p.top + p.top - 1]);
+    }
+    all.m = fmaxf(all.m, part[i].m);
+  }
+  all.m = warp_max(all.m);
+  least = warp_largest(least);
+#pragma unroll
+  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
+    part[i].move(all.m);
+    all.z += part[i].z;
+    all.w += part[i].w;
+    all.before += part[i].before;
+  }
+  all.z = warp_sum(all.z);
+  all.w = warp_sum(all.w);
+  all.before = __reduce_add_sync(0xffffffffu, all.before);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.splits * p.top; i += THREADS) {
+    const unsigned long long key = p.keys[(size_t)r * p.splits * p.top + i];
+    if (key != 0 && key >= least) list[atomicAdd(&listed, 1)] = key;
+  }
+  __syncthreads();
+  if (p.top > 0) choose(list, listed, p.top, scratch);
+  answer(p, r, all, own, known, list);
+}
+
+// Logits of a chunk: as many as a block passes over in a few rounds, so that the last blocks of a launch do not run alone; single rounds where
+// all of them are on the device at a time.
+int chunk_of(int rows, int vocab) {
+  const int rounds = (vocab + ROUND - 1) / ROUND;
+  int mine = (long long)rows * rounds <= 2ll * tge_sm_count() ? 1 : 4;
+  if (mine * MOST_SPLITS < rounds) mine = (rounds + MOST_SPLITS - 1) / MOST_SPLITS;
+  return mine >= rounds ? vocab : mine * ROUND;
+}
+int splits_of(int rows, int vocab) {
+  const int chunk = chunk_of(rows, vocab);
+  return (vocab + chunk - 1) / chunk;
 }
 
 }  // namespace
 
+// float32 scratch numbers of tge_token_logprobs (16-byte aligned).
+TGE_API long long tge_token_logprobs_floats(int rows, int vocab, int top) {
+  if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+  const int splits = splits_of(rows, vocab);
+  return splits == 1 ? 0 : (long long)rows * splits * (4 + 2 * top);
+}
+
 TGE_API int tge_token_logprobs(const void* logits, int is_bf16, long long stride, const int* tokens, int rows, int vocab, int top,
-                               float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs, int* status,
-                               cudaStream_t stream) {
-  TGE_REQUIRE(rows >= 0 && vocab > 0 && stride >= vocab, "token_logprobs: bad sizes rows=%d vocab=%d stride=%lld", rows, vocab, stride);
+                               float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs, float* scratch,
+                               long long scratch_floats, int* status, cudaStream_t stream) {
+  TGE_REQUIRE(rows >= 0 && vocab > 0 && vocab < 0x7fff0000 && stride >= vocab, "token_logprobs: bad sizes rows=%d vocab=%d stride=%lld", rows, vocab, stride);
   TGE_REQUIRE(top >= 0 && top <= MOST_TOP && top <= vocab, "token_logprobs: %d alternatives of %d tokens, at most %d", top, vocab, MOST_TOP);
   if (rows == 0) return 0;
-  if (is_bf16)
-    tge_launch(token_logprobs_simple_kernel<__nv_bfloat16>, rows, THREADS, 0, stream, (const __nv_bfloat16*)logits, stride, tokens, vocab, top,
-               logprob, entropy, rank, top_ids, top_logprobs, status);
-  else
-    tge_launch(token_logprobs_simple_kernel<float>, rows, THREADS, 0, stream, (const float*)logits, stride, tokens, vocab, top, logprob,
-               entropy, rank, top_ids, top_logprobs, status);
-  return tge_launched("token_logprobs", 1);
+  LogprobParams p{logits, tokens, stride, rows, vocab, top, splits_of(rows, vocab), chunk_of(rows, vocab), logprob, entropy, top_logprobs,
+                  rank, top_ids, scratch, nullptr, status};
+  TGE_REQUIRE((long long)rows * p.splits < 0x7fffffffll, "token_logprobs: %d rows of %d logits", rows, vocab);
+  TGE_REQUIRE(scratch_floats >= tge_token_logprobs_floats(rows, vocab, top), "token_logprobs: %lld floats of scratch memory", scratch_floats);
+  p.keys = reinterpret_cast<unsigned long long*>(scratch + 4 * (size_t)rows * p.splits);
+  const int element = is_bf16 ? 2 : 4;
+  const bool vector = (uintptr_t)logits % 16 == 0 && stride * element % 16 == 0;
+  auto run = [&](auto type) {
+    using T = decltype(type);
+    if (vector) tge_launch(token_logprobs_kernel<T, true>, rows * p.splits, THREADS, 0, stream, p);
+    else tge_launch(token_logprobs_kernel<T, false>, rows * p.splits, THREADS, 0, stream, p);
+    if (p.splits == 1) return tge_launched("token_logprobs", 1);
+    tge_launch(token_logprobs_join_kernel<T>, rows, THREADS, 0, stream, p);
+    return tge_launched("token_logprobs", 2);
+  };
+  return is_bf16 ? run(__nv_bfloat16()) : run(float());
 }

@@ -217,7 +217,9 @@ def core() -> ctypes.CDLL:
                                                     _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ll, _c_int, _c_int,
                                                     _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_ptr])
         _declare(lib, "tge_token_logprobs", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                                             _c_ptr, _c_ptr, _c_ptr])
+                                             _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr])
+        lib.tge_token_logprobs_floats.argtypes = [_c_int] * 3
+        lib.tge_token_logprobs_floats.restype = _c_ll
         lib.tge_device_sm_count.restype = _c_int
         lib.tge_sample_cuts_padded.argtypes = [_c_int]
         lib.tge_sample_cuts_padded.restype = _c_ll
@@ -1638,9 +1640,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     top_ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=device)
     top_logprobs = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=device)
     lib = core()
+    need = lib.tge_token_logprobs_floats(rows, vocab, int(top))
+    scratch = torch.empty(need, dtype=torch.float32, device=device) if need else None
     _check(lib.tge_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride, tokens.data_ptr(), rows, vocab, int(top),
                                   logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(),
-                                  status_word().data_ptr(), _stream()), lib)
+                                  _ptr(scratch), need, status_word().data_ptr(), _stream()), lib)
     return logprob, entropy, rank, top_ids, top_logprobs
 
 
