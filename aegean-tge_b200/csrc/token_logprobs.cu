@@ -171,9 +171,10 @@ __device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[
 
 // One pass over a chunk of a row.  What bounds it is reading the logits: a thread holds its next sixteen on their way while it works on
 // these, keeps sums of its own, and looks at single logits only where its largest reaches the smallest of the best so far.  Those that do are listed
-// with the block's others; a list that grows beyond SORTED_AT_ONCE is cut to the best again.  After the first round the best are a
-// choice among the largest of 32 half warps' logits and whatever passes the n-th of those, so that of random rows some hundred
-// logits are ever listed, and of no row more than there is room for.
+// with the block's others; the list is cut to the best now and then.  After the first round the best are a
+// choice among the largest of 32 half warps' logits and whatever passes the n-th of those, then whatever passes the n-th of the chunk's
+// first 1, 2, 4, 8, ... rounds: of random rows some hundred logits are ever listed.  A row that lists more than there is room
+// for (rising logits) is looked through again.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const LogprobParams p) {
   constexpr int per = 16 / sizeof(T);
@@ -201,7 +202,38 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
   unsigned long long least = 0;                  // the smallest of the best so far (0: not as many yet)
   __syncthreads();
 
-  for (int first = begin; first < end; first += ROUND) {
+  auto index_of = [&](int first, int i) { return first + ((i / per) * THREADS + (int)threadIdx.x) * per + i % per; };
+  // Cuts the list to the best of the chunk up to `upto`.
+  auto settle = [&](int upto) {
+    __syncthreads();
+    const int count = listed;
+    if (count <= ROOM) {
+      least = max(least, choose(list, count, p.top, scratch));
+      if (threadIdx.x == 0) listed = min(count, p.top);
+      __syncthreads();
+      return;
+    }
+    // More than there is room for: all of the chunk up to here again, a load of every thread at a time.
+    __syncthreads();
+    if (threadIdx.x == 0) listed = 0;
+    least = 0;
+    __syncthreads();
+    for (int from = begin; from < upto; from += THREADS * per) {
+      for (int i = 0; i < per; ++i) {
+        const int index = from + (int)threadIdx.x * per + i;
+        const unsigned long long key = index < upto ? key_of(to_float<T>(x[index]), index) : 0ull;
+        if (key > least) list[atomicAdd(&listed, 1)] = key;
+      }
+      __syncthreads();
+      const int so_far = listed;
+      least = max(least, choose(list, so_far, p.top, scratch));
+      if (threadIdx.x == 0) listed = min(so_far, p.top);
+      __syncthreads();
+    }
+  };
+
+  float bar = __int_as_float(0x7fc00000);        // the logit of `least`; NaN where anything may enter
+  for (int first = begin, round = 1; first < end; first += ROUND, ++round) {
     if (first + ROUND < end) take<T, VECTOR>(x, first + ROUND, end, ahead);
     float largest = v[0];
 #pragma unroll
@@ -216,98 +248,63 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
     }
     mine.z += z;
     mine.w += w;
-    auto index_of = [&](int i) { return first + ((i / per) * THREADS + (int)threadIdx.x) * per + i % per; };
-    if (!token_is_nan) {
+    if (!token_is_nan && (token < first || token >= first + ROUND)) {
+      const float from = first < token ? own : above;
 #pragma unroll
-      for (int k = 0; k < MINE / per; ++k) {
-        const int at = index_of(per * k);
-        if (at <= token && token < at + per) {
+      for (int i = 0; i < MINE; ++i) mine.before += v[i] >= from ? 1 : 0;
+    } else {
 #pragma unroll
-          for (int i = 0; i < per; ++i) mine.before += v[per * k + i] >= (at + i < token ? own : above) ? 1 : 0;
-        } else {
-          const float from = at < token ? own : above;
-#pragma unroll
-          for (int i = 0; i < per; ++i) mine.before += v[per * k + i] >= from ? 1 : 0;
-        }
+      for (int i = 0; i < MINE; ++i) {
+        const int index = index_of(first, i);
+        const bool ahead_of = token_is_nan ? v[i] == v[i] || index < token : v[i] >= (index < token ? own : above);
+        mine.before += index < end && ahead_of ? 1 : 0;
       }
-    } else {                                     // it comes behind all that are numbers
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) mine.before += index_of(i) < end && (v[i] == v[i] || index_of(i) < token) ? 1 : 0;
     }
 
     if (p.top > 0) {
-      if (first == begin) {                      // the n-th of the half warps' largest keys: that many logits are no smaller
+      if (round == 1) {                          // the n-th of the half warps' largest keys: that many logits are no smaller
         unsigned long long key = 0;
 #pragma unroll
         for (int i = 0; i < MINE; ++i)
-          if (index_of(i) < end) key = max(key, key_of(v[i], index_of(i)));
+          if (index_of(first, i) < end) key = max(key, key_of(v[i], index_of(first, i)));
         key = warp_largest(key, 16);
         if ((lane & 15) == 0) scratch[threadIdx.x >> 4] = key;
         __syncthreads();
-        key = scratch[lane];
-        int in_front = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) in_front += __shfl_sync(0xffffffffu, key, i) > key ? 1 : 0;
-        const unsigned nth = __ballot_sync(0xffffffffu, key != 0 && in_front == p.top - 1);
-        // keys of at least the n-th: those above its predecessor
-        least = nth ? __shfl_sync(0xffffffffu, key, __ffs(nth) - 1) - 1 : 0ull;
+        if (threadIdx.x < 32) {
+          key = scratch[lane];
+          int in_front = 0;
+          for (int i = 0; i < 32; ++i) in_front += __shfl_sync(0xffffffffu, key, i) > key ? 1 : 0;
+          const unsigned nth = __ballot_sync(0xffffffffu, key != 0 && in_front == p.top - 1);
+          // keys of at least the n-th: those above its predecessor
+          if (lane == 0) scratch[32] = nth ? scratch[__ffs(nth) - 1] - 1 : 0ull;
+        }
+        __syncthreads();
+        least = scratch[32];
+        bar = logit_of(least);
       }
-      const float bar = logit_of(least);         // NaN where anything may enter
-      int entering = 0;
-      if (!(largest < bar)) {
+      if (__any_sync(0xffffffffu, !(largest < bar))) {
+        uint32_t which = 0;
 #pragma unroll
-        for (int i = 0; i < MINE; ++i)
-          if (!(v[i] < bar)) entering += index_of(i) < end && key_of(v[i], index_of(i)) > least ? 1 : 0;
-      }
-      int place = 0;
-      if (entering > 0) {
-        place = atomicAdd(&listed, entering);
-        int at = place;
+        for (int i = 0; i < MINE; ++i) which |= !(v[i] < bar) && index_of(first, i) < end && key_of(v[i], index_of(first, i)) > least ? 1u << i : 0u;
+        if (which != 0) {
+          int at = atomicAdd(&listed, __popc(which));
 #pragma unroll
-        for (int i = 0; i < MINE; ++i)
-          if (index_of(i) < end && key_of(v[i], index_of(i)) > least) {
-            if (at < ROOM) list[at] = key_of(v[i], index_of(i));
-            ++at;
-          }
-      }
-      const bool full = __syncthreads_or(place + entering > SORTED_AT_ONCE);
-      if (full || first == begin) {
-        const int count = listed;
-        if (count <= ROOM) {
-          least = max(least, choose(list, count, p.top, scratch));
-          if (threadIdx.x == 0) listed = min(count, p.top);
-          __syncthreads();
-        } else {
-          // more than there is room for: again, a load of every thread at a time.  What the list held before this round lies in
-          // front of it no longer (threads wrote in any order): the whole chunk up to here is looked through.
-          __syncthreads();
-          if (threadIdx.x == 0) listed = 0;
-          least = 0;
-          __syncthreads();
-          for (int from = begin; from <= first; from += ROUND)
-            for (int k = 0; k < MINE / per; ++k) {
-              const int at0 = from + (k * THREADS + (int)threadIdx.x) * per;
-              for (int i = 0; i < per; ++i) {
-                const int index = at0 + i;
-                const unsigned long long key = index < end ? key_of(to_float<T>(x[index]), index) : 0ull;
-                if (key > least) list[atomicAdd(&listed, 1)] = key;
-              }
-              __syncthreads();
-              const int so_far = listed;
-              least = max(least, choose(list, so_far, p.top, scratch));
-              if (threadIdx.x == 0) listed = min(so_far, p.top);
-              __syncthreads();
+          for (int i = 0; i < MINE; ++i)
+            if (which >> i & 1) {
+              if (at < ROOM) list[at] = key_of(v[i], index_of(first, i));
+              ++at;
             }
         }
+      }
+      if ((round & (round - 1)) == 0) {          // after rounds 1, 2, 4, 8, ...: the bar rises as the best get rarer
+        settle(min(first + ROUND, end));
+        bar = logit_of(least);
       }
     }
 #pragma unroll
     for (int i = 0; i < MINE; ++i) v[i] = ahead[i];
   }
-  if (p.top > 0) {
-    __syncthreads();
-    choose(list, listed, p.top, scratch);
-  }
+  if (p.top > 0) settle(end);
   const int found = p.top > 0 ? min(listed, p.top) : 0;
   mine = block_sums(mine, floats, counts);
   if (p.splits == 1) {
@@ -368,13 +365,22 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const Logp
   answer(p, r, all, own, known, list);
 }
 
-// Logits of a chunk: as many as a block passes over in a few rounds, so that the last blocks of a launch do not run alone; single rounds where
-// all of them are on the device at a time.
+// Logits of a chunk.  A block costs its rounds and about two more (the first choice, the joining), and as many run at a time as the device holds:
+// of all cuts the one that is done first, the fewest chunks among equals.
 int chunk_of(int rows, int vocab) {
   const int rounds = (vocab + ROUND - 1) / ROUND;
-  int mine = (long long)rows * rounds <= 2ll * tge_sm_count() ? 1 : 4;
-  if (mine * MOST_SPLITS < rounds) mine = (rounds + MOST_SPLITS - 1) / MOST_SPLITS;
-  return mine >= rounds ? vocab : mine * ROUND;
+  const long long at_once = 2ll * tge_sm_count();
+  long long best = 0;
+  int chunk = vocab;
+  for (int splits = 1; splits <= rounds && splits <= MOST_SPLITS; ++splits) {
+    const int mine = (rounds + splits - 1) / splits;
+    const long long cost = ((long long)rows * splits + at_once - 1) / at_once * (mine + 2);
+    if (splits == 1 || cost < best) {
+      best = cost;
+      chunk = splits == 1 ? vocab : mine * ROUND;
+    }
+  }
+  return chunk;
 }
 int splits_of(int rows, int vocab) {
   const int chunk = chunk_of(rows, vocab);
