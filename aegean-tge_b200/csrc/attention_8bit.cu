@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // that holds a whole unit writes its output; parts of units are left as (maximum, sum, unnormalised output) in scratch memory, at
 // most two per block, and a second kernel joins them in the order of the positions.
 // ---------------------------------------------------------------------------
-constexpr int DWARPS = 8;
+constexpr int DWARPS = 4;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float HELD = 64.0f;                   // probabilities are held times this
@@ -161,13 +161,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Codes of bytes `which` of two words as two float16.
+// Codes of bytes `which` of two words as two float16, plus 1,152.
 __device__ __forceinline__ uint32_t two_codes(uint32_t a, uint32_t b, uint32_t which) {
-  uint32_t r = __byte_perm(a, b, which), v;
+  const uint32_t r = __byte_perm(a, b, which);
+  uint32_t v;
   asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;\n" : "=r"(v) : "r"(r));       // (r & mask) ^ pattern: 1,024 + (byte ^ 128)
-  asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0xe480e480u));            // - 1,152
-  return r;
+  return v;
 }
+constexpr uint32_t LESS = 0xe480e480u;          // -1,152, twice
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -251,10 +252,10 @@ __device__ __forceinline__ void four(const T* q, bool vector, float (&x)[4]) {
 }
 
 // A row of queries as DIGITS whole numbers to the base 128 per number, four numbers to a word, in the order of the codes' words; the lane has
-// a quarter of the row, the four lanes of a row agree on its largest number.  Returns what the whole numbers are to be multiplied with
-// (NaN if a number is not finite).
+// a quarter of the row, the four lanes of a row agree on its largest number.  Words w of chunk j go to to[j][digit][lane], four side by
+// side.  Returns what the whole numbers are to be multiplied with (NaN if a number is not finite).
 template <typename T, int HD, int DIGITS>
-__device__ __forceinline__ float query_digits(const T* q, bool valid, bool vector, int t, uint32_t (&b)[HD / 64][4][DIGITS]) {
+__device__ __forceinline__ float query_digits(const T* q, bool valid, bool vector, int t, uint32_t (*to)[DIGITS][32][4]) {
   constexpr float TOP = DIGITS == 2 ? 16256.0f : 2080768.0f;          // 127 x 128^(DIGITS - 1)
   float most = 0.0f;
   bool fine = true;
@@ -291,7 +292,7 @@ __device__ __forceinline__ float query_digits(const T* q, bool valid, bool vecto
         here[i] = digit > 0 ? whole[i] - 128 * rest : whole[i];
         whole[i] = rest;
       }
-      b[j][w][digit] = __byte_perm(__byte_perm(here[0], here[1], 0x0040), __byte_perm(here[2], here[3], 0x0040), 0x5410);
+      to[j][digit][threadIdx.x & 31][w] = __byte_perm(__byte_perm(here[0], here[1], 0x0040), __byte_perm(here[2], here[3], 0x0040), 0x5410);
     }
   });
   // a number that is not finite in any quarter
@@ -307,13 +308,17 @@ __device__ __forceinline__ int number_of(int pair) {
   return VB * (g + 8 * j) + 2 * (i - j * (VB / 2));
 }
 
+// Blocks on an SM, by what registers allow.
+__host__ __device__ constexpr int decode_blocks_per_sm(int head_dim, int tiles) { return head_dim * tiles <= 64 ? 6 : head_dim * tiles <= 128 ? 5 : 3; }
+
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 ? 2 : 1) decode_8bit_kernel(const Decode8 p) {
+__global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) decode_8bit_kernel(const Decode8 p) {
   constexpr int DIGITS = sizeof(T) == 2 ? 2 : 3, PARTS = sizeof(T) == 2 ? 1 : 2;
   constexpr int HEADS = 8 * NT, MTILES = HD / 16, PITCH = HD + 4;
   using C = Codes<HD>;
   extern __shared__ float merge_o[];                              // [warps][HEADS][PITCH], a head's numbers in the order of the accumulators
-  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS];
+  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS], factors[HEADS];
+  __shared__ __align__(16) uint32_t queries[NT][C::KC][DIGITS][32][4];
   __shared__ int start_of[4];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = uniform_warp_index();
@@ -361,35 +366,41 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
     const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
     const int token = p.q_start[seq];
     const int* table = p.a.block_table + (size_t)seq * p.a.max_pages;
-    const int first = s.first + skip, last = first + length;
+    // the warps' shares of the run's slices, one behind the other
+    const int first = s.first + skip + length * warp / DWARPS, last = s.first + skip + length * (warp + 1) / DWARPS;
     bool bad = false;
-    auto page_of = [&](int slice) {
-      const int index = (slice << 4) >> p.page_shift;
-      return slice < last && index < p.a.max_pages ? table[index] : -1;
-    };
-    // the entry at which a slice starts; a page outside the pool reads page 0, unseen
-    auto row_of = [&](int slice, int page) {
-      const bool here = page >= 0 && page < p.a.num_pages;
-      return ((size_t)((here ? page : 0) * p.a.kv_heads + kvh) << p.page_shift) + ((slice << 4) & (p.a.page_size - 1));
+    auto page_at = [&](int index) { return index < p.a.max_pages ? table[index] : -1; };
+    // where a page's entries start; one outside the pool reads page 0, unseen
+    auto start_at = [&](int page) { return (size_t)((page >= 0 && page < p.a.num_pages ? page : 0) * p.a.kv_heads + kvh) << p.page_shift; };
+    // the slice to ask for next, its page and the one behind it
+    int asked = first, page = page_at((first << 4) >> p.page_shift), page_behind = page_at(((first << 4) >> p.page_shift) + 1);
+    size_t row = start_at(page) + ((first << 4) & (p.a.page_size - 1));
+    auto advance = [&] {
+      ++asked;
+      row += 16;
+      if (((asked << 4) & (p.a.page_size - 1)) == 0) {
+        page = page_behind;
+        page_behind = page_at(((asked << 4) >> p.page_shift) + 1);
+        row = start_at(page);
+      }
     };
     C c;
-    int slice = first + warp;
-    int page = page_of(slice), page_next = page_of(slice + DWARPS);
-    if (slice < last) {
-      const size_t row = row_of(slice, page);
+    if (first < last) {
       load_keys<HD>(p, c, row, g, t);
       load_values<HD>(p, c, row, g, t);
     }
-
-    uint32_t q[NT][HD / 64][4][DIGITS];
+    if (warp < NT) {
+      const bool valid = 8 * warp + g < heads_here;
+      const T* src = static_cast<const T*>(p.a.q) + (size_t)token * p.a.q_stride + (size_t)(head0 + (valid ? 8 * warp + g : 0)) * HD;
+      const float unit_of = query_digits<T, HD, DIGITS>(src, valid, p.q_by_eight != 0, t, queries[warp]) * (p.a.scale * (LOG2E / 127.0f));
+      if (t == 0) factors[8 * warp + g] = unit_of;
+    }
+    __syncthreads();
     float factor[NT][2];                                          // of the scores of heads 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const bool valid = 8 * nt + g < heads_here;
-      const T* src = static_cast<const T*>(p.a.q) + (size_t)token * p.a.q_stride + (size_t)(head0 + (valid ? 8 * nt + g : 0)) * HD;
-      const float unit_of = query_digits<T, HD, DIGITS>(src, valid, p.q_by_eight != 0, t, q[nt]) * (p.a.scale * (LOG2E / 127.0f));
-      factor[nt][0] = __shfl_sync(0xffffffffu, unit_of, 8 * t);
-      factor[nt][1] = __shfl_sync(0xffffffffu, unit_of, 8 * t + 4);
+      factor[nt][0] = factors[8 * nt + 2 * t];
+      factor[nt][1] = factors[8 * nt + 2 * t + 1];
     }
     float o[NT][MTILES][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -403,13 +414,10 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
     }
     float v_most = 1e-30f, v_over = HELD / 1e-30f;                // the largest scale of the values so far, and what scales are multiplied with
 
-    for (; slice < last; slice += DWARPS) {
-      const int next = slice + DWARPS;
-      const size_t row_next = row_of(next, page_next);
-      const bool here = page >= 0 && page < p.a.num_pages;
+    for (int slice = first; slice < last; ++slice) {
+      const bool here = page >= 0 && page < p.a.num_pages;         // `asked` is this slice still
       bad |= !here;
-      page = page_next;
-      page_next = page_of(next + DWARPS);
+      advance();
 
       float sc[NT][4];
 #pragma unroll
@@ -422,10 +430,11 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
 #pragma unroll
         for (int j = 0; j < C::KC; ++j)
 #pragma unroll
-          for (int w = 0; w < 4; w += 2)
-#pragma unroll
-            for (int digit = 0; digit < DIGITS; ++digit)
-              mma_s8(acc[digit], c.k[0][j][w], c.k[1][j][w], c.k[0][j][w + 1], c.k[1][j][w + 1], q[nt][j][w][digit], q[nt][j][w + 1][digit]);
+          for (int digit = 0; digit < DIGITS; ++digit) {
+            const uint4 q = *reinterpret_cast<const uint4*>(queries[nt][j][digit][lane]);
+            mma_s8(acc[digit], c.k[0][j][0], c.k[1][j][0], c.k[0][j][1], c.k[1][j][1], q.x, q.y);
+            mma_s8(acc[digit], c.k[0][j][2], c.k[1][j][2], c.k[0][j][3], c.k[1][j][3], q.z, q.w);
+          }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           // at most 256 x 127 x 127 in a digit's sum: two of them fit 32 bits, the third is added in float32
@@ -434,22 +443,35 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
           sc[nt][e] = sum;
         }
       }
-      const int k0 = slice * 16 + g;
-      const bool see0 = here && k0 >= s.lo && k0 < s.hi, see1 = here && k0 + 8 >= s.lo && k0 + 8 < s.hi;
       const float f0 = c.ks[0], f1 = c.ks[1];
-      // an unseen position's scales may be anything, NaN too
-      const float v0 = see0 ? c.vs[0] : 0.0f, v1 = see1 ? c.vs[1] : 0.0f;
-      if (next < last) load_keys<HD>(p, c, row_next, g, t);
+      float v0 = c.vs[0], v1 = c.vs[1];
+      if (slice + 1 < last) load_keys<HD>(p, c, row, g, t);
 
-      bool raise = fmaxf(v0, v1) > 2.0f * v_most;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sc[nt][e] = see0 ? sc[nt][e] * (f0 * factor[nt][e]) : -INFINITY;
-          sc[nt][2 + e] = see1 ? sc[nt][2 + e] * (f1 * factor[nt][e]) : -INFINITY;
-          raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + 8.0f;
+          sc[nt][e] *= f0 * factor[nt][e];
+          sc[nt][2 + e] *= f1 * factor[nt][e];
         }
+      if (!here || slice * 16 < s.lo || slice * 16 + 16 > s.hi) {    // some of the slice's positions are not seen
+        const int k0 = slice * 16 + g;
+        const bool see0 = here && k0 >= s.lo && k0 < s.hi, see1 = here && k0 + 8 >= s.lo && k0 + 8 < s.hi;
+        v0 = see0 ? v0 : 0.0f;                                       // their scales may be anything, NaN too
+        v1 = see1 ? v1 : 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sc[nt][e] = see0 ? sc[nt][e] : -INFINITY;
+            sc[nt][2 + e] = see1 ? sc[nt][2 + e] : -INFINITY;
+          }
+      }
+      bool raise = fmaxf(v0, v1) > 2.0f * v_most;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + 8.0f;
       if (__any_sync(0xffffffffu, raise)) {
         float v_now = fmaxf(fmaxf(v0, v1), v_most);
 #pragma unroll
@@ -512,9 +534,13 @@ __global__ void __launch_bounds__(DWARPS * 32, HD * NT * (sizeof(T) / 2) <= 128 
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int part = 0; part < PARTS; ++part) mma_f16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
+              for (int part = 0; part < PARTS; ++part) {
+                // 1,152 + c and, in the same breath, 1,152 less: no more than the slice's own sum is ever off by the rounding of that much
+                mma_f16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
+                mma_f16(o[nt][i], LESS, LESS, LESS, LESS, pr[nt][part][0], pr[nt][part][1]);
+              }
           }
-      if (next < last) load_values<HD>(p, c, row_next, g, t);
+      if (slice + 1 < last) load_values<HD>(p, c, row, g, t);
     }
     if (bad && lane == 0) atomicOr(p.a.status, TGE_STATUS_BAD_PAGE);
 
@@ -692,7 +718,7 @@ int launch_decode(Decode8 p, int blocks, cudaStream_t stream) {
 }
 
 // Blocks of a launch: all that are on the device at a time, so that all runs advance together.
-int decode_blocks(int head_dim, int tile_heads, bool is_bf16) { return tge_sm_count() * (head_dim * (tile_heads / 8) * (is_bf16 ? 1 : 2) <= 128 ? 2 : 1); }
+int decode_blocks(int head_dim, int tile_heads) { return tge_sm_count() * decode_blocks_per_sm(head_dim, tile_heads / 8); }
 
 }  // namespace
 
@@ -708,7 +734,7 @@ TGE_API long long tge_attention_8bit_decode_floats(int is_bf16, int num_seqs, in
   // places in the row of all slices are counted in 32 bits, units along a grid's second axis
   if (units > 65535 || (long long)max_pages * page_size > (1ll << 30) ||
       units * num_seqs * ((long long)max_pages * page_size / 16 + 1) > (1ll << 30)) return -1;
-  return 2ll * decode_blocks(head_dim, tile, is_bf16 != 0) * tile * (head_dim + 2);
+  return 2ll * decode_blocks(head_dim, tile) * tile * (head_dim + 2);
 }
 
 TGE_API int tge_attention_8bit_decode(const void* q, int is_bf16, long long q_stride, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -730,13 +756,13 @@ TGE_API int tge_attention_8bit_decode(const void* q, int is_bf16, long long q_st
   p.start_pos = start_pos;
   p.head_tiles = (group + tile - 1) / tile;
   p.units = kv_heads * p.head_tiles;
-  p.least = DWARPS;
+  p.least = 2 * DWARPS;
   const int element = is_bf16 ? 2 : 4;
   p.q_by_eight = (uintptr_t)q % 8 == 0 && q_stride * element % 8 == 0;
   p.page_shift = __builtin_ctz(page_size);
   p.block_shift = __builtin_ctz(block);
   p.parts = parts;
-  const int blocks = decode_blocks(head_dim, tile, is_bf16 != 0);
+  const int blocks = decode_blocks(head_dim, tile);
   auto run = [&](auto type) {
     using T = decltype(type);
     if (head_dim == 256) return launch_decode<T, 256, 1>(p, blocks, stream);

@@ -61,7 +61,11 @@ struct StoreParams {
   int* status;
 };
 
-// Number i of this lane (d = lane + 32 i) of a head's row at `src`, rotated for position `pos`.
+// One product rounded, the other inside the sum: spelled out, so that every kernel here rounds alike.
+__device__ __forceinline__ float turned_lo(float lo, float hi, float c, float s) { return __fmaf_rn(lo, c, -__fmul_rn(hi, s)); }
+__device__ __forceinline__ float turned_hi(float lo, float hi, float c, float s) { return __fmaf_rn(lo, s, __fmul_rn(hi, c)); }
+
+// Number d of a head's row at `src`, rotated for position `pos`.
 template <typename T>
 __device__ __forceinline__ float rotated(const StoreParams& p, const T* src, int d, int pos, bool rotate) {
   const float own = to_float<T>(src[d]);
@@ -69,7 +73,7 @@ __device__ __forceinline__ float rotated(const StoreParams& p, const T* src, int
   const int half = p.rotary >> 1, j = d < half ? d : d - half;
   const float other = to_float<T>(src[d < half ? d + half : d - half]);
   const float c = p.cos_table[(size_t)pos * half + j], s = p.sin_table[(size_t)pos * half + j];
-  return d < half ? own * c - other * s : other * s + own * c;
+  return d < half ? turned_lo(own, other, c, s) : turned_hi(other, own, c, s);
 }
 
 // One warp per (token, head): a query head is rotated into q_out; a key or value head is quantised by the warp of the block's first
@@ -143,6 +147,241 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 }
 
 // ---------------------------------------------------------------------------
+// The same by units of eight numbers, for head sizes 16, 32, ..., 256 that are rotated whole or not at all and rows on 16 bytes.  Bound by
+// the rows' bytes.  HEAD / 16 lanes (a group) have a head's row, eight numbers of its first half and the eight that they are rotated
+// with.  The first blocks have a token each: its groups take its query heads (and, with blocks of one position, its key and value heads) in
+// turn, three rows on their way at a time, the angles loaded once.  With larger blocks the others have a (block of positions, key or value
+// head) each: its groups take the block's rows in turn, once for the scale and, from cache, once for the codes.
+// ---------------------------------------------------------------------------
+constexpr int UNIT_THREADS = 128, UNIT_AHEAD = 3;
+
+struct Eight { float x[8]; };
+__device__ __forceinline__ Eight eight(const __nv_bfloat16* src) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(src);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  Eight e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e.x[2 * i] = __uint_as_float(w[i] << 16);
+    e.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  return e;
+}
+__device__ __forceinline__ Eight eight(const float* src) {
+  const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+  return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ void put_eight(__nv_bfloat16* dst, const Eight& e) {
+  uint4 raw;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(e.x[2 * i], e.x[2 * i + 1]);
+  *reinterpret_cast<uint4*>(dst) = raw;
+}
+__device__ __forceinline__ void put_eight(float* dst, const Eight& e) {
+  reinterpret_cast<float4*>(dst)[0] = make_float4(e.x[0], e.x[1], e.x[2], e.x[3]);
+  reinterpret_cast<float4*>(dst)[1] = make_float4(e.x[4], e.x[5], e.x[6], e.x[7]);
+}
+__device__ __forceinline__ void turn(Eight& lo, Eight& hi, const Eight& c, const Eight& s) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float l = lo.x[i], h = hi.x[i];
+    lo.x[i] = turned_lo(l, h, c.x[i], s.x[i]);
+    hi.x[i] = turned_hi(l, h, c.x[i], s.x[i]);
+  }
+}
+__device__ __forceinline__ float largest_of(const Eight& lo, const Eight& hi) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = larger(larger(most, magnitude(lo.x[i])), magnitude(hi.x[i]));
+  return most;
+}
+__device__ __forceinline__ void put_codes(int8_t* dst, const Coder& coder, const Eight& e) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(coder.code(e.x[4 * i]), coder.code(e.x[4 * i + 1]), 0x0040),
+                       __byte_perm(coder.code(e.x[4 * i + 2]), coder.code(e.x[4 * i + 3]), 0x0040), 0x5410);
+  *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+}
+
+template <typename T, int HEAD>
+__global__ void __launch_bounds__(UNIT_THREADS) store_8bit_units_kernel(const StoreParams p) {
+  constexpr int LANES = HEAD / 16, GROUPS = UNIT_THREADS / LANES, HALF = HEAD / 2;
+  __shared__ float scales[GROUPS];
+  __shared__ int found[2];
+  pdl_trigger();
+  const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
+  const bool rotate = p.rotary > 0;
+  const T* rows = static_cast<const T*>(p.qkv) + 8 * j;
+  auto angles = [&](int pos, Eight& c, Eight& s) {
+    if (rotate) {
+      c = eight(p.cos_table + (size_t)pos * HALF + 8 * j);
+      s = eight(p.sin_table + (size_t)pos * HALF + 8 * j);
+    }
+  };
+  auto all_lanes = [&](float most) {                              // over the lanes of a head
+#pragma unroll
+    for (int offset = LANES / 2; offset > 0; offset >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, offset));
+    return most;
+  };
+  if ((int)blockIdx.x < p.tokens) {
+    const int t = blockIdx.x, pos = p.positions[t], seq = p.seq_of_token[t];
+    if (pos < 0 || (rotate && pos >= p.table_rows) || seq < 0 || seq >= p.num_seqs) {
+      if (threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+      pdl_wait();
+      return;
+    }
+    Eight c, s;
+    angles(pos, c, s);
+    const int page_index = pos / p.page_size, slot = pos - page_index * p.page_size;
+    const int page = page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+    const bool here = page >= 0 && page < p.num_pages;
+    if (!here && p.block == 1 && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+    pdl_wait();
+    const T* row = rows + (size_t)t * p.row_stride;
+    const int heads = p.heads + (p.block == 1 ? 2 * p.kv_heads : 0);
+    for (int h0 = group; h0 < heads + group; h0 += UNIT_AHEAD * GROUPS) {       // the same number of rounds for every lane of a warp
+      Eight lo[UNIT_AHEAD], hi[UNIT_AHEAD];
+#pragma unroll
+      for (int i = 0; i < UNIT_AHEAD; ++i) {
+        const int h = min(h0 + i * GROUPS, heads - 1);
+        lo[i] = eight(row + (size_t)h * HEAD);
+        hi[i] = eight(row + (size_t)h * HEAD + HALF);
+      }
+#pragma unroll
+      for (int i = 0; i < UNIT_AHEAD; ++i) {
+        const int h = h0 + i * GROUPS;
+        const bool valid = h < heads, to_cache = h >= p.heads;
+        if (rotate && h < p.heads + p.kv_heads) turn(lo[i], hi[i], c, s);
+        if (valid && !to_cache) {
+          T* dst = static_cast<T*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * HEAD + 8 * j;
+          put_eight(dst, lo[i]);
+          put_eight(dst + HALF, hi[i]);
+        }
+        if (__any_sync(0xffffffffu, valid && to_cache)) {
+          const float scale = all_lanes(largest_of(lo[i], hi[i]));
+          if (valid && to_cache && here) {
+            const bool is_key = h < p.heads + p.kv_heads;
+            const size_t entry = ((size_t)page * p.kv_heads + (h - p.heads - (is_key ? 0 : p.kv_heads))) * p.page_size + slot;
+            const Coder coder(scale);
+            int8_t* codes = (is_key ? p.k_pages : p.v_pages) + entry * HEAD + 8 * j;
+            put_codes(codes, coder, lo[i]);
+            put_codes(codes + HALF, coder, hi[i]);
+            if (j == 0) (is_key ? p.k_scale : p.v_scale)[entry] = scale;
+          }
+        }
+      }
+    }
+    return;
+  }
+  // a block of positions of one request: the requests' blocks one after the other
+  const int shift = __ffs(p.block) - 1, number = blockIdx.x - p.tokens;
+  const int item = number / (2 * p.kv_heads), head = number - item * 2 * p.kv_heads;
+  if (threadIdx.x < 32) {
+    int before = 0, seq_found = -1, index = 0;
+    for (int base = 0; base < p.num_seqs && seq_found < 0; base += 32) {
+      const int seq = base + threadIdx.x;
+      int n = 0, first = 0;
+      if (seq < p.num_seqs) {
+        const int start = p.q_start[seq], count = p.q_start[seq + 1] - start;
+        if (count > 0 && start >= 0 && start < p.tokens) {
+          const int pos = p.positions[start];
+          first = pos >> shift;
+          n = pos >= 0 ? ((pos + count - 1) >> shift) - first + 1 : 0;
+        }
+      }
+      int upto = n;
+#pragma unroll
+      for (int offset = 1; offset < 32; offset <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, offset);
+        if ((int)threadIdx.x >= offset) upto += v;
+      }
+      const unsigned mine = __ballot_sync(0xffffffffu, item < before + upto);
+      if (mine != 0) {
+        const int who = __ffs(mine) - 1;
+        seq_found = base + who;
+        index = item - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, n, who)) + __shfl_sync(0xffffffffu, first, who);
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (threadIdx.x == 0) { found[0] = seq_found; found[1] = index; }
+  }
+  __syncthreads();
+  const int seq = found[0];
+  pdl_wait();
+  if (seq < 0) return;
+  const int start = p.q_start[seq], count = p.q_start[seq + 1] - start, first_pos = p.positions[start];
+  const int lo_pos = found[1] << shift, from = max(lo_pos, first_pos), to = min(lo_pos + p.block, first_pos + count);
+  const bool is_key = head < p.kv_heads, rotated_here = rotate && is_key;
+  const int page_index = lo_pos / p.page_size;
+  const int page = page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+  if (page < 0 || page >= p.num_pages || start + (to - first_pos) > p.tokens) {
+    if (threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+    return;
+  }
+  if (rotated_here && to > p.table_rows) {
+    if (threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    return;
+  }
+  const size_t entry = ((size_t)page * p.kv_heads + (is_key ? head : head - p.kv_heads)) * p.page_size + (lo_pos - page_index * p.page_size);
+  int8_t* codes = (is_key ? p.k_pages : p.v_pages) + entry * HEAD + 8 * j;     // of the block's first position
+  float* scale_at = (is_key ? p.k_scale : p.v_scale) + (entry >> shift);
+  const float before = from > lo_pos ? *scale_at : 0.0f;
+  const T* row0 = rows + (size_t)(p.heads + head) * HEAD + (size_t)(start - first_pos) * p.row_stride;    // position pos at pos rows from here
+  auto row_of = [&](int pos, Eight& lo, Eight& hi) {
+    const T* row = row0 + (long long)pos * p.row_stride;
+    lo = eight(row);
+    hi = eight(row + HALF);
+    if (rotated_here) {
+      Eight c, s;
+      angles(pos, c, s);
+      turn(lo, hi, c, s);
+    }
+  };
+  float most = 0.0f;
+  for (int pos = from + group; pos < to; pos += GROUPS) {
+    Eight lo, hi;
+    row_of(pos, lo, hi);
+    most = larger(most, largest_of(lo, hi));
+  }
+  most = all_lanes(most);
+  if (j == 0) scales[group] = most;
+  __syncthreads();
+  most = before;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) most = larger(most, scales[i]);
+  const Coder coder(most);
+  if (from > lo_pos && !(before >= most))                          // the scale grew: what the block held is rounded again
+    for (int i = group; i < from - lo_pos; i += GROUPS)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        int8_t* at = codes + (size_t)i * HEAD + half * HALF;
+        const uint2 raw = *reinterpret_cast<const uint2*>(at);
+        uint32_t w[2] = {raw.x, raw.y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          int again[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float stands = (float)(int8_t)(w[k] >> (8 * b)) * (before * coder.shrink);
+            again[b] = coder.any ? __float2int_rn(__fdiv_rn(stands, coder.over)) : 0;
+          }
+          w[k] = __byte_perm(__byte_perm(again[0], again[1], 0x0040), __byte_perm(again[2], again[3], 0x0040), 0x5410);
+        }
+        *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+      }
+  for (int pos = from + group; pos < to; pos += GROUPS) {
+    Eight lo, hi;
+    row_of(pos, lo, hi);
+    put_codes(codes + (size_t)(pos - lo_pos) * HEAD, coder, lo);
+    put_codes(codes + (size_t)(pos - lo_pos) * HEAD + HALF, coder, hi);
+  }
+  __syncthreads();                                                 // every thread has read the scale
+  if (threadIdx.x == 0) *scale_at = most;
+}
+
+// ---------------------------------------------------------------------------
 // Entries read back: the positions that a step's queries may see, request after request, in runs of 64 positions
 // [runs, kv_heads, 64, head_dim] (zeros behind a request's last), a block table over those runs and (starts, if wanted) the requests'
 // first tokens counted from the first one's.
@@ -168,7 +407,7 @@ __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
   return s;
 }
 
-template <typename T>
+template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ int found[3];
   pdl_trigger();
@@ -223,6 +462,52 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   }
   const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
   if (kvh == 0 && threadIdx.x == 0 && tile < p.width) p.table[(size_t)(seq - p.first_seq) * p.width + tile] = run;
+  if constexpr (UNITS) {
+    // sixteen codes of a position to a thread and turn, all loads of a turn of keys and values on their way together
+    const int units = p.head_dim >> 4, shift = __ffs(p.block) - 1, blocks = p.page_size >> shift;
+    constexpr int AHEAD = 2;
+    for (int u0 = threadIdx.x; u0 < 64 * units; u0 += AHEAD * blockDim.x) {
+      uint4 raw[AHEAD][2];
+      float scale[AHEAD][2];
+      int at[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int u = u0 + i * blockDim.x, j = u / units, part = u - j * units, pos = tile * 64 + j;
+        at[i] = u < 64 * units ? j * p.head_dim + 16 * part : -1;
+        const int page_index = pos / p.page_size, slot = pos - page_index * p.page_size;
+        const bool held_here = at[i] >= 0 && pos < held;
+        const int page = held_here && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+        const bool here = page >= 0 && page < p.num_pages;
+        if (held_here && !here) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+        raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+        scale[i][0] = scale[i][1] = 0.0f;
+        if (here) {
+          const size_t head = (size_t)page * p.kv_heads + kvh;
+          raw[i][0] = *reinterpret_cast<const uint4*>(p.k_pages + (head * p.page_size + slot) * p.head_dim + 16 * part);
+          raw[i][1] = *reinterpret_cast<const uint4*>(p.v_pages + (head * p.page_size + slot) * p.head_dim + 16 * part);
+          scale[i][0] = p.k_scale[head * blocks + (slot >> shift)];
+          scale[i][1] = p.v_scale[head * blocks + (slot >> shift)];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (at[i] >= 0) {
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const float s = __fdiv_rn(scale[i][kv], 127.0f);
+            const uint32_t w[4] = {raw[i][kv].x, raw[i][kv].y, raw[i][kv].z, raw[i][kv].w};
+            Eight e[2];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)       // 2^23 + (byte ^ 128), less 2^23 + 128: the code, exactly
+              e[k >> 3].x[k & 7] = (__uint_as_float(__byte_perm(w[k >> 2] ^ 0x80808080u, 0x4b000000u, 0x7440 + (k & 3))) - 8388736.0f) * s;
+            T* dst = (kv ? v_dst : k_dst) + at[i];
+            put_eight(dst, e[0]);
+            put_eight(dst + 8, e[1]);
+          }
+        }
+    }
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int j = warp; j < 64; j += 8) {
     const int pos = tile * 64 + j;
@@ -263,6 +548,26 @@ TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, v
   const StoreParams p{qkv, q_out, row_stride, q_stride, cos_table, sin_table, table_rows, positions, seq_of_token, q_start, block_table,
                       max_pages, (int8_t*)k_pages, (int8_t*)v_pages, k_scale, v_scale, num_pages, page_size, block, tokens, num_seqs,
                       heads, kv_heads, head_dim, rotary, status};
+  const size_t bytes = is_bf16 ? 16 : 32;                          // of eight numbers
+  const bool power = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0;
+  const long long blocks = tokens + (block > 1 ? ((long long)tokens / block + 2ll * num_seqs) * 2 * kv_heads : 0);
+  if (power && (rotary == 0 || rotary == head_dim) && blocks < 0x7fffffffll && row_stride * bytes / 8 % 16 == 0 && q_stride * bytes / 8 % 16 == 0 &&
+      ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0) {
+    auto run = [&](auto type) {
+      using T = decltype(type);
+      auto launch = [&](void (*kernel)(StoreParams)) { tge_launch(kernel, dim3((unsigned)blocks), UNIT_THREADS, 0, stream, p); };
+      switch (head_dim) {
+        case 16: launch(store_8bit_units_kernel<T, 16>); break;
+        case 32: launch(store_8bit_units_kernel<T, 32>); break;
+        case 64: launch(store_8bit_units_kernel<T, 64>); break;
+        case 128: launch(store_8bit_units_kernel<T, 128>); break;
+        default: launch(store_8bit_units_kernel<T, 256>); break;
+      }
+    };
+    if (is_bf16) run(__nv_bfloat16());
+    else run(float());
+    return tge_launched("store_8bit", 1);
+  }
   const dim3 grid(tokens, (heads + 2 * kv_heads + WARPS - 1) / WARPS);
   if (is_bf16)
     tge_launch(store_8bit_kernel<__nv_bfloat16>, grid, WARPS * 32, 0, stream, p);
@@ -282,9 +587,10 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
                      page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, starts, runs, width, status};
   const dim3 grid(runs + 1, kv_heads);
+  const bool units = head_dim % 16 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (is_bf16)
-    tge_launch(read_8bit_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);
+    tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
-    tge_launch(read_8bit_kernel<float>, grid, 256, 0, stream, p);
+    tge_launch(units ? read_8bit_kernel<float, true> : read_8bit_kernel<float, false>, grid, 256, 0, stream, p);
   return tge_launched("read_8bit", 1);
 }
