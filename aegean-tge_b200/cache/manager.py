@@ -82,6 +82,7 @@ class PageGroup:
     # differ from layer to layer (other head counts and sizes).  Layers whose entries are equal are stacked in one
     # tensor per entry, a *variant*: (entries, its layers in order).
     variants: List[Tuple[Tuple, List[int]]] = field(default_factory=list)
+    variant_specs: List[PagedCacheSpec] = field(default_factory=list)              # per variant: what its entries are held in
     variant_storage: List[Dict[str, torch.Tensor]] = field(default_factory=list)   # per variant: name -> [layers, pages, ...]
 
     @property
@@ -90,14 +91,8 @@ class PageGroup:
         return self.variant_storage[0] if self.variant_storage else {}
 
     def bytes_per_page(self, element_size: int) -> int:
-        per_token = 0
-        for entries, layers in self.variants:
-            for _, shape in entries:
-                count = 1
-                for d in shape:
-                    count *= d
-                per_token += count * len(layers)
-        return per_token * self.page_size * element_size
+        return round(sum(spec.bytes_per_token(element_size) * len(layers) * self.page_size
+                         for spec, (_entries, layers) in zip(self.variant_specs, self.variants)))
 
     def first_needed_page(self, computed_tokens: int) -> int:
         """Index of the first logical page a query at position >= computed_tokens can still read."""
@@ -203,13 +198,14 @@ class CacheManager:
         group.layers.append(layer)
         self.layer_group[layer] = index
         for number, (entries, layers) in enumerate(group.variants):
-            if entries == cache.entries:
+            if entries == cache.entries and group.variant_specs[number].formats == cache.formats:
                 self.layer_variant[layer], self.layer_row[layer] = number, len(layers)
                 layers.append(layer)
                 break
         else:
             self.layer_variant[layer], self.layer_row[layer] = len(group.variants), 0
             group.variants.append((cache.entries, [layer]))
+            group.variant_specs.append(cache)
 
     def set_pool_sizes(self, pages_per_group: Sequence[int]) -> None:
         if len(pages_per_group) != len(self.groups):
@@ -254,11 +250,14 @@ class CacheManager:
         """
         for group in self.groups:
             group.variant_storage = []
-            for entries, layers in group.variants:
+            for spec, (entries, layers) in zip(group.variant_specs, group.variants):
                 tensors = {}
                 for name, shape in entries:
-                    full = (len(layers), group.pool.capacity + 1, *shape[:-1], self.page_size, shape[-1])
-                    tensors[name] = torch.zeros(full, dtype=dtype, device=device)
+                    kind, positions = spec.format_of(name, dtype)
+                    if self.page_size % positions:
+                        raise ValueError(f"cache manager: entries of {positions} positions in pages of {self.page_size}")
+                    full = (len(layers), group.pool.capacity + 1, *shape[:-1], self.page_size // positions, shape[-1])
+                    tensors[name] = torch.zeros(full, dtype=kind, device=device)
                 group.variant_storage.append(tensors)
         self.state_storage = {}
         for layer, spec in self.state_specs.items():

@@ -7,6 +7,7 @@
     tge bench prefill|decode --model DIR [--prompt-len N] [--batch B] [--n N] [--repeat R]
     tge bench mixed --model DIR [--batch B] [--prompt-len N] [--portion P]      (B single tokens beside a prompt portion)
     tge fidelity --model DIR [--context N] [--tokens N] [--corpus FILE]
+    tge score --model DIR --tokens "a b c" | --corpus FILE | --prompt-len N [--top N] [--cache-dtype int8 [--compare]]
     tge bench continuous --model DIR [--requests N] [--tokens N] [--sequences N] [--prompt-tokens N] [--prompt-max N]
     tge make-random --config FILE --out DIR [--seed S] [--dtype float32|bfloat16]
     tge replay --model DIR --dtype D --out DIR --max-tokens N          (same as bin/trace_run)
@@ -55,6 +56,12 @@ def _model_args(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--max-batch-tokens", type=int, default=2048, help="token budget of one step")
     parser.add_argument("--chunk", type=int, help="largest prompt portion in one step (default: the budget)")
     parser.add_argument("--max-requests", type=int, default=64)
+    _cache_args(parser)
+
+
+def _cache_args(parser: argparse.ArgumentParser) -> None:
+    parser.add_argument("--cache-dtype", choices=["int8"], help="hold keys and values in 8 bits (default: in --dtype)")
+    parser.add_argument("--cache-block", type=int, default=1, help="positions that share a scale of an 8-bit cache (default 1)")
 
 
 def _sampling_args(parser: argparse.ArgumentParser) -> None:
@@ -78,6 +85,7 @@ def build_parser() -> argparse.ArgumentParser:
     plan.add_argument("--sessions", type=int, default=1)
     plan.add_argument("--bandwidth", type=float, help="GB/s (default: the measured or nominal HBM figure)")
     plan.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    _cache_args(plan)
     generate = commands.add_parser("generate", help="generate tokens and report token rates")
     _model_args(generate)
     _sampling_args(generate)
@@ -107,6 +115,13 @@ def build_parser() -> argparse.ArgumentParser:
     _model_args(fidelity)
     fidelity.add_argument("--corpus", help="file of token ids separated by white space (default: seeded random ids)")
     fidelity.add_argument("--tokens", type=int, default=256, help="positions to compare (default 256)")
+    score = commands.add_parser("score", help="log probabilities of given tokens, entropies, ranks, best alternatives")
+    _model_args(score)
+    score.add_argument("--tokens", help='token ids, "a b c": every one but the first is scored')
+    score.add_argument("--corpus", help="file of token ids separated by white space")
+    score.add_argument("--prompt-len", type=int, help="random ids, so many, instead of --tokens or --corpus")
+    score.add_argument("--top", type=int, default=0, help="also the so many best tokens at every place (at most 32)")
+    score.add_argument("--compare", action="store_true", help="with --cache-dtype: also score with the cache in --dtype, and say how far the two are apart")
     make = commands.add_parser("make-random", help="write a model folder with seeded random weights")
     make.add_argument("--config", required=True, help="a config.json")
     make.add_argument("--out", required=True)
@@ -132,7 +147,7 @@ def _engine_from(args):
             random_config = json.load(handle)
     return Engine(args.model, random_config=random_config, seed=args.weights_seed, dtype=args.dtype,
                   context=args.context, num_pages=args.num_pages, max_batch_tokens=args.max_batch_tokens,
-                  chunk=args.chunk, max_requests=args.max_requests,
+                  chunk=args.chunk, max_requests=args.max_requests, cache_dtype=args.cache_dtype, cache_block=args.cache_block,
                   **({} if args.page_size is None else {"page_size": args.page_size}))
 
 
@@ -175,7 +190,8 @@ def command_plan(args) -> int:
     arch = architecture_of(raw)
     spec = arch.build_spec(arch.parse_config(raw))
     env = BuildEnv(dtype=parse_dtype(args.dtype), device=torch.device("cpu"), hidden_size=spec.hidden_size,
-                   max_positions=min(spec.max_positions, args.context), page_size=PAGE_SIZE, ops=None)
+                   max_positions=min(spec.max_positions, args.context), page_size=PAGE_SIZE, ops=None,
+                   cache_block=None if args.cache_dtype is None else args.cache_block)
     model = DecoderModel(spec, env)
     weights = model.weight_bytes()
     decode_bytes = model.step_param_bytes()                 # everything but the embedding rows (plan.cpp:42-46)
@@ -280,8 +296,10 @@ def command_fidelity(args) -> int:
     logits = {}
     tokens = None
     load_seconds = 0.0
+    candidate_cache = args.cache_dtype
     for dtype in ("float32", "bfloat16"):
         args.dtype = dtype
+        args.cache_dtype = candidate_cache if dtype == "bfloat16" else None      # the oracle's cache is never of 8 bits
         args.max_requests = 1
         t0 = time.time()
         engine = _engine_from(args)
@@ -315,14 +333,62 @@ def command_fidelity(args) -> int:
     kl = (log_p.exp() * (log_p - log_q)).sum(-1)
     agree = int((reference.argmax(-1) == candidate.argmax(-1)).sum())
     positions = reference.shape[0]
-    print("fidelity : float32 path vs bfloat16 kernels (prompt of %d tokens, then %d single tokens)"
-          % (max(len(tokens) // 2, 1), positions - max(len(tokens) // 2, 1)))
+    print("fidelity : float32 path vs bfloat16 kernels%s (prompt of %d tokens, then %d single tokens)"
+          % (f" over a cache of {candidate_cache}" if candidate_cache else "", max(len(tokens) // 2, 1), positions - max(len(tokens) // 2, 1)))
     print(f"load     : {load_seconds * 1e3:.1f} ms")
     print(f"corpus   : {positions} positions")
     print(f"KL       : mean {float(kl.mean()):.3e}, worst {float(kl.max()):.3e} nats")
     print(f"logits   : max |diff| {float((reference - candidate).abs().max()):.3e} (largest |logit| {float(reference.abs().max()):.3e})")
     print(f"top-1    : {agree}/{positions} agree")
     print(f"time     : {time.time() - started:.2f} s")
+    return 0
+
+
+def command_score(args) -> int:
+    """What the model thinks of given tokens: one line per token (id, log probability, entropy, rank, best alternatives) and the mean.  With
+    ``--cache-dtype int8 --compare`` also how far that cache moves the answers from those with the cache in the run's dtype."""
+    import gc
+    import math
+    import random
+    import torch
+    if sum(option is not None for option in (args.tokens, args.corpus, args.prompt_len)) != 1:
+        raise UsageError("score: give one of --tokens, --corpus and --prompt-len")
+    if args.compare and not args.cache_dtype:
+        raise UsageError("score: --compare is for --cache-dtype int8")
+    if not 0 <= args.top <= 32:
+        raise UsageError("score: --top is at most 32")
+    args.max_requests = 1
+    started = time.time()
+    engine = _engine_from(args)
+    print(f"load     : {(time.time() - started) * 1e3:.1f} ms")
+    if args.tokens is not None:
+        tokens = _parse_ids(args.tokens)
+    elif args.corpus is not None:
+        with open(args.corpus, "r", encoding="utf-8") as handle:
+            tokens = _parse_ids(handle.read())[:engine.max_model_len + 1]
+    else:
+        rnd = random.Random(0)
+        tokens = [rnd.randrange(engine.spec.vocab_size) for _ in range(args.prompt_len)]
+    if len(tokens) < 2 or any(not 0 <= t < engine.spec.vocab_size for t in tokens) or len(tokens) - 1 > engine.max_model_len:
+        raise UsageError(f"score: two tokens or more, within the vocabulary of {engine.spec.vocab_size} and the {engine.max_model_len} token context")
+    started = time.time()
+    scores = engine.score(tokens, top=min(args.top, engine.spec.vocab_size))
+    took = time.time() - started
+    for i, token in enumerate(tokens[1:]):
+        best = " ".join(f"{id}:{lp:.4f}" for id, lp in zip(scores.top_ids[i].tolist(), scores.top_logprobs[i].tolist()))
+        print(f"{token:>9}: {float(scores.logprob[i]):9.4f}  entropy {float(scores.entropy[i]):7.4f}  rank {int(scores.rank[i])}" + (f"  best {best}" if best else ""))
+    mean = float(scores.logprob.double().mean())
+    print(f"score    : {len(tokens) - 1} tokens, mean log probability {mean:.5f}, perplexity {math.exp(min(-mean, 700.0)):.4f}, "
+          f"mean entropy {float(scores.entropy.double().mean()):.5f} ({took * 1e3:.1f} ms)")
+    if args.compare:
+        del engine
+        gc.collect()
+        torch.cuda.empty_cache()
+        args.cache_dtype = None
+        other = _engine_from(args).score(tokens)
+        apart = (scores.logprob.double() - other.logprob.double()).abs()
+        print(f"compare  : cache in {args.dtype}: mean log probability {float(other.logprob.double().mean()):.5f}; |difference| mean "
+              f"{float(apart.mean()):.3e}, worst {float(apart.max()):.3e}; equal ranks {int((scores.rank == other.rank).sum())}/{len(tokens) - 1}")
     return 0
 
 
@@ -450,6 +516,8 @@ def main(argv: Optional[List[str]] = None) -> int:
             return command_bench(args)
         if args.command == "fidelity":
             return command_fidelity(args)
+        if args.command == "score":
+            return command_score(args)
         if args.command == "make-random":
             return command_make_random(args)
         if args.command == "replay":

@@ -3,6 +3,8 @@
     engine = Engine("path/to/model", dtype="bfloat16")
     ids = engine.generate([5, 17, 3], n=32)                      # greedy
     ids = engine.generate([[1, 2], [3]], n=8, sampling=SamplingParams(temperature=0.8, seed=7))
+    engine = Engine("path/to/model", cache_dtype="int8")          # keys and values in 8 bits
+    scores = engine.score([5, 17, 3, 9], top=5)                   # log probabilities of 17, 3, 9, with the five best beside each
 
 Options carry the reference's names and meanings where it has them
 (``generate --model --tokens --n --temp --top-k --top-p --min-p
@@ -20,7 +22,7 @@ from __future__ import annotations
 
 import os
 import time
-from typing import Any, Dict, Hashable, List, Optional, Sequence, Union
+from typing import Any, Dict, Hashable, List, NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -47,12 +49,23 @@ DEFAULT_CONTEXT = 4096      # the reference's default KV length (src/models/qwen
 PAGE_SIZE = 64
 
 
+class Scores(NamedTuple):
+    """What the model thinks of a sequence's tokens, from the second on; host tensors, a row per token."""
+
+    logprob: torch.Tensor         # float32 [n - 1], nats
+    entropy: torch.Tensor         # float32 [n - 1], of the distribution that the token was one draw of
+    rank: torch.Tensor            # int32 [n - 1], how many tokens are likelier (the lower id first among equals)
+    top_ids: torch.Tensor         # int32 [n - 1, top]
+    top_logprobs: torch.Tensor    # float32 [n - 1, top]
+
+
 class Engine:
     def __init__(self, model_dir: Optional[str] = None, *, dtype: str = "bfloat16", context: Optional[int] = None,
                  max_tokens: Optional[int] = None, num_pages: Optional[int] = None, max_batch_tokens: int = 2048,
                  max_requests: int = 64, chunk: Optional[int] = None, device: str = "cuda:0",
                  memory_fraction: float = 0.9, random_config: Optional[Dict[str, Any]] = None, seed: int = 0,
-                 page_size: int = PAGE_SIZE, run_ahead: bool = True, use_graphs: bool = True):
+                 page_size: int = PAGE_SIZE, run_ahead: bool = True, use_graphs: bool = True, cache_dtype: Optional[str] = None,
+                 cache_block: int = 1):
         """``model_dir``: folder with config.json and model.safetensors.  Alternatively
         ``random_config`` (a config.json as a dict) and ``seed``: random weights drawn on the device.
 
@@ -60,6 +73,9 @@ class Engine:
         tokens in total; else ``memory_fraction`` of the memory left after the weights.
         ``run_ahead`` / ``use_graphs``: switches for the step queued ahead and for CUDA graph replay of
         single-token steps (both on; off for A/B comparisons).
+        ``cache_dtype``: None keeps keys and values in ``dtype``; "int8" as 8-bit codes with a float32 scale per head and ``cache_block``
+        positions (a power of two that divides the page).  With blocks of one, the default, what a position's entry is does not
+        depend on the steps that brought it; larger blocks save up to 4 bytes a position and head.
         """
         if not torch.cuda.is_available():
             raise RuntimeError("this engine runs on a CUDA device only; none is available")
@@ -67,6 +83,11 @@ class Engine:
             raise ValueError("give either model_dir or random_config")
         if page_size <= 0 or 64 % page_size != 0:
             raise ValueError(f"page_size {page_size} must divide 64, the attention kernels' tile of key positions")
+        if cache_dtype not in (None, "int8"):
+            raise ValueError(f"cache_dtype {cache_dtype!r} is neither None (the run's dtype) nor 'int8'")
+        if cache_dtype is not None and (cache_block <= 0 or cache_block & (cache_block - 1) or page_size % cache_block):
+            raise ValueError(f"cache_block {cache_block} must be a power of two that divides the page of {page_size}")
+        self.cache_dtype = cache_dtype
         self.device = torch.device(device)
         torch.cuda.set_device(self.device)
         self.dtype = parse_dtype(dtype)
@@ -81,7 +102,8 @@ class Engine:
         self.max_model_len = min(self.spec.max_positions, limit)
         started = time.time()
         env = BuildEnv(dtype=self.dtype, device=self.device, hidden_size=self.spec.hidden_size,
-                       max_positions=self.max_model_len, page_size=page_size, ops=_ops)
+                       max_positions=self.max_model_len, page_size=page_size, ops=_ops,
+                       cache_block=None if cache_dtype is None else int(cache_block))
         _ops.core()     # builds and loads the kernels now, or fails loudly
         self.model = DecoderModel(self.spec, env)
         if model_dir is not None:
@@ -248,6 +270,36 @@ class Engine:
             self.scheduler.finished.pop(i, None)
         return outputs[0] if single else outputs
 
+    def score(self, tokens: Sequence[int], top: int = 0) -> Scores:
+        """Log probabilities of ``tokens[1:]``, each behind the tokens before it, with entropies, ranks and the ``top`` (at most 32) best.
+
+        The tokens run as portions of the step's budget through the engine's own cache, which needs room for them beside the requests
+        that are live; nothing of them stays.
+        """
+        tokens = [int(t) for t in tokens]
+        if len(tokens) < 2:
+            raise ValueError("score: at least two tokens")
+        if len(tokens) - 1 > self.max_model_len:
+            raise ValueError(f"score: {len(tokens)} tokens exceed the {self.max_model_len} token context")
+        if not 0 <= top <= min(32, self.spec.vocab_size):
+            raise ValueError(f"score: {top} alternatives, at most {min(32, self.spec.vocab_size)}")
+        for token in tokens:
+            if not 0 <= token < self.spec.vocab_size:
+                raise ValueError(f"token {token} is outside the vocabulary")
+        name, parts, budget = object(), [], self.scheduler.max_batch_tokens
+        try:
+            for first in range(0, len(tokens) - 1, budget):
+                portion = tokens[first:min(first + budget, len(tokens) - 1)]
+                logits = self.runner.step([Portion(name, portion, list(range(len(portion))))])
+                given = torch.tensor(tokens[first + 1:first + 1 + len(portion)], dtype=torch.int32, device=self.device)
+                parts.append(_ops.token_logprobs(logits, given, top=top))
+        finally:
+            if self.cache.is_live(name):
+                self.runner.finish(name)
+        scores = Scores(*(torch.cat(column).cpu() for column in zip(*parts)))
+        _ops.check_status()
+        return scores
+
     # -- facts ----------------------------------------------------------------
     def stats(self) -> Dict[str, Any]:
         out = dict(self.scheduler.counters)
@@ -269,6 +321,7 @@ class Engine:
             "architecture": self.spec.architecture, "dtype": str(self.dtype).replace("torch.", ""),
             "layers": len(self.spec.layers), "hidden_size": self.spec.hidden_size, "vocab_size": self.spec.vocab_size,
             "max_model_len": self.max_model_len, "page_size": self.cache.page_size,
+            "cache_dtype": self.cache_dtype or str(self.dtype).replace("torch.", ""),
             "pages_per_group": [g.pool.capacity for g in self.cache.groups],
             "param_bytes_per_step": self.model.step_param_bytes(),
             "cache_bytes_per_token": self.model.cache_bytes_per_token(),

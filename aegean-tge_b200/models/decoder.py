@@ -46,6 +46,11 @@ class DecoderModel:
                 self.blocks.append(block_class(mixer, ffn, norm1, norm2, env, params=dict(layer.block_params)))
             else:
                 self.blocks.append(block_class(mixer, ffn, norm1, norm2, env))
+        if env.cache_block is not None:
+            for index, block in enumerate(self.blocks):
+                if (block.mixer.cache_spec() is not None or block.mixer.extra_cache_specs()) and not block.mixer.holds_8bit:
+                    raise ValueError(f"layers[{index}]: {spec.layers[index].mixer.kind} as this model has it keeps its cache in the run "
+                                     f"dtype; one of 8 bits is for rotated keys and values without norms, biases or gates")
         self.layer_caches: List[LayerCache] = [LayerCache() for _ in spec.layers]
         # single-token steps may be replayed from a CUDA graph only if every part says so
         self.graph_safe = all(part.graph_safe for _where, part, _spec in self.named_parts())
@@ -133,12 +138,8 @@ class DecoderModel:
         for block, layer in zip(self.blocks, self.spec.layers):
             spec = block.mixer.cache_spec() if layer.cache_from is None else None
             if spec is not None:
-                for _name, shape in spec.entries:
-                    count = 1
-                    for extent in shape:
-                        count *= int(extent)
-                    total += count * self.env.dtype.itemsize
-        return total
+                total += spec.bytes_per_token(self.env.dtype.itemsize)
+        return round(total)
 
     def decode_cache_bytes(self, context: int) -> int:
         """Bytes of cache and state a single-token step moves for one request that holds ``context`` tokens, over the

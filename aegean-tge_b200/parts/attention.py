@@ -49,6 +49,9 @@ input, that multiplies the head's output where the attention writes it; and a la
 (``own_kv: False``) because it reads an earlier layer's cache.  The gate's rows lie below q, k and v in the one input
 product; one kernel normalises and stores, and the attention adds the bias and applies the gate.
 
+The plain layer (rotation, values of the keys' size, window, sinks) can hold its cache in 8 bits (``BuildEnv.cache_block``): codes of
+keys and values, and a scale per block of positions and head.  Product, one kernel that rotates, quantises and stores, attention over codes.
+
 On the general path, too: the norm of q and k after their rotation, with or without weights (``qk_norm`` with
 ``"after_rotation": True``); a sink whose score is a constant and not learned (``sink_score``); and one gate per number of
 the output (``output_gate``), the logistic function of a projection of the same input, applied where the attention writes.
@@ -197,6 +200,9 @@ class GQAttention(Mixer):
             self.gate_rows = self.heads + -(self.q_dim + kv + self.heads) % 16
         elif self.output_gate:
             self.gate_rows = self.o_dim + -(self.q_dim + self.kv_dim + self.v_dim + self.o_dim) % 16
+        # a cache of 8-bit codes: the plain layer, with a rotation that the kernels know
+        self.cache_block = env.cache_block
+        self.holds_8bit = self.plain and not self.general and not self.separate and tables is not None and self.head_dim <= 256
         self.conv_w: Optional[torch.Tensor] = None
         self.q_norm_w: Optional[torch.Tensor] = None
         self.k_norm_w: Optional[torch.Tensor] = None
@@ -369,6 +375,12 @@ class GQAttention(Mixer):
         # with pooled blocks a token is also read when its block is averaged, which is when the block's last token
         # arrives: the pages keep whichever reaches further back, the window or a block
         window = None if self.window is None else max(int(self.window), self.pool)
+        if self.cache_block is not None and self.holds_8bit:
+            block = self.cache_block
+            return PagedCacheSpec(entries=(("k", (self.kv_heads, self.head_dim)), ("v", (self.kv_heads, self.head_dim)),
+                                           ("k_scale", (self.kv_heads, 1)), ("v_scale", (self.kv_heads, 1))), window=window,
+                                  formats=(("k", torch.int8, 1), ("v", torch.int8, 1), ("k_scale", torch.float32, block),
+                                           ("v_scale", torch.float32, block)))
         return PagedCacheSpec(entries=(("k", (self.kv_heads, self.head_dim)), ("v", (self.kv_heads, self.value_dim))),
                               window=window, keep_first=self.keep_first)
 
@@ -412,6 +424,25 @@ class GQAttention(Mixer):
                              lead_longest=ctx.lead_longest, rest_ctx_len=ctx.rest_ctx_len, sink=self.sink,
                              out=out, gate=gate, **pooled)
 
+    def attend_8bit(self, h, ctx: StepContext, cache: LayerCache, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Product with its biases; rotation, codes and scales of k and v stored; attention over the codes."""
+        ops = self.ops
+        held = (cache.paged["k"], cache.paged["v"], cache.paged["k_scale"].squeeze(-1), cache.paged["v_scale"].squeeze(-1))
+        table = ctx.block_tables[cache.group]
+        cos, sin, rotary = self.position.rotary_tables()
+        qkv = ops.linear(h, self.w_qkv, self.b_qkv, ops.GEMM_STORE, settled=True)
+        if cache.owner:
+            q = ops.rope_kv_store_8bit(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, ctx.q_start, table, *held, self.heads,
+                                       self.kv_heads, self.head_dim)
+        else:
+            ops.rope_kv_store(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, table, None, None, self.heads, self.kv_heads, self.head_dim)
+            q = qkv[:, :self.q_dim]
+        if ctx.max_q_len > 1 and "ctx_lens" not in ctx.scratch:
+            ctx.scratch["ctx_lens"] = [start + count for start, count in zip(ctx.host_start_pos, ctx.host_q_lens)]
+        return ops.attention_8bit(q, *held, table, ctx.q_start, ctx.start_pos, ctx.positions, ctx.seq_of_token, ctx.num_seqs, ctx.max_q_len,
+                                  ctx.max_ctx_len, self.heads, self.kv_heads, self.head_dim, self.scale, window=int(self.window or 0), out=out,
+                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"))
+
     def share_input_projection(self, rows: torch.Tensor) -> Optional[torch.Tensor]:
         """A block offers the rows of another product over the same input (a feed-forward's up weight) to be
         multiplied together with q, k and v.  A mixer whose small-batch kernel can carry them (whole-projection
@@ -436,6 +467,9 @@ class GQAttention(Mixer):
         if self.general or self.values_are_keys or self.separate:
             attend = self.attend_keyed if self.values_are_keys else self.attend_separate if self.separate else self.attend_general
             a = attend(h, ctx, cache, out=out)
+            return a if beside is None else (a, False)
+        if self.cache_block is not None:
+            a = self.attend_8bit(h, ctx, cache, out=out)
             return a if beside is None else (a, False)
         ops = self.ops
         k_pages, v_pages = cache.paged["k"], cache.paged["v"]

@@ -64,23 +64,41 @@ class PagedCacheSpec:
     is whole; entry b of a request then sits where position b would.
     ``keep_first``: with a window, the first so many tokens of a request stay readable beside it, and their pages
     are kept.
+    ``formats``: (name, dtype, positions) of the entries that are not one per token in the run dtype: one per so many
+    positions (which divide a page) in a type of their own, for instance a cache's 8-bit codes and their scales.
     """
 
     entries: Tuple[Tuple[str, Tuple[int, ...]], ...]
     window: Optional[int] = None
     stride: int = 1
     keep_first: int = 0
+    formats: Tuple[Tuple[str, torch.dtype, int], ...] = ()
+
+    def format_of(self, name: str, dtype: Optional[torch.dtype]) -> Tuple[Optional[torch.dtype], int]:
+        """(type, positions per entry) of an entry; ``dtype``: the run dtype."""
+        return next(((kind, positions) for entry, kind, positions in self.formats if entry == name), (dtype, 1))
+
+    def bytes_per_token(self, element_size: int) -> float:
+        """Bytes that one position's entries take (``element_size``: of the run dtype)."""
+        total = 0
+        for name, shape in self.entries:
+            count = 1
+            for extent in shape:
+                count *= int(extent)
+            kind, positions = self.format_of(name, None)
+            total += count * (element_size if kind is None else kind.itemsize) / positions
+        return total
 
     def group_key(self) -> Tuple:
-        return (self.entries, self.window, self.stride, self.keep_first)
+        return (self.entries, self.window, self.stride, self.keep_first, self.formats)
 
     def covering(self, other: "PagedCacheSpec") -> "PagedCacheSpec":
         """This spec, keeping also whatever ``other`` may read of the same entries (another layer's mixer over them)."""
-        if other.entries != self.entries or other.stride != self.stride:
+        if other.entries != self.entries or other.stride != self.stride or other.formats != self.formats:
             raise ValueError(f"a mixer reads entries {other.entries} of a cache that keeps {self.entries}")
         if self.window is None or other.window is None:
-            return PagedCacheSpec(self.entries, None, self.stride)
-        return PagedCacheSpec(self.entries, max(self.window, other.window), self.stride, max(self.keep_first, other.keep_first))
+            return PagedCacheSpec(self.entries, None, self.stride, formats=self.formats)
+        return PagedCacheSpec(self.entries, max(self.window, other.window), self.stride, max(self.keep_first, other.keep_first), self.formats)
 
 
 @dataclass(frozen=True)
@@ -100,6 +118,7 @@ class BuildEnv:
     max_positions: int
     page_size: int
     ops: Any                           # the kernel bindings (aegean_tge_b200.ops)
+    cache_block: Optional[int] = None  # keys and values held in 8 bits, a scale per so many positions and head (None: in the run dtype)
 
 
 @dataclass
@@ -231,6 +250,8 @@ class StreamStep(Part):
 
 class Mixer(Part):
     """Mixes information between the tokens of a request."""
+    # A mixer with a paged cache that can hold it in 8 bits (``BuildEnv.cache_block``) says so; a model with one that cannot refuses.
+    holds_8bit = False
 
     def cache_spec(self) -> Optional[PagedCacheSpec]:
         return None
@@ -254,7 +275,7 @@ class Mixer(Part):
         spec = self.cache_spec()
         if spec is not None:
             seen = context if spec.window is None else min(context, int(spec.window) + int(spec.keep_first))
-            total += seen * per_entry(spec) * self.env.dtype.itemsize
+            total += int(seen * spec.bytes_per_token(self.env.dtype.itemsize))
         for extra in self.extra_cache_specs().values():
             total += (context // extra.stride) * per_entry(extra) * self.env.dtype.itemsize
         state = self.state_spec()
