@@ -407,27 +407,30 @@ __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
   return s;
 }
 
+// The block table over the runs, and the first tokens.  A kernel of its own: the attention kernels look block tables and first tokens up
+// while the kernel in front of them still runs, so these have to be there before that one lets them start.
+__global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p) {
+  pdl_trigger();
+  pdl_wait();
+  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += blockDim.x)
+    p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
+  int total = 0;
+  for (int seq = p.first_seq; seq < p.num_seqs; ++seq) {
+    const Span s = span_of(p, seq);
+    for (int i = threadIdx.x; i < p.width; i += blockDim.x)
+      p.table[(size_t)(seq - p.first_seq) * p.width + i] = i >= s.first && i < s.first + s.count ? total + i - s.first : -1;
+    if (s.first + s.count > p.width && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    total += s.count;
+  }
+  if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+}
+
 template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
-  __shared__ int found[3];
-  pdl_trigger();
+  __shared__ int found[2];
   const int run = blockIdx.x, kvh = blockIdx.y;
-  if (run == p.runs) {                         // the last block: table entries that name no run, and a look at the sum of all
-    pdl_wait();
-    if (kvh != 0) return;
-    for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += blockDim.x)
-      p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
-    int total = 0;
-    for (int seq = p.first_seq; seq < p.num_seqs; ++seq) {
-      const Span s = span_of(p, seq);
-      for (int i = threadIdx.x; i < p.width; i += blockDim.x)
-        if (i < s.first || i >= s.first + s.count) p.table[(size_t)(seq - p.first_seq) * p.width + i] = -1;
-      if (s.first + s.count > p.width && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-      total += s.count;
-    }
-    if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-    return;
-  }
+  pdl_wait();
+  pdl_trigger();                               // behind the wait: see the kernel above
   if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
     int before = 0, seq_found = -1, first_run = 0, index = 0;
     for (int base = p.first_seq; base < p.num_seqs && seq_found < 0; base += 32) {
@@ -455,13 +458,11 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   const int seq = found[0], tile = found[1];
   T* k_dst = static_cast<T*>(p.k_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
   T* v_dst = static_cast<T*>(p.v_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
-  pdl_wait();
   if (seq < 0) {                               // the caller counted more runs than there are
     for (int i = threadIdx.x; i < 64 * p.head_dim; i += blockDim.x) k_dst[i] = v_dst[i] = from_float<T>(0.0f);
     return;
   }
   const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
-  if (kvh == 0 && threadIdx.x == 0 && tile < p.width) p.table[(size_t)(seq - p.first_seq) * p.width + tile] = run;
   if constexpr (UNITS) {
     // sixteen codes of a position to a thread and turn, all loads of a turn of keys and values on their way together
     const int units = p.head_dim >> 4, shift = __ffs(p.block) - 1, blocks = p.page_size >> shift;
@@ -586,11 +587,13 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   if (num_seqs == first_seq || width == 0) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
                      page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, starts, runs, width, status};
-  const dim3 grid(runs + 1, kv_heads);
+  tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
+  if (runs == 0) return tge_launched("read_8bit", 1);
+  const dim3 grid(runs, kv_heads);
   const bool units = head_dim % 16 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (is_bf16)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
     tge_launch(units ? read_8bit_kernel<float, true> : read_8bit_kernel<float, false>, grid, 256, 0, stream, p);
-  return tge_launched("read_8bit", 1);
+  return tge_launched("read_8bit", 2);
 }
