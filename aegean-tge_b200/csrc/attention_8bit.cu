@@ -114,11 +114,13 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // sums of probabilities stay in their lanes until the end.
 //
 // Work: the slices of all (request, kv head, tile of heads) units in one row, cut into equal runs, one per block, whatever the
-// requests' lengths; the blocks work that out from the lengths on the device, so a captured graph stays right as they grow.  A run
+// requests' lengths; the blocks work that out from the lengths on the device, so a captured graph stays right as they grow.  A unit
+// counts as BEGIN slices more than it has: what a block spends on its queries, its first copies and the joining of its warps.  A run
 // that holds a whole unit writes its output; parts of units are left as (maximum, sum, unnormalised output) in scratch memory, at
 // most two per block, and a second kernel joins them in the order of the positions.
 // ---------------------------------------------------------------------------
 constexpr int DWARPS = 4;
+constexpr int BEGIN = 12;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float HELD = 64.0f;                   // probabilities are held times this
@@ -145,10 +147,10 @@ __device__ __forceinline__ Slices slices_of(const Decode8& p, int seq) {
   return s;
 }
 
-// Sum of the slice counts of requests [0, upto), by the whole warp.
+// What requests [0, upto) count for in the row, by the whole warp.
 __device__ __forceinline__ int slices_before(const Decode8& p, int upto, int lane) {
   int n = 0;
-  for (int seq = lane; seq < upto; seq += 32) n += slices_of(p, seq).count;
+  for (int seq = lane; seq < upto; seq += 32) n += (slices_of(p, seq).count + BEGIN) * p.units;
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) n += __shfl_xor_sync(0xffffffffu, n, offset);
   return n;
@@ -319,16 +321,26 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
   extern __shared__ float merge_o[];                              // [warps][HEADS][PITCH], a head's numbers in the order of the accumulators
   __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS], factors[HEADS];
   __shared__ __align__(16) uint32_t queries[NT][C::KC][DIGITS][32][4];
-  __shared__ int start_of[4];
+  __shared__ int start_of[5];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = uniform_warp_index();
   const int g = lane >> 2, t = lane & 3;
   if (warp == 0) {                                                // where this block's run begins
-    const int total = slices_before(p, p.a.num_seqs, lane) * p.units, run = run_length(p, total, gridDim.x);
+    // 32 requests at a time; the first of them stay where they are
+    const int first_count = lane < p.a.num_seqs ? (slices_of(p, lane).count + BEGIN) * p.units : 0;
+    const int first_token = lane < p.a.num_seqs ? p.q_start[lane] : 0;
+    int total = __reduce_add_sync(0xffffffffu, first_count);
+    for (int seq = 32 + lane; seq - lane < p.a.num_seqs; seq += 32)
+      total += __reduce_add_sync(0xffffffffu, seq < p.a.num_seqs ? (slices_of(p, seq).count + BEGIN) * p.units : 0);
+    const int run = run_length(p, total, gridDim.x);
     const int from = (int)min((long long)run * blockIdx.x, (long long)total);
-    int seq = 0, base = 0;
-    while (seq < p.a.num_seqs) {                                  // 32 requests at a time
-      const int n = seq + lane < p.a.num_seqs ? slices_of(p, seq + lane).count * p.units : 0;
+    int seq = 0, base = 0, token = first_token;
+    while (seq < p.a.num_seqs) {
+      int n = first_count;
+      if (seq > 0) {
+        n = seq + lane < p.a.num_seqs ? (slices_of(p, seq + lane).count + BEGIN) * p.units : 0;
+        token = seq + lane < p.a.num_seqs ? p.q_start[seq + lane] : 0;
+      }
       int upto = n;
 #pragma unroll
       for (int offset = 1; offset < 32; offset <<= 1) {
@@ -338,6 +350,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       const unsigned here = __ballot_sync(0xffffffffu, from < base + upto);
       const int who = here ? __ffs(here) - 1 : 31;
       const int behind = __shfl_sync(0xffffffffu, upto, who), mine = __shfl_sync(0xffffffffu, n, who);
+      token = __shfl_sync(0xffffffffu, token, who);
       if (here) {
         base += behind - mine;
         seq += who;
@@ -351,20 +364,24 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       start_of[1] = base;
       start_of[2] = from;
       start_of[3] = min(from + run, total);
+      start_of[4] = token;
     }
   }
   __syncthreads();
-  int seq = start_of[0], base = start_of[1], at = start_of[2];
+  int seq = start_of[0], base = start_of[1], at = start_of[2], token = start_of[4];
   const int end = start_of[3];
-  pdl_wait();
+  bool waited = false;
 
   while (at < end) {
     const Slices s = slices_of(p, seq);
-    const int unit = (at - base) / s.count, skip = (at - base) - unit * s.count;
-    const int length = min(s.count - skip, end - at);
+    const int unit = (at - base) / (s.count + BEGIN), begin = base + unit * (s.count + BEGIN);
+    const int upto = min(begin + s.count + BEGIN, end);            // where this unit's part of the run ends
+    const int skip = max(at - begin - BEGIN, 0), length = upto - begin - BEGIN - skip;
+    at = upto;
+    const bool next_seq = unit == p.units - 1 && upto == begin + s.count + BEGIN;
+    if (length <= 0) continue;                                     // no more than the begin of a unit
     const int kvh = unit / p.head_tiles, tile = unit - kvh * p.head_tiles;
     const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
-    const int token = p.q_start[seq];
     const int* table = p.a.block_table + (size_t)seq * p.a.max_pages;
     // the warps' shares of the run's slices, one behind the other
     const int first = s.first + skip + length * warp / DWARPS, last = s.first + skip + length * (warp + 1) / DWARPS;
@@ -384,6 +401,8 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         row = start_at(page);
       }
     };
+    if (!waited) pdl_wait();                                       // all above is what the step was given
+    waited = true;
     C c;
     if (first < last) {
       load_keys<HD>(p, c, row, g, t);
@@ -598,12 +617,13 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         if (pair == 0) *reinterpret_cast<float2*>(p.states + (place + head) * 2) = make_float2(most, sum);
       }
     }
-    at += length;
-    if (at == base + s.count * p.units) {
+    if (next_seq && at < end) {
       base = at;
       ++seq;
+      token = p.q_start[seq];
     }
   }
+  if (!waited) pdl_wait();
 }
 
 // Joins the parts of the units that more than one block worked on: one block per unit, two warps per head, which take the first and the
@@ -618,8 +638,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const
   pdl_trigger();
   const int seq = blockIdx.x, unit = blockIdx.y, lane = threadIdx.x & 31, warp = uniform_warp_index();
   if (warp == 0) {
-    const int total = slices_before(p, p.a.num_seqs, lane) * p.units, run = run_length(p, total, blocks);
-    const int count = slices_of(p, seq).count, from = slices_before(p, seq, lane) * p.units + unit * count;
+    const int total = slices_before(p, p.a.num_seqs, lane), run = run_length(p, total, blocks);
+    const int count = slices_of(p, seq).count, from = slices_before(p, seq, lane) + unit * (count + BEGIN) + BEGIN;
     if (lane == 0) {
       where[0] = from / run;
       where[1] = (from + count - 1) / run;
@@ -648,6 +668,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const
       const int count = min(32, to - b0);
       float2 state = make_float2(NONE, 0.0f);
       if (lane < count) state = *reinterpret_cast<const float2*>(p.states + place(b0 + lane) * 2);
+      float2 x[JOIN_AHEAD][PAIRS];
+      auto load = [&](int b) {
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k)
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i)
+            x[k][i] = b + k < count ? *reinterpret_cast<const float2*>(p.parts + place(b0 + b + k) * HD + 2 * (lane + 32 * i)) : make_float2(0.0f, 0.0f);
+      };
+      load(0);                                                     // on their way while the states' maximum is found
       const float top = fmaxf(most, warp_max(state.x));
       const float weight = exp2_fast(state.x - top), down = exp2_fast(most - top);
       sum = fmaf(sum, down, warp_sum(weight * state.y));
@@ -655,12 +684,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) { acc[i].x *= down; acc[i].y *= down; }
       for (int b = 0; b < count; b += JOIN_AHEAD) {
-        float2 x[JOIN_AHEAD][PAIRS];
-#pragma unroll
-        for (int k = 0; k < JOIN_AHEAD; ++k)
-#pragma unroll
-          for (int i = 0; i < PAIRS; ++i)
-            x[k][i] = b + k < count ? *reinterpret_cast<const float2*>(p.parts + place(b0 + b + k) * HD + 2 * (lane + 32 * i)) : make_float2(0.0f, 0.0f);
+        if (b > 0) load(b);
 #pragma unroll
         for (int k = 0; k < JOIN_AHEAD; ++k) {
           const float f = __shfl_sync(0xffffffffu, weight, (b + k) & 31);
@@ -733,7 +757,7 @@ TGE_API long long tge_attention_8bit_decode_floats(int is_bf16, int num_seqs, in
   const long long units = (long long)kv_heads * ((heads / kv_heads + tile - 1) / tile);
   // places in the row of all slices are counted in 32 bits, units along a grid's second axis
   if (units > 65535 || (long long)max_pages * page_size > (1ll << 30) ||
-      units * num_seqs * ((long long)max_pages * page_size / 16 + 1) > (1ll << 30)) return -1;
+      units * num_seqs * ((long long)max_pages * page_size / 16 + 1 + BEGIN) > (1ll << 30)) return -1;
   return 2ll * decode_blocks(head_dim, tile) * tile * (head_dim + 2);
 }
 

@@ -407,11 +407,8 @@ __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
   return s;
 }
 
-// The block table over the runs, and the first tokens.  A kernel of its own: the attention kernels look block tables and first tokens up
-// while the kernel in front of them still runs, so these have to be there before that one lets them start.
-__global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p) {
-  pdl_trigger();
-  pdl_wait();
+// The block table over the runs, and the first tokens if wanted.
+__device__ __forceinline__ void plan_runs(const ReadParams& p) {
   for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += blockDim.x)
     p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
   int total = 0;
@@ -425,12 +422,24 @@ __global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p)
   if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
 }
 
+// A kernel of its own where attention follows: the attention kernels look block tables and first tokens up while the kernel in front of
+// them still runs, so these have to be there before that one lets them start.
+__global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p) {
+  pdl_trigger();
+  pdl_wait();
+  plan_runs(p);
+}
+
 template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ int found[2];
   const int run = blockIdx.x, kvh = blockIdx.y;
   pdl_wait();
   pdl_trigger();                               // behind the wait: see the kernel above
+  if (run == p.runs) {                         // the block behind the runs, where no kernel in front has planned them
+    if (kvh == 0) plan_runs(p);
+    return;
+  }
   if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
     int before = 0, seq_found = -1, first_run = 0, index = 0;
     for (int base = p.first_seq; base < p.num_seqs && seq_found < 0; base += 32) {
@@ -587,13 +596,14 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   if (num_seqs == first_seq || width == 0) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
                      page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, starts, runs, width, status};
-  tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
-  if (runs == 0) return tge_launched("read_8bit", 1);
-  const dim3 grid(runs, kv_heads);
+  const bool planned = starts != nullptr;
+  if (planned) tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
+  if (planned && runs == 0) return tge_launched("read_8bit", 1);
+  const dim3 grid(runs + (planned ? 0 : 1), kv_heads);
   const bool units = head_dim % 16 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (is_bf16)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
     tge_launch(units ? read_8bit_kernel<float, true> : read_8bit_kernel<float, false>, grid, 256, 0, stream, p);
-  return tge_launched("read_8bit", 2);
+  return tge_launched("read_8bit", planned ? 2 : 1);
 }

@@ -1092,20 +1092,22 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
 def _cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
                 num_seqs: int, kv_heads: int, head_dim: int) -> Tuple[int, int, int]:
     """(pages, positions in a page, positions in a block) of a cache held in 8 bits."""
-    for name, t, dtype in (("k pages", k_pages, torch.int8), ("v pages", v_pages, torch.int8), ("k scales", k_scale, torch.float32),
-                           ("v scales", v_scale, torch.float32), ("block table", block_table, torch.int32)):
-        _want(t, name, dtype)
-    if k_pages.dim() != 4 or k_pages.shape[1] != kv_heads or k_pages.shape[3] != head_dim or v_pages.shape != k_pages.shape:
-        raise KernelError(f"8-bit pages must be [pages, {kv_heads}, page_size, {head_dim}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    num_pages, _, page_size, _ = k_pages.shape
-    blocks = k_scale.shape[2] if k_scale.dim() == 3 else 0
-    if tuple(k_scale.shape) != (num_pages, kv_heads, blocks) or v_scale.shape != k_scale.shape or blocks <= 0 or page_size % blocks:
-        raise KernelError(f"scales must be [{num_pages}, {kv_heads}, blocks of a page], got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
-    block = page_size // blocks
+    _want(k_pages, "k pages", torch.int8)
+    _want(v_pages, "v pages", torch.int8)
+    _want(k_scale, "k scales", torch.float32)
+    _want(v_scale, "v scales", torch.float32)
+    _want(block_table, "block table", torch.int32)
+    shape, scales, table = k_pages.shape, k_scale.shape, block_table.shape
+    if len(shape) != 4 or shape[1] != kv_heads or shape[3] != head_dim or v_pages.shape != shape:
+        raise KernelError(f"8-bit pages must be [pages, {kv_heads}, page_size, {head_dim}], got {tuple(shape)} and {tuple(v_pages.shape)}")
+    num_pages, _, page_size, _ = shape
+    if len(scales) != 3 or scales[0] != num_pages or scales[1] != kv_heads or v_scale.shape != scales or scales[2] <= 0 or page_size % scales[2]:
+        raise KernelError(f"scales must be [{num_pages}, {kv_heads}, blocks of a page], got {tuple(scales)} and {tuple(v_scale.shape)}")
+    block = page_size // scales[2]
     if block & (block - 1):
         raise KernelError(f"a block of {block} positions: blocks are a power of two")
-    if block_table.dim() != 2 or block_table.shape[0] < num_seqs or block_table.shape[1] == 0:
-        raise KernelError(f"the block table must be [{num_seqs}, pages], got {tuple(block_table.shape)}")
+    if len(table) != 2 or table[0] < num_seqs or table[1] == 0:
+        raise KernelError(f"the block table must be [{num_seqs}, pages], got {tuple(table)}")
     return num_pages, page_size, block
 
 
@@ -1121,6 +1123,18 @@ def _per_token(positions: torch.Tensor, seq_of_token: torch.Tensor, tokens: int)
     _want(seq_of_token, "seq_of_token", torch.int32)
     if positions.numel() < tokens or seq_of_token.numel() < tokens:
         raise KernelError(f"{tokens} tokens with {positions.numel()} positions and {seq_of_token.numel()} portions")
+
+
+def _rows_like(x: torch.Tensor, width: int, out: Optional[torch.Tensor], name: str) -> Tuple[torch.Tensor, int]:
+    """(``out`` or a new tensor of x's rows and type, ``width`` wide; its row stride)."""
+    tokens = x.shape[0]
+    if out is None:
+        # (half the price of torch.empty with its keywords, in a call that the host's time decides)
+        return (torch.empty_like(x) if x.shape[1] == width and x.is_contiguous() else x.new_empty((tokens, width))), width
+    _want(out, name, x.dtype, contiguous=False)
+    if out.dim() != 2 or out.shape[0] != tokens or out.shape[1] != width:
+        raise KernelError(f"{name} must be [{tokens}, {width}], got {tuple(out.shape)}")
+    return out, _rows_2d(out, name)
 
 
 def rope_kv_store_8bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary: int, positions: torch.Tensor,
@@ -1150,13 +1164,9 @@ def rope_kv_store_8bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Opti
     _want(q_start, "q_start", torch.int32)
     num_seqs = q_start.numel() - 1
     num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
-    if out is None:
-        out = torch.empty((tokens, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-    _want(out, "rotated queries", qkv.dtype, contiguous=False)
-    if tuple(out.shape) != (tokens, heads * head_dim):
-        raise KernelError(f"rotated queries must be [{tokens}, {heads * head_dim}], got {tuple(out.shape)}")
+    out, out_stride = _rows_like(qkv, heads * head_dim, out, "rotated queries")
     lib = core()
-    _check(lib.tge_store_8bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), _rows_2d(out, "rotated queries"),
+    _check(lib.tge_store_8bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), out_stride,
                               _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0], rotary, positions.data_ptr(),
                               seq_of_token.data_ptr(), q_start.data_ptr(), num_seqs, block_table.data_ptr(), block_table.shape[1],
                               k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size,
@@ -1189,15 +1199,18 @@ def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_p
     # a window may leave out runs in front: the sum is then a bound
     mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
     runs, width = sum(mine), max(mine, default=0)
-    k = torch.empty((runs, kv_heads, 64, head_dim), dtype=dtype, device=k_pages.device)
+    k = k_scale.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    table = torch.empty((len(mine), width), dtype=torch.int32, device=k_pages.device)
+    table = block_table.new_empty((len(mine), width))
     lib = core()
     _check(lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                              block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
                              kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), int(dtype == torch.bfloat16), table.data_ptr(),
                              _ptr(starts), runs, width, status_word().data_ptr(), _stream()), lib)
     return k, v, table
+
+
+_decode_8bit_floats: Dict[tuple, int] = {}      # scratch numbers by sizes: asking the library costs a microsecond a call
 
 
 def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -1228,20 +1241,21 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         _want(sink, "attention sinks", torch.float32)
         if sink.numel() != heads:
             raise KernelError(f"attention: {sink.numel()} sinks for {heads} heads")
-    if out is None:
-        out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=q.device)
-    _want(out, "attention output", q.dtype, contiguous=False)
-    if tuple(out.shape) != (tokens, heads * head_dim):
-        raise KernelError(f"attention: the output must be [{tokens}, {heads * head_dim}], got {tuple(out.shape)}")
-    out_stride, is_bf16 = _rows_2d(out, "attention output"), int(q.dtype == torch.bfloat16)
+    out, out_stride = _rows_like(q, heads * head_dim, out, "attention output")
+    is_bf16 = int(q.dtype == torch.bfloat16)
     lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                           block_table.data_ptr(), block_table.shape[1])
     singles = num_seqs if max_q_len <= 1 else decode_prefix
     done = 0                                            # requests, and so tokens, that are served
     if singles:
-        need = lib.tge_attention_8bit_decode_floats(is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
+        sizes = (is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
+        need = _decode_8bit_floats.get(sizes)
+        if need is None:
+            if len(_decode_8bit_floats) >= 1024:
+                _decode_8bit_floats.clear()
+            need = _decode_8bit_floats[sizes] = lib.tge_attention_8bit_decode_floats(*sizes)
         if need >= 0:
-            parts = torch.empty(need, dtype=torch.float32, device=q.device)
+            parts = k_scale.new_empty(need)
             rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
                                                out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
                                                parts.data_ptr(), need, status_word().data_ptr(), _stream())
@@ -1250,17 +1264,21 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if done == num_seqs:
         return out
     ctx_lens = [max_ctx_len] * num_seqs if ctx_lens is None else ctx_lens
+    rest = (q, out, start_pos, positions, seq_of_token)
+    if done:
+        rest = (q[done:], out[done:], start_pos[done:], positions[done:], seq_of_token[done:])
+    rows, rows_out, rest_pos, rest_positions, rest_seq = rest
     if max_q_len > 1 and done == singles and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
                                               else head_dim in (16, 32, 64, 128) and sink is None):
         # portions: their keys and values are read once into run-type pages of 64, which the prefill kernels take; a query tile of
         # those reads each of them again, so that turning codes into numbers there would be done many times over
-        starts = torch.empty(num_seqs - done + 1, dtype=torch.int32, device=q.device)
+        starts = q_start.new_empty(num_seqs - done + 1)
         k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, done, starts)
-        attention(q[done:, :heads * head_dim], k, v, table, starts, start_pos[done:], positions[done:], seq_of_token[done:], num_seqs - done,
-                  max_q_len, max(ctx_lens[done:]), heads, kv_heads, head_dim, scale, window=window, out=out[done:], sink=sink)
+        attention(rows, k, v, table, starts, rest_pos, rest_positions, rest_seq, num_seqs - done, max_q_len, max(ctx_lens[done:]), heads, kv_heads,
+                  head_dim, scale, window=window, out=rows_out, sink=sink)
         return out
-    _check(lib.tge_attention_8bit_simple(q[done:].data_ptr(), is_bf16, q_stride, *cache, positions[done:].data_ptr(), seq_of_token[done:].data_ptr(),
-                                         num_seqs, tokens - done, out[done:].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale),
+    _check(lib.tge_attention_8bit_simple(rows.data_ptr(), is_bf16, q_stride, *cache, rest_positions.data_ptr(), rest_seq.data_ptr(),
+                                         num_seqs, tokens - done, rows_out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale),
                                          int(window), _ptr(sink), status_word().data_ptr(), _stream()), lib)
     return out
 
@@ -1631,17 +1649,16 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     stride = _rows_2d(logits, "logits")
     rows, vocab = logits.shape
     _want(tokens, "tokens", torch.int32)
-    if tokens.numel() != rows:
-        raise KernelError(f"token_logprobs: {tokens.numel()} tokens for {rows} rows")
-    device = logits.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=device)
-    entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    rank = torch.empty(rows, dtype=torch.int32, device=device)
-    top_ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=device)
-    top_logprobs = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=device)
+    if tuple(tokens.shape) != (rows,):
+        raise KernelError(f"token_logprobs: {tuple(tokens.shape)} tokens for {rows} rows")
+    wide = max(top, 0)
+    logprob, entropy = logits.new_empty((2, rows), dtype=torch.float32).unbind(0)
+    rank = torch.empty_like(tokens)
+    top_ids = tokens.new_empty((rows, wide))
+    top_logprobs = entropy.new_empty((rows, wide))
     lib = core()
     need = lib.tge_token_logprobs_floats(rows, vocab, int(top))
-    scratch = torch.empty(need, dtype=torch.float32, device=device) if need else None
+    scratch = entropy.new_empty(need) if need else None
     _check(lib.tge_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride, tokens.data_ptr(), rows, vocab, int(top),
                                   logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(),
                                   _ptr(scratch), need, status_word().data_ptr(), _stream()), lib)
