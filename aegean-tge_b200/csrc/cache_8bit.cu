@@ -12,6 +12,8 @@
 //   lo' = lo cos - hi sin ; hi' = lo sin + hi cos
 // keys are quantised from these float32 numbers, with no rounding to the run's type in between.  127 x is exact for a bfloat16 x and
 // the division is rounded once, so x = s (k + 1/2) / 127 meets its tie exactly and goes to even wherever it is computed.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace {
@@ -156,9 +158,14 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 constexpr int UNIT_THREADS = 128, UNIT_AHEAD = 3;
 
 struct Eight { float x[8]; };
-__device__ __forceinline__ Eight eight(const __nv_bfloat16* src) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(src);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+// Eight numbers as they lie in memory.
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> { uint4 w; };
+template <> struct Raw<float> { float4 a, b; };
+__device__ __forceinline__ Raw<__nv_bfloat16> raw_eight(const __nv_bfloat16* src) { return {*reinterpret_cast<const uint4*>(src)}; }
+__device__ __forceinline__ Raw<float> raw_eight(const float* src) { return {reinterpret_cast<const float4*>(src)[0], reinterpret_cast<const float4*>(src)[1]}; }
+__device__ __forceinline__ Eight eight(const Raw<__nv_bfloat16>& r) {
+  const uint32_t w[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
   Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -167,10 +174,10 @@ __device__ __forceinline__ Eight eight(const __nv_bfloat16* src) {
   }
   return e;
 }
-__device__ __forceinline__ Eight eight(const float* src) {
-  const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-  return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
+__device__ __forceinline__ Eight eight(const Raw<float>& r) { return Eight{{r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w}}; }
+template <typename T>
+__device__ __forceinline__ Eight eight(const T* src) { return eight(raw_eight(src)); }
+
 __device__ __forceinline__ void put_eight(__nv_bfloat16* dst, const Eight& e) {
   uint4 raw;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
@@ -206,7 +213,7 @@ __device__ __forceinline__ void put_codes(int8_t* dst, const Coder& coder, const
 }
 
 template <typename T, int HEAD>
-__global__ void __launch_bounds__(UNIT_THREADS) store_8bit_units_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 6 : 5) store_8bit_units_kernel(const StoreParams p) {
   constexpr int LANES = HEAD / 16, GROUPS = UNIT_THREADS / LANES, HALF = HEAD / 2;
   __shared__ float scales[GROUPS];
   __shared__ int found[2];
@@ -227,9 +234,22 @@ __global__ void __launch_bounds__(UNIT_THREADS) store_8bit_units_kernel(const St
   };
   if ((int)blockIdx.x < p.tokens) {
     const int t = blockIdx.x, pos = p.positions[t], seq = p.seq_of_token[t];
+    pdl_wait();
+    // the first rows are on their way before anything has to be looked up
+    const T* row = rows + (size_t)t * p.row_stride;
+    const int heads = p.heads + (p.block == 1 ? 2 * p.kv_heads : 0);
+    Raw<T> lo_raw[UNIT_AHEAD], hi_raw[UNIT_AHEAD];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int i = 0; i < UNIT_AHEAD; ++i) {
+        const int h = min(h0 + i * GROUPS, heads - 1);
+        lo_raw[i] = raw_eight(row + (size_t)h * HEAD);
+        hi_raw[i] = raw_eight(row + (size_t)h * HEAD + HALF);
+      }
+    };
+    load(group);
     if (pos < 0 || (rotate && pos >= p.table_rows) || seq < 0 || seq >= p.num_seqs) {
       if (threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-      pdl_wait();
       return;
     }
     Eight c, s;
@@ -238,36 +258,28 @@ __global__ void __launch_bounds__(UNIT_THREADS) store_8bit_units_kernel(const St
     const int page = page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
     const bool here = page >= 0 && page < p.num_pages;
     if (!here && p.block == 1 && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
-    pdl_wait();
-    const T* row = rows + (size_t)t * p.row_stride;
-    const int heads = p.heads + (p.block == 1 ? 2 * p.kv_heads : 0);
     for (int h0 = group; h0 < heads + group; h0 += UNIT_AHEAD * GROUPS) {       // the same number of rounds for every lane of a warp
-      Eight lo[UNIT_AHEAD], hi[UNIT_AHEAD];
-#pragma unroll
-      for (int i = 0; i < UNIT_AHEAD; ++i) {
-        const int h = min(h0 + i * GROUPS, heads - 1);
-        lo[i] = eight(row + (size_t)h * HEAD);
-        hi[i] = eight(row + (size_t)h * HEAD + HALF);
-      }
+      if (h0 != group) load(h0);
 #pragma unroll
       for (int i = 0; i < UNIT_AHEAD; ++i) {
         const int h = h0 + i * GROUPS;
+        Eight lo = eight(lo_raw[i]), hi = eight(hi_raw[i]);
         const bool valid = h < heads, to_cache = h >= p.heads;
-        if (rotate && h < p.heads + p.kv_heads) turn(lo[i], hi[i], c, s);
+        if (rotate && h < p.heads + p.kv_heads) turn(lo, hi, c, s);
         if (valid && !to_cache) {
           T* dst = static_cast<T*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * HEAD + 8 * j;
-          put_eight(dst, lo[i]);
-          put_eight(dst + HALF, hi[i]);
+          put_eight(dst, lo);
+          put_eight(dst + HALF, hi);
         }
         if (__any_sync(0xffffffffu, valid && to_cache)) {
-          const float scale = all_lanes(largest_of(lo[i], hi[i]));
+          const float scale = all_lanes(largest_of(lo, hi));
           if (valid && to_cache && here) {
             const bool is_key = h < p.heads + p.kv_heads;
             const size_t entry = ((size_t)page * p.kv_heads + (h - p.heads - (is_key ? 0 : p.kv_heads))) * p.page_size + slot;
             const Coder coder(scale);
             int8_t* codes = (is_key ? p.k_pages : p.v_pages) + entry * HEAD + 8 * j;
-            put_codes(codes, coder, lo[i]);
-            put_codes(codes + HALF, coder, hi[i]);
+            put_codes(codes, coder, lo);
+            put_codes(codes + HALF, coder, hi);
             if (j == 0) (is_key ? p.k_scale : p.v_scale)[entry] = scale;
           }
         }
@@ -433,11 +445,11 @@ __global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p)
 template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ int found[2];
-  const int run = blockIdx.x, kvh = blockIdx.y;
+  const int run = blockIdx.x;
   pdl_wait();
   pdl_trigger();                               // behind the wait: see the kernel above
   if (run == p.runs) {                         // the block behind the runs, where no kernel in front has planned them
-    if (kvh == 0) plan_runs(p);
+    if (blockIdx.y == 0) plan_runs(p);
     return;
   }
   if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
@@ -465,11 +477,12 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   }
   __syncthreads();
   const int seq = found[0], tile = found[1];
+  for (int kvh = blockIdx.y; kvh < p.kv_heads; kvh += gridDim.y) {
   T* k_dst = static_cast<T*>(p.k_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
   T* v_dst = static_cast<T*>(p.v_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
   if (seq < 0) {                               // the caller counted more runs than there are
     for (int i = threadIdx.x; i < 64 * p.head_dim; i += blockDim.x) k_dst[i] = v_dst[i] = from_float<T>(0.0f);
-    return;
+    continue;
   }
   const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
   if constexpr (UNITS) {
@@ -516,7 +529,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
           }
         }
     }
-    return;
+    continue;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int j = warp; j < 64; j += 8) {
@@ -532,6 +545,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
       k_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.k_pages[entry * p.head_dim + d] * ks : 0.0f);
       v_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.v_pages[entry * p.head_dim + d] * vs : 0.0f);
     }
+  }
   }
 }
 
@@ -599,7 +613,9 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   const bool planned = starts != nullptr;
   if (planned) tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
   if (planned && runs == 0) return tge_launched("read_8bit", 1);
-  const dim3 grid(runs + (planned ? 0 : 1), kv_heads);
+  // a block takes several heads of its run where there are many runs: finding whose it is costs as much as a head
+  const int at_once = 10 * tge_sm_count();
+  const dim3 grid(runs + (planned ? 0 : 1), std::max(1, std::min(kv_heads, (at_once + runs) / (runs + 1))));
   const bool units = head_dim % 16 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (is_bf16)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);

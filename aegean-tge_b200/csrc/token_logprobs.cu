@@ -9,12 +9,11 @@
 
 namespace {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int MOST_TOP = 32;
 constexpr int MINE = 16;                        // logits of a thread and round
 constexpr int ROUND = THREADS * MINE;
-constexpr int ROOM = 4096 + MOST_TOP;           // keys in the list of candidates: what one load of all threads may add to a full choice
-constexpr int SORTED_AT_ONCE = 512;             // more are chosen one after the other
+constexpr int ROOM = 8 * THREADS + MOST_TOP;    // keys in the list of candidates: what one load of all threads may add to a full choice
 constexpr int MOST_SPLITS = 128;
 constexpr float LEAST = -3.402823466e38f;       // where a thread's reference starts: finite, so that -inf less it is -inf
 constexpr float LOG2E = 1.4426950408889634f;
@@ -88,17 +87,60 @@ __device__ __forceinline__ Sums block_sums(Sums mine, float* scratch, int* count
   return mine;
 }
 
-// The `top` largest of the `count` keys at `list`, sorted, to its start; the smallest of them (0 if there are fewer).
-__device__ __forceinline__ unsigned long long choose(unsigned long long* list, int count, int top, unsigned long long* scratch) {
+constexpr int GROUPS = THREADS / 4;             // groups of four lanes
+static_assert(GROUPS == 64, "two groups to a lane");
+
+// A bar that at least `top` keys pass (are above) and not many more: just below the top-th largest of the groups' largest keys, if so many
+// groups have one, else 0.  `key`: the thread's largest (0: none).  scratch: 64 keys and one for the result.
+__device__ __forceinline__ unsigned long long bar_of(unsigned long long key, int top, unsigned long long* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  key = warp_largest(key, 4);
   __syncthreads();
-  if (count <= SORTED_AT_ONCE) {
+  if ((lane & 3) == 0) scratch[threadIdx.x >> 2] = key;
+  if (threadIdx.x == 0) scratch[64] = 0ull;
+  __syncthreads();
+  const unsigned long long a = scratch[lane], b = scratch[lane + 32];
+#pragma unroll
+  for (int i = 0; i < GROUPS * 32 / THREADS; ++i) {
+    const unsigned long long mine = scratch[warp * (GROUPS * 32 / THREADS) + i];
+    const int in_front = __popc(__ballot_sync(0xffffffffu, a > mine)) + __popc(__ballot_sync(0xffffffffu, b > mine));
+    if (lane == 0 && mine != 0ull && in_front == top - 1) scratch[64] = mine - 1;
+  }
+  __syncthreads();
+  return scratch[64];
+}
+
+// The `top` largest of the `count` keys at `list`, sorted, to its start; the smallest of them (0 if there are fewer).  Few keys find their
+// places by counting those in front of them; of many, those above a bar come to the start first.  MOST: a bound of `count`.
+template <int MOST>
+__device__ __forceinline__ unsigned long long choose(unsigned long long* list, int count, int top, unsigned long long* scratch, int* counter) {
+  constexpr int EACH = (MOST + THREADS - 1) / THREADS;
+  __syncthreads();
+  if (count > 64) {
+    unsigned long long mine[EACH], largest = 0ull;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int at = threadIdx.x + i * THREADS;
+      mine[i] = at < count ? list[at] : 0ull;
+      largest = max(largest, mine[i]);
+    }
+    const unsigned long long bar = bar_of(largest, top, scratch);
+    if (threadIdx.x == 0) *counter = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (mine[i] > bar) list[atomicAdd(counter, 1)] = mine[i];
+    __syncthreads();
+    count = *counter;
+  }
+  if (count <= THREADS) {
     const unsigned long long mine = (int)threadIdx.x < count ? list[threadIdx.x] : 0ull;
     int ahead = 0;
     if ((int)(threadIdx.x & ~31) < count)
       for (int i = 0; i < count; ++i) ahead += list[i] > mine ? 1 : 0;
     __syncthreads();
     if ((int)threadIdx.x < count && ahead < top) list[ahead] = mine;
-  } else {
+  } else {                                       // keys that rise with their place, say: one after the other
     unsigned long long last = ~0ull;
     for (int k = 0; k < top; ++k) {
       unsigned long long next = 0;
@@ -172,15 +214,15 @@ __device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[
 // One pass over a chunk of a row.  What bounds it is reading the logits: a thread holds its next sixteen on their way while it works on
 // these, keeps sums of its own, and looks at single logits only where its largest reaches the smallest of the best so far.  Those that do are listed
 // with the block's others; the list is cut to the best now and then.  After the first round the best are a
-// choice among the largest of 32 half warps' logits and whatever passes the n-th of those, then whatever passes the n-th of the chunk's
+// choice among the largest of 64 groups of four lanes and whatever passes the n-th of those, then whatever passes the n-th of the chunk's
 // first 1, 2, 4, 8, ... rounds: of random rows some hundred logits are ever listed.  A row that lists more than there is room
 // for (rising logits) is looked through again.
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const LogprobParams p) {
   constexpr int per = 16 / sizeof(T);
-  __shared__ unsigned long long list[ROOM], scratch[64];
+  __shared__ unsigned long long list[ROOM], scratch[65];
   __shared__ float floats[32];
-  __shared__ int counts[32], listed;
+  __shared__ int counts[32], listed, counter;
   pdl_trigger();
   const int r = blockIdx.x / p.splits, split = blockIdx.x - r * p.splits, lane = threadIdx.x & 31;
   const int begin = split * p.chunk, end = min(begin + p.chunk, p.vocab);
@@ -208,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
     __syncthreads();
     const int count = listed;
     if (count <= ROOM) {
-      least = max(least, choose(list, count, p.top, scratch));
+      least = max(least, choose<ROOM>(list, count, p.top, scratch, &counter));
       if (threadIdx.x == 0) listed = min(count, p.top);
       __syncthreads();
       return;
@@ -226,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
       }
       __syncthreads();
       const int so_far = listed;
-      least = max(least, choose(list, so_far, p.top, scratch));
+      least = max(least, choose<ROOM>(list, so_far, p.top, scratch, &counter));
       if (threadIdx.x == 0) listed = min(so_far, p.top);
       __syncthreads();
     }
@@ -235,19 +277,31 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
   float bar = __int_as_float(0x7fc00000);        // the logit of `least`; NaN where anything may enter
   for (int first = begin, round = 1; first < end; first += ROUND, ++round) {
     if (first + ROUND < end) take<T, VECTOR>(x, first + ROUND, end, ahead);
-    float largest = v[0];
+    float quad[MINE / 4];                        // the largest of four
 #pragma unroll
-    for (int i = 1; i < MINE; ++i) largest = fmaxf(largest, v[i]);
+    for (int k = 0; k < MINE / 4; ++k) quad[k] = fmaxf(fmaxf(v[4 * k], v[4 * k + 1]), fmaxf(v[4 * k + 2], v[4 * k + 3]));
+    const float largest = fmaxf(fmaxf(quad[0], quad[1]), fmaxf(quad[2], quad[3]));
     if (largest > mine.m + 16.0f) mine.move(largest);
     float z = 0.0f, w = 0.0f;
+    if (fabsf(mine.m) < 64.0f) {                // m log2 e rounded once, 4e-6 off at most; w in units of ln 2
+      const float less = -mine.m * LOG2E;
 #pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const float d = v[i] - mine.m, e = exp2_fast(d * LOG2E);
-      z += e;
-      w = fmaf(e, fmaxf(d, -200.0f), w);        // -inf has no weight (and NaN shows in z)
+      for (int i = 0; i < MINE; ++i) {
+        const float d = fmaf(v[i], LOG2E, less), e = exp2_fast(d);
+        z += e;
+        w = fmaf(e, fmaxf(d, -200.0f), w);      // -inf has no weight (and NaN shows in z)
+      }
+      mine.w = fmaf(w, 0.6931471805599453f, mine.w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const float d = v[i] - mine.m, e = exp2_fast(d * LOG2E);
+        z += e;
+        w = fmaf(e, fmaxf(d, -200.0f), w);
+      }
+      mine.w += w;
     }
     mine.z += z;
-    mine.w += w;
     if (!token_is_nan && (token < first || token >= first + ROUND)) {
       const float from = first < token ? own : above;
 #pragma unroll
@@ -262,39 +316,29 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
     }
 
     if (p.top > 0) {
-      if (round == 1) {                          // the n-th of the half warps' largest keys: that many logits are no smaller
-        unsigned long long key = 0;
+      if (round == 1) {                          // the first of a thread's largest logits, of all that it has
+        int at = -1;
 #pragma unroll
-        for (int i = 0; i < MINE; ++i)
-          if (index_of(first, i) < end) key = max(key, key_of(v[i], index_of(first, i)));
-        key = warp_largest(key, 16);
-        if ((lane & 15) == 0) scratch[threadIdx.x >> 4] = key;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-          key = scratch[lane];
-          int in_front = 0;
-          for (int i = 0; i < 32; ++i) in_front += __shfl_sync(0xffffffffu, key, i) > key ? 1 : 0;
-          const unsigned nth = __ballot_sync(0xffffffffu, key != 0 && in_front == p.top - 1);
-          // keys of at least the n-th: those above its predecessor
-          if (lane == 0) scratch[32] = nth ? scratch[__ffs(nth) - 1] - 1 : 0ull;
-        }
-        __syncthreads();
-        least = scratch[32];
+        for (int i = MINE - 1; i >= 0; --i) at = v[i] == largest ? i : at;
+        const int index = index_of(first, max(at, 0));
+        least = bar_of(at >= 0 && index < end ? key_of(largest, index) : 0ull, p.top, scratch);
         bar = logit_of(least);
       }
       if (__any_sync(0xffffffffu, !(largest < bar))) {
-        uint32_t which = 0;
 #pragma unroll
-        for (int i = 0; i < MINE; ++i) which |= !(v[i] < bar) && index_of(first, i) < end && key_of(v[i], index_of(first, i)) > least ? 1u << i : 0u;
-        if (which != 0) {
-          int at = atomicAdd(&listed, __popc(which));
+        for (int k = 0; k < MINE / 4; ++k)
+          if (__any_sync(0xffffffffu, !(quad[k] < bar))) {
 #pragma unroll
-          for (int i = 0; i < MINE; ++i)
-            if (which >> i & 1) {
-              if (at < ROOM) list[at] = key_of(v[i], index_of(first, i));
-              ++at;
-            }
-        }
+            for (int i = 4 * k; i < 4 * k + 4; ++i)
+              if (!(v[i] < bar)) {
+                const int index = index_of(first, i);
+                const unsigned long long key = key_of(v[i], index);
+                if (index < end && key > least) {
+                  const int at = atomicAdd(&listed, 1);
+                  if (at < ROOM) list[at] = key;
+                }
+              }
+          }
       }
       if ((round & (round - 1)) == 0) {          // after rounds 1, 2, 4, 8, ...: the bar rises as the best get rarer
         settle(min(first + ROUND, end));
@@ -319,8 +363,8 @@ __global__ void __launch_bounds__(THREADS, 2) token_logprobs_kernel(const Logpro
 // The chunks of a row joined: their sums in order, and the best of their best.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const LogprobParams p) {
-  __shared__ unsigned long long list[ROOM], scratch[64];
-  __shared__ int listed;
+  __shared__ unsigned long long list[MOST_SPLITS * MOST_TOP], scratch[65];
+  __shared__ int listed, counter;
   pdl_trigger();
   const int r = blockIdx.x, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) listed = 0;
@@ -361,7 +405,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const Logp
     if (key != 0 && key >= least) list[atomicAdd(&listed, 1)] = key;
   }
   __syncthreads();
-  if (p.top > 0) choose(list, listed, p.top, scratch);
+  if (p.top > 0) choose<MOST_SPLITS * MOST_TOP>(list, listed, p.top, scratch, &counter);
   answer(p, r, all, own, known, list);
 }
 
@@ -369,7 +413,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const Logp
 // of all cuts the one that is done first, the fewest chunks among equals.
 int chunk_of(int rows, int vocab) {
   const int rounds = (vocab + ROUND - 1) / ROUND;
-  const long long at_once = 2ll * tge_sm_count();
+  const long long at_once = 4ll * tge_sm_count();
   long long best = 0;
   int chunk = vocab;
   for (int splits = 1; splits <= rounds && splits <= MOST_SPLITS; ++splits) {
