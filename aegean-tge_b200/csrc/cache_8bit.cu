@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 // turn, three rows on their way at a time, the angles loaded once.  With larger blocks the others have a (block of positions, key or value
 // head) each: its groups take the block's rows in turn, once for the scale and, from cache, once for the codes.
 // ---------------------------------------------------------------------------
-constexpr int UNIT_THREADS = 128, UNIT_AHEAD = 3;
+constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns
 
 struct Eight { float x[8]; };
 // Eight numbers as they lie in memory.
@@ -213,9 +213,10 @@ __device__ __forceinline__ void put_codes(int8_t* dst, const Coder& coder, const
 }
 
 template <typename T, int HEAD>
-__global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 6 : 5) store_8bit_units_kernel(const StoreParams p) {
-  constexpr int LANES = HEAD / 16, GROUPS = UNIT_THREADS / LANES, HALF = HEAD / 2;
-  __shared__ float scales[GROUPS];
+__global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_8bit_units_kernel(const StoreParams p) {
+  constexpr int LANES = HEAD / 16, HALF = HEAD / 2;
+  const int GROUPS = blockDim.x / LANES;
+  __shared__ float scales[UNIT_THREADS / LANES];
   __shared__ int found[2];
   pdl_trigger();
   const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
@@ -361,7 +362,6 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 6 : 5) store_8b
   if (j == 0) scales[group] = most;
   __syncthreads();
   most = before;
-#pragma unroll
   for (int i = 0; i < GROUPS; ++i) most = larger(most, scales[i]);
   const Coder coder(most);
   if (from > lo_pos && !(before >= most))                          // the scale grew: what the block held is rounded again
@@ -486,30 +486,44 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   }
   const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
   if constexpr (UNITS) {
-    // sixteen codes of a position to a thread and turn, all loads of a turn of keys and values on their way together
-    const int units = p.head_dim >> 4, shift = __ffs(p.block) - 1, blocks = p.page_size >> shift;
-    constexpr int AHEAD = 2;
-    for (int u0 = threadIdx.x; u0 < 64 * units; u0 += AHEAD * blockDim.x) {
-      uint4 raw[AHEAD][2];
+    // 16 bytes of the output to a thread and turn, side by side across a warp, four turns' codes of keys and values on their way together
+    // (head sizes and pages are powers of two here: a division per eight numbers would cost more than they do)
+    constexpr int EACH = 16 / sizeof(T), AHEAD = 4;
+    const int unit_shift = __ffs(p.head_dim / EACH) - 1, page_shift = __ffs(p.page_size) - 1, shift = __ffs(p.block) - 1;
+    const int part = threadIdx.x & ((1 << unit_shift) - 1), apart = blockDim.x >> unit_shift;      // positions between two of a thread's turns
+    for (int j0 = threadIdx.x >> unit_shift; j0 < 64; j0 += AHEAD * apart) {
+      uint32_t raw[AHEAD][2][EACH / 4];
       float scale[AHEAD][2];
       int at[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        const int u = u0 + i * blockDim.x, j = u / units, part = u - j * units, pos = tile * 64 + j;
-        at[i] = u < 64 * units ? j * p.head_dim + 16 * part : -1;
-        const int page_index = pos / p.page_size, slot = pos - page_index * p.page_size;
-        const bool held_here = at[i] >= 0 && pos < held;
+        const int j = j0 + i * apart, pos = tile * 64 + j;
+        at[i] = j < 64 ? j * p.head_dim + EACH * part : -1;
+        const int page_index = pos >> page_shift, slot = pos & (p.page_size - 1);
+        const bool held_here = j < 64 && pos < held;
         const int page = held_here && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
         const bool here = page >= 0 && page < p.num_pages;
         if (held_here && !here) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
-        raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
-        scale[i][0] = scale[i][1] = 0.0f;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          scale[i][kv] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < EACH / 4; ++k) raw[i][kv][k] = 0u;
+        }
         if (here) {
-          const size_t head = (size_t)page * p.kv_heads + kvh;
-          raw[i][0] = *reinterpret_cast<const uint4*>(p.k_pages + (head * p.page_size + slot) * p.head_dim + 16 * part);
-          raw[i][1] = *reinterpret_cast<const uint4*>(p.v_pages + (head * p.page_size + slot) * p.head_dim + 16 * part);
-          scale[i][0] = p.k_scale[head * blocks + (slot >> shift)];
-          scale[i][1] = p.v_scale[head * blocks + (slot >> shift)];
+          const size_t entry = ((size_t)(page * p.kv_heads + kvh) << page_shift) + slot, from = entry * p.head_dim + EACH * part;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int8_t* src = (kv ? p.v_pages : p.k_pages) + from;
+            if constexpr (EACH == 8) {
+              const uint2 x = *reinterpret_cast<const uint2*>(src);
+              raw[i][kv][0] = x.x;
+              raw[i][kv][1] = x.y;
+            } else {
+              raw[i][kv][0] = *reinterpret_cast<const uint32_t*>(src);
+            }
+            scale[i][kv] = (kv ? p.v_scale : p.k_scale)[entry >> shift];
+          }
         }
       }
 #pragma unroll
@@ -517,15 +531,14 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
         if (at[i] >= 0) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const float s = __fdiv_rn(scale[i][kv], 127.0f);
-            const uint32_t w[4] = {raw[i][kv].x, raw[i][kv].y, raw[i][kv].z, raw[i][kv].w};
-            Eight e[2];
+            const float s = scale[i][kv] * (1.0f / 127.0f);
+            float x[EACH];
 #pragma unroll
-            for (int k = 0; k < 16; ++k)       // 2^23 + (byte ^ 128), less 2^23 + 128: the code, exactly
-              e[k >> 3].x[k & 7] = (__uint_as_float(__byte_perm(w[k >> 2] ^ 0x80808080u, 0x4b000000u, 0x7440 + (k & 3))) - 8388736.0f) * s;
+            for (int k = 0; k < EACH; ++k)     // 2^23 + (byte ^ 128), less 2^23 + 128: the code, exactly
+              x[k] = (__uint_as_float(__byte_perm(raw[i][kv][k >> 2] ^ 0x80808080u, 0x4b000000u, 0x7440 + (k & 3))) - 8388736.0f) * s;
             T* dst = (kv ? v_dst : k_dst) + at[i];
-            put_eight(dst, e[0]);
-            put_eight(dst + 8, e[1]);
+            if constexpr (EACH == 8) put_eight(dst, Eight{{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]}});
+            else *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
           }
         }
     }
@@ -579,7 +592,9 @@ TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, v
       ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0) {
     auto run = [&](auto type) {
       using T = decltype(type);
-      auto launch = [&](void (*kernel)(StoreParams)) { tge_launch(kernel, dim3((unsigned)blocks), UNIT_THREADS, 0, stream, p); };
+      const int lanes = (heads + (block == 1 ? 2 * kv_heads : 0) + UNIT_AHEAD - 1) / UNIT_AHEAD * (head_dim / 16);
+      const int threads = std::min(UNIT_THREADS, std::max(64, (lanes + 31) / 32 * 32));
+      auto launch = [&](void (*kernel)(StoreParams)) { tge_launch(kernel, dim3((unsigned)blocks), threads, 0, stream, p); };
       switch (head_dim) {
         case 16: launch(store_8bit_units_kernel<T, 16>); break;
         case 32: launch(store_8bit_units_kernel<T, 32>); break;
@@ -616,7 +631,8 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   // a block takes several heads of its run where there are many runs: finding whose it is costs as much as a head
   const int at_once = 10 * tge_sm_count();
   const dim3 grid(runs + (planned ? 0 : 1), std::max(1, std::min(kv_heads, (at_once + runs) / (runs + 1))));
-  const bool units = head_dim % 16 == 0 && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
+  const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
+                     (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (is_bf16)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
