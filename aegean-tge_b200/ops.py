@@ -1211,6 +1211,16 @@ def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_p
 
 
 _decode_8bit_floats: Dict[tuple, int] = {}      # scratch numbers by sizes: asking the library costs a microsecond a call
+BESIDE_8BIT_FLOPS = 1e11                         # bound of the portions' work from which single tokens run beside them (some 130 us of it)
+_side_streams: Dict[int, "torch.cuda.Stream"] = {}
+
+
+def _side_stream() -> "torch.cuda.Stream":
+    """A stream of higher priority than the default, one per device."""
+    index = _current_device()
+    if index not in _side_streams:
+        _side_streams[index] = torch.cuda.Stream(device=index, priority=-1)
+    return _side_streams[index]
 
 
 def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -1246,40 +1256,68 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                           block_table.data_ptr(), block_table.shape[1])
     singles = num_seqs if max_q_len <= 1 else decode_prefix
-    done = 0                                            # requests, and so tokens, that are served
-    if singles:
+    if singles < num_seqs and ctx_lens is None:
+        ctx_lens = [max_ctx_len] * num_seqs
+
+    def single_tokens() -> int:
+        """Serves the requests that bring one token each, if the kernel takes their sizes; returns how many."""
         sizes = (is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
         need = _decode_8bit_floats.get(sizes)
         if need is None:
             if len(_decode_8bit_floats) >= 1024:
                 _decode_8bit_floats.clear()
             need = _decode_8bit_floats[sizes] = lib.tge_attention_8bit_decode_floats(*sizes)
-        if need >= 0:
-            parts = k_scale.new_empty(need)
-            rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
-                                               out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
-                                               parts.data_ptr(), need, status_word().data_ptr(), _stream())
-            if _check(rc, lib) != UNSUPPORTED:
-                done = singles
+        if need < 0:
+            return 0
+        parts = k_scale.new_empty(need)
+        rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
+                                           out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
+                                           parts.data_ptr(), need, status_word().data_ptr(), _stream())
+        return singles if _check(rc, lib) != UNSUPPORTED else 0
+
+    def portions(first: int, read=None) -> None:
+        """The requests from ``first`` on.  Their keys and values are read once into run-type pages of 64, which the prefill kernels take:
+        a query tile of those reads each of them again, so that turning codes into numbers there would be done many times over."""
+        starts = q_start.new_empty(num_seqs - first + 1)
+        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, first, starts)
+        if read is not None:
+            read.record()
+        rows = (q, start_pos, positions, seq_of_token, out)
+        if first:
+            rows = (q[first:], start_pos[first:], positions[first:], seq_of_token[first:], out[first:])
+        attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, max(ctx_lens[first:]), heads, kv_heads, head_dim, scale,
+                  window=window, out=rows[4], sink=sink)
+
+    as_portions = max_q_len > 1 and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
+                                     else head_dim in (16, 32, 64, 128) and sink is None)
+    if as_portions and MIN_DECODE_PREFIX <= singles < num_seqs and not torch.cuda.is_current_stream_capturing():
+        reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
+        if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
+            # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
+            # the read-back, on SMs that its last wave leaves.  63 of 2,048 beside 1,985 after 6,143 (40 heads over 8) 425 -> 377 us, 31 of 2,048
+            # beside 1,000 after 1,000 (28 over 4) 71 -> 61, 32 of 1,024 beside 2,016 (40 over 8) 107 -> 104; small steps wait for the host,
+            # whom the second stream costs 12 us.
+            main, side = torch.cuda.current_stream(), _side_stream()
+            read = torch.cuda.Event()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                portions(singles, read)
+            main.wait_event(read)
+            served = single_tokens()
+            main.wait_stream(side)
+            if served == singles:
+                return out
+            as_portions = False          # (sizes that the single tokens' kernel does not take: all go the simple way below)
+    done = single_tokens() if singles else 0            # requests, and so tokens, that are served
     if done == num_seqs:
         return out
-    ctx_lens = [max_ctx_len] * num_seqs if ctx_lens is None else ctx_lens
-    rest = (q, out, start_pos, positions, seq_of_token)
-    if done:
-        rest = (q[done:], out[done:], start_pos[done:], positions[done:], seq_of_token[done:])
-    rows, rows_out, rest_pos, rest_positions, rest_seq = rest
-    if max_q_len > 1 and done == singles and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
-                                              else head_dim in (16, 32, 64, 128) and sink is None):
-        # portions: their keys and values are read once into run-type pages of 64, which the prefill kernels take; a query tile of
-        # those reads each of them again, so that turning codes into numbers there would be done many times over
-        starts = q_start.new_empty(num_seqs - done + 1)
-        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, done, starts)
-        attention(rows, k, v, table, starts, rest_pos, rest_positions, rest_seq, num_seqs - done, max_q_len, max(ctx_lens[done:]), heads, kv_heads,
-                  head_dim, scale, window=window, out=rows_out, sink=sink)
+    if as_portions and done == singles:
+        portions(done)
         return out
-    _check(lib.tge_attention_8bit_simple(rows.data_ptr(), is_bf16, q_stride, *cache, rest_positions.data_ptr(), rest_seq.data_ptr(),
-                                         num_seqs, tokens - done, rows_out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale),
-                                         int(window), _ptr(sink), status_word().data_ptr(), _stream()), lib)
+    rows = (q, out, positions, seq_of_token) if done == 0 else (q[done:], out[done:], positions[done:], seq_of_token[done:])
+    _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
+                                         tokens - done, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
+                                         _ptr(sink), status_word().data_ptr(), _stream()), lib)
     return out
 
 

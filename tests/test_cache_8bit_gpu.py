@@ -432,3 +432,25 @@ def test_refusals(ops):
     with pytest.raises(ops.KernelError):
         attention(q=torch.zeros(1, 4 * 320, device=DEV), kp=wide[0], vp=wide[0], ks=wide[1], vs=wide[1], dim=320)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 32)])
+def test_side_by_side_is_the_same(ops, monkeypatch, dtype, heads, kv, dim):
+    """Single tokens beside portions on two streams: the bits of one, from any stream, time and again; head sizes that only the portions'
+    kernels take as well."""
+    held = [1, 5, 64, 65, 200, 17, 128, 90, 400, 33, 300, 270]
+    lens = [1] * 10 + [200, 64]
+    cache = Cache(held, kv, dim, 16, 1)
+    want, _ = attend(ops, cache, lens, heads, dtype, decode_prefix=10, ctx_lens=held)
+    monkeypatch.setattr(ops, "BESIDE_8BIT_FLOPS", 0.0)
+    for _ in range(4):
+        got, _ = attend(ops, cache, lens, heads, dtype, decode_prefix=10, ctx_lens=held)
+        assert torch.equal(got, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, _ = attend(ops, cache, lens, heads, dtype, decode_prefix=10, ctx_lens=held)
+    side.synchronize()
+    if dim == 128:
+        assert torch.equal(got, want)
