@@ -163,14 +163,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Codes of bytes `which` of two words as two float16, plus 1,152.
+// Codes of bytes `which` of two words as two float16.
 __device__ __forceinline__ uint32_t two_codes(uint32_t a, uint32_t b, uint32_t which) {
-  const uint32_t r = __byte_perm(a, b, which);
-  uint32_t v;
+  uint32_t r = __byte_perm(a, b, which), v;
   asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;\n" : "=r"(v) : "r"(r));       // (r & mask) ^ pattern: 1,024 + (byte ^ 128)
-  return v;
+  asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0xe480e480u));            // - 1,152
+  return r;
 }
-constexpr uint32_t LESS = 0xe480e480u;          // -1,152, twice
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -553,11 +552,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int part = 0; part < PARTS; ++part) {
-                // 1,152 + c and, in the same breath, 1,152 less: no more than the slice's own sum is ever off by the rounding of that much
-                mma_f16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
-                mma_f16(o[nt][i], LESS, LESS, LESS, LESS, pr[nt][part][0], pr[nt][part][1]);
-              }
+              for (int part = 0; part < PARTS; ++part) mma_f16(o[nt][i], a0, a1, a2, a3, pr[nt][part][0], pr[nt][part][1]);
           }
       if (slice + 1 < last) load_values<HD>(p, c, row, g, t);
     }
