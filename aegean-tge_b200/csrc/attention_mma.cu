@@ -86,6 +86,7 @@ struct AttnParams {
   int trigger_late, beside;
   unsigned long long ticket;
   float scale_log2;
+  const int* page_exponents;      // the two-tile prefill kernel over float16 pages: of every page and kv head, f below and e above
 };
 
 // Tickets of side-by-side launches: a number of its own for every such pair of launches, in the place that it falls on.  The first
@@ -1275,8 +1276,8 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// The tensor map of a page pool, made once per (address, geometry) and kept.
-const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int page_size) {
+// The tensor map of a page pool, made once per (address, geometry) and kept; with `into`, for pages of one call, made there and not kept.
+const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int page_size, CUtensorMap* into = nullptr) {
   static EncodeTiledFn encode = nullptr;
   static bool tried = false;
   static std::map<std::tuple<const void*, int, int, int>, CUtensorMap> maps;
@@ -1294,7 +1295,7 @@ const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int 
   }
   const auto key = std::make_tuple(pages, num_pages, kv_heads, page_size);
   auto found = maps.find(key);
-  if (found != maps.end()) return &found->second;
+  if (into == nullptr && found != maps.end()) return &found->second;
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)num_pages * kv_heads * page_size};
   cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
@@ -1306,6 +1307,10 @@ const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int 
   if (rc != CUDA_SUCCESS) {
     tge_set_error("attention_decode: cuTensorMapEncodeTiled failed with code %d", (int)rc);
     return nullptr;
+  }
+  if (into != nullptr) {
+    *into = map;
+    return into;
   }
   return &maps.emplace(key, map).first->second;
 }
@@ -1487,7 +1492,8 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
                               int kv_heads, float scale, int window, int split_tokens, float* scratch, int* status,
                               int first_token, const float* sink, int leave_states, int v_pitch, const float* dist_bias,
                               int dist_span, int keep_first, const void* gate, int gate_stride, int gate_elements,
-                              int shared_keys, cudaStream_t stream, LeadingTokens* lead = nullptr, unsigned long long beside = 0) {
+                              int shared_keys, cudaStream_t stream, LeadingTokens* lead = nullptr, unsigned long long beside = 0,
+                              const int* page_exponents = nullptr) {
   TGE_REQUIRE(tokens >= 0 && num_seqs >= 0, "attention_mma: negative sizes");
   TGE_REQUIRE(dist_bias == nullptr || (dist_span > 0 && scale != 0.0f), "attention_mma: a bias by distance needs its span");
   TGE_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
@@ -1524,6 +1530,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
   TGE_REQUIRE(!shared_keys || (single && p.v_in_keys), "attention_mma: runs of heads over the same keys are for single tokens and values inside the keys");
   p.kv_pool = shared_keys ? 1 : kv_heads;
   p.trigger_late = 0;
+  p.page_exponents = page_exponents;
   p.beside = beside != 0;
   p.ticket = beside;
   p.q_stride = q_stride; p.out_stride = out_stride;
@@ -1628,6 +1635,32 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
     return 1;
   }
 #if TGE_TMA_KERNELS
+  if (page_exponents != nullptr) {
+    // float16 pages with exponents: pages of one call, the two-tile kernel, two query tiles per block and one block per SM
+    p.bq = tc2::ROWS / group;
+    const int range = (num_splits > 1 ? p.split_tokens : max_ctx_len) + 2 * BKV;
+    const size_t smem = tc2::smem_bytes(range / BKV, true);
+    if (!tc2::FITS || page_size != BKV || smem > tc2::MOST_SMEM || q_stride % 8 != 0 || (uintptr_t)q % 16 != 0 || out_stride % 8 != 0 ||
+        (uintptr_t)out % 16 != 0)
+      return TGE_UNSUPPORTED;
+    CUtensorMap map_k, map_v;
+    if (!pool_map(k_pages, num_pages, kv_heads, page_size, &map_k) || !pool_map(v_pages, num_pages, kv_heads, page_size, &map_v)) return -3;
+    static std::atomic<size_t> configured{0};
+    if (smem > configured) {
+      const cudaError_t err = cudaFuncSetAttribute(tc2::attention_prefill_tc2_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc2::MOST_SMEM);
+      TGE_REQUIRE(err == cudaSuccess, "attention_prefill_tc2: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(err));
+      configured = tc2::MOST_SMEM;
+    }
+    const int pairs = ((tokens - first_token + p.bq - 1) / p.bq + 1) / 2 + num_seqs;
+    tge_launch(tc2::attention_prefill_tc2_kernel<true>, dim3(pairs * kv_heads, 1, num_splits), tc2::THREADS, smem, stream, map_k, map_v, p);
+    const int rc = tge_check_launch("attention_prefill_tc2");
+    if (rc != 0) return rc;
+    if (num_splits > 1) {
+      launch_merge(p, positions, first_token, stream);
+      return tge_launched("attention_merge", 2);
+    }
+    return 1;
+  }
   if (max_q_len > 1 && group <= 64 && page_size >= 8) {
     const CUtensorMap* map_k = pool_map(k_pages, num_pages, kv_heads, page_size);
     const CUtensorMap* map_v = pool_map(v_pages, num_pages, kv_heads, page_size);
@@ -1645,7 +1678,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
         const size_t smem2 = tc2::smem_bytes(range >> p.page_shift);
         static size_t configured_tc2 = 0;
         if (smem2 > configured_tc2) {
-          cudaError_t err = cudaFuncSetAttribute(tc2::attention_prefill_tc2_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem2);
+          cudaError_t err = cudaFuncSetAttribute(tc2::attention_prefill_tc2_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem2);
           if (err != cudaSuccess) {
             tge_set_error("attention_prefill_tc2: cannot reserve %zu bytes of shared memory: %s", smem2, cudaGetErrorString(err));
             return -2;
@@ -1654,7 +1687,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
         }
         const int pairs = ((tokens - first_token + p.bq - 1) / p.bq + 1) / 2 + num_seqs;
         dim3 grid2(pairs * kv_heads, 1, num_splits);
-        tge_launch(tc2::attention_prefill_tc2_kernel, grid2, tc2::THREADS, smem2, stream, *map_k, *map_v, p);
+        tge_launch(tc2::attention_prefill_tc2_kernel<false>, grid2, tc2::THREADS, smem2, stream, *map_k, *map_v, p);
         int rc2 = tge_check_launch("attention_prefill_tc2");
         if (rc2 != 0) return rc2;
         if (num_splits > 1 && !p.leave_states) {
@@ -1734,6 +1767,33 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
     return tge_launched("attention_merge", 2);
   }
   return 1;
+}
+
+// Portions over float16 pages of 64 positions whose keys and values are over 2^e and 2^f of their page and kv head, whole numbers of -120 to 120 in
+// `page_exponents` ([num_pages, kv_heads], f in the lower 16 bits and e in the upper).  Whether this library's kernel takes
+// portions whose longest context is `max_ctx_len`:
+TGE_API int tge_attention_mma_halves_fit(int max_ctx_len, int split_tokens) {
+#if TGE_TMA_KERNELS
+  const int range = (split_tokens > 0 && split_tokens < max_ctx_len ? split_tokens : max_ctx_len) + 2 * BKV;
+  return tc2::FITS && tc2::smem_bytes(range / BKV, true) <= tc2::MOST_SMEM;
+#else
+  return 0;
+#endif
+}
+
+TGE_API int tge_attention_mma_halves(const void* q, int q_stride, const void* k_pages, const void* v_pages, const int* page_exponents,
+                                      const int* block_table, int max_pages, int num_pages, const int* q_start,
+                                      const int* start_pos, const int* positions, int num_seqs, int tokens, int max_q_len, int max_ctx_len,
+                                      void* out, int out_stride, int heads, int kv_heads, float scale, int window, int split_tokens,
+                                      float* scratch, int* status, const float* sink, cudaStream_t stream) {
+  TGE_REQUIRE(page_exponents != nullptr && max_q_len > 1 && scale > 0.0f, "attention_mma: float16 pages are for portions and positive scales");
+#if TGE_TMA_KERNELS
+  return attention_dispatch(q, q_stride, k_pages, v_pages, block_table, max_pages, num_pages, BKV, q_start, start_pos, positions, num_seqs, tokens,
+                            max_q_len, max_ctx_len, out, out_stride, heads, kv_heads, scale, window, split_tokens, scratch, status, 0, sink, 0, 0,
+                            nullptr, 0, 0, nullptr, 0, 0, 0, stream, nullptr, 0, page_exponents);
+#else
+  return TGE_UNSUPPORTED;
+#endif
 }
 
 // `leave_states`: the keys are cut into at least two runs and the runs' unnormalised states (sums, maxima in base-2

@@ -14,6 +14,17 @@
 //     tokens, a third one nothing), one warp issuing copies; three stages of K and V; P in buffers of its own.
 // While the tensor core adds one tile's P V, the other tile's softmax runs.
 // Masking, splits along the keys, the rescaling threshold and the output layout are those of attention_tc.cuh.
+//
+// HALVES: keys and values of a cache of 8-bit codes, read back into float16 pages of 64 positions.  float16 holds them, and the probabilities,
+// to 2^-12 where bfloat16 rounds them to 2^-9: a prompt of 2,048 tokens at 28 heads over 4 comes to 1.7e-3 of float64, which is the rounding
+// of the result, and to 3.7e-3 with everything in bfloat16, for 64 us beside 60.  (Whole codes in bfloat16 with a factor per key on the
+// scores: 2.7e-3, 64 us; with a factor per value on the probabilities too: 2.3e-3, 71 us.)
+// float16's range is short, so a page's keys and values are held over powers of two 2^e and 2^f of that page and kv head ((f, e) in
+// `page_exponents`), no larger than 1, and a row of queries over one of its own.  2^e joins the scale of the tile's scores; e and f are
+// multiples of 8, so that few tiles bring new ones and a tile like the last costs a row a comparison and two products.  (Exponents that
+// change by one from tile to tile, and loads of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at
+// most 2^15: the reference moves at 2^8), and the accumulator follows where f changes; they keep 11 bits down to 2^-21 of a probability of
+// 1 and some down to 2^-31.
 #pragma once
 
 namespace tc2 {
@@ -40,11 +51,22 @@ constexpr int TMEM_COLS = 512;
 constexpr bool FITS = 2 * QTILES * BKV + QTILES * HD <= TMEM_COLS;
 constexpr int BARRIER_BYTES = 256;
 
-constexpr size_t smem_bytes(int table_entries) {
+constexpr float HELD = 7.0f;                       // probabilities are held times 2^7
+constexpr size_t MOST_SMEM = 227 * 1024 - 64;      // of one block, beside its few static bytes
+
+constexpr size_t smem_bytes(int table_entries, bool halves = false) {
   return 1024 + (size_t)QTILES * (Q_BYTES + P_BYTES) + (size_t)STAGES * TMA_STAGE_BYTES + BARRIER_BYTES +
-         ((size_t)table_entries + 2) * sizeof(int);
+         ((size_t)table_entries + 2) * (halves ? 2 : 1) * sizeof(int);
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 to 127
+
+template <bool HALVES>
 __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
   extern __shared__ unsigned char smem_dyn[];
@@ -64,6 +86,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
   const uint32_t o_bar = p_bar + 8 * QTILES;              // [query tile]
   const uint32_t free_bar = o_bar + 8 * QTILES;           // [query tile][score buffer]: the softmax has read the scores
   int* local_table = reinterpret_cast<int*>(generic + (stages - base) + STAGES * TMA_STAGE_BYTES + BARRIER_BYTES);
+  [[maybe_unused]] int* local_exponents;                  // behind it, as many
 
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index();
   const int kvh = (int)blockIdx.x % p.kv_heads, pair_rank = (int)blockIdx.x / p.kv_heads, split = blockIdx.z;
@@ -95,6 +118,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
   const int num_tiles = keys.num_tiles;
   const int first_page = keys.start(0) >> p.page_shift;
   const int last_page = (keys.start(num_tiles - 1) + BKV - 1) >> p.page_shift;
+  local_exponents = local_table + (last_page - first_page + 1);
   for (int i = first_page + tid; i <= last_page; i += THREADS) {
     int page = i < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + i] : -1;
     if (page >= p.num_pages) page = -2;
@@ -184,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     // two phases behind cannot tell them apart by parity).
     asm volatile("bar.sync 1, %0;\n" ::"n"((SOFTMAX_WARPS + 1) * 32) : "memory");          // the queries are there
     if (elect_one()) {
-      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+      const uint32_t idesc_s = (1u << 4) | (HALVES ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       for (int tile = 0; tile < num_tiles; ++tile) {
         const int stage = tile % STAGES;
         mbar_wait_bounded(k_bar + 8 * stage, (uint32_t)(tile / STAGES) & 1u, p.status);
@@ -208,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
   } else if (warp == MMA_WARP) {
     // ------------------------------- P V products -------------------------------
     if (elect_one()) {
-      const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+      const uint32_t idesc_o = (1u << 4) | (HALVES ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       for (int it = 0; it < num_tiles; ++it) {
         const int stage = it % STAGES;
         const uint64_t v_desc = desc_mn_major(stages + stage * TMA_STAGE_BYTES + TMA_TILE_BYTES, BKV * 128);
@@ -233,11 +257,36 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     // Q row into the K-major swizzled tile of its query tile: 64-column blocks of [128 rows][128 bytes]
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)row_token * p.q_stride + (size_t)row_head * HD);
     unsigned char* q_tile = generic + qt * Q_BYTES;
+    float row_scale = p.scale_log2;                      // what the row's scores are multiplied with (2^e of their tile apart)
+    if constexpr (HALVES) {
+      for (int i = tid; i <= last_page - first_page; i += SOFTMAX_WARPS * 32) {      // (e, f) of the tiles, behind the barrier of the queries
+        const int page = max(local_table[i], 0);
+        local_exponents[i] = p.page_exponents[(size_t)page * p.kv_heads + kvh];
+      }
+      // over a power of two above the row's largest number (NaN and infinities stay what they are)
+      uint4 row[HD / 8];
+      float most = 0.0f;
 #pragma unroll
-    for (int c = 0; c < HD / 8; ++c) {
-      const uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
-      const int block = c >> 3, chunk = c & 7;
-      *reinterpret_cast<uint4*>(q_tile + block * (ROWS * 128) + r * 128 + ((chunk ^ (r & 7)) << 4)) = v;
+      for (int c = 0; c < HD / 8; ++c) row[c] = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        for (uint32_t w : {row[c].x, row[c].y, row[c].z, row[c].w})
+          most = tc::max3(most, fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u)));
+      const int up = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 120) : 0;
+      const float over = power_of_two(-up);
+      row_scale *= power_of_two(up);
+      auto halves = [&](uint32_t w) { return pack_f16(__uint_as_float(w << 16) * over, __uint_as_float(w & 0xffff0000u) * over); };
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(halves(row[c].x), halves(row[c].y), halves(row[c].z), halves(row[c].w));
+    } else {
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
+        const int block = c >> 3, chunk = c & 7;
+        *reinterpret_cast<uint4*>(q_tile + block * (ROWS * 128) + r * 128 + ((chunk ^ (r & 7)) << 4)) = v;
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");     // the queries, before the tensor core reads them
     asm volatile("bar.sync 1, %0;\n" ::"n"((SOFTMAX_WARPS + 1) * 32) : "memory");
@@ -247,10 +296,34 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     const uint32_t my_o = o_tmem(qt);
     const uint32_t p_row = p_smem + qt * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.0f;            // m_run: the row's reference, in raw score units
-    const float step_raw = tc::RESCALE_STEP / p.scale_log2;
+    const float step = HALVES ? tc::RESCALE_STEP : tc::RESCALE_STEP / row_scale;
+    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), f - F + 7, 2 to its negative.
+    // The row's reference is in units of the exponentials there.
+    [[maybe_unused]] int now = -1;
+    [[maybe_unused]] float held = 0.0f, more = 0.0f, less = 1.0f;
+    float scale_now = row_scale;
     bool bad_page = false;
     for (int it = 0; it < num_tiles; ++it) {
       const int k0 = keys.start(it);
+      float again = 1.0f;                              // what the accumulator takes as F moves
+      if constexpr (HALVES) {
+        const int both = local_exponents[(k0 >> p.page_shift) - first_page];
+        if (both != now) {
+          now = both;
+          scale_now = row_scale * power_of_two(both >> 16);
+          const float f = (float)(short)both;
+          if (m_run == -INFINITY) {
+            held = f;                                       // nothing seen, nothing in the accumulator
+          } else if (f != held) {
+            // (down by no more than 80 at a time: the accumulator's numbers stay far from float32's largest)
+            const float to = fmaxf(f, held - 80.0f);
+            again = power_of_two(max((int)(held - to), -126));
+            held = to;
+          }
+          more = fmaxf(f - held + HELD, -60.0f);        // (float16 has nothing left there)
+          less = power_of_two((int)-more);
+        }
+      }
       mbar_wait_bounded(my_s_bar + 8 * (it & 1), (uint32_t)(it >> 1) & 1u, p.status);
       fence_after();
       if (local_table[(keys.probe(k0) >> p.page_shift) - first_page] < 0) bad_page = true;
@@ -294,12 +367,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
           mx = fmaxf(mx, sv);
         }
       }
-      const bool moved = mx > m_run + step_raw || m_run == -INFINITY;
+      if constexpr (HALVES) mx *= scale_now;
+      const bool moved = mx > m_run + step || m_run == -INFINITY;
       const float m_new = moved ? mx : m_run;
       const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-      const float corr = exp2f((m_run - m_use) * p.scale_log2);            // exp2(-inf) = 0 while nothing was visible yet
-      const float shift = -m_use * p.scale_log2;
-      const uint64_t scale2 = tc::pair(p.scale_log2, p.scale_log2), shift2 = tc::pair(shift, shift);
+      const float corr = exp2f(HALVES ? m_run - m_use : (m_run - m_use) * row_scale);      // exp2(-inf) = 0 while nothing was visible yet
+      const float shift = HALVES ? more - m_use : -m_use * row_scale;
+      const uint64_t scale2 = tc::pair(scale_now, scale_now), shift2 = tc::pair(shift, shift);
       uint64_t sum2 = tc::pair(0.0f, 0.0f);
       if (it > 0) {
         // P has one buffer per query tile, and the accumulator may be rescaled below: the previous tile's
@@ -319,17 +393,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
           sum2 = tc::add2(sum2, tc::pair(pv[e], pv[e + 1]));
         }
         const uint32_t dst = p_row + ((c ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(pack_bf16(pv[0], pv[1])),
-                     "r"(pack_bf16(pv[2], pv[3])), "r"(pack_bf16(pv[4], pv[5])), "r"(pack_bf16(pv[6], pv[7])) : "memory");
+        auto packed = [](float lo, float hi) { return HALVES ? pack_f16(lo, hi) : pack_bf16(lo, hi); };
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(packed(pv[0], pv[1])),
+                     "r"(packed(pv[2], pv[3])), "r"(packed(pv[4], pv[5])), "r"(packed(pv[6], pv[7])) : "memory");
       }
       float sum_even, sum_odd;
       tc::unpair(sum2, sum_even, sum_odd);
-      l_run = l_run * corr + (sum_even + sum_odd);
-      const bool rescale = it > 0 && moved && m_run != -INFINITY;
+      l_run = l_run * corr + (HALVES ? (sum_even + sum_odd) * less : sum_even + sum_odd);
+      const bool rescale = it > 0 && ((moved && m_run != -INFINITY) || (HALVES && again != 1.0f));
       m_run = m_new;
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // P, before the tensor core reads it
       if (it > 0 && __any_sync(0xffffffffu, rescale)) {
-        const float factor = rescale ? corr : 1.0f;
+        const float factor = HALVES ? corr * again : rescale ? corr : 1.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o_bits[32];
@@ -348,8 +423,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     mbar_wait_bounded(my_o_bar, (uint32_t)(num_tiles - 1) & 1u, p.status);
     fence_after();
     // the running maximum is kept in the scores' own units here; the sink joins in scaled base-2 units
-    const float l_all = p.num_splits == 1 ? with_sink(p, row_head, m_run == -INFINITY ? -INFINITY : m_run * p.scale_log2, l_run) : l_run;
-    const float inv = (p.num_splits == 1) ? (l_all > 0.0f ? 1.0f / l_all : 0.0f) * head_gate(p, row_token, row_head) : 1.0f;
+    const float l_all = p.num_splits == 1 ? with_sink(p, row_head, HALVES || m_run == -INFINITY ? m_run : m_run * row_scale, l_run) : l_run;
+    const float unheld = HALVES ? exp2f(held - HELD) : 1.0f;
+    const float inv = (p.num_splits == 1) ? (HALVES ? l_all != 0.0f : l_all > 0.0f) ? unheld / l_all * head_gate(p, row_token, row_head) : 0.0f : unheld;
     const size_t slot = ((size_t)split * p.total_tokens + row_token) * p.heads + row_head;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
@@ -379,12 +455,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
         float4* dst = reinterpret_cast<float4*>(p.partial_o + slot * HD + c * 32);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          dst[e] = make_float4(__uint_as_float(o_bits[e * 4]), __uint_as_float(o_bits[e * 4 + 1]),
-                               __uint_as_float(o_bits[e * 4 + 2]), __uint_as_float(o_bits[e * 4 + 3]));
+          dst[e] = make_float4(__uint_as_float(o_bits[e * 4]) * inv, __uint_as_float(o_bits[e * 4 + 1]) * inv,
+                               __uint_as_float(o_bits[e * 4 + 2]) * inv, __uint_as_float(o_bits[e * 4 + 3]) * inv);
       }
     }
     if (row_valid && p.num_splits > 1) {
-      p.partial_ml[slot * 2] = m_run == -INFINITY ? -INFINITY : m_run * p.scale_log2;   // merged in scaled base-2 units
+      p.partial_ml[slot * 2] = HALVES || m_run == -INFINITY ? m_run : m_run * row_scale;      // merged in scaled base-2 units
       p.partial_ml[slot * 2 + 1] = l_run;
     }
   }

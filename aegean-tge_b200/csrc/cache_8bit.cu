@@ -12,9 +12,15 @@
 //   lo' = lo cos - hi sin ; hi' = lo sin + hi cos
 // keys are quantised from these float32 numbers, with no rounding to the run's type in between.  127 x is exact for a bfloat16 x and
 // the division is rounded once, so x = s (k + 1/2) / 127 meets its tie exactly and goes to even wherever it is computed.
+#include <cuda_fp16.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
+
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
 namespace {
 
@@ -183,6 +189,13 @@ __device__ __forceinline__ void put_eight(__nv_bfloat16* dst, const Eight& e) {
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(e.x[2 * i], e.x[2 * i + 1]);
+  *reinterpret_cast<uint4*>(dst) = raw;
+}
+__device__ __forceinline__ void put_eight(__half* dst, const Eight& e) {
+  uint4 raw;
+  __half2* h = reinterpret_cast<__half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(e.x[2 * i], e.x[2 * i + 1]);
   *reinterpret_cast<uint4*>(dst) = raw;
 }
 __device__ __forceinline__ void put_eight(float* dst, const Eight& e) {
@@ -396,7 +409,9 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_8b
 // ---------------------------------------------------------------------------
 // Entries read back: the positions that a step's queries may see, request after request, in runs of 64 positions
 // [runs, kv_heads, 64, head_dim] (zeros behind a request's last), a block table over those runs and (starts, if wanted) the requests'
-// first tokens counted from the first one's.
+// first tokens counted from the first one's.  In float16 with a power of two for each run and head, for the attention kernel that takes these.
+// For attention (starts are wanted): it multiplies every value of a tile with a probability, unseen ones with zero, so values are finite there:
+// a position whose values' scale is not gets a key that is not, which whoever sees it turns into the same and nobody else looks at.
 // ---------------------------------------------------------------------------
 struct ReadParams {
   const int8_t *k_pages, *v_pages;
@@ -404,6 +419,7 @@ struct ReadParams {
   const int *block_table, *q_start, *start_pos;
   int max_pages, num_pages, page_size, block, first_seq, num_seqs, kv_heads, head_dim, window;
   void *k_out, *v_out;
+  int* exponents;                              // [runs, kv_heads], for float16 output: f below, e above
   int *table, *starts;
   int runs, width;
   int* status;
@@ -442,9 +458,18 @@ __global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p)
   plan_runs(p);
 }
 
+// float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ,
+// and what is lost is nothing (the largest numbers of a run are above 2^-9, float16 keeps its 11 bits down to 2^-14).
+__device__ __forceinline__ int exponent_above(float s) {      // of such a power that is no smaller than s > 0
+  return min(max(((int)(__float_as_uint(s) >> 23) - 126 + 7) & ~7, -120), 120);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
+  constexpr bool HALVES = std::is_same<T, __half>::value;
   __shared__ int found[2];
+  __shared__ float most[2][2];                 // float16: the largest scales of the run's first and second 32 positions, keys' and values'
   const int run = blockIdx.x;
   pdl_wait();
   pdl_trigger();                               // behind the wait: see the kernel above
@@ -482,6 +507,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   T* v_dst = static_cast<T*>(p.v_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
   if (seq < 0) {                               // the caller counted more runs than there are
     for (int i = threadIdx.x; i < 64 * p.head_dim; i += blockDim.x) k_dst[i] = v_dst[i] = from_float<T>(0.0f);
+    if (HALVES && threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = 0;
     continue;
   }
   const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
@@ -490,6 +516,28 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
     // (head sizes and pages are powers of two here: a division per eight numbers would cost more than they do)
     constexpr int EACH = 16 / sizeof(T), AHEAD = 4;
     const int unit_shift = __ffs(p.head_dim / EACH) - 1, page_shift = __ffs(p.page_size) - 1, shift = __ffs(p.block) - 1;
+    [[maybe_unused]] float k_over = 1.0f, v_over = 1.0f;
+    if constexpr (HALVES) {
+      __syncthreads();                         // whoever still reads those of the head before
+      if (threadIdx.x < 64) {
+        const int pos = tile * 64 + threadIdx.x, page_index = pos >> page_shift;
+        const int page = pos < held && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
+        const bool here = page >= 0 && page < p.num_pages;
+        const size_t block = ((((size_t)(page * p.kv_heads + kvh) << page_shift) + (pos & (p.page_size - 1))) >> shift);
+        const float ks = here ? fabsf(p.k_scale[block]) : 0.0f, vs = here ? fabsf(p.v_scale[block]) : 0.0f;
+        const float k = warp_max(ks < INFINITY ? ks : 0.0f), v = warp_max(vs < INFINITY ? vs : 0.0f);
+        if ((threadIdx.x & 31) == 0) {
+          most[threadIdx.x >> 5][0] = k;
+          most[threadIdx.x >> 5][1] = v;
+        }
+      }
+      __syncthreads();
+      const float k = fmaxf(most[0][0], most[1][0]), v = fmaxf(most[0][1], most[1][1]);
+      const int e = k > 0.0f ? exponent_above(k) : 0, f = v > 0.0f ? exponent_above(v) : 0;
+      k_over = power_of_two(-e);
+      v_over = power_of_two(-f);
+      if (threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = (int)((uint32_t)e << 16 | ((uint32_t)f & 0xffffu));
+    }
     const int part = threadIdx.x & ((1 << unit_shift) - 1), apart = blockDim.x >> unit_shift;      // positions between two of a thread's turns
     for (int j0 = threadIdx.x >> unit_shift; j0 < 64; j0 += AHEAD * apart) {
       uint32_t raw[AHEAD][2][EACH / 4];
@@ -531,7 +579,9 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
         if (at[i] >= 0) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const float s = scale[i][kv] * (1.0f / 127.0f);
+            float s = scale[i][kv] * (1.0f / 127.0f);
+            if constexpr (HALVES) s *= kv == 0 ? k_over : v_over;
+            if (!(fabsf(scale[i][1]) < INFINITY) && p.starts != nullptr) s = kv == 0 ? NAN : 0.0f;
             float x[EACH];
 #pragma unroll
             for (int k = 0; k < EACH; ++k)     // 2^23 + (byte ^ 128), less 2^23 + 128: the code, exactly
@@ -552,8 +602,12 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
     const bool here = page >= 0 && page < p.num_pages;
     if (!here && pos < held && lane == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
     const size_t entry = here ? ((size_t)page * p.kv_heads + kvh) * p.page_size + pos % p.page_size : 0;
-    const float ks = here ? __fdiv_rn(p.k_scale[entry / p.block], 127.0f) : 0.0f;
-    const float vs = here ? __fdiv_rn(p.v_scale[entry / p.block], 127.0f) : 0.0f;
+    float ks = here ? p.k_scale[entry / p.block] * (1.0f / 127.0f) : 0.0f;
+    float vs = here ? p.v_scale[entry / p.block] * (1.0f / 127.0f) : 0.0f;
+    if (!(fabsf(vs) < INFINITY) && p.starts != nullptr) {
+      ks = NAN;
+      vs = 0.0f;
+    }
     for (int d = lane; d < p.head_dim; d += 32) {
       k_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.k_pages[entry * p.head_dim + d] * ks : 0.0f);
       v_dst[j * p.head_dim + d] = from_float<T>(here ? (float)p.v_pages[entry * p.head_dim + d] * vs : 0.0f);
@@ -617,23 +671,26 @@ TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, v
 
 TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int num_pages, int page_size,
                           int block, const int* block_table, int max_pages, const int* q_start, const int* start_pos, int first_seq,
-                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int is_bf16, int* table, int* starts, int runs,
-                          int width, int* status, cudaStream_t stream) {
+                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int type, int* exponents, int* table,
+                          int* starts, int runs, int width, int* status, cudaStream_t stream) {
   const int rc = cache_shape("read_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
   if (rc != 0) return rc;
   TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
   if (num_seqs == first_seq || width == 0) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
-                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, table, starts, runs, width, status};
+                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, exponents, table, starts, runs, width, status};
+  const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
+                     (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
+  if (type == 2 && (!units || exponents == nullptr)) return TGE_UNSUPPORTED;
   const bool planned = starts != nullptr;
   if (planned) tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
   if (planned && runs == 0) return tge_launched("read_8bit", 1);
   // a block takes several heads of its run where there are many runs: finding whose it is costs as much as a head
   const int at_once = 10 * tge_sm_count();
   const dim3 grid(runs + (planned ? 0 : 1), std::max(1, std::min(kv_heads, (at_once + runs) / (runs + 1))));
-  const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
-                     (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
-  if (is_bf16)
+  if (type == 2)
+    tge_launch(read_8bit_kernel<__half, true>, grid, 256, 0, stream, p);
+  else if (type == 1)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
     tge_launch(units ? read_8bit_kernel<float, true> : read_8bit_kernel<float, false>, grid, 256, 0, stream, p);

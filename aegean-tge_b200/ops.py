@@ -206,8 +206,8 @@ def core() -> ctypes.CDLL:
                                          _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                          _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr])
         _declare(lib, "tge_read_8bit", [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr,
-                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int,
-                                        _c_ptr, _c_ptr])
+                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                                        _c_int, _c_ptr, _c_ptr])
         lib.tge_attention_8bit_decode_floats.argtypes = [_c_int] * 7
         lib.tge_attention_8bit_decode_floats.restype = _c_ll
         _declare(lib, "tge_attention_8bit_decode", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
@@ -237,6 +237,9 @@ def attention_lib(head_dim: int, value_dim: int = 0) -> ctypes.CDLL:
                                             _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_int,
                                             _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr,
                                             _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr])
+        _declare(lib, "tge_attention_mma_halves", [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr,
+                                                    _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_float,
+                                                    _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr])
         lib.tge_attention_mma_scratch_floats.argtypes = [_c_int, _c_int, _c_int]
         lib.tge_attention_mma_scratch_floats.restype = _c_ll
         if lib.tge_attention_mma_head_dim() != head_dim or lib.tge_attention_mma_value_dim() != value_dim:
@@ -1192,7 +1195,9 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
 
 
 def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
-    """:func:`read_cache_8bit`, and the requests' q_start counted from ``first_seq``'s into ``starts``."""
+    """:func:`read_cache_8bit`, and the requests' q_start counted from ``first_seq``'s into ``starts``.  ``dtype`` float16: for the attention
+    over such pages, with a fourth result, their exponents (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over 2^f, at most 1; a
+    position whose values' scale is not finite has a key that is not); None for a cache that this is not built for."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
     num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
     _portions(q_start, start_pos, num_seqs)
@@ -1202,12 +1207,15 @@ def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_p
     k = k_scale.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
     table = block_table.new_empty((len(mine), width))
+    exponents = block_table.new_empty((runs, kv_heads)) if dtype == torch.float16 else None
     lib = core()
-    _check(lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
-                             block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
-                             kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), int(dtype == torch.bfloat16), table.data_ptr(),
-                             _ptr(starts), runs, width, status_word().data_ptr(), _stream()), lib)
-    return k, v, table
+    rc = lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
+                           block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
+                           kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), 2 if exponents is not None else int(dtype == torch.bfloat16),
+                           _ptr(exponents), table.data_ptr(), _ptr(starts), runs, width, status_word().data_ptr(), _stream())
+    if _check(rc, lib) == UNSUPPORTED:
+        return None
+    return (k, v, table) if exponents is None else (k, v, table, exponents)
 
 
 _decode_8bit_floats: Dict[tuple, int] = {}      # scratch numbers by sizes: asking the library costs a microsecond a call
@@ -1259,16 +1267,17 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if singles < num_seqs and ctx_lens is None:
         ctx_lens = [max_ctx_len] * num_seqs
 
-    def single_tokens() -> int:
-        """Serves the requests that bring one token each, if the kernel takes their sizes; returns how many."""
+    need = -1                                           # scratch numbers of the single tokens' kernel; -1: sizes that it does not take
+    if singles:
         sizes = (is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
         need = _decode_8bit_floats.get(sizes)
         if need is None:
             if len(_decode_8bit_floats) >= 1024:
                 _decode_8bit_floats.clear()
             need = _decode_8bit_floats[sizes] = lib.tge_attention_8bit_decode_floats(*sizes)
-        if need < 0:
-            return 0
+
+    def single_tokens() -> int:
+        """Serves the requests that bring one token each, if the kernel takes them; returns how many."""
         parts = k_scale.new_empty(need)
         rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
                                            out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
@@ -1277,20 +1286,41 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     def portions(first: int, read=None) -> None:
         """The requests from ``first`` on.  Their keys and values are read once into run-type pages of 64, which the prefill kernels take:
-        a query tile of those reads each of them again, so that turning codes into numbers there would be done many times over."""
-        starts = q_start.new_empty(num_seqs - first + 1)
-        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, first, starts)
-        if read is not None:
-            read.record()
+        a query tile of those reads each of them again, so that turning codes into numbers there would be done many times over.
+        bfloat16 runs, heads of 64 or 128: in float16 over powers of two, three bits more than bfloat16 has.  Else in the run type."""
+        starts, longest = q_start.new_empty(num_seqs - first + 1), max(ctx_lens[first:])
         rows = (q, start_pos, positions, seq_of_token, out)
         if first:
             rows = (q[first:], start_pos[first:], positions[first:], seq_of_token[first:], out[first:])
-        attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, max(ctx_lens[first:]), heads, kv_heads, head_dim, scale,
+        if is_bf16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and out_stride % 8 == 0 and (rows[0].data_ptr() | rows[4].data_ptr()) % 16 == 0:
+            span = longest if window == 0 else min(longest, (-(-window // 64) + 1) * 64)
+            split = choose_attention_split(tokens - first, num_seqs - first, max_q_len, span, heads, kv_heads, bound=span)
+            prefill = attention_lib(head_dim)
+            held = None
+            if prefill.tge_attention_mma_halves_fit(longest, split):
+                held = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, torch.float16, window, first, starts)
+            if held is not None:
+                if read is not None:
+                    read.record()
+                k, v, table, exponents = held
+                splits = 1 if split == 0 or longest <= split else -(-longest // split)
+                states = prefill.tge_attention_mma_scratch_floats(tokens - first, heads, splits)
+                scratch = k_scale.new_empty(states) if states > 0 else None
+                _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), exponents.data_ptr(),
+                                                        table.data_ptr(), table.shape[1], k.shape[0], starts.data_ptr(), rows[1].data_ptr(),
+                                                        rows[2].data_ptr(), num_seqs - first, tokens - first, max_q_len, longest,
+                                                        rows[4].data_ptr(), out_stride, heads, kv_heads, float(scale), int(window), split,
+                                                        _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
+                return
+        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, first, starts)
+        if read is not None:
+            read.record()
+        attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
                   window=window, out=rows[4], sink=sink)
 
     as_portions = max_q_len > 1 and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
                                      else head_dim in (16, 32, 64, 128) and sink is None)
-    if as_portions and MIN_DECODE_PREFIX <= singles < num_seqs and not torch.cuda.is_current_stream_capturing():
+    if as_portions and need >= 0 and MIN_DECODE_PREFIX <= singles < num_seqs and not torch.cuda.is_current_stream_capturing():
         reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
         if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
             # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
@@ -1307,8 +1337,8 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             main.wait_stream(side)
             if served == singles:
                 return out
-            as_portions = False          # (sizes that the single tokens' kernel does not take: all go the simple way below)
-    done = single_tokens() if singles else 0            # requests, and so tokens, that are served
+            as_portions = False          # (a cache that the single tokens' kernel does not take: all go the simple way below)
+    done = single_tokens() if need >= 0 else 0            # requests, and so tokens, that are served
     if done == num_seqs:
         return out
     if as_portions and done == singles:

@@ -454,3 +454,64 @@ def test_side_by_side_is_the_same(ops, monkeypatch, dtype, heads, kv, dim):
     side.synchronize()
     if dim == 128:
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64), (6, 2, 32), (4, 2, 80), (2, 2, 256)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_a_block_that_reads_as_nan_in_a_portion(ops, dtype, heads, kv, dim, window):
+    """Rows in front of it, rows behind its window and other requests do not see it, in whatever tile of keys it lies."""
+    held, lens = [300, 150, 70], [300, 90, 6]
+    cache = Cache(held, kv, dim, 16, 1)
+    bad = {0: (170, "v"), 1: (63, "k"), 2: (66, "v")}
+    for request, (pos, name) in bad.items():
+        cache.scales[name][cache.table[request, pos // 16].item(), 1, pos % 16] = math.nan
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+    q = torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    out = ops.attention_8bit(q, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 3, 300, 300, heads, kv, dim, 0.09, window=window, ctx_lens=held)
+    nan = torch.isnan(out.view(-1, heads, dim)).cpu()
+    want, at = torch.zeros(sum(lens), heads, dtype=torch.bool), 0
+    for r, n in enumerate(lens):
+        for i in range(n):
+            pos = held[r] - n + i
+            sees = bad[r][0] <= pos and (not window or bad[r][0] > pos - window)
+            want[at + i, heads // kv:2 * (heads // kv)] = sees
+        at += n
+    assert torch.equal(nan.all(-1), want) and torch.equal(nan.any(-1), want)
+
+
+@pytest.mark.parametrize("splits", [128, 192])
+def test_portions_whose_keys_are_cut(ops, monkeypatch, splits):
+    """The runs of keys that a short portion deep in a long context is cut into, and their merging."""
+    monkeypatch.setattr(ops, "choose_attention_split", lambda *a, **k: splits)
+    cache = Cache([700, 64, 1000], 2, 128, 64, 1)
+    out, want = attend(ops, cache, [9, 64, 30], 14, torch.bfloat16, ctx_lens=[700, 64, 1000], sink=True)
+    assert rel_error(out, want) < TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_portions_over_scales_far_apart(ops, heads, kv, dim, window):
+    """Values whose size changes by up to 2^120 from one run of 64 positions to the next, keys by 2^3; queries of 2^60 over keys of 2^-60."""
+    held, lens = [640, 150, 130], [600, 150, 6]
+    cache = Cache(held, kv, dim, 64, 1)
+    for r, (size, sizes) in enumerate(zip((60, 0, -60), ([0, 30, -30, 0, 5, 60, -60, 1, 0, -1], [-40, 20, 0], [1, 0, -100]))):
+        for run, f in enumerate(sizes):
+            where = cache.table[r, run].item()
+            cache.scales["v"][where] *= 2.0 ** f
+            cache.scales["k"][where] *= 2.0 ** (run % 4 - size)
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+    q = torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(2))
+    q = (q * 2.0 ** torch.tensor([60.0, 0, -60]).repeat_interleave(torch.tensor(lens))[:, None]).bfloat16()
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 3, 600, 640, heads, kv, dim, 0.02,
+                             window=window, ctx_lens=held)
+    ops.check_status()
+    at = 0
+    for r, n in enumerate(lens):
+        k, v, rows = cache.values("k", r), cache.values("v", r), q[at:at + n].view(n, heads, dim)
+        want = plain.attend(rows, k, v, held[r] - n, 0.02, window, None)
+        # a row and head's error against the largest sum of probabilities times magnitudes: each product's roundings are of its own size
+        size = plain.attend(rows, k, v.abs(), held[r] - n, 0.02, window, None).amax(-1)
+        error = (out[at:at + n].cpu().double().view(n, heads, dim) - want).abs().amax(-1)
+        assert float((error / size).max()) < 2 ** -7
+        at += n
