@@ -1183,9 +1183,10 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
     """What the requests of a step hold in a cache of 8-bit codes, as values: (k, v, table).
 
     ``ctx_lens``: for every request how many positions it holds after the step (host numbers; the device has them as
-    start_pos + q_start's differences).  k and v [runs, kv_heads, 64, head_dim] in ``dtype`` (float32 or bfloat16): the requests' positions one request after the
-    other in runs of 64, zeros behind a request's last position; table [requests, runs of the longest]: run i of a request, -1
-    where there is none.  With a ``window`` only runs that the step's queries may see.  ``first_seq``: leave out the requests before.
+    start_pos + q_start's differences).  k and v [runs, kv_heads, 64, head_dim] in ``dtype`` (float32 or bfloat16): the requests'
+    positions one request after the other in runs of 64, zeros behind a request's last position; table [requests, runs of the
+    longest]: run i of a request, -1 where there is none.  With a ``window`` only runs that the step's queries may see.
+    ``first_seq``: leave out the requests before.
     """
     if k_pages.dim() != 4:
         raise KernelError(f"8-bit pages must be [pages, kv_heads, page_size, head_dim], got {tuple(k_pages.shape)}")
@@ -1195,9 +1196,10 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
 
 
 def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
-    """:func:`read_cache_8bit`, and the requests' q_start counted from ``first_seq``'s into ``starts``.  ``dtype`` float16: for the attention
-    over such pages, with a fourth result, their exponents (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over 2^f, at most 1; a
-    position whose values' scale is not finite has a key that is not); None for a cache that this is not built for."""
+    """:func:`read_cache_8bit`; with ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a position
+    whose values' scale is not finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a
+    fourth result, their exponents (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over
+    2^f, at most 1); None for a cache that this is not built for."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
     num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
     _portions(q_start, start_pos, num_seqs)
@@ -1324,7 +1326,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
         if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
             # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
-            # the read-back, on SMs that its last wave leaves.  63 of 2,048 beside 1,985 after 6,143 (40 heads over 8) 425 -> 377 us, 31 of 2,048
+            # the read-back, on SMs that its last wave leaves.  63 of 2,048 beside 1,985 after 6,143 (40 heads over 8) 475 -> 421 us, 31 of 2,048
             # beside 1,000 after 1,000 (28 over 4) 71 -> 61, 32 of 1,024 beside 2,016 (40 over 8) 107 -> 104; small steps wait for the host,
             # whom the second stream costs 12 us.
             main, side = torch.cuda.current_stream(), _side_stream()
