@@ -119,13 +119,13 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // that holds a whole unit writes its output; parts of units are left as (maximum, sum, unnormalised output) in scratch memory, at
 // most two per block, and a second kernel joins them in the order of the positions.
 //
-// Measured, with the joining: 64 requests of 4,096 positions at 40 heads over 8 (425 MB with their scales) 80.5 us, 5.3 TB/s or 0.81 of a
+// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (425 MB with their scales) 80.5 us, 5.3 TB/s or 0.81 of a
 // copy's rate; a kernel that only reads the same pages takes 71.7.  Four of 32,768 45 us, eight of 2,048 at 28 heads over 4 13.7, one 12, of
 // which most are two launches and the joining.  Not taken: the codes through rings in shared memory (117 us where this took 83), two slices of
 // each warp on their way (94), slices dealt to the warps in turn instead of in runs (91 beside 81), pages asked into L2 a slice ahead (86).
 // ---------------------------------------------------------------------------
 constexpr int DWARPS = 4;
-// 64 requests of 4,096 at 0 / 12 / 24: 80.9 / 80.2 / 82.5 us, four of 32,768 47.8 / 45.6 / 45.9, eight of 2,048 16.5 / 14.4 / 14.4
+// The 64 requests at 0 / 12 / 24: 80.9 / 80.2 / 82.5 us, four of 32,768 47.8 / 45.6 / 45.9, eight of 2,048 16.5 / 14.4 / 14.4
 constexpr int BEGIN = 12;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
 constexpr float LOG2E = 1.4426950408889634f;
@@ -316,7 +316,7 @@ __device__ __forceinline__ int number_of(int pair) {
 }
 
 // Blocks on an SM.  Codes on their way are what hides the memory's latency, and they are in registers: five blocks of heads of 128 numbers have
-// room too, but bring more parts to join (eight requests of 2,048 14.4 us, with four 13.7; 64 of 4,096 80 both).
+// room too, but bring more parts to join (eight requests of 2,048 14.4 us, with four 13.7; the 64 of up to 4,096 80 both; with three 87).
 __host__ __device__ constexpr int decode_blocks_per_sm(int head_dim, int tiles) { return head_dim * tiles <= 64 ? 6 : head_dim * tiles <= 128 ? 4 : 3; }
 
 template <typename T, int HD, int NT>

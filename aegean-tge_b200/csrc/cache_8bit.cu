@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 // turn, three rows on their way at a time, the angles loaded once.  With larger blocks the others have a (block of positions, key or value
 // head) each: its groups take the block's rows in turn, once for the scale and, from cache, once for the codes.
 // With the read-back below: one token 8.4 us; a prompt of 2,048 tokens at 28 heads over 4 15 us (43 MB; 6.6 at a copy's rate); 64 tokens
-// behind 511 each at 40 heads over 8, blocks of 16, 48 us (166 MB, 25 at that rate).  With a warp to a head, as above: 25, 57 and 92 us.
+// of requests that hold up to 512 (25,109 together) at 40 heads over 8, blocks of 16, 48 us (165 MB, 25 at that rate).  With a warp to a head, as above: 25, 57 and 92 us.
 // ---------------------------------------------------------------------------
 constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns
 

@@ -211,12 +211,16 @@ __device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[
   }
 }
 
-// One pass over a chunk of a row.  What bounds it is reading the logits: a thread holds its next sixteen on their way while it works on
-// these, keeps sums of its own, and looks at single logits only where its largest reaches the smallest of the best so far.  Those that do are listed
-// with the block's others; the list is cut to the best now and then.  After the first round the best are a
-// choice among the largest of 64 groups of four lanes and whatever passes the n-th of those, then whatever passes the n-th of the chunk's
-// first 1, 2, 4, 8, ... rounds: of random rows some hundred logits are ever listed.  A row that lists more than there is room
-// for (rising logits) is looked through again.
+// One pass over a chunk of a row: a thread holds its next sixteen logits on their way while it works on these, keeps sums of its own, and looks
+// at single logits only where its largest reaches the smallest of the best so far.  Those that do are listed with the block's others; the list
+// is cut to the best now and then.  After the first round the best are a choice among the largest of 64 groups of four lanes and whatever
+// passes the n-th of those, then whatever passes the n-th of the chunk's first 1, 2, 4, 8, ... rounds: of random rows some hundred logits are
+// ever listed.  A row that lists more than there is room for (rising logits) is looked through again.
+//
+// 1,024 rows of 152,064 float32 logits with the 20 best: 120 us, 5.2 TB/s or 0.79 of a copy's rate (without alternatives 109); 70 % of the issue
+// slots are taken, some 20 instructions a logit.  In bfloat16 155 us, for the same number of instructions and the conversions.  One row in 38
+// chunks 10.4 us, most of it two launches and the trips of the first round.  Not taken: cuts after rounds 1, 4, 16, ... only (127 us); a bar that
+// stays where the first round put it, with a barrier every round (365).
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const LogprobParams p) {
   constexpr int per = 16 / sizeof(T);
