@@ -117,11 +117,12 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // requests' lengths; the blocks work that out from the lengths on the device, so a captured graph stays right as they grow.  A unit
 // counts as BEGIN slices more than it has: what a block spends on its queries, its first copies and the joining of its warps.  A run
 // that holds a whole unit writes its output; parts of units are left as (maximum, sum, unnormalised output) in scratch memory, at
-// most two per block, and a second kernel joins them in the order of the positions.
+// most two per block, and a second kernel joins them in the order of the positions.  Few units over short contexts (decode_cluster) go without: a
+// cluster of blocks has a unit, its slices in equal shares, and joins them through its shared memory.
 //
 // Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (425 MB with their scales) 80.5 us, 5.3 TB/s or 0.81 of a
-// copy's rate; a kernel that only reads the same pages takes 71.7.  Four of 32,768 45 us, eight of 2,048 at 28 heads over 4 13.7, one 12, of
-// which most are two launches and the joining.  Not taken: the codes through rings in shared memory (117 us where this took 83), two slices of
+// copy's rate; a kernel that only reads the same pages takes 71.7.  Four of 32,768 45 us, eight of 2,048 at 28 heads over 4 (a cluster each unit)
+// 10.3, of 512 8.2: the trips to memory one behind the other.  Not taken: the codes through rings in shared memory (117 us where this took 83), two slices of
 // each warp on their way (94), slices dealt to the warps in turn instead of in runs (91 beside 81), pages asked into L2 a slice ahead (86).
 // ---------------------------------------------------------------------------
 constexpr int DWARPS = 4;
@@ -315,11 +316,33 @@ __device__ __forceinline__ int number_of(int pair) {
   return VB * (g + 8 * j) + 2 * (i - j * (VB / 2));
 }
 
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_size() {
+  int n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+// What lies at `mine`'s place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ float2 of_rank(const float2* mine, int rank) {
+  uint32_t at;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
 // Blocks on an SM.  Codes on their way are what hides the memory's latency, and they are in registers: five blocks of heads of 128 numbers have
 // room too, but bring more parts to join (eight requests of 2,048 14.4 us, with four 13.7; the 64 of up to 4,096 80 both; with three 87).
 __host__ __device__ constexpr int decode_blocks_per_sm(int head_dim, int tiles) { return head_dim * tiles <= 64 ? 6 : head_dim * tiles <= 128 ? 4 : 3; }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) decode_8bit_kernel(const Decode8 p) {
   constexpr int DIGITS = sizeof(T) == 2 ? 2 : 3, PARTS = sizeof(T) == 2 ? 1 : 2;
   constexpr int HEADS = 8 * NT, MTILES = HD / 16, PITCH = HD + 4;
@@ -328,10 +351,11 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
   __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS], factors[HEADS];
   __shared__ __align__(16) uint32_t queries[NT][C::KC][DIGITS][32][4];
   __shared__ int start_of[5];
+  __shared__ float2 part_state[CLUSTER ? HEADS : 1];              // what merge_o's first place is over: (maximum, sum)
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = uniform_warp_index();
   const int g = lane >> 2, t = lane & 3;
-  if (warp == 0) {                                                // where this block's run begins
+  if (!CLUSTER && warp == 0) {                                    // where this block's run begins
     // 32 requests at a time; the first of them stay where they are
     const int first_count = lane < p.a.num_seqs ? (slices_of(p, lane).count + BEGIN) * p.units : 0;
     const int first_token = lane < p.a.num_seqs ? p.q_start[lane] : 0;
@@ -373,19 +397,42 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       start_of[4] = token;
     }
   }
-  __syncthreads();
-  int seq = start_of[0], base = start_of[1], at = start_of[2], token = start_of[4];
-  const int end = start_of[3];
+  int seq, base = 0, at = 0, end = 1, token, unit = 0, rank = 0, ranks = 1;
+  if constexpr (CLUSTER) {
+    rank = cluster_rank();
+    ranks = cluster_size();
+    const int which = blockIdx.x / ranks;
+    seq = which / p.units;
+    unit = which - seq * p.units;
+    token = p.q_start[seq];
+  } else {
+    __syncthreads();
+    seq = start_of[0];
+    base = start_of[1];
+    at = start_of[2];
+    end = start_of[3];
+    token = start_of[4];
+  }
   bool waited = false;
 
   while (at < end) {
     const Slices s = slices_of(p, seq);
-    const int unit = (at - base) / (s.count + BEGIN), begin = base + unit * (s.count + BEGIN);
-    const int upto = min(begin + s.count + BEGIN, end);            // where this unit's part of the run ends
-    const int skip = max(at - begin - BEGIN, 0), length = upto - begin - BEGIN - skip;
-    at = upto;
-    const bool next_seq = unit == p.units - 1 && upto == begin + s.count + BEGIN;
-    if (length <= 0) continue;                                     // no more than the begin of a unit
+    int skip, length;
+    bool next_seq = false;
+    if constexpr (CLUSTER) {
+      skip = s.count * rank / ranks;
+      length = s.count * (rank + 1) / ranks - skip;                // (none is fine)
+      at = end;
+    } else {
+      unit = (at - base) / (s.count + BEGIN);
+      const int begin = base + unit * (s.count + BEGIN);
+      const int upto = min(begin + s.count + BEGIN, end);          // where this unit's part of the run ends
+      skip = max(at - begin - BEGIN, 0);
+      length = upto - begin - BEGIN - skip;
+      at = upto;
+      next_seq = unit == p.units - 1 && upto == begin + s.count + BEGIN;
+      if (length <= 0) continue;                                   // no more than the begin of a unit
+    }
     const int kvh = unit / p.head_tiles, tile = unit - kvh * p.head_tiles;
     const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
     const int* table = p.a.block_table + (size_t)seq * p.a.max_pages;
@@ -586,7 +633,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       }
     }
     __syncthreads();
-    const bool whole = length == s.count;
+    const bool whole = !CLUSTER && length == s.count;
     const size_t place = (size_t)(2 * blockIdx.x + (skip == 0 ? 1 : 0)) * HEADS;
     for (int i = threadIdx.x; i < heads_here * (HD / 2); i += DWARPS * 32) {
       const int head = i / (HD / 2), pair = i - head * (HD / 2);
@@ -614,10 +661,37 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         T* dst = static_cast<T*>(p.a.out) + (size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD + number_of<HD>(pair);
         dst[0] = from_float<T>(acc.x * over);
         dst[1] = from_float<T>(acc.y * over);
-      } else {
+      } else if (!CLUSTER) {
         *reinterpret_cast<float2*>(p.parts + (place + head) * HD + 2 * pair) = acc;
         if (pair == 0) *reinterpret_cast<float2*>(p.states + (place + head) * 2) = make_float2(most, sum);
+      } else {
+        *reinterpret_cast<float2*>(merge_o + head * PITCH + 2 * pair) = acc;             // in the first warp's place: read by this thread alone
+        if (pair == 0) part_state[head] = make_float2(most, sum);
       }
+    }
+    if constexpr (CLUSTER) {
+      cluster_sync();
+      for (int i = rank * DWARPS * 32 + threadIdx.x; i < heads_here * (HD / 2); i += ranks * DWARPS * 32) {
+        const int head = i / (HD / 2), pair = i - head * (HD / 2);
+        const float sink = p.a.sink != nullptr ? p.a.sink[head0 + head] * LOG2E : NONE;
+        float top = sink, all = 0.0f;
+        for (int r = 0; r < ranks; ++r) top = fmaxf(top, of_rank(&part_state[head], r).x);
+        float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+        for (int r = 0; r < ranks; ++r) {
+          const float2 state = of_rank(&part_state[head], r), x = of_rank(reinterpret_cast<const float2*>(merge_o + head * PITCH + 2 * pair), r);
+          const float f = exp2_fast(state.x - top);
+          all = fmaf(state.y, f, all);
+          acc.x = fmaf(x.x, f, acc.x);
+          acc.y = fmaf(x.y, f, acc.y);
+        }
+        if (p.a.sink != nullptr) all += exp2_fast(sink - top);
+        const float over = all == 0.0f ? 0.0f : 1.0f / all;
+        T* dst = static_cast<T*>(p.a.out) + (size_t)token * p.a.out_stride + (size_t)(head0 + head) * HD + number_of<HD>(pair);
+        dst[0] = from_float<T>(acc.x * over);
+        dst[1] = from_float<T>(acc.y * over);
+      }
+      cluster_sync();                                             // nobody leaves while another reads its memory
     }
     if (next_seq && at < end) {
       base = at;
@@ -727,18 +801,24 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const
 }
 
 template <typename T, int HD, int NT>
-int launch_decode(Decode8 p, int blocks, cudaStream_t stream) {
+int launch_decode(Decode8 p, int blocks, int cluster, cudaStream_t stream) {
   constexpr int smem = DWARPS * 8 * NT * (HD + 4) * 4;
-  static bool ready[64] = {};                                     // shared memory beyond 48 KB is asked for once per device
+  static bool ready[64] = {};                                     // shared memory beyond 48 KB, clusters of 16: asked for once per device
   int device = 0;
   cudaGetDevice(&device);
-  if (smem > 48 * 1024 && (device >= 64 || !ready[device])) {
-    const cudaError_t rc = cudaFuncSetAttribute(decode_8bit_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    TGE_REQUIRE(rc == cudaSuccess, "attention_8bit: %d bytes of shared memory: %s", smem, cudaGetErrorString(rc));
+  if (device >= 64 || !ready[device]) {
+    cudaError_t rc = cudaFuncSetAttribute(decode_8bit_kernel<T, HD, NT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (rc == cudaSuccess && smem > 48 * 1024) rc = cudaFuncSetAttribute(decode_8bit_kernel<T, HD, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc == cudaSuccess && smem > 48 * 1024) rc = cudaFuncSetAttribute(decode_8bit_kernel<T, HD, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    TGE_REQUIRE(rc == cudaSuccess, "attention_8bit: %d bytes of shared memory, clusters of 16: %s", smem, cudaGetErrorString(rc));
     if (device < 64) ready[device] = true;
   }
+  if (cluster > 0) {
+    tge_launch_clusters(decode_8bit_kernel<T, HD, NT, true>, dim3(p.a.num_seqs * p.units * cluster), DWARPS * 32, smem, cluster, stream, p);
+    return tge_launched("attention_8bit", 1);
+  }
   p.states = p.parts + (size_t)2 * blocks * 8 * NT * HD;
-  tge_launch(decode_8bit_kernel<T, HD, NT>, blocks, DWARPS * 32, smem, stream, p);
+  tge_launch(decode_8bit_kernel<T, HD, NT, false>, blocks, DWARPS * 32, smem, stream, p);
   tge_launch(decode_8bit_join_kernel<T, HD, NT>, dim3(p.a.num_seqs, p.units), JOIN_WARPS * 32, 0, stream, p, blocks);
   return tge_launched("attention_8bit", 2);
 }
@@ -752,6 +832,16 @@ int decode_blocks(int head_dim, int tile_heads) { return tge_sm_count() * decode
 // heads of 256 numbers have no registers for).
 static int decode_tile(int group, int head_dim) { return group <= 8 || head_dim > 128 ? 8 : 16; }
 
+// Blocks of a cluster per unit, which joins its parts itself; 0: runs of slices and a second kernel.  A rule on what the host knows, the units and the
+// bound of their lengths.  Clusters of 8 while all of them are on the device at a time, us with them / with runs: one to 16 requests of 512
+// at 28 heads over 4 8.2 to 10.3 / 10.3 to 11.8, of 2,048 10.3 to 13.3 / 10.3 to 14.7, of 4,096 12.3 to 18.5 / 12.3 to 18.5 (8 of them 14.4 / 16.2); of
+// 8,192 18 / 16.  Clusters of 16 for few units and longer bounds: one to four requests of 4,096 10.3 to 12.3, of 8,192 14 to 15, of 16,384 18.5
+// to 22 / 18.6 to 18.9; 32 units of them are not on the device at a time (18.5 us where 8 take 10.3).
+static int decode_cluster(long long units, int head_dim, int tile, long long positions) {
+  if (units <= 16 && positions > 2048 && positions <= 8192) return 16;
+  return 8 * units <= decode_blocks(head_dim, tile) && positions <= 4096 ? 8 : 0;
+}
+
 // float32 scratch numbers of tge_attention_8bit_decode; -1: sizes that it does not take.
 TGE_API long long tge_attention_8bit_decode_floats(int is_bf16, int num_seqs, int heads, int kv_heads, int head_dim, int page_size, int max_pages) {
   if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size < 16 || (page_size & (page_size - 1)) != 0 || kv_heads <= 0 || heads % kv_heads != 0) return -1;
@@ -760,6 +850,7 @@ TGE_API long long tge_attention_8bit_decode_floats(int is_bf16, int num_seqs, in
   // places in the row of all slices are counted in 32 bits, units along a grid's second axis
   if (units > 65535 || (long long)max_pages * page_size > (1ll << 30) ||
       units * num_seqs * ((long long)max_pages * page_size / 16 + 1 + BEGIN) > (1ll << 30)) return -1;
+  if (decode_cluster(units * num_seqs, head_dim, tile, (long long)max_pages * page_size) > 0) return 0;
   return 2ll * decode_blocks(head_dim, tile) * tile * (head_dim + 2);
 }
 
@@ -789,11 +880,12 @@ TGE_API int tge_attention_8bit_decode(const void* q, int is_bf16, long long q_st
   p.block_shift = __builtin_ctz(block);
   p.parts = parts;
   const int blocks = decode_blocks(head_dim, tile);
+  const int cluster = decode_cluster((long long)p.units * num_seqs, head_dim, tile, (long long)max_pages * page_size);
   auto run = [&](auto type) {
     using T = decltype(type);
-    if (head_dim == 256) return launch_decode<T, 256, 1>(p, blocks, stream);
-    if (head_dim == 128) return tile == 8 ? launch_decode<T, 128, 1>(p, blocks, stream) : launch_decode<T, 128, 2>(p, blocks, stream);
-    return tile == 8 ? launch_decode<T, 64, 1>(p, blocks, stream) : launch_decode<T, 64, 2>(p, blocks, stream);
+    if (head_dim == 256) return launch_decode<T, 256, 1>(p, blocks, cluster, stream);
+    if (head_dim == 128) return tile == 8 ? launch_decode<T, 128, 1>(p, blocks, cluster, stream) : launch_decode<T, 128, 2>(p, blocks, cluster, stream);
+    return tile == 8 ? launch_decode<T, 64, 1>(p, blocks, cluster, stream) : launch_decode<T, 64, 2>(p, blocks, cluster, stream);
   };
   return is_bf16 ? run(__nv_bfloat16()) : run(float());
 }

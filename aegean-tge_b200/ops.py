@@ -1280,10 +1280,10 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     def single_tokens() -> int:
         """Serves the requests that bring one token each, if the kernel takes them; returns how many."""
-        parts = k_scale.new_empty(need)
+        parts = k_scale.new_empty(need) if need else None
         rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
                                            out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
-                                           parts.data_ptr(), need, status_word().data_ptr(), _stream())
+                                           _ptr(parts), need, status_word().data_ptr(), _stream())
         return singles if _check(rc, lib) != UNSUPPORTED else 0
 
     def portions(first: int, read=None) -> None:

@@ -515,3 +515,34 @@ def test_portions_over_scales_far_apart(ops, heads, kv, dim, window):
         error = (out[at:at + n].cpu().double().view(n, heads, dim) - want).abs().amax(-1)
         assert float((error / size).max()) < 2 ** -7
         at += n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 128), (14, 2, 64), (5, 1, 256), (24, 2, 128)])
+@pytest.mark.parametrize("columns", [16, 33, 64, 66, 128, 130])
+@pytest.mark.parametrize("window,sink", [(0, True), (70, False)])
+def test_single_tokens_under_every_bound(ops, dtype, heads, kv, dim, columns, window, sink):
+    """The bound of the contexts (the block table's columns, of 64 positions here) decides how a unit's keys are shared out: clusters of 8 and 16
+    blocks, runs; requests of one position, of less than a slice to a block, of more."""
+    cache = Cache([1, 17, 1000, 130, 64], kv, dim, 64, 1)
+    wide = torch.full((5, columns), -1, dtype=torch.int32)
+    wide[:, :cache.table.shape[1]] = cache.table
+    cache.table = wide
+    out, want = attend(ops, cache, [1] * 5, heads, dtype, window=window, sink=sink)
+    assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("columns", [16, 66, 130])
+def test_a_page_outside_the_pool_under_every_bound(ops, columns):
+    """A unit whose keys are partly or wholly outside the pool: reported, unread, zero where nothing is seen."""
+    cache = Cache([40, 300], 1, 128, 64, 1)
+    wide = torch.full((2, columns), -1, dtype=torch.int32)
+    wide[1, :5] = cache.table[1, :5]
+    positions, seq, q_start, start_pos = batch_index([1, 1], [39, 299], DEV)
+    q = torch.randn(2, 8 * 128, device=DEV).bfloat16()
+    out = ops.attention_8bit(q, *cache.device(), wide.to(DEV), q_start, start_pos, positions, seq, 2, 1, 300, 8, 1, 128, 0.09)
+    with pytest.raises(ops.DeviceStatusError, match="page"):
+        ops.check_status()
+    assert (out[0] == 0).all()
+    want = plain.attend(q[1:].cpu().view(1, 8, 128), cache.values("k", 1), cache.values("v", 1), 299, 0.09, 0, None)
+    assert rel_error(out[1:], want.flatten(1)) < TOL[torch.bfloat16]
