@@ -14,7 +14,7 @@ constexpr int MOST_TOP = 32;
 constexpr int MINE = 16;                        // logits of a thread and round
 constexpr int ROUND = THREADS * MINE;
 constexpr int ROOM = 8 * THREADS + MOST_TOP;    // keys in the list of candidates: what one load of all threads may add to a full choice
-constexpr int MOST_SPLITS = 128;
+constexpr int MOST_SPLITS = 128, MOST_CLUSTER = 16;
 constexpr float LEAST = -3.402823466e38f;       // where a thread's reference starts: finite, so that -inf less it is -inf
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -184,6 +184,51 @@ __device__ __forceinline__ void answer(const LogprobParams& p, int r, const Sums
   }
 }
 
+// The chunks of a row, SPLITS of them at most, joined by a block: their sums in order, and the best of their best (`list`: room for all of them).
+template <int SPLITS>
+__device__ void join_chunks(const LogprobParams& p, int r, float own, bool known, unsigned long long* list, unsigned long long* scratch, int* listed,
+                            int* counter) {
+  constexpr int PER_LANE = (SPLITS + 31) / 32;
+  const int lane = threadIdx.x & 31;
+  __syncthreads();                               // whoever still reads the block's own list
+  if (threadIdx.x == 0) *listed = 0;
+  // every warp for itself, splits lane by lane
+  Sums part[PER_LANE], all{LEAST, 0.0f, 0.0f, 0};
+  unsigned long long least = 0;
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i) {
+    const int split = lane + 32 * i;
+    part[i] = Sums{LEAST, 0.0f, 0.0f, 0};
+    if (split < p.splits) {
+      const float4 s = *reinterpret_cast<const float4*>(p.sums + 4 * ((size_t)r * p.splits + split));
+      part[i] = Sums{s.x, s.y, s.z, __float_as_int(s.w)};
+      // no key below the last of a chunk's best is among the row's
+      if (p.top > 0) least = max(least, p.keys[((size_t)r * p.splits + split) * p.top + p.top - 1]);
+    }
+    all.m = fmaxf(all.m, part[i].m);
+  }
+  all.m = warp_max(all.m);
+  least = warp_largest(least);
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i) {
+    part[i].move(all.m);
+    all.z += part[i].z;
+    all.w += part[i].w;
+    all.before += part[i].before;
+  }
+  all.z = warp_sum(all.z);
+  all.w = warp_sum(all.w);
+  all.before = __reduce_add_sync(0xffffffffu, all.before);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.splits * p.top; i += THREADS) {
+    const unsigned long long key = p.keys[(size_t)r * p.splits * p.top + i];
+    if (key != 0 && key >= least) list[atomicAdd(listed, 1)] = key;
+  }
+  __syncthreads();
+  if (p.top > 0) choose<SPLITS * MOST_TOP>(list, *listed, p.top, scratch, counter);
+  answer(p, r, all, own, known, list);
+}
+
 // Sixteen logits of a thread in loads of 16 bytes, `per` of them each: load k holds those from first + (k THREADS + thread) per on.
 // What lies behind the chunk is -inf (and told apart by its index where that matters).
 template <typename T, bool VECTOR>
@@ -218,10 +263,10 @@ __device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[
 // ever listed.  A row that lists more than there is room for (rising logits) is looked through again.
 //
 // 1,024 rows of 152,064 float32 logits with the 20 best: 120 us, 5.2 TB/s or 0.79 of a copy's rate (without alternatives 109); 70 % of the issue
-// slots are taken, some 20 instructions a logit.  In bfloat16 155 us, for the same number of instructions and the conversions.  One row in 38
-// chunks 10.4 us, most of it two launches and the trips of the first round.  Not taken: cuts after rounds 1, 4, 16, ... only (127 us); a bar that
+// slots are taken, some 20 instructions a logit.  In bfloat16 155 us, for the same number of instructions and the conversions.  One row
+// with 5 alternatives 10.4 us: the trips of three rounds and of the joining.  Not taken: cuts after rounds 1, 4, 16, ... only (127 us); a bar that
 // stays where the first round put it, with a barrier every round (365).
-template <typename T, bool VECTOR>
+template <typename T, bool VECTOR, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const LogprobParams p) {
   constexpr int per = 16 / sizeof(T);
   __shared__ unsigned long long list[ROOM], scratch[65];
@@ -355,84 +400,73 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Logpro
   if (p.top > 0) settle(end);
   const int found = p.top > 0 ? min(listed, p.top) : 0;
   mine = block_sums(mine, floats, counts);
-  if (p.splits == 1) {
+  if (!CLUSTER && p.splits == 1) {
     answer(p, r, mine, own, known, list);
     return;
   }
   const size_t place = (size_t)r * p.splits + split;
   if (threadIdx.x == 0) *reinterpret_cast<float4*>(p.sums + 4 * place) = make_float4(mine.m, mine.z, mine.w, __int_as_float(mine.before));
   if ((int)threadIdx.x < p.top) p.keys[place * p.top + threadIdx.x] = (int)threadIdx.x < found ? list[threadIdx.x] : 0ull;
+  if constexpr (CLUSTER) {                       // a row's blocks are a cluster: its first one joins them
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+    if (split == 0) join_chunks<MOST_CLUSTER>(p, r, own, known, list, scratch, &listed, &counter);
+  }
 }
 
-// The chunks of a row joined: their sums in order, and the best of their best.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) token_logprobs_join_kernel(const LogprobParams p) {
   __shared__ unsigned long long list[MOST_SPLITS * MOST_TOP], scratch[65];
   __shared__ int listed, counter;
   pdl_trigger();
-  const int r = blockIdx.x, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) listed = 0;
   pdl_wait();
-  const int token = p.tokens[r];
+  const int token = p.tokens[blockIdx.x];
   const bool known = token >= 0 && token < p.vocab;
-  const float own = known ? to_float<T>(static_cast<const T*>(p.logits)[(size_t)r * p.stride + token]) : 0.0f;
-  // every warp for itself, splits lane by lane
-  Sums part[MOST_SPLITS / 32], all{LEAST, 0.0f, 0.0f, 0};
-  unsigned long long least = 0;
-#pragma unroll
-  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
-    const int split = lane + 32 * i;
-    part[i] = Sums{LEAST, 0.0f, 0.0f, 0};
-    if (split < p.splits) {
-      const float4 s = *reinterpret_cast<const float4*>(p.sums + 4 * ((size_t)r * p.splits + split));
-      part[i] = Sums{s.x, s.y, s.z, __float_as_int(s.w)};
-      // no key below the last of a chunk's best is among the row's
-      if (p.top > 0) least = max(least, p.keys[((size_t)r * p.splits + split) * p.top + p.top - 1]);
-    }
-    all.m = fmaxf(all.m, part[i].m);
-  }
-  all.m = warp_max(all.m);
-  least = warp_largest(least);
-#pragma unroll
-  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
-    part[i].move(all.m);
-    all.z += part[i].z;
-    all.w += part[i].w;
-    all.before += part[i].before;
-  }
-  all.z = warp_sum(all.z);
-  all.w = warp_sum(all.w);
-  all.before = __reduce_add_sync(0xffffffffu, all.before);
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.splits * p.top; i += THREADS) {
-    const unsigned long long key = p.keys[(size_t)r * p.splits * p.top + i];
-    if (key != 0 && key >= least) list[atomicAdd(&listed, 1)] = key;
-  }
-  __syncthreads();
-  if (p.top > 0) choose<MOST_SPLITS * MOST_TOP>(list, listed, p.top, scratch, &counter);
-  answer(p, r, all, own, known, list);
+  const float own = known ? to_float<T>(static_cast<const T*>(p.logits)[(size_t)blockIdx.x * p.stride + token]) : 0.0f;
+  join_chunks<MOST_SPLITS>(p, blockIdx.x, own, known, list, scratch, &listed, &counter);
 }
 
-// Logits of a chunk.  A block costs its rounds and about two more (the first choice, the joining), and as many run at a time as the device holds:
-// of all cuts the one that is done first, the fewest chunks among equals.
-int chunk_of(int rows, int vocab) {
+// How rows are cut into chunks of one block each.  A block costs its rounds and about two more (the first choice, the joining), and as many run at a
+// time as the device holds; a second kernel costs about three.  Few rows go in clusters of 8 or 16 blocks (16 of these clusters are on the
+// device at a time), which need none.  Of all cuts the one that is done first, the fewest chunks among equals.  Rows of 152,064 with 20
+// alternatives, us with clusters / a second kernel: one 12.5 / 12.5 (from the host, with 5, 22 / 24), 8 14.5 / 16.6, 64 24.8 / 26.8; with 32 one
+// 16.5 / 12.6 and 64 31 / 33.
+struct Cut { int splits, chunk, cluster; };
+Cut cut_of(int rows, int vocab) {
   const int rounds = (vocab + ROUND - 1) / ROUND;
   const long long at_once = 4ll * tge_sm_count();
-  long long best = 0;
-  int chunk = vocab;
-  for (int splits = 1; splits <= rounds && splits <= MOST_SPLITS; ++splits) {
+  long long best = (rows + at_once - 1) / at_once * (rounds + 2);
+  Cut cut{1, vocab, 0};
+  for (int splits = 2; splits <= rounds && splits <= MOST_SPLITS; ++splits) {
     const int mine = (rounds + splits - 1) / splits;
-    const long long cost = ((long long)rows * splits + at_once - 1) / at_once * (mine + 2);
-    if (splits == 1 || cost < best) {
+    const long long cost = ((long long)rows * splits + at_once - 1) / at_once * (mine + 2) + 3;
+    if (cost < best) {
       best = cost;
-      chunk = splits == 1 ? vocab : mine * ROUND;
+      cut = Cut{(vocab + mine * ROUND - 1) / (mine * ROUND), mine * ROUND, 0};
     }
   }
-  return chunk;
+  for (int blocks = 8; blocks <= MOST_CLUSTER; blocks += 8) {
+    const int chunk = ((vocab + blocks - 1) / blocks + 63) / 64 * 64;
+    const long long cost = (chunk + ROUND - 1) / ROUND + 2;
+    if ((long long)chunk * (blocks - 1) < vocab && rows <= (blocks == 8 ? at_once / 8 : 16) && cost < best) {
+      best = cost;
+      cut = Cut{blocks, chunk, blocks};
+    }
+  }
+  return cut;
 }
-int splits_of(int rows, int vocab) {
-  const int chunk = chunk_of(rows, vocab);
-  return (vocab + chunk - 1) / chunk;
+
+template <typename T, bool VECTOR>
+int in_clusters(const LogprobParams& p, int blocks, cudaStream_t stream) {
+  static bool ready[64] = {};                    // clusters of 16: asked for once per device
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device >= 64 || !ready[device]) {
+    const cudaError_t rc = cudaFuncSetAttribute(token_logprobs_kernel<T, VECTOR, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    TGE_REQUIRE(rc == cudaSuccess, "token_logprobs: clusters of 16: %s", cudaGetErrorString(rc));
+    if (device < 64) ready[device] = true;
+  }
+  tge_launch_clusters(token_logprobs_kernel<T, VECTOR, true>, dim3(p.rows * p.splits), THREADS, 0, blocks, stream, p);
+  return tge_launched("token_logprobs", 1);
 }
 
 }  // namespace
@@ -440,7 +474,7 @@ int splits_of(int rows, int vocab) {
 // float32 scratch numbers of tge_token_logprobs (16-byte aligned).
 TGE_API long long tge_token_logprobs_floats(int rows, int vocab, int top) {
   if (rows <= 0 || vocab <= 0 || top < 0) return 0;
-  const int splits = splits_of(rows, vocab);
+  const int splits = cut_of(rows, vocab).splits;
   return splits == 1 ? 0 : (long long)rows * splits * (4 + 2 * top);
 }
 
@@ -450,7 +484,8 @@ TGE_API int tge_token_logprobs(const void* logits, int is_bf16, long long stride
   TGE_REQUIRE(rows >= 0 && vocab > 0 && vocab < 0x7fff0000 && stride >= vocab, "token_logprobs: bad sizes rows=%d vocab=%d stride=%lld", rows, vocab, stride);
   TGE_REQUIRE(top >= 0 && top <= MOST_TOP && top <= vocab, "token_logprobs: %d alternatives of %d tokens, at most %d", top, vocab, MOST_TOP);
   if (rows == 0) return 0;
-  LogprobParams p{logits, tokens, stride, rows, vocab, top, splits_of(rows, vocab), chunk_of(rows, vocab), logprob, entropy, top_logprobs,
+  const Cut cut = cut_of(rows, vocab);
+  LogprobParams p{logits, tokens, stride, rows, vocab, top, cut.splits, cut.chunk, logprob, entropy, top_logprobs,
                   rank, top_ids, scratch, nullptr, status};
   TGE_REQUIRE((long long)rows * p.splits < 0x7fffffffll, "token_logprobs: %d rows of %d logits", rows, vocab);
   TGE_REQUIRE(scratch_floats >= tge_token_logprobs_floats(rows, vocab, top), "token_logprobs: %lld floats of scratch memory", scratch_floats);
@@ -459,8 +494,9 @@ TGE_API int tge_token_logprobs(const void* logits, int is_bf16, long long stride
   const bool vector = (uintptr_t)logits % 16 == 0 && stride * element % 16 == 0;
   auto run = [&](auto type) {
     using T = decltype(type);
-    if (vector) tge_launch(token_logprobs_kernel<T, true>, rows * p.splits, THREADS, 0, stream, p);
-    else tge_launch(token_logprobs_kernel<T, false>, rows * p.splits, THREADS, 0, stream, p);
+    if (cut.cluster > 0) return vector ? in_clusters<T, true>(p, cut.cluster, stream) : in_clusters<T, false>(p, cut.cluster, stream);
+    if (vector) tge_launch(token_logprobs_kernel<T, true, false>, rows * p.splits, THREADS, 0, stream, p);
+    else tge_launch(token_logprobs_kernel<T, false, false>, rows * p.splits, THREADS, 0, stream, p);
     if (p.splits == 1) return tge_launched("token_logprobs", 1);
     tge_launch(token_logprobs_join_kernel<T>, rows, THREADS, 0, stream, p);
     return tge_launched("token_logprobs", 2);

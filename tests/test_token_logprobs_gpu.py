@@ -119,3 +119,14 @@ def test_refusals(ops):
         with pytest.raises(ops.KernelError):
             call()
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,top", [(20, 40001, 32), (70, 33333, 5), (17, 100003, 0), (100, 50000, 20), (80, 70001, 32), (16, 16500, 1), (1, 12289, 32)])
+def test_rows_cut_every_way(ops, dtype, rows, vocab, top):
+    """Chunks that a cluster of 8 or 16 blocks joins, chunks that a second kernel joins, of odd vocabularies."""
+    gen = torch.Generator().manual_seed(rows)
+    logits = torch.randn(rows, vocab, generator=gen).to(dtype)
+    logits[0, :vocab // 2] = -math.inf
+    logits[-1] = torch.arange(vocab).to(dtype) / vocab
+    check(ops, logits, torch.randint(0, vocab, (rows,), generator=gen).tolist(), top)
