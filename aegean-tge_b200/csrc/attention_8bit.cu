@@ -142,11 +142,18 @@ struct Decode8 {
   float *parts, *states;                        // [2 x blocks][heads of a tile][head_dim], [2 x blocks][heads of a tile][2]
 };
 
-// The slices of 16 positions that request `seq` sees: [first, first + count).
+// The row of a request's token; -1: it brings none.
+__device__ __forceinline__ int row_of(const Decode8& p, int seq) {
+  const int row = p.q_start[seq], behind = p.q_start[seq + 1];
+  return behind > row ? row : -1;
+}
+
+// The slices of 16 positions that request `seq` sees: [first, first + count), one at least.
 struct Slices { int lo, hi, first, count; };
 __device__ __forceinline__ Slices slices_of(const Decode8& p, int seq) {
   Slices s;
-  const int pos = p.start_pos[seq];
+  const int start = p.start_pos[seq], here = p.q_start[seq], behind = p.q_start[seq + 1];      // one trip to memory
+  const int pos = behind > here ? start : -1;
   s.hi = min(max(pos + 1, 0), p.a.max_pages << p.page_shift);
   s.lo = p.a.window > 0 ? max(pos - p.a.window + 1, 0) : 0;
   s.first = s.lo >> 4;
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
   if (!CLUSTER && warp == 0) {                                    // where this block's run begins
     // 32 requests at a time; the first of them stay where they are
     const int first_count = lane < p.a.num_seqs ? (slices_of(p, lane).count + BEGIN) * p.units : 0;
-    const int first_token = lane < p.a.num_seqs ? p.q_start[lane] : 0;
+    const int first_token = lane < p.a.num_seqs ? row_of(p, lane) : 0;
     int total = __reduce_add_sync(0xffffffffu, first_count);
     for (int seq = 32 + lane; seq - lane < p.a.num_seqs; seq += 32)
       total += __reduce_add_sync(0xffffffffu, seq < p.a.num_seqs ? (slices_of(p, seq).count + BEGIN) * p.units : 0);
@@ -369,7 +376,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       int n = first_count;
       if (seq > 0) {
         n = seq + lane < p.a.num_seqs ? (slices_of(p, seq + lane).count + BEGIN) * p.units : 0;
-        token = seq + lane < p.a.num_seqs ? p.q_start[seq + lane] : 0;
+        token = seq + lane < p.a.num_seqs ? row_of(p, seq + lane) : 0;
       }
       int upto = n;
 #pragma unroll
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
     const int which = blockIdx.x / ranks;
     seq = which / p.units;
     unit = which - seq * p.units;
-    token = p.q_start[seq];
+    token = row_of(p, seq);
   } else {
     __syncthreads();
     seq = start_of[0];
@@ -462,8 +469,8 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       load_values<HD>(p, c, row, g, t);
     }
     if (warp < NT) {
-      const bool valid = 8 * warp + g < heads_here;
-      const T* src = static_cast<const T*>(p.a.q) + (size_t)token * p.a.q_stride + (size_t)(head0 + (valid ? 8 * warp + g : 0)) * HD;
+      const bool valid = token >= 0 && 8 * warp + g < heads_here;
+      const T* src = static_cast<const T*>(p.a.q) + (size_t)max(token, 0) * p.a.q_stride + (size_t)(head0 + (valid ? 8 * warp + g : 0)) * HD;
       const float unit_of = query_digits<T, HD, DIGITS>(src, valid, p.q_by_eight != 0, t, queries[warp]) * (p.a.scale * (LOG2E / 127.0f));
       if (t == 0) factors[8 * warp + g] = unit_of;
     }
@@ -610,7 +617,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
           }
       if (slice + 1 < last) load_values<HD>(p, c, row, g, t);
     }
-    if (bad && lane == 0) atomicOr(p.a.status, TGE_STATUS_BAD_PAGE);
+    if (bad && token >= 0 && lane == 0) atomicOr(p.a.status, TGE_STATUS_BAD_PAGE);
 
     // the warps' states meet in shared memory: the two numbers of a lane and a tile side by side, then the lanes g, then the tiles
     __syncthreads();                                              // whoever still reads the unit before
@@ -651,6 +658,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         acc.y = fmaf(fv, x.y, acc.y);
       }
       if (whole) {
+        if (token < 0) continue;
         if (p.a.sink != nullptr) {
           const float sink = p.a.sink[head0 + head] * LOG2E, top = fmaxf(most, sink), down = exp2_fast(most - top);
           sum = fmaf(sum, down, exp2_fast(sink - top));
@@ -671,7 +679,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
     }
     if constexpr (CLUSTER) {
       cluster_sync();
-      for (int i = rank * DWARPS * 32 + threadIdx.x; i < heads_here * (HD / 2); i += ranks * DWARPS * 32) {
+      for (int i = rank * DWARPS * 32 + threadIdx.x; token >= 0 && i < heads_here * (HD / 2); i += ranks * DWARPS * 32) {
         const int head = i / (HD / 2), pair = i - head * (HD / 2);
         const float sink = p.a.sink != nullptr ? p.a.sink[head0 + head] * LOG2E : NONE;
         float top = sink, all = 0.0f;
@@ -696,7 +704,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
     if (next_seq && at < end) {
       base = at;
       ++seq;
-      token = p.q_start[seq];
+      token = row_of(p, seq);
     }
   }
   if (!waited) pdl_wait();
@@ -727,7 +735,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_8bit_join_kernel(const
   if (first == last) return;
   const int kvh = unit / p.head_tiles, tile = unit - kvh * p.head_tiles;
   const int heads_here = min(HEADS, p.a.group - tile * HEADS), head0 = kvh * p.a.group + tile * HEADS;
-  const int token = p.q_start[seq];
+  const int token = row_of(p, seq);
+  if (token < 0) return;
   const int middle = first + (last - first + 2) / 2;
   const bool second = warp >= 8;
   for (int head = warp & 7; head < (heads_here + 7) / 8 * 8; head += 8) {

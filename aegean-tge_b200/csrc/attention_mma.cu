@@ -1640,7 +1640,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
     p.bq = tc2::ROWS / group;
     const int range = (num_splits > 1 ? p.split_tokens : max_ctx_len) + 2 * BKV;
     const size_t smem = tc2::smem_bytes(range / BKV, true);
-    if (!tc2::FITS || page_size != BKV || smem > tc2::MOST_SMEM || q_stride % 8 != 0 || (uintptr_t)q % 16 != 0 || out_stride % 8 != 0 ||
+    if (!tc2::FITS || page_size != BKV || group > 64 || smem > tc2::MOST_SMEM || q_stride % 8 != 0 || (uintptr_t)q % 16 != 0 || out_stride % 8 != 0 ||
         (uintptr_t)out % 16 != 0)
       return TGE_UNSUPPORTED;
     CUtensorMap map_k, map_v;

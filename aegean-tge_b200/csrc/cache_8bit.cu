@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ float most[2][2];                 // float16: the largest scales of the run's first and second 32 positions, keys' and values'
   const int run = blockIdx.x;
   pdl_wait();
-  pdl_trigger();                               // behind the wait: see the kernel above
+  if (p.starts != nullptr) pdl_trigger();      // behind the wait: see the kernel above; not at all where the table is written here
   if (run == p.runs) {                         // the block behind the runs, where no kernel in front has planned them
     if (blockIdx.y == 0) plan_runs(p);
     return;

@@ -1308,12 +1308,13 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                 splits = 1 if split == 0 or longest <= split else -(-longest // split)
                 states = prefill.tge_attention_mma_scratch_floats(tokens - first, heads, splits)
                 scratch = k_scale.new_empty(states) if states > 0 else None
-                _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), exponents.data_ptr(),
-                                                        table.data_ptr(), table.shape[1], k.shape[0], starts.data_ptr(), rows[1].data_ptr(),
-                                                        rows[2].data_ptr(), num_seqs - first, tokens - first, max_q_len, longest,
-                                                        rows[4].data_ptr(), out_stride, heads, kv_heads, float(scale), int(window), split,
-                                                        _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
-                return
+                rc = _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), exponents.data_ptr(),
+                                                             table.data_ptr(), table.shape[1], k.shape[0], starts.data_ptr(), rows[1].data_ptr(),
+                                                             rows[2].data_ptr(), num_seqs - first, tokens - first, max_q_len, longest,
+                                                             rows[4].data_ptr(), out_stride, heads, kv_heads, float(scale), int(window), split,
+                                                             _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
+                if rc != UNSUPPORTED:
+                    return
         k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, first, starts)
         if read is not None:
             read.record()

@@ -23,7 +23,7 @@ def quantise(x, scale):
 def append(quotients, scales, rows, start, block):
     """One request and one head.  ``quotients`` [n, dim] and ``scales`` [blocks]: what its cache holds for positions below ``start``
     (whole numbers there) and gets for those from there on: codes before their rounding.  ``rows`` [new, dim] float64."""
-    for b in range(start // block, -(-(start + len(rows)) // block)):
+    for b in range(start // block, -(-(start + len(rows)) // block) if len(rows) else 0):
         lo, hi = b * block, min((b + 1) * block, start + len(rows))
         new = rows[max(lo, start) - start:hi - start]
         before = 0.0 if lo >= start else float(scales[b])
