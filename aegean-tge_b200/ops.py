@@ -1192,17 +1192,19 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
         raise KernelError(f"8-bit pages must be [pages, kv_heads, page_size, head_dim], got {tuple(k_pages.shape)}")
     if dtype not in _FLOAT:
         raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
-    return _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, None)
+    sizes = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, len(ctx_lens), k_pages.shape[1], k_pages.shape[3])
+    _portions(q_start, start_pos, len(ctx_lens))
+    return _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, None)
 
 
-def _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
-    """:func:`read_cache_8bit`; with ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a position
-    whose values' scale is not finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a
-    fourth result, their exponents (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over
-    2^f, at most 1); None for a cache that this is not built for."""
+def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
+    """What :func:`read_cache_8bit` does, of arguments that were looked over (``sizes``: pages, positions in a page and in a block).  With
+    ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a position whose values' scale is not
+    finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a fourth result, their exponents
+    (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over 2^f, at most 1); None for a cache
+    that this is not built for."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
-    num_pages, page_size, block = _cache_8bit(k_pages, v_pages, k_scale, v_scale, block_table, num_seqs, kv_heads, head_dim)
-    _portions(q_start, start_pos, num_seqs)
+    num_pages, page_size, block = sizes
     # a window may leave out runs in front: the sum is then a bound
     mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
     runs, width = sum(mine), max(mine, default=0)
@@ -1294,13 +1296,19 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         rows = (q, start_pos, positions, seq_of_token, out)
         if first:
             rows = (q[first:], start_pos[first:], positions[first:], seq_of_token[first:], out[first:])
-        if is_bf16 and head_dim in (64, 128) and scale > 0 and q_stride % 8 == 0 and out_stride % 8 == 0 and (rows[0].data_ptr() | rows[4].data_ptr()) % 16 == 0:
+
+        def read_as(dtype):
+            return _read_8bit((num_pages, page_size, block), k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens,
+                              dtype, window, first, starts)
+
+        aligned = q_stride % 8 == 0 and out_stride % 8 == 0 and (rows[0].data_ptr() | rows[4].data_ptr()) % 16 == 0
+        if is_bf16 and head_dim in (64, 128) and scale > 0 and aligned:
             span = longest if window == 0 else min(longest, (-(-window // 64) + 1) * 64)
             split = choose_attention_split(tokens - first, num_seqs - first, max_q_len, span, heads, kv_heads, bound=span)
             prefill = attention_lib(head_dim)
             held = None
             if prefill.tge_attention_mma_halves_fit(longest, split):
-                held = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, torch.float16, window, first, starts)
+                held = read_as(torch.float16)
             if held is not None:
                 if read is not None:
                     read.record()
@@ -1315,7 +1323,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                                              _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
                 if rc != UNSUPPORTED:
                     return
-        k, v, table = _read_8bit(k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, q.dtype, window, first, starts)
+        k, v, table = read_as(q.dtype)
         if read is not None:
             read.record()
         attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
