@@ -293,7 +293,7 @@ __device__ __forceinline__ float query_digits(const T* q, bool valid, bool vecto
   });
   most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
   most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-  const float over = most > 1e-30f ? TOP / most : 0.0f;               // rows below that are zeros
+  const float over = most > TOP * 3e-39f ? TOP / most : 0.0f;         // (float32 has no larger factor: rows below that are zeros)
   each([&](int j, int w, const float (&x)[4]) {
     int whole[4];
 #pragma unroll
@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       m[nt][0] = m[nt][1] = NONE;
       l[nt][0] = l[nt][1] = 0.0f;
     }
-    float v_most = 1e-30f, v_over = HELD / 1e-30f;                // the largest scale of the values so far, and what scales are multiplied with
+    // the largest scale of the values so far, from the smallest whose factor float32 has, and what scales are multiplied with
+    float v_most = 3e-37f, v_over = HELD / 3e-37f;
 
     for (int slice = first; slice < last; ++slice) {
       const bool here = page >= 0 && page < p.a.num_pages;         // `asked` is this slice still

@@ -589,3 +589,24 @@ def test_attention_over_a_cache_that_was_read_back(ops):
         runs.fill_(-1)
         assert rel_error(out, want) < TOL[torch.bfloat16]
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [40, 1, 70]])
+@pytest.mark.parametrize("values,keys", [(1e-35, 1.0), (1e35, 1.0), (1.0, 1e-25), (1e-32, 1e25)])
+def test_attention_at_the_ends_of_the_range(ops, dtype, lens, values, keys):
+    """Values of very small and large scales; keys of them under queries that make up for it."""
+    heads, kv, dim = 6, 2, 128
+    cache = Cache([300, 1, 90], kv, dim, 64, 1)
+    cache.scales["v"] *= values
+    cache.scales["k"] *= keys
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(cache.held, lens)], DEV)
+    q = (torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(9)) * (0.5 / keys)).to(dtype)
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 3, max(lens), 300, heads, kv, dim, 0.09)
+    ops.check_status()
+    want, at = [], 0
+    for r, n in enumerate(lens):
+        want.append(plain.attend(q[at:at + n].view(n, heads, dim), cache.values("k", r), cache.values("v", r), cache.held[r] - n, 0.09, 0, None))
+        at += n
+    want = torch.cat(want).flatten(1)
+    assert rel_error(out.cpu().double() / values, want / values) < TOL[dtype]
