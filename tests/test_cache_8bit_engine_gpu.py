@@ -176,3 +176,31 @@ def test_command_line(folder):
     assert 0 < worst < 0.5 and math.isfinite(worst)
     assert "ids      :" in tge("generate", "--model", folder, "--tokens", "1 2 3", "--n", "4", "--cache-dtype", "int8", "--print-ids", "--num-pages", "8")
     assert "over a cache of int8" in tge("fidelity", "--model", folder, "--tokens", "20", "--cache-dtype", "int8", "--num-pages", "8", "--context", "64")
+
+
+def test_a_layer_that_reads_an_earlier_layers_cache(monkeypatch):
+    """It rotates its queries and stores nothing; the cut changes nothing, and the codes move its logits by little."""
+    import dataclasses
+
+    from aegean_tge_b200 import Engine, registry
+    from aegean_tge_b200.registry import Architecture, architecture_of, register_architecture
+    base = architecture_of(CONFIG)
+
+    def shared(config):
+        spec = base.build_spec(config)
+        return dataclasses.replace(spec, layers=(spec.layers[0], dataclasses.replace(spec.layers[1], cache_from=0)))
+
+    monkeypatch.setattr(registry, "_ARCHITECTURES", dict(registry._ARCHITECTURES))
+    register_architecture(Architecture("SharedCacheForCausalLM", base.parse_config, shared, base.random_plan))
+    raw = dict(CONFIG, architectures=["SharedCacheForCausalLM"])
+    tokens = prompt(90)
+
+    def rows(cuts, cache_dtype):
+        eng = Engine(random_config=raw, dtype="float32", context=256, max_tokens=4096, page_size=16, cache_dtype=cache_dtype)
+        assert len(eng.cache.groups) == 1
+        return run(eng, cuts, tokens)
+
+    whole, exact = rows([90], "int8"), rows([90], None)
+    assert float((rows([30, 1, 1, 58], "int8") - whole).abs().max()) < 2e-3 * float(whole.abs().max())
+    moved = float((whole - exact).abs().max()) / float(exact.abs().max())
+    assert 1e-6 < moved < 5e-2
