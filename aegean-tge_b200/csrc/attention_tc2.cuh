@@ -297,10 +297,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     const uint32_t p_row = p_smem + qt * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.0f;            // m_run: the row's reference, in raw score units
     const float step = HALVES ? tc::RESCALE_STEP : tc::RESCALE_STEP / row_scale;
-    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), f - F + 7, 2 to its negative.
+    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), the highest f seen, f - F + 7, 2 to its negative.
     // The row's reference is in units of the exponentials there.
     [[maybe_unused]] int now = -1;
-    [[maybe_unused]] float held = 0.0f, more = 0.0f, less = 1.0f;
+    [[maybe_unused]] float held = 0.0f, highest = 0.0f, more = 0.0f, less = 1.0f;
     float scale_now = row_scale;
     bool bad_page = false;
     for (int it = 0; it < num_tiles; ++it) {
@@ -312,15 +312,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
           now = both;
           scale_now = row_scale * power_of_two(both >> 16);
           const float f = (float)(short)both;
-          if (m_run == -INFINITY) {
-            held = f;                                       // nothing seen, nothing in the accumulator
-          } else if (f != held) {
-            // (down by no more than 80 at a time: the accumulator's numbers stay far from float32's largest)
-            const float to = fmaxf(f, held - 80.0f);
-            again = power_of_two(max((int)(held - to), -126));
-            held = to;
-          }
-          more = fmaxf(f - held + HELD, -60.0f);        // (float16 has nothing left there)
+          highest = m_run == -INFINITY ? f : fmaxf(highest, f);
+          // (2^-80 of the largest values seen is as far as it goes down: the accumulator's numbers stay below float32's largest)
+          const float to = fmaxf(f, highest - 80.0f);
+          if (m_run != -INFINITY) again = power_of_two(max((int)(held - to), -126));      // (else nothing is in the accumulator)
+          held = to;
+          more = fmaxf(f - held + HELD, -60.0f);            // (float16 has nothing left there)
           less = power_of_two((int)-more);
         }
       }

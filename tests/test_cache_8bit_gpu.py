@@ -491,11 +491,11 @@ def test_portions_whose_keys_are_cut(ops, monkeypatch, splits):
 
 @pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64)])
 @pytest.mark.parametrize("window", [0, 70])
-def test_portions_over_scales_far_apart(ops, heads, kv, dim, window):
+def test_portions_over_scales_far_apart(ops, heads, kv, dim, window, first=(0, 30, -30, 0, 5, 60, -60, 1, 0, -1)):
     """Values whose size changes by up to 2^120 from one run of 64 positions to the next, keys by 2^3; queries of 2^60 over keys of 2^-60."""
     held, lens = [640, 150, 130], [600, 150, 6]
     cache = Cache(held, kv, dim, 64, 1)
-    for r, (size, sizes) in enumerate(zip((60, 0, -60), ([0, 30, -30, 0, 5, 60, -60, 1, 0, -1], [-40, 20, 0], [1, 0, -100]))):
+    for r, (size, sizes) in enumerate(zip((60, 0, -60), (first, [-40, 20, 0], [1, 0, -100]))):
         for run, f in enumerate(sizes):
             where = cache.table[r, run].item()
             cache.scales["v"][where] *= 2.0 ** f
@@ -610,3 +610,10 @@ def test_attention_at_the_ends_of_the_range(ops, dtype, lens, values, keys):
         at += n
     want = torch.cat(want).flatten(1)
     assert rel_error(out.cpu().double() / values, want / values) < TOL[dtype]
+
+
+@pytest.mark.parametrize("first", [(100, 20, -60, -100, 40, 100, 10, -70, 0, 90), (-100, -20, 60, 110, 30, -50, -110, 0, 80, -80)])
+@pytest.mark.parametrize("window", [0, 70, 200])
+def test_portions_over_scales_that_fall_and_rise(ops, window, first):
+    """By 2^80 and more from run to run, several times in a row."""
+    test_portions_over_scales_far_apart(ops, 14, 2, 128, window, first)
