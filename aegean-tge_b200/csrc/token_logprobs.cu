@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Logpro
       mine.w += w;
     }
     mine.z += z;
-    if (!token_is_nan && (token < first || token >= first + ROUND)) {
+    // (in front of the token's round only where the round is all of this chunk's: what take() puts behind the chunk counts as -inf too)
+    if (!token_is_nan && (token < first || (token >= first + ROUND && first + ROUND <= end))) {
       const float from = first < token ? own : above;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) mine.before += v[i] >= from ? 1 : 0;

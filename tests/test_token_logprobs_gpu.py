@@ -130,3 +130,21 @@ def test_rows_cut_every_way(ops, dtype, rows, vocab, top):
     logits[0, :vocab // 2] = -math.inf
     logits[-1] = torch.arange(vocab).to(dtype) / vocab
     check(ops, logits, torch.randint(0, vocab, (rows,), generator=gen).tolist(), top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 152064), (16, 152064), (64, 152064), (17, 100003), (600, 20001)])
+def test_ranks_of_tokens_that_cannot_come(ops, dtype, rows, vocab):
+    """Rows of -inf but for a few: a token of -inf comes behind those and the -inf of lower index, whatever chunks a row is cut into."""
+    there = [7, vocab // 3, vocab // 2 + 1, vocab - 1]
+    borders = [b for blocks in (8, 16) for chunk in [-(-(-(-vocab // blocks)) // 64) * 64] for b in range(chunk, vocab, chunk)]
+    masked = sorted({t for b in [0, 100, 4096, 8192, vocab - 2, *borders] for t in (b - 1, b, b + 1, b + 2500) if 0 <= t < vocab} - set(there))
+    logits = torch.full((rows, vocab), -math.inf, device=DEV)
+    logits[:, there] = torch.tensor([2.0, -3e38, 0.5, -40.0], device=DEV)
+    logits = logits.to(dtype)
+    for first in range(0, len(masked), rows):
+        tokens = [masked[(first + r) % len(masked)] for r in range(rows)]
+        lp, _, rank, _, _ = ops.token_logprobs(logits, torch.tensor(tokens, dtype=torch.int32, device=DEV), top=0)
+        assert (lp == -math.inf).all()
+        assert rank.tolist() == [len(there) + t - sum(i < t for i in there) for t in tokens]
+    ops.check_status()
