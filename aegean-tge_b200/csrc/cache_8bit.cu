@@ -428,12 +428,15 @@ struct ReadParams {
   int* status;
 };
 
+// The first position that a step's queries see, from `start` on.  Pages in front of it are given back, also where they lie in its run of 64:
+// those positions are zeros and nobody's fault.
+__device__ __forceinline__ int first_seen(const ReadParams& p, int start) { return p.window > 0 ? max(start - p.window + 1, 0) : 0; }
+
 struct Span { int first, count; };             // a request's runs: from position 64 first on
 __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
   const int start = p.start_pos[seq], held = start + p.q_start[seq + 1] - p.q_start[seq];
-  const int lo = p.window > 0 ? max(start - p.window + 1, 0) : 0;
   Span s;
-  s.first = lo >> 6;
+  s.first = first_seen(p, start) >> 6;
   s.count = max((held + 63) / 64 - s.first, 0);
   return s;
 }
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
     if (HALVES && threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = 0;
     continue;
   }
-  const int held = p.start_pos[seq] + p.q_start[seq + 1] - p.q_start[seq];
+  const int start = p.start_pos[seq], held = start + p.q_start[seq + 1] - p.q_start[seq], seen_from = first_seen(p, start);
   if constexpr (UNITS) {
     // 16 bytes of the output to a thread and turn, side by side across a warp, four turns' codes of keys and values on their way together
     // (head sizes and pages are powers of two here: a division per eight numbers would cost more than they do)
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
         const bool held_here = j < 64 && pos < held;
         const int page = held_here && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
         const bool here = page >= 0 && page < p.num_pages;
-        if (held_here && !here) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+        if (held_here && !here && pos >= seen_from) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           scale[i][kv] = 0.0f;
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
     const int page_index = pos / p.page_size;
     const int page = pos < held && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
     const bool here = page >= 0 && page < p.num_pages;
-    if (!here && pos < held && lane == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+    if (!here && pos >= seen_from && pos < held && lane == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
     const size_t entry = here ? ((size_t)page * p.kv_heads + kvh) * p.page_size + pos % p.page_size : 0;
     float ks = here ? p.k_scale[entry / p.block] * (1.0f / 127.0f) : 0.0f;
     float vs = here ? p.v_scale[entry / p.block] * (1.0f / 127.0f) : 0.0f;

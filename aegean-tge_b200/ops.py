@@ -1185,7 +1185,8 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
     ``ctx_lens``: for every request how many positions it holds after the step (host numbers; the device has them as
     start_pos + q_start's differences).  k and v [runs, kv_heads, 64, head_dim] in ``dtype`` (float32 or bfloat16): the requests'
     positions one request after the other in runs of 64, zeros behind a request's last position; table [requests, runs of the
-    longest]: run i of a request, -1 where there is none.  With a ``window`` only runs that the step's queries may see.
+    longest]: run i of a request, -1 where there is none.  With a ``window`` only runs that the step's queries may see; positions in
+    front of the first one that they see may lie on pages that were given back, and are zeros there.
     ``first_seq``: leave out the requests before.
     """
     if k_pages.dim() != 4:

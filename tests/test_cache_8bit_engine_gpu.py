@@ -204,3 +204,34 @@ def test_a_layer_that_reads_an_earlier_layers_cache(monkeypatch):
     assert float((rows([30, 1, 1, 58], "int8") - whole).abs().max()) < 2e-3 * float(whole.abs().max())
     moved = float((whole - exact).abs().max()) / float(exact.abs().max())
     assert 1e-6 < moved < 5e-2
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_layers_over_a_window_whose_pages_are_given_back(monkeypatch, dtype):
+    """Pages behind the window are released as a request grows: cut prompts and single tokens go on without a fault."""
+    import dataclasses
+
+    from aegean_tge_b200 import Engine, ops, registry
+    from aegean_tge_b200.registry import Architecture, architecture_of, register_architecture
+    base = architecture_of(CONFIG)
+
+    def windowed(config):
+        spec = base.build_spec(config)
+        narrow = [dataclasses.replace(layer, mixer=dataclasses.replace(layer.mixer, params=dict(layer.mixer.params, window=100))) for layer in spec.layers]
+        return dataclasses.replace(spec, layers=tuple(narrow))
+
+    monkeypatch.setattr(registry, "_ARCHITECTURES", dict(registry._ARCHITECTURES))
+    register_architecture(Architecture("WindowedForCausalLM", base.parse_config, windowed, base.random_plan))
+    raw = dict(CONFIG, architectures=["WindowedForCausalLM"])
+    tokens = prompt(400)
+
+    def rows(cuts, cache_dtype):
+        eng = Engine(random_config=raw, dtype=dtype, context=512, max_tokens=4096, page_size=16, cache_dtype=cache_dtype)
+        found = run(eng, cuts, tokens)
+        ops.check_status()
+        return found
+
+    whole, exact = rows([400], "int8"), rows([400], None)
+    cut = rows([130, 70, 90, 1, 50, 1, 1, 57], "int8")
+    assert float((cut - whole).abs().max()) < {"float32": 2e-3, "bfloat16": 3.5e-2}[dtype] * float(whole.abs().max())
+    assert float((whole - exact).abs().max()) < 5e-2 * float(exact.abs().max())

@@ -617,3 +617,31 @@ def test_attention_at_the_ends_of_the_range(ops, dtype, lens, values, keys):
 def test_portions_over_scales_that_fall_and_rise(ops, window, first):
     """By 2^80 and more from run to run, several times in a row."""
     test_portions_over_scales_far_apart(ops, 14, 2, 128, window, first)
+
+
+def released(cache, lens, window):
+    """The cache's table as its manager leaves it over a window: pages wholly behind the first query's window are given back."""
+    table = cache.table.clone()
+    for r, (held, n) in enumerate(zip(cache.held, lens)):
+        table[r, :max(held - n - window + 1, 0) // cache.page] = -1
+    return table
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64), (4, 2, 80), (2, 1, 256)])
+@pytest.mark.parametrize("page,window", [(16, 100), (32, 33), (16, 1)])
+def test_windows_over_released_pages(ops, dtype, heads, kv, dim, page, window):
+    """Pages behind the window are nobody's: not read, and no fault of the call's.  One that a query sees is."""
+    lens = [70, 1, 30, 65, 40, 2]
+    cache = Cache([200, 150, 290, 65, 350, 131], kv, dim, page, 1)
+    cache.table = released(cache, lens, window)
+    out, want = attend(ops, cache, lens, heads, dtype, window=window, ctx_lens=cache.held)
+    assert rel_error(out, want) < TOL[dtype]
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(cache.held, lens)], DEV)
+    ops.read_cache_8bit(*cache.device(), cache.table.to(DEV), q_start, start_pos, cache.held, dtype, window=window)
+    ops.check_status()
+    missing = cache.table.clone()
+    missing[4, (350 - 40 - window + 1) // page] = -1
+    with pytest.raises(ops.DeviceStatusError, match="page"):
+        ops.read_cache_8bit(*cache.device(), missing.to(DEV), q_start, start_pos, cache.held, dtype, window=window)
+        ops.check_status()
