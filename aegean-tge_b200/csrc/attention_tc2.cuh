@@ -23,8 +23,8 @@
 // `page_exponents`), no larger than 1, and a row of queries over one of its own.  2^e joins the scale of the tile's scores; e and f are
 // multiples of 8, so that few tiles bring new ones and a tile like the last costs a row a comparison and two products.  (Exponents that
 // change by one from tile to tile, and loads of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at
-// most 2^15: the reference moves at 2^8), and the accumulator follows where f changes; they keep 11 bits down to 2^-21 of a probability of
-// 1 and some down to 2^-31.
+// most 2^15: the reference moves at 2^8), and the accumulator follows where f changes, row by row: how far goes by what the row sees of the
+// tile.  They keep 11 bits down to 2^-21 of a probability of 1 and some down to 2^-31.
 #pragma once
 
 namespace tc2 {
@@ -297,28 +297,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     const uint32_t p_row = p_smem + qt * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.0f;            // m_run: the row's reference, in raw score units
     const float step = HALVES ? tc::RESCALE_STEP : tc::RESCALE_STEP / row_scale;
-    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), the highest f seen, f - F + 7, 2 to its negative.
-    // The row's reference is in units of the exponentials there.
+    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), a bound 2^highest of what each key has added to
+    // the sum.  The row's reference is in units of the exponentials there.
     [[maybe_unused]] int now = -1;
-    [[maybe_unused]] float held = 0.0f, highest = 0.0f, more = 0.0f, less = 1.0f;
+    [[maybe_unused]] float held = 0.0f, highest = 0.0f;
     float scale_now = row_scale;
     bool bad_page = false;
     for (int it = 0; it < num_tiles; ++it) {
       const int k0 = keys.start(it);
-      float again = 1.0f;                              // what the accumulator takes as F moves
       if constexpr (HALVES) {
         const int both = local_exponents[(k0 >> p.page_shift) - first_page];
         if (both != now) {
           now = both;
           scale_now = row_scale * power_of_two(both >> 16);
-          const float f = (float)(short)both;
-          highest = m_run == -INFINITY ? f : fmaxf(highest, f);
-          // (2^-80 of the largest values seen is as far as it goes down: the accumulator's numbers stay below float32's largest)
-          const float to = fmaxf(f, highest - 80.0f);
-          if (m_run != -INFINITY) again = power_of_two(max((int)(held - to), -126));      // (else nothing is in the accumulator)
-          held = to;
-          more = fmaxf(f - held + HELD, -60.0f);            // (float16 has nothing left there)
-          less = power_of_two((int)-more);
         }
       }
       mbar_wait_bounded(my_s_bar + 8 * (it & 1), (uint32_t)(it >> 1) & 1u, p.status);
@@ -369,6 +360,32 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       const float m_new = moved ? mx : m_run;
       const float m_use = m_new == -INFINITY ? 0.0f : m_new;
       const float corr = exp2f(HALVES ? m_run - m_use : (m_run - m_use) * row_scale);      // exp2(-inf) = 0 while nothing was visible yet
+      float factor = corr;                             // what the accumulator takes as the reference and F move
+      bool follow = moved;
+      [[maybe_unused]] float more = HELD, less = 1.0f / 128.0f;      // probabilities go to the tensor core times 2^more; 2^-more
+      if constexpr (HALVES) {
+        // F follows the tile's f where that is lower, so that small values keep their bits, and what the row's largest probability makes of
+        // 2^f where that is higher.  A tile that the row does not see moves nothing; f = F is nearly always.
+        if (moved) highest = m_run == -INFINITY ? -INFINITY : highest - (m_new - m_run);
+        const float f = (float)(short)now;
+        if (f != held) {
+          const float lead = f + (mx - m_use);
+          float to = held;
+          if (mx > -INFINITY) {
+            // (2^-80 of the largest products is as far as it goes down: the accumulator's numbers stay below float32's largest)
+            if (m_run == -INFINITY || f < held) to = fmaxf(f, ceilf(highest) - 80.0f);
+            else if (lead > held) to = ceilf(lead);
+          }
+          if (to != held) {
+            factor = exp2f((m_run - m_use) + (held - to));         // (in one: the two may be far apart on either side)
+            follow = true;
+            held = to;
+          }
+          more = fmaxf(f - held + HELD, -60.0f);            // (float16 has nothing left there)
+          less = power_of_two(max((int)-more, -126));       // (nor the sum)
+        }
+        highest = fmaxf(highest, held);
+      }
       const float shift = HALVES ? more - m_use : -m_use * row_scale;
       const uint64_t scale2 = tc::pair(scale_now, scale_now), shift2 = tc::pair(shift, shift);
       uint64_t sum2 = tc::pair(0.0f, 0.0f);
@@ -397,11 +414,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       float sum_even, sum_odd;
       tc::unpair(sum2, sum_even, sum_odd);
       l_run = l_run * corr + (HALVES ? (sum_even + sum_odd) * less : sum_even + sum_odd);
-      const bool rescale = it > 0 && ((moved && m_run != -INFINITY) || (HALVES && again != 1.0f));
+      const bool rescale = it > 0 && follow && m_run != -INFINITY;          // (else nothing is in the accumulator)
       m_run = m_new;
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // P, before the tensor core reads it
       if (it > 0 && __any_sync(0xffffffffu, rescale)) {
-        const float factor = HALVES ? corr * again : rescale ? corr : 1.0f;
+        if (!rescale) factor = 1.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o_bits[32];

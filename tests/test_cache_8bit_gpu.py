@@ -645,3 +645,61 @@ def test_windows_over_released_pages(ops, dtype, heads, kv, dim, page, window):
     with pytest.raises(ops.DeviceStatusError, match="page"):
         ops.read_cache_8bit(*cache.device(), missing.to(DEV), q_start, start_pos, cache.held, dtype, window=window)
         ops.check_status()
+
+
+def row_errors(out, q, cache, lens, heads, scale, window=0):
+    """Of every row and head the error over the sum of its probabilities times magnitudes of values, the largest number's."""
+    worst, at = 0.0, 0
+    for r, n in enumerate(lens):
+        k, v, rows = cache.values("k", r), cache.values("v", r), q[at:at + n].view(n, heads, cache.dim)
+        want = plain.attend(rows, k, v, cache.held[r] - n, scale, window, None)
+        size = plain.attend(rows, k, v.abs(), cache.held[r] - n, scale, window, None).amax(-1)
+        got = out[at:at + n].cpu().double().view(n, heads, cache.dim)
+        assert torch.isfinite(got).all()
+        worst = max(worst, float(((got - want).abs().amax(-1) / size).max()))
+        at += n
+    return worst
+
+
+def portions_of(ops, cache, lens, heads, q, scale, window=0):
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(cache.held, lens)], DEV)
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, len(lens), max(lens), max(cache.held),
+                             heads, cache.kv_heads, cache.dim, scale, window=window, ctx_lens=cache.held)
+    ops.check_status()
+    return out
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("powers", [(-70, 70, -70), (-100, 100, 0), (100, -100, 100), (0, 115, -115), (-120, 120, -120)])
+@pytest.mark.parametrize("window", [0, 70])
+def test_portions_over_scales_that_jump_inside_a_block_of_queries(ops, heads, kv, dim, powers, window):
+    """Values whose size changes by up to 2^240 where one run of 64 positions ends and the next begins: rows that see the next run and rows that do not
+    lie in one block of queries."""
+    held = lens = [192, 100]
+    cache = Cache(held, kv, dim, 64, 1)
+    for r in range(2):
+        for run in range(cache.table.shape[1]):
+            if cache.table[r, run] >= 0:
+                cache.scales["v"][cache.table[r, run].item()] *= 2.0 ** powers[run]
+    q = (torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(4))).bfloat16()
+    out = portions_of(ops, cache, lens, heads, q, 0.02, window)
+    assert row_errors(out, q, cache, lens, heads, 0.02, window) < 2 ** -7
+
+
+@pytest.mark.parametrize("far", [60, 100, 200, 400])
+@pytest.mark.parametrize("base,power", [(0, 20), (0, 60), (0, 120), (-110, 230)])
+@pytest.mark.parametrize("order", [(0, 1), (1, 0)])
+def test_portions_that_hardly_weigh_a_run_of_large_values(ops, far, base, power, order):
+    """A run whose values are 2^120 the others' size and more, and whose scores lie far below theirs."""
+    heads, kv, dim, held = 4, 2, 128, [128]
+    cache = Cache(held, kv, dim, 64, 1)
+    codes = torch.randint(-127, 128, (dim,), generator=torch.Generator().manual_seed(3)).to(torch.int8)
+    near, away = (cache.table[0, i].item() for i in order)
+    cache.codes["k"][near], cache.codes["k"][away] = codes, -codes
+    cache.scales["k"].fill_(1.0)
+    cache.scales["v"][near] *= 2.0 ** base
+    cache.scales["v"][away] *= 2.0 ** (base + power)
+    q = (codes.float() / 127).repeat(128, heads, 1).flatten(1).bfloat16()
+    scale = far / 2 * math.log(2) / float((codes.float() / 127).pow(2).sum())            # scores of far / 2 and its negative, in powers of two
+    out = portions_of(ops, cache, held, heads, q, scale)
+    assert row_errors(out, q, cache, held, heads, scale) < 2 ** -7
