@@ -17,12 +17,12 @@
 //
 // HALVES: keys and values of a cache of 8-bit codes, read back into float16 pages of 64 positions.  float16 holds them, and the probabilities,
 // to 2^-12 where bfloat16 rounds them to 2^-9: a prompt of 2,048 tokens at 28 heads over 4 comes to 1.7e-3 of float64, which is the rounding
-// of the result, and to 3.7e-3 with everything in bfloat16, for 64 us beside 60.  (Whole codes in bfloat16 with a factor per key on the
+// of the result, and to 3.7e-3 with everything in bfloat16, for 63 us beside 60.  (Whole codes in bfloat16 with a factor per key on the
 // scores: 2.7e-3, 64 us; with a factor per value on the probabilities too: 2.3e-3, 71 us.)
 // float16's range is short, so a page's keys and values are held over powers of two 2^e and 2^f of that page and kv head ((f, e) in
 // `page_exponents`), no larger than 1, and a row of queries over one of its own.  2^e joins the scale of the tile's scores; e and f are
-// multiples of 8, so that few tiles bring new ones and a tile like the last costs a row a comparison and two products.  (Exponents that
-// change by one from tile to tile, and loads of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at
+// multiples of 8, so that few tiles bring a new f and the accumulator's rescaling.  (Exponents that change by one from tile to tile, and loads
+// of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at
 // most 2^15: the reference moves at 2^8), and the accumulator follows where f changes, row by row: how far goes by what the row sees of the
 // tile.  They keep 11 bits down to 2^-21 of a probability of 1 and some down to 2^-31.
 #pragma once
@@ -65,6 +65,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return d;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }      // -126 to 127
+// x 2^e for e of -240 to 240.  Never 0 or infinite, which would make NaN of a masked score or of a score of 0: below 2^-110 it is x 2^-110 (scores
+// that small are zeros), and it ends at float32's largest number.
+__device__ __forceinline__ float times_power(float x, int e) {
+  return fminf(fmaxf(x * 65536.0f * power_of_two(min(max(e - 16, -126), 127)), 1.17549435e-38f), 3.402823466e38f);
+}
 
 template <bool HALVES>
 __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
@@ -257,7 +262,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     // Q row into the K-major swizzled tile of its query tile: 64-column blocks of [128 rows][128 bytes]
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)row_token * p.q_stride + (size_t)row_head * HD);
     unsigned char* q_tile = generic + qt * Q_BYTES;
-    float row_scale = p.scale_log2;                      // what the row's scores are multiplied with (2^e of their tile apart)
+    const float row_scale = p.scale_log2;                // what the row's scores are multiplied with, times 2^(up + e) over float16 pages
+    [[maybe_unused]] int up = 0;
     if constexpr (HALVES) {
       for (int i = tid; i <= last_page - first_page; i += SOFTMAX_WARPS * 32) {      // (e, f) of the tiles, behind the barrier of the queries
         const int page = max(local_table[i], 0);
@@ -272,9 +278,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       for (int c = 0; c < HD / 8; ++c)
         for (uint32_t w : {row[c].x, row[c].y, row[c].z, row[c].w})
           most = tc::max3(most, fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u)));
-      const int up = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 120) : 0;
+      up = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 120) : 0;
       const float over = power_of_two(-up);
-      row_scale *= power_of_two(up);
       auto halves = [&](uint32_t w) { return pack_f16(__uint_as_float(w << 16) * over, __uint_as_float(w & 0xffff0000u) * over); };
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c)
@@ -297,20 +302,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     const uint32_t p_row = p_smem + qt * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.0f;            // m_run: the row's reference, in raw score units
     const float step = HALVES ? tc::RESCALE_STEP : tc::RESCALE_STEP / row_scale;
-    // float16 pages: the tile's exponents, F (the accumulator's values are over 2^(F - 7)), a bound 2^highest of what each key has added to
-    // the sum.  The row's reference is in units of the exponentials there.
-    [[maybe_unused]] int now = -1;
+    // float16 pages: F (the accumulator's values are over 2^(F - 7)), a bound 2^highest of what each key has added to the sum.  The row's
+    // reference is in units of the exponentials there.
     [[maybe_unused]] float held = 0.0f, highest = 0.0f;
-    float scale_now = row_scale;
     bool bad_page = false;
     for (int it = 0; it < num_tiles; ++it) {
       const int k0 = keys.start(it);
+      [[maybe_unused]] int now = 0;                    // the tile's exponents
+      float scale_now = row_scale;
       if constexpr (HALVES) {
-        const int both = local_exponents[(k0 >> p.page_shift) - first_page];
-        if (both != now) {
-          now = both;
-          scale_now = row_scale * power_of_two(both >> 16);
-        }
+        now = local_exponents[(k0 >> p.page_shift) - first_page];
+        scale_now = times_power(row_scale, up + (now >> 16));
       }
       mbar_wait_bounded(my_s_bar + 8 * (it & 1), (uint32_t)(it >> 1) & 1u, p.status);
       fence_after();

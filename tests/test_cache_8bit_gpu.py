@@ -703,3 +703,16 @@ def test_portions_that_hardly_weigh_a_run_of_large_values(ops, far, base, power,
     scale = far / 2 * math.log(2) / float((codes.float() / 127).pow(2).sum())            # scores of far / 2 and its negative, in powers of two
     out = portions_of(ops, cache, held, heads, q, scale)
     assert row_errors(out, q, cache, held, heads, scale) < 2 ** -7
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("keys,queries,scale", [(-90, -90, 0.09), (-120, -60, 0.09), (-60, -120, 0.09), (-120, 118, 2.0), (-128, 118, 300.0)])
+def test_portions_of_queries_and_keys_at_the_ends_of_the_range(ops, window, keys, queries, scale):
+    """Scores that float32 has no number for are zeros: every key weighs the same, and masked ones nothing.  Queries whose product with the scale alone
+    float32 has no number for."""
+    heads, kv, dim, held = 6, 2, 128, [150]
+    cache = Cache(held, kv, dim, 64, 1)
+    cache.scales["k"] *= 2.0 ** keys
+    q = (torch.randn(150, heads * dim, generator=torch.Generator().manual_seed(6)) * 2.0 ** queries).bfloat16()
+    out = portions_of(ops, cache, held, heads, q, scale, window)
+    assert row_errors(out, q, cache, held, heads, scale, window) < 2 ** -7
