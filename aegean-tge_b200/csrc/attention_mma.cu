@@ -25,6 +25,7 @@
 #include <atomic>
 #include <map>
 #include <tuple>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -86,7 +87,10 @@ struct AttnParams {
   int trigger_late, beside;
   unsigned long long ticket;
   float scale_log2;
-  const int* page_exponents;      // the two-tile prefill kernel over float16 pages: of every page and kv head, f below and e above
+  // the two-tile prefill kernel over float16 pages: of every page and kv head, f below and e above; 1 in it: codes as they are, and of every
+  // position (what a score is multiplied with, the logarithm of what a value is)
+  const int* page_exponents;
+  const float4* page_factors;     // [pages, kv_heads, 32], two positions each
 };
 
 // Tickets of side-by-side launches: a number of its own for every such pair of launches, in the place that it falls on.  The first
@@ -1493,7 +1497,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
                               int first_token, const float* sink, int leave_states, int v_pitch, const float* dist_bias,
                               int dist_span, int keep_first, const void* gate, int gate_stride, int gate_elements,
                               int shared_keys, cudaStream_t stream, LeadingTokens* lead = nullptr, unsigned long long beside = 0,
-                              const int* page_exponents = nullptr) {
+                              const void* page_factors = nullptr) {
   TGE_REQUIRE(tokens >= 0 && num_seqs >= 0, "attention_mma: negative sizes");
   TGE_REQUIRE(dist_bias == nullptr || (dist_span > 0 && scale != 0.0f), "attention_mma: a bias by distance needs its span");
   TGE_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
@@ -1530,7 +1534,8 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
   TGE_REQUIRE(!shared_keys || (single && p.v_in_keys), "attention_mma: runs of heads over the same keys are for single tokens and values inside the keys");
   p.kv_pool = shared_keys ? 1 : kv_heads;
   p.trigger_late = 0;
-  p.page_exponents = page_exponents;
+  p.page_factors = static_cast<const float4*>(page_factors);
+  p.page_exponents = page_factors == nullptr ? nullptr : static_cast<const int*>(page_factors) + (size_t)num_pages * kv_heads * 128;
   p.beside = beside != 0;
   p.ticket = beside;
   p.q_stride = q_stride; p.out_stride = out_stride;
@@ -1635,7 +1640,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
     return 1;
   }
 #if TGE_TMA_KERNELS
-  if (page_exponents != nullptr) {
+  if (page_factors != nullptr) {
     // float16 pages with exponents: pages of one call, the two-tile kernel, two query tiles per block and one block per SM
     p.bq = tc2::ROWS / group;
     const int range = (num_splits > 1 ? p.split_tokens : max_ctx_len) + 2 * BKV;
@@ -1769,9 +1774,10 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
   return 1;
 }
 
-// Portions over float16 pages of 64 positions whose keys and values are over 2^e and 2^f of their page and kv head, whole numbers of -120 to 120 in
-// `page_exponents` ([num_pages, kv_heads], f in the lower 16 bits and e in the upper).  Whether this library's kernel takes
-// portions whose longest context is `max_ctx_len`:
+// Portions over float16 pages of 64 positions as cache_8bit.cu reads them back: keys and values over 2^e and 2^f of their page and kv head, multiples of
+// 8 from -120 to 120, or codes over 128 with factors.  `page_factors` (on 16 bytes): two numbers a position, [num_pages, kv_heads, 64, 2], and
+// behind them a word a page and kv head, f in its lower 16 bits and e in the upper, plus 1 where the page has factors.
+// Whether this library's kernel takes portions whose longest context is `max_ctx_len`:
 TGE_API int tge_attention_mma_halves_fit(int max_ctx_len, int split_tokens) {
 #if TGE_TMA_KERNELS
   const int range = (split_tokens > 0 && split_tokens < max_ctx_len ? split_tokens : max_ctx_len) + 2 * BKV;
@@ -1781,16 +1787,17 @@ TGE_API int tge_attention_mma_halves_fit(int max_ctx_len, int split_tokens) {
 #endif
 }
 
-TGE_API int tge_attention_mma_halves(const void* q, int q_stride, const void* k_pages, const void* v_pages, const int* page_exponents,
+TGE_API int tge_attention_mma_halves(const void* q, int q_stride, const void* k_pages, const void* v_pages, const void* page_factors,
                                       const int* block_table, int max_pages, int num_pages, const int* q_start,
                                       const int* start_pos, const int* positions, int num_seqs, int tokens, int max_q_len, int max_ctx_len,
                                       void* out, int out_stride, int heads, int kv_heads, float scale, int window, int split_tokens,
                                       float* scratch, int* status, const float* sink, cudaStream_t stream) {
-  TGE_REQUIRE(page_exponents != nullptr && max_q_len > 1 && scale > 0.0f, "attention_mma: float16 pages are for portions and positive scales");
+  TGE_REQUIRE(page_factors != nullptr && (uintptr_t)page_factors % 16 == 0 && max_q_len > 1 && scale > 0.0f,
+              "attention_mma: float16 pages are for portions and positive scales");
 #if TGE_TMA_KERNELS
   return attention_dispatch(q, q_stride, k_pages, v_pages, block_table, max_pages, num_pages, BKV, q_start, start_pos, positions, num_seqs, tokens,
                             max_q_len, max_ctx_len, out, out_stride, heads, kv_heads, scale, window, split_tokens, scratch, status, 0, sink, 0, 0,
-                            nullptr, 0, 0, nullptr, 0, 0, 0, stream, nullptr, 0, page_exponents);
+                            nullptr, 0, 0, nullptr, 0, 0, 0, stream, nullptr, 0, page_factors);
 #else
   return TGE_UNSUPPORTED;
 #endif

@@ -22,9 +22,12 @@
 // float16's range is short, so a page's keys and values are held over powers of two 2^e and 2^f of that page and kv head ((f, e) in
 // `page_exponents`), no larger than 1, and a row of queries over one of its own.  2^e joins the scale of the tile's scores; e and f are
 // multiples of 8, so that few tiles bring a new f and the accumulator's rescaling.  (Exponents that change by one from tile to tile, and loads
-// of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at
-// most 2^15: the reference moves at 2^8), and the accumulator follows where f changes, row by row: how far goes by what the row sees of the
-// tile.  They keep 11 bits down to 2^-21 of a probability of 1 and some down to 2^-31.
+// of them beside the scores, took 70 us.)  Probabilities go to the tensor core times 2^7 (at most 2^15: the reference moves at 2^8), and the
+// accumulator follows where f changes, row by row: how far goes by what the row sees of the tile.  They keep 11 bits down to 2^-21 of a
+// probability of 1 and some down to 2^-31.
+// A page whose scales lie too far apart for that holds whole codes, and two factors a position in `page_factors`: a key's on its score; a value's,
+// as a logarithm, on its probability, over a power of two above the largest such product that the row sees.  So what a row cannot see, or hardly
+// weighs, does not decide how many bits the rest keeps.
 #pragma once
 
 namespace tc2 {
@@ -69,6 +72,13 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // that small are zeros), and it ends at float32's largest number.
 __device__ __forceinline__ float times_power(float x, int e) {
   return fminf(fmaxf(x * 65536.0f * power_of_two(min(max(e - 16, -126), 127)), 1.17549435e-38f), 3.402823466e38f);
+}
+
+// A load that stays where it stands: a row of them in front of their use would take the registers of the scores.
+__device__ __forceinline__ float4 load_in_turn(const float4* src) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(src) : "memory");
+  return v;
 }
 
 template <bool HALVES>
@@ -306,13 +316,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
     // reference is in units of the exponentials there.
     [[maybe_unused]] float held = 0.0f, highest = 0.0f;
     bool bad_page = false;
+    auto all_tiles = [&](auto apart) {
+    constexpr bool SOME_APART = decltype(apart)::value;       // float16 pages of which some hold whole codes
     for (int it = 0; it < num_tiles; ++it) {
       const int k0 = keys.start(it);
       [[maybe_unused]] int now = 0;                    // the tile's exponents
+      [[maybe_unused]] const float4* factors = nullptr;      // the tile's, if its page holds whole codes
       float scale_now = row_scale;
       if constexpr (HALVES) {
-        now = local_exponents[(k0 >> p.page_shift) - first_page];
+        const int index = (k0 >> p.page_shift) - first_page;
+        now = local_exponents[index];
         scale_now = times_power(row_scale, up + (now >> 16));
+        if (SOME_APART && (now & 1)) factors = p.page_factors + ((size_t)max(local_table[index], 0) * p.kv_heads + kvh) * (BKV / 2);
       }
       mbar_wait_bounded(my_s_bar + 8 * (it & 1), (uint32_t)(it >> 1) & 1u, p.status);
       fence_after();
@@ -340,6 +355,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
             s_bits[j] = __float_as_uint(fmaf(bias_row[min(max(d0 - j, 0), p.dist_span - 1)], p.bias_to_raw, __uint_as_float(s_bits[j])));
         }
       }
+      if (SOME_APART && factors != nullptr) {          // a factor for each score
+        const float half = power_of_two(up / 2), rest = times_power(row_scale, up - up / 2);
+        auto scaled = [&](uint32_t raw, float x) {
+          return __float_as_uint(__uint_as_float(raw) * fminf(fmaxf(x * half * rest, 1.17549435e-38f), 3.402823466e38f));
+        };
+#pragma unroll
+        for (int j = 0; j < BKV; j += 2) {
+          const float4 by = load_in_turn(factors + j / 2);
+          s_bits[j] = scaled(s_bits[j], by.x);
+          s_bits[j + 1] = scaled(s_bits[j + 1], by.z);
+        }
+        scale_now = 1.0f;
+      }
       // a tile that every row of the warp sees whole needs no mask
       // (rows beyond the tile's queries hold zeros and are never stored: they need none either)
       const bool whole = !row_valid || (k0 + BKV - 1 <= row_pos && ((k0 >= first_key && k0 >= lo) || k0 + BKV <= keys.keep) && k0 + BKV <= hi);
@@ -365,18 +393,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       float factor = corr;                             // what the accumulator takes as the reference and F move
       bool follow = moved;
       [[maybe_unused]] float more = HELD, less = 1.0f / 128.0f;      // probabilities go to the tensor core times 2^more; 2^-more
+      [[maybe_unused]] float sum_apart = 0.0f;           // the probabilities' sum where what goes to the tensor core is not they
       if constexpr (HALVES) {
         // F follows the tile's f where that is lower, so that small values keep their bits, and what the row's largest probability makes of
         // 2^f where that is higher.  A tile that the row does not see moves nothing; f = F is nearly always.
         if (moved) highest = m_run == -INFINITY ? -INFINITY : highest - (m_new - m_run);
-        const float f = (float)(short)now;
+        float f = (float)(short)(now & ~1), lead = f + (mx - m_use);
+        if (SOME_APART && factors != nullptr) {
+          // a probability and its value's scale go to the tensor core as one number, over what the row's largest such number is below
+          float most = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < BKV; j += 2) {
+            const float4 by = load_in_turn(factors + j / 2);
+            const float a = __uint_as_float(s_bits[j]) - m_use, b = __uint_as_float(s_bits[j + 1]) - m_use;
+            sum_apart += tc::ex2(a) + tc::ex2(b);
+            most = tc::max3(most, a + by.y, b + by.w);
+            s_bits[j] = __float_as_uint(a + by.y);
+            s_bits[j + 1] = __float_as_uint(b + by.w);
+          }
+          lead = most;
+          f = fminf(fmaxf(ceilf(lead), -120.0f), 128.0f);
+        }
         if (f != held) {
-          const float lead = f + (mx - m_use);
           float to = held;
           if (mx > -INFINITY) {
             // (2^-80 of the largest products is as far as it goes down: the accumulator's numbers stay below float32's largest)
             if (m_run == -INFINITY || f < held) to = fmaxf(f, ceilf(highest) - 80.0f);
-            else if (lead > held) to = ceilf(lead);
+            else if (lead > held) to = fminf(ceilf(lead), 128.0f);
           }
           if (to != held) {
             factor = exp2f((m_run - m_use) + (held - to));         // (in one: the two may be far apart on either side)
@@ -386,9 +429,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
           more = fmaxf(f - held + HELD, -60.0f);            // (float16 has nothing left there)
           less = power_of_two(max((int)-more, -126));       // (nor the sum)
         }
+        if (SOME_APART && factors != nullptr) more = HELD - held;
         highest = fmaxf(highest, held);
       }
-      const float shift = HALVES ? more - m_use : -m_use * row_scale;
+      const float shift = SOME_APART && factors != nullptr ? more : HALVES ? more - m_use : -m_use * row_scale;
       const uint64_t scale2 = tc::pair(scale_now, scale_now), shift2 = tc::pair(shift, shift);
       uint64_t sum2 = tc::pair(0.0f, 0.0f);
       if (it > 0) {
@@ -415,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       }
       float sum_even, sum_odd;
       tc::unpair(sum2, sum_even, sum_odd);
-      l_run = l_run * corr + (HALVES ? (sum_even + sum_odd) * less : sum_even + sum_odd);
+      l_run = l_run * corr + (!HALVES ? sum_even + sum_odd : SOME_APART && factors != nullptr ? sum_apart : (sum_even + sum_odd) * less);
       const bool rescale = it > 0 && follow && m_run != -INFINITY;          // (else nothing is in the accumulator)
       m_run = m_new;
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // P, before the tensor core reads it
@@ -435,6 +479,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_tc2_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(my_p_bar);
     }
+    };
+    // (two loops: one that looks for factors in every tile takes a prompt of 2,048 tokens from 62 to 67 us)
+    bool some_apart = false;
+    if constexpr (HALVES) {
+      for (int i = lane; i <= last_page - first_page; i += 32) some_apart |= local_exponents[i] & 1;
+      some_apart = __any_sync(0xffffffffu, some_apart);
+    }
+    if (some_apart) all_tiles(std::integral_constant<bool, HALVES>());
+    else all_tiles(std::false_type());
     if (bad_page && p.status) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
     mbar_wait_bounded(my_o_bar, (uint32_t)(num_tiles - 1) & 1u, p.status);
     fence_after();

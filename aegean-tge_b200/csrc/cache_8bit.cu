@@ -422,7 +422,8 @@ struct ReadParams {
   const int *block_table, *q_start, *start_pos;
   int max_pages, num_pages, page_size, block, first_seq, num_seqs, kv_heads, head_dim, window;
   void *k_out, *v_out;
-  int* exponents;                              // [runs, kv_heads], for float16 output: f below, e above
+  float2* factors;                             // [runs, kv_heads, 64], for float16 output: of runs whose scales lie far apart, see below
+  int* exponents;                              // [runs, kv_heads], for float16 output: f below, e above; 1: the run has factors
   int *table, *starts;
   int runs, width;
   int* status;
@@ -464,8 +465,11 @@ __global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p)
   plan_runs(p);
 }
 
-// float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ,
-// and what is lost is nothing (the largest numbers of a run are above 2^-9, float16 keeps its 11 bits down to 2^-14).
+// float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ.
+// float16's numbers are 2^-24 apart below 2^-14, so a position whose scale is at least 2^-13 of the power keeps 2^-12 of its own largest
+// number, which is what float16 keeps of any.  A run with a smaller scale (its largest one is above 2^-8 of the power: they lie 2^5 apart at
+// least) holds whole codes over 128, which float16 has exactly, and the scales go to the attention as factors: what multiplies a key's scores,
+// and the logarithm to the base 2 of what multiplies a value's probability.
 __device__ __forceinline__ int exponent_above(float s) {      // of such a power that is no smaller than s > 0
   return min(max(((int)(__float_as_uint(s) >> 23) - 126 + 7) & ~7, -120), 120);
 }
@@ -475,7 +479,7 @@ template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   constexpr bool HALVES = std::is_same<T, __half>::value;
   __shared__ int found[2];
-  __shared__ float most[2][2];                 // float16: the largest scales of the run's first and second 32 positions, keys' and values'
+  __shared__ float most[2][2], least[2][2];    // float16: the largest and smallest scales of the run's first and second 32 positions, keys' and values'
   const int run = blockIdx.x;
   pdl_wait();
   if (p.starts != nullptr) pdl_trigger();      // behind the wait: see the kernel above; not at all where the table is written here
@@ -523,18 +527,24 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
     constexpr int EACH = 16 / sizeof(T), AHEAD = 4;
     const int unit_shift = __ffs(p.head_dim / EACH) - 1, page_shift = __ffs(p.page_size) - 1, shift = __ffs(p.block) - 1;
     [[maybe_unused]] float k_over = 1.0f, v_over = 1.0f;
+    [[maybe_unused]] bool whole_codes = false;
     if constexpr (HALVES) {
       __syncthreads();                         // whoever still reads those of the head before
+      float ks = 0.0f, vs = 0.0f;
       if (threadIdx.x < 64) {
         const int pos = tile * 64 + threadIdx.x, page_index = pos >> page_shift;
         const int page = pos < held && page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
         const bool here = page >= 0 && page < p.num_pages;
         const size_t block = ((((size_t)(page * p.kv_heads + kvh) << page_shift) + (pos & (p.page_size - 1))) >> shift);
-        const float ks = here ? fabsf(p.k_scale[block]) : 0.0f, vs = here ? fabsf(p.v_scale[block]) : 0.0f;
+        ks = here ? fabsf(p.k_scale[block]) : 0.0f;
+        vs = here ? fabsf(p.v_scale[block]) : 0.0f;
         const float k = warp_max(ks < INFINITY ? ks : 0.0f), v = warp_max(vs < INFINITY ? vs : 0.0f);
+        const float k_least = -warp_max(ks > 0.0f ? -ks : -INFINITY), v_least = -warp_max(vs > 0.0f ? -vs : -INFINITY);
         if ((threadIdx.x & 31) == 0) {
           most[threadIdx.x >> 5][0] = k;
           most[threadIdx.x >> 5][1] = v;
+          least[threadIdx.x >> 5][0] = k_least;
+          least[threadIdx.x >> 5][1] = v_least;
         }
       }
       __syncthreads();
@@ -542,7 +552,12 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
       const int e = k > 0.0f ? exponent_above(k) : 0, f = v > 0.0f ? exponent_above(v) : 0;
       k_over = power_of_two(-e);
       v_over = power_of_two(-f);
-      if (threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = (int)((uint32_t)e << 16 | ((uint32_t)f & 0xffffu));
+      whole_codes = fminf(least[0][0], least[1][0]) < power_of_two(e) * 0x1p-13f || fminf(least[0][1], least[1][1]) < power_of_two(f) * 0x1p-13f;
+      if (threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = (int)((uint32_t)e << 16 | ((uint32_t)f & 0xffffu)) | (whole_codes ? 1 : 0);
+      // (no factor is infinite or NaN, whatever the scale: a masked position has one too)
+      if (whole_codes && threadIdx.x < 64)
+        p.factors[((size_t)run * p.kv_heads + kvh) * 64 + threadIdx.x] =
+            make_float2(ks < INFINITY ? fminf(ks * (128.0f / 127.0f), 3.402823466e38f) : 1.0f, vs > 0.0f && vs < INFINITY ? log2f(vs) + 0.0113153133f : -200.0f);
     }
     const int part = threadIdx.x & ((1 << unit_shift) - 1), apart = blockDim.x >> unit_shift;      // positions between two of a thread's turns
     for (int j0 = threadIdx.x >> unit_shift; j0 < 64; j0 += AHEAD * apart) {
@@ -586,7 +601,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             float s = scale[i][kv] * (1.0f / 127.0f);
-            if constexpr (HALVES) s *= kv == 0 ? k_over : v_over;
+            if constexpr (HALVES) s = whole_codes ? (s == 0.0f || !(fabsf(s) < INFINITY) ? s : copysignf(1.0f / 128.0f, s)) : s * (kv == 0 ? k_over : v_over);
             if (!(fabsf(scale[i][1]) < INFINITY) && p.starts != nullptr) s = kv == 0 ? NAN : 0.0f;
             float x[EACH];
 #pragma unroll
@@ -677,17 +692,18 @@ TGE_API int tge_store_8bit(const void* qkv, int is_bf16, long long row_stride, v
 
 TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int num_pages, int page_size,
                           int block, const int* block_table, int max_pages, const int* q_start, const int* start_pos, int first_seq,
-                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int type, int* exponents, int* table,
+                          int num_seqs, int kv_heads, int head_dim, int window, void* k_out, void* v_out, int type, void* factors, int* table,
                           int* starts, int runs, int width, int* status, cudaStream_t stream) {
   const int rc = cache_shape("read_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
   if (rc != 0) return rc;
   TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
   if (num_seqs == first_seq || width == 0) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
-                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, exponents, table, starts, runs, width, status};
+                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, static_cast<float2*>(factors),
+                     factors == nullptr ? nullptr : static_cast<int*>(factors) + (size_t)runs * kv_heads * 128, table, starts, runs, width, status};
   const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
                      (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
-  if (type == 2 && (!units || exponents == nullptr)) return TGE_UNSUPPORTED;
+  if (type == 2 && (!units || factors == nullptr || (uintptr_t)factors % 16 != 0)) return TGE_UNSUPPORTED;
   const bool planned = starts != nullptr;
   if (planned) tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
   if (planned && runs == 0) return tge_launched("read_8bit", 1);

@@ -1201,9 +1201,9 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
 def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
     """What :func:`read_cache_8bit` does, of arguments that were looked over (``sizes``: pages, positions in a page and in a block).  With
     ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a position whose values' scale is not
-    finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a fourth result, their exponents
-    (int32 [runs, kv_heads], f in the lower half and e in the upper: keys are over 2^e, values over 2^f, at most 1); None for a cache
-    that this is not built for."""
+    finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a fourth result, what their numbers
+    stand for (int32: two factors a position, and behind them a word a run and head with their exponents, f in the lower half and e in
+    the upper: keys are over 2^e, values over 2^f, at most 1; 1 in it where the factors count); None for a cache that this is not built for."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
     num_pages, page_size, block = sizes
     # a window may leave out runs in front: the sum is then a bound
@@ -1212,15 +1212,15 @@ def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, 
     k = k_scale.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
     table = block_table.new_empty((len(mine), width))
-    exponents = block_table.new_empty((runs, kv_heads)) if dtype == torch.float16 else None
+    factors = block_table.new_empty(runs * kv_heads * (128 + 1)) if dtype == torch.float16 else None
     lib = core()
     rc = lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                            block_table.data_ptr(), block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, num_seqs,
-                           kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), 2 if exponents is not None else int(dtype == torch.bfloat16),
-                           _ptr(exponents), table.data_ptr(), _ptr(starts), runs, width, status_word().data_ptr(), _stream())
+                           kv_heads, head_dim, int(window), k.data_ptr(), v.data_ptr(), 2 if factors is not None else int(dtype == torch.bfloat16),
+                           _ptr(factors), table.data_ptr(), _ptr(starts), runs, width, status_word().data_ptr(), _stream())
     if _check(rc, lib) == UNSUPPORTED:
         return None
-    return (k, v, table) if exponents is None else (k, v, table, exponents)
+    return (k, v, table) if factors is None else (k, v, table, factors)
 
 
 _decode_8bit_floats: Dict[tuple, int] = {}      # scratch numbers by sizes: asking the library costs a microsecond a call
@@ -1313,11 +1313,11 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             if held is not None:
                 if read is not None:
                     read.record()
-                k, v, table, exponents = held
+                k, v, table, factors = held
                 splits = 1 if split == 0 or longest <= split else -(-longest // split)
                 states = prefill.tge_attention_mma_scratch_floats(tokens - first, heads, splits)
                 scratch = k_scale.new_empty(states) if states > 0 else None
-                rc = _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), exponents.data_ptr(),
+                rc = _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), factors.data_ptr(),
                                                              table.data_ptr(), table.shape[1], k.shape[0], starts.data_ptr(), rows[1].data_ptr(),
                                                              rows[2].data_ptr(), num_seqs - first, tokens - first, max_q_len, longest,
                                                              rows[4].data_ptr(), out_stride, heads, kv_heads, float(scale), int(window), split,
