@@ -148,13 +148,15 @@ __device__ __forceinline__ int row_of(const Decode8& p, int seq) {
   return behind > row ? row : -1;
 }
 
-// The slices of 16 positions that request `seq` sees: [first, first + count), one at least.
-struct Slices { int lo, hi, first, count; };
+// The slices of 16 positions that request `seq` sees: [first, first + count), one at least.  `wrong`: what is to be reported of a token whose
+// position is none, or one that the block table has no room for; the others are served as far as they go.
+struct Slices { int lo, hi, first, count, wrong; };
 __device__ __forceinline__ Slices slices_of(const Decode8& p, int seq) {
   Slices s;
   const int start = p.start_pos[seq], here = p.q_start[seq], behind = p.q_start[seq + 1];      // one trip to memory
-  const int pos = behind > here ? start : -1;
-  s.hi = min(max(pos + 1, 0), p.a.max_pages << p.page_shift);
+  const int pos = behind > here ? start : -1, room = p.a.max_pages << p.page_shift;
+  s.hi = min(max(pos, -1), room - 1) + 1;
+  s.wrong = behind <= here ? 0 : start < 0 ? TGE_STATUS_BAD_ROW : start >= room ? TGE_STATUS_BAD_PAGE : 0;
   s.lo = p.a.window > 0 ? max(pos - p.a.window + 1, 0) : 0;
   s.first = s.lo >> 4;
   s.count = max((s.hi + 15) / 16 - s.first, 1);
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
           }
       if (slice + 1 < last) load_values<HD>(p, c, row, g, t);
     }
-    if (bad && token >= 0 && lane == 0) atomicOr(p.a.status, TGE_STATUS_BAD_PAGE);
+    if (token >= 0 && lane == 0 && (bad || s.wrong != 0)) atomicOr(p.a.status, s.wrong != 0 ? s.wrong : TGE_STATUS_BAD_PAGE);
 
     // the warps' states meet in shared memory: the two numbers of a lane and a tile side by side, then the lanes g, then the tiles
     __syncthreads();                                              // whoever still reads the unit before

@@ -807,3 +807,31 @@ def test_a_run_of_scales_far_apart_with_blocks_of_zeros_and_nan(ops, heads, kv, 
         for i in range(held[r]):
             want[first + i, heads // kv:] = bad[r][0] <= i and (not window or bad[r][0] > i - window)
     assert torch.equal(nan.all(-1), want) and torch.equal(nan.any(-1), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("requests,kv,dim,columns,held", [(3, 2, 128, 2, 300), (40, 2, 128, 2, 300), (3, 1, 128, 130, 8330), (3, 2, 80, 2, 300), (2, 1, 256, 1, 65)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_single_tokens_beyond_their_block_table_are_reported(ops, dtype, requests, kv, dim, columns, held, window):
+    """A context that the table has no room for, and one that starts in front of position 0: as faults, whatever kernel serves them."""
+    heads = 4 * kv
+    cache = Cache([held] + [60] * (requests - 1), kv, dim, 64, 1)
+    device, short = cache.device(), cache.table[:, :columns].contiguous().to(DEV)
+    q = torch.randn(requests, heads * dim, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+
+    def call(starts, table):
+        positions, seq, q_start, start_pos = batch_index([1] * requests, starts, DEV)
+        return ops.attention_8bit(q, *device, table, q_start, start_pos, positions, seq, requests, 1, held, heads, kv, dim, 0.09, window=window)
+
+    good = call([n - 1 for n in cache.held], cache.table.to(DEV))
+    ops.check_status()
+    out = call([n - 1 for n in cache.held], short)
+    with pytest.raises(ops.DeviceStatusError, match="page"):
+        ops.check_status()
+    assert rel_error(out[1:], good[1:]) < TOL[dtype]
+    out = call([-1] + [n - 1 for n in cache.held[1:]], cache.table.to(DEV))
+    with pytest.raises(ops.DeviceStatusError, match="row"):
+        ops.check_status()
+    assert (out[0] == 0).all() and rel_error(out[1:], good[1:]) < TOL[dtype]
+    call([columns * 64 - 1] + [n - 1 for n in cache.held[1:]], short)           # the last position that the table has room for
+    ops.check_status()
