@@ -1330,6 +1330,13 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
                   window=window, out=rows[4], sink=sink)
 
+    def simply(first: int, last: int) -> None:
+        """The rows [first, last), a warp each."""
+        rows = (q, out, positions, seq_of_token) if first == 0 else (q[first:], out[first:], positions[first:], seq_of_token[first:])
+        _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
+                                             last - first, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
+                                             _ptr(sink), status_word().data_ptr(), _stream()), lib)
+
     as_portions = max_q_len > 1 and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
                                      else head_dim in (16, 32, 64, 128) and sink is None)
     if as_portions and need >= 0 and MIN_DECODE_PREFIX <= singles < num_seqs and not torch.cuda.is_current_stream_capturing():
@@ -1348,19 +1355,19 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             main.wait_event(read)
             served = single_tokens()
             main.wait_stream(side)
-            if served == singles:
-                return out
-            as_portions = False          # (a cache that the single tokens' kernel does not take: all go the simple way below)
+            if served < singles:
+                simply(served, singles)                   # (a cache that the single tokens' kernel does not take)
+            return out
     done = single_tokens() if need >= 0 else 0            # requests, and so tokens, that are served
+    if done < singles and as_portions:
+        simply(done, singles)                             # (the portions behind them go the way that they go alone)
+        done = singles
     if done == num_seqs:
         return out
-    if as_portions and done == singles:
+    if as_portions:
         portions(done)
-        return out
-    rows = (q, out, positions, seq_of_token) if done == 0 else (q[done:], out[done:], positions[done:], seq_of_token[done:])
-    _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
-                                         tokens - done, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
-                                         _ptr(sink), status_word().data_ptr(), _stream()), lib)
+    else:
+        simply(done, tokens)
     return out
 
 

@@ -835,3 +835,23 @@ def test_single_tokens_beyond_their_block_table_are_reported(ops, dtype, request
     assert (out[0] == 0).all() and rel_error(out[1:], good[1:]) < TOL[dtype]
     call([columns * 64 - 1] + [n - 1 for n in cache.held[1:]], short)           # the last position that the table has room for
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim,page", [(6, 2, 32, 16), (6, 2, 80, 16), (14, 2, 128, 8)])
+@pytest.mark.parametrize("singles", [1, 9])
+def test_a_portion_goes_the_same_way_beside_single_tokens(ops, dtype, heads, kv, dim, page, singles):
+    """Caches that the single tokens' kernel does not take: the bits of both parts on their own."""
+    held = [40 + 3 * i for i in range(singles)] + [100, 70]
+    lens = [1] * singles + [64, 70]
+    cache = Cache(held, kv, dim, page, 1)
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+    q = torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(5)).to(dtype).to(DEV)
+    device, table = cache.device(), cache.table.to(DEV)
+    rest = (heads, kv, dim, dim ** -0.5)
+    both = ops.attention_8bit(q, *device, table, q_start, start_pos, positions, seq, len(lens), 70, max(held), *rest, decode_prefix=singles, ctx_lens=held)
+    first = ops.attention_8bit(q[:singles], *device, table, q_start, start_pos, positions, seq, singles, 1, max(held), *rest, ctx_lens=held[:singles])
+    second = ops.attention_8bit(q[singles:], *device, table[singles:].contiguous(), q_start[singles:] - singles, start_pos[singles:].clone(),
+                                positions[singles:].clone(), seq[singles:] - singles, 2, 70, 100, *rest, ctx_lens=held[singles:])
+    ops.check_status()
+    assert torch.equal(both[:singles], first) and torch.equal(both[singles:], second)
