@@ -1350,11 +1350,13 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             main, side = torch.cuda.current_stream(), _side_stream()
             read = torch.cuda.Event()
             side.wait_stream(main)
-            with torch.cuda.stream(side):
-                portions(singles, read)
-            main.wait_event(read)
-            served = single_tokens()
-            main.wait_stream(side)
+            try:
+                with torch.cuda.stream(side):
+                    portions(singles, read)
+                main.wait_event(read)
+                served = single_tokens()
+            finally:
+                main.wait_stream(side)       # also when a part raises: what the side stream uses is the main one's again afterwards
             if served < singles:
                 simply(served, singles)                   # (a cache that the single tokens' kernel does not take)
             return out

@@ -855,3 +855,34 @@ def test_a_portion_goes_the_same_way_beside_single_tokens(ops, dtype, heads, kv,
                                 positions[singles:].clone(), seq[singles:] - singles, 2, 70, 100, *rest, ctx_lens=held[singles:])
     ops.check_status()
     assert torch.equal(both[:singles], first) and torch.equal(both[singles:], second)
+
+
+class Refusing:
+    """The kernels' library, with one entry that refuses."""
+
+    def __init__(self, lib, name):
+        self._lib, self._name = lib, name
+
+    def __getattr__(self, name):
+        return (lambda *args: -1) if name == self._name else getattr(self._lib, name)
+
+
+def test_side_by_side_joins_its_stream_when_a_part_is_refused(ops, monkeypatch):
+    """What the second stream still uses is the caller's again once the call has raised: the caller's stream waits for it."""
+    held, lens, heads = [1, 5, 64, 65, 200, 17, 128, 90, 400, 200], [1] * 9 + [100], 14
+    cache = Cache(held, 2, 128, 16, 1)
+    want, _ = attend(ops, cache, lens, heads, torch.bfloat16, decode_prefix=9, ctx_lens=held)
+    monkeypatch.setattr(ops, "BESIDE_8BIT_FLOPS", 0.0)
+    waits, wait_stream = [], torch.cuda.Stream.wait_stream
+    monkeypatch.setattr(torch.cuda.Stream, "wait_stream", lambda self, other: (waits.append((self, other)), wait_stream(self, other))[1])
+    lib = ops.core()
+    main, side = torch.cuda.current_stream(), ops._side_stream()
+    for refused in ("tge_attention_8bit_decode", "tge_read_8bit"):
+        waits.clear()
+        with monkeypatch.context() as patch:
+            patch.setattr(ops, "core", lambda: Refusing(lib, refused))
+            with pytest.raises(ops.KernelError):
+                attend(ops, cache, lens, heads, torch.bfloat16, decode_prefix=9, ctx_lens=held)
+        assert waits[0] == (side, main) and waits[-1] == (main, side)
+    got, _ = attend(ops, cache, lens, heads, torch.bfloat16, decode_prefix=9, ctx_lens=held)
+    assert torch.equal(got, want)
