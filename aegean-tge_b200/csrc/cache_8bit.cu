@@ -442,27 +442,46 @@ __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
   return s;
 }
 
-// The block table over the runs, and the first tokens if wanted.
-__device__ __forceinline__ void plan_runs(const ReadParams& p) {
-  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += blockDim.x)
-    p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
-  int total = 0;
-  for (int seq = p.first_seq; seq < p.num_seqs; ++seq) {
-    const Span s = span_of(p, seq);
-    for (int i = threadIdx.x; i < p.width; i += blockDim.x)
-      p.table[(size_t)(seq - p.first_seq) * p.width + i] = i >= s.first && i < s.first + s.count ? total + i - s.first : -1;
-    if (s.first + s.count > p.width && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-    total += s.count;
-  }
-  if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-}
-
-// A kernel of its own where attention follows: the attention kernels look block tables and first tokens up while the kernel in front of
-// them still runs, so these have to be there before that one lets them start.
-__global__ void __launch_bounds__(256) read_8bit_plan_kernel(const ReadParams p) {
+// The block table over the runs, and the first tokens if wanted.  A kernel of its own: attention kernels look block tables and first tokens up while
+// the kernel in front of them still runs, so these have to be there before that one lets them start.  One block, a request to a thread at a time:
+// one request after the other took 64 of them 9 us longer.
+constexpr int PLAN_THREADS = 256;
+__global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const ReadParams p) {
+  __shared__ int first_run[PLAN_THREADS], count[PLAN_THREADS], runs_upto[PLAN_THREADS], of_warp[PLAN_THREADS / 32];
   pdl_trigger();
   pdl_wait();
-  plan_runs(p);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += PLAN_THREADS)
+    p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
+  int total = 0;
+  for (int base = p.first_seq; base < p.num_seqs; base += PLAN_THREADS) {
+    const int here = min(PLAN_THREADS, p.num_seqs - base);
+    Span s{0, 0};
+    if ((int)threadIdx.x < here) s = span_of(p, base + threadIdx.x);
+    if (s.first + s.count > p.width) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    int upto = s.count;
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, offset);
+      if (lane >= offset) upto += v;
+    }
+    first_run[threadIdx.x] = s.first;
+    count[threadIdx.x] = s.count;
+    runs_upto[threadIdx.x] = upto - s.count;
+    if (lane == 31) of_warp[warp] = upto;
+    __syncthreads();
+    for (int r = warp; r < here; r += PLAN_THREADS / 32) {
+      int before = total + runs_upto[r];
+      for (int w = 0; w < r >> 5; ++w) before += of_warp[w];
+      for (int i = lane; i < p.width; i += 32) {
+        const int at = i - first_run[r];
+        p.table[(size_t)(base - p.first_seq + r) * p.width + i] = at >= 0 && at < count[r] ? before + at : -1;
+      }
+    }
+    for (int w = 0; w < PLAN_THREADS / 32; ++w) total += of_warp[w];
+    __syncthreads();
+  }
+  if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
 }
 
 // float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ.
@@ -482,11 +501,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ float most[2][2], least[2][2];    // float16: the largest and smallest scales of the run's first and second 32 positions, keys' and values'
   const int run = blockIdx.x;
   pdl_wait();
-  if (p.starts != nullptr) pdl_trigger();      // behind the wait: see the kernel above; not at all where the table is written here
-  if (run == p.runs) {                         // the block behind the runs, where no kernel in front has planned them
-    if (blockIdx.y == 0) plan_runs(p);
-    return;
-  }
+  pdl_trigger();                               // behind the wait: see the kernel above
   if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
     int before = 0, seq_found = -1, first_run = 0, index = 0;
     for (int base = p.first_seq; base < p.num_seqs && seq_found < 0; base += 32) {
@@ -697,24 +712,23 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   const int rc = cache_shape("read_8bit", num_pages, page_size, block, kv_heads, head_dim, max_pages);
   if (rc != 0) return rc;
   TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
-  if (num_seqs == first_seq || width == 0) return 0;
+  if (num_seqs == first_seq) return 0;
   const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
                      page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, static_cast<float2*>(factors),
                      factors == nullptr ? nullptr : static_cast<int*>(factors) + (size_t)runs * kv_heads * 128, table, starts, runs, width, status};
   const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
                      (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (type == 2 && (!units || factors == nullptr || (uintptr_t)factors % 16 != 0)) return TGE_UNSUPPORTED;
-  const bool planned = starts != nullptr;
-  if (planned) tge_launch(read_8bit_plan_kernel, 1, 256, 0, stream, p);
-  if (planned && runs == 0) return tge_launched("read_8bit", 1);
+  tge_launch(read_8bit_plan_kernel, 1, PLAN_THREADS, 0, stream, p);
+  if (runs == 0) return tge_launched("read_8bit", 1);
   // a block takes several heads of its run where there are many runs: finding whose it is costs as much as a head
   const int at_once = 10 * tge_sm_count();
-  const dim3 grid(runs + (planned ? 0 : 1), std::max(1, std::min(kv_heads, (at_once + runs) / (runs + 1))));
+  const dim3 grid(runs, std::max(1, std::min(kv_heads, (at_once + runs) / (runs + 1))));
   if (type == 2)
     tge_launch(read_8bit_kernel<__half, true>, grid, 256, 0, stream, p);
   else if (type == 1)
     tge_launch(units ? read_8bit_kernel<__nv_bfloat16, true> : read_8bit_kernel<__nv_bfloat16, false>, grid, 256, 0, stream, p);
   else
     tge_launch(units ? read_8bit_kernel<float, true> : read_8bit_kernel<float, false>, grid, 256, 0, stream, p);
-  return tge_launched("read_8bit", planned ? 2 : 1);
+  return tge_launched("read_8bit", 2);
 }

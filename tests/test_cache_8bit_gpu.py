@@ -886,3 +886,31 @@ def test_side_by_side_joins_its_stream_when_a_part_is_refused(ops, monkeypatch):
         assert waits[0] == (side, main) and waits[-1] == (main, side)
     got, _ = attend(ops, cache, lens, heads, torch.bfloat16, decode_prefix=9, ctx_lens=held)
     assert torch.equal(got, want)
+
+
+def test_a_read_back_is_planned_by_a_kernel_of_its_own(ops):
+    """Its block table is there before the kernel that reads entries lets the next one start; requests that hold nothing have a plan too."""
+    cache = Cache([130, 0, 40], 2, 64, 16, 1)
+    _, _, q_start, start_pos = batch_index([1, 0, 1], [129, 0, 39], DEV)
+    device, table = cache.device(), cache.table.to(DEV)
+    before = ops.launches
+    k, _v, runs = ops.read_cache_8bit(*device, table, q_start, start_pos, cache.held, torch.bfloat16)
+    assert ops.launches - before == 2 and k.shape[0] == 4 and runs.tolist() == [[0, 1, 2], [-1, -1, -1], [3, -1, -1]]
+    many = [i * 37 % 300 for i in range(600)]                     # more requests than the plan takes at a time
+    lens = [min(n, 2) for n in many]
+    cache = Cache(many, 1, 64, 16, 1)
+    _, _, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(many, lens)], DEV)
+    for window, first in ((0, 0), (70, 5)):
+        found = ops.read_cache_8bit(*cache.device(), cache.table.to(DEV), q_start, start_pos, many, torch.bfloat16, window=window, first_seq=first)[2].tolist()
+        at = 0
+        for held, n, row in zip(many[first:], lens[first:], found):
+            seen = max(held - n - window + 1, 0) // 64 if window else 0
+            count = max(-(-held // 64) - seen, 0)
+            assert row == [-1] * seen + list(range(at, at + count)) + [-1] * (len(row) - seen - count)
+            at += count
+    _, _, q_start, start_pos = batch_index([1, 0, 1], [129, 0, 39], DEV)
+    starts = torch.full((2,), -7, dtype=torch.int32, device=DEV)
+    before = ops.launches
+    found = ops._read_8bit((device[0].shape[0], 16, 1), *device, table, q_start, start_pos, [130, 0], torch.bfloat16, 0, 1, starts)
+    assert ops.launches - before == 1 and found[0].shape[0] == 0 and starts.tolist() == [0, 0]
+    ops.check_status()
