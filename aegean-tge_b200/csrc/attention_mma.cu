@@ -24,6 +24,7 @@
 
 #include <atomic>
 #include <map>
+#include <mutex>
 #include <tuple>
 #include <type_traits>
 
@@ -1280,26 +1281,39 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// The tensor map of a page pool, made once per (address, geometry) and kept; with `into`, for pages of one call, made there and not kept.
+// The tensor maps of page pools, made once per (address, geometry) and kept.
+struct PoolMaps {
+  std::mutex lock;
+  std::map<std::tuple<const void*, int, int, int>, CUtensorMap> maps;
+};
+PoolMaps& pool_maps() {
+  static PoolMaps kept;
+  return kept;
+}
+
+EncodeTiledFn tiled_encoder() {
+  void* ptr = nullptr;
+  cudaDriverEntryPointQueryResult result;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) == cudaSuccess &&
+      result == cudaDriverEntryPointSuccess)
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  return nullptr;
+}
+
+// The tensor map of a page pool; with `into`, for pages of one call, made there and not kept.
 const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int page_size, CUtensorMap* into = nullptr) {
-  static EncodeTiledFn encode = nullptr;
-  static bool tried = false;
-  static std::map<std::tuple<const void*, int, int, int>, CUtensorMap> maps;
-  if (!tried) {
-    tried = true;
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) == cudaSuccess &&
-        result == cudaDriverEntryPointSuccess)
-      encode = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
+  static const EncodeTiledFn encode = tiled_encoder();
   if (!encode) {
     tge_set_error("attention_decode: the driver does not export cuTensorMapEncodeTiled");
     return nullptr;
   }
+  PoolMaps& kept = pool_maps();
   const auto key = std::make_tuple(pages, num_pages, kv_heads, page_size);
-  auto found = maps.find(key);
-  if (into == nullptr && found != maps.end()) return &found->second;
+  if (into == nullptr) {
+    std::lock_guard<std::mutex> held(kept.lock);
+    auto found = kept.maps.find(key);
+    if (found != kept.maps.end()) return &found->second;
+  }
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)num_pages * kv_heads * page_size};
   cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
@@ -1316,7 +1330,8 @@ const CUtensorMap* pool_map(const void* pages, int num_pages, int kv_heads, int 
     *into = map;
     return into;
   }
-  return &maps.emplace(key, map).first->second;
+  std::lock_guard<std::mutex> held(kept.lock);
+  return &kept.maps.emplace(key, map).first->second;
 }
 #endif  // TGE_TMA_KERNELS
 
@@ -1497,7 +1512,7 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
                               int first_token, const float* sink, int leave_states, int v_pitch, const float* dist_bias,
                               int dist_span, int keep_first, const void* gate, int gate_stride, int gate_elements,
                               int shared_keys, cudaStream_t stream, LeadingTokens* lead = nullptr, unsigned long long beside = 0,
-                              const void* page_factors = nullptr) {
+                              const void* page_factors = nullptr, bool own_pages = false) {
   TGE_REQUIRE(tokens >= 0 && num_seqs >= 0, "attention_mma: negative sizes");
   TGE_REQUIRE(dist_bias == nullptr || (dist_span > 0 && scale != 0.0f), "attention_mma: a bias by distance needs its span");
   TGE_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
@@ -1562,8 +1577,9 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
 
 #if TGE_TMA_KERNELS
   if (max_q_len <= 1 && tokens == num_seqs && group <= 16 && page_size >= 8) {
-    const CUtensorMap* map_k = pool_map(k_pages, num_pages, kv_heads, page_size);
-    const CUtensorMap* map_v = pool_map(v_pages, num_pages, kv_heads, page_size);
+    CUtensorMap own_k, own_v;
+    const CUtensorMap* map_k = pool_map(k_pages, num_pages, kv_heads, page_size, own_pages ? &own_k : nullptr);
+    const CUtensorMap* map_v = pool_map(v_pages, num_pages, kv_heads, page_size, own_pages ? &own_v : nullptr);
     if (!map_k || !map_v) return -3;
     const int range = (num_splits > 1 ? p.split_tokens : key_span) + 2 * BKV;
     // No more blocks than SMs, each with many keys: a block has its SM to itself and runs two groups of warps on
@@ -1667,8 +1683,9 @@ static int attention_dispatch(const void* q, int q_stride, const void* k_pages, 
     return 1;
   }
   if (max_q_len > 1 && group <= 64 && page_size >= 8) {
-    const CUtensorMap* map_k = pool_map(k_pages, num_pages, kv_heads, page_size);
-    const CUtensorMap* map_v = pool_map(v_pages, num_pages, kv_heads, page_size);
+    CUtensorMap own_k, own_v;
+    const CUtensorMap* map_k = pool_map(k_pages, num_pages, kv_heads, page_size, own_pages ? &own_k : nullptr);
+    const CUtensorMap* map_v = pool_map(v_pages, num_pages, kv_heads, page_size, own_pages ? &own_v : nullptr);
     if (!map_k || !map_v) return -3;
     p.bq = (PRE_WARPS * 16) / group;
     const int range = (num_splits > 1 ? p.split_tokens : max_ctx_len) + 2 * BKV;
@@ -1803,6 +1820,16 @@ TGE_API int tge_attention_mma_halves(const void* q, int q_stride, const void* k_
 #endif
 }
 
+// How many tensor maps of page pools this library keeps.
+TGE_API int tge_attention_mma_kept_maps() {
+#if TGE_TMA_KERNELS
+  std::lock_guard<std::mutex> held(pool_maps().lock);
+  return (int)pool_maps().maps.size();
+#else
+  return 0;
+#endif
+}
+
 // `leave_states`: the keys are cut into at least two runs and the runs' unnormalised states (sums, maxima in base-2
 // units, denominators) stay in the scratch memory unmerged, [runs, tokens, heads, DV] and then [runs, tokens, heads, 2]:
 // the caller has more to merge into the softmax (pooled blocks) and writes the output itself.
@@ -1817,7 +1844,8 @@ TGE_API int tge_attention_mma_halves(const void* q, int q_stride, const void* k_
 // gate_stride], or null): logits of one gate per token and head; whoever writes a head's output multiplies it by their
 // logistic function.  `shared_keys`: for single tokens whose values lie inside the keys, all kv_heads runs of heads read the one
 // key/value head that the pages hold.  Single tokens over a window (without kept first positions): split_tokens cuts the window's
-// span, from its first tile on.  `gate_elements`: one gate per number of a head's output instead, [tokens, heads * DV].
+// span, from its first tile on.  `gate_elements`: one gate per number of a head's output instead, [tokens, heads * DV].  `own_pages`: the pages
+// are this call's own, and nothing is kept of where they lie.
 TGE_API int tge_attention_mma(const void* q, int q_stride, const void* k_pages, const void* v_pages,
                               const int* block_table, int max_pages, int num_pages, int page_size,
                               const int* q_start, const int* start_pos, const int* positions, int num_seqs,
@@ -1825,7 +1853,7 @@ TGE_API int tge_attention_mma(const void* q, int q_stride, const void* k_pages, 
                               int kv_heads, float scale, int window, int split_tokens, float* scratch, int* status,
                               int decode_prefix, int prefix_split_tokens, const float* sink, int leave_states,
                               int v_pitch, const float* dist_bias, int dist_span, int keep_first, const void* gate,
-                              int gate_stride, int gate_elements, int shared_keys, int rest_ctx_len, cudaStream_t stream) {
+                              int gate_stride, int gate_elements, int shared_keys, int rest_ctx_len, int own_pages, cudaStream_t stream) {
   TGE_REQUIRE(decode_prefix >= 0 && decode_prefix <= num_seqs, "attention_mma: %d leading single tokens of %d sequences",
               decode_prefix, num_seqs);
   TGE_REQUIRE(prefix_split_tokens >= 0 && prefix_split_tokens % BKV == 0,
@@ -1833,7 +1861,8 @@ TGE_API int tge_attention_mma(const void* q, int q_stride, const void* k_pages, 
   if (decode_prefix == 0 || max_q_len <= 1 || decode_prefix == num_seqs || kv_heads <= 0 || heads / kv_heads > 16)
     return attention_dispatch(q, q_stride, k_pages, v_pages, block_table, max_pages, num_pages, page_size, q_start, start_pos,
                               positions, num_seqs, tokens, max_q_len, max_ctx_len, out, out_stride, heads, kv_heads, scale,
-                              window, split_tokens, scratch, status, 0, sink, leave_states, v_pitch, dist_bias, dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream);
+                              window, split_tokens, scratch, status, 0, sink, leave_states, v_pitch, dist_bias, dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream, nullptr, 0,
+                              nullptr, own_pages != 0);
   // Side by side where nothing but keys, queries and constants is read (gates may be the kernel in front's work) and where the
   // scratch memory holds the states of one of the two calls only.  (31 single tokens of up to 4,096 beside a prompt of 1,187, 40 heads over 8, us
   // a layer in a step: 88 and 50 one after the other, 95 and 25 so; eight layers of such a step 6,084 and 6,029.)
@@ -1855,13 +1884,14 @@ TGE_API int tge_attention_mma(const void* q, int q_stride, const void* k_pages, 
   const int first = attention_dispatch(q, q_stride, k_pages, v_pages, block_table, max_pages, num_pages, page_size, q_start,
                                        start_pos, positions, decode_prefix, decode_prefix, 1, max_ctx_len, out, out_stride,
                                        heads, kv_heads, scale, window, prefix_split_tokens, scratch, status, 0, sink, leave_states, v_pitch, dist_bias,
-                                       dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream, ask);
+                                       dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream, ask, 0, nullptr, own_pages != 0);
   if (first < 0) return first;
   int rest = attention_dispatch(q, q_stride, k_pages, v_pages, block_table + (size_t)decode_prefix * max_pages, max_pages,
                                 num_pages, page_size, q_start + decode_prefix, start_pos + decode_prefix, positions,
                                 num_seqs - decode_prefix, tokens, max_q_len, rest_ctx, out, out_stride, heads,
                                 kv_heads, scale, window, split_tokens, scratch, status, decode_prefix, sink, leave_states, v_pitch, dist_bias,
-                                dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream, nullptr, lead.late ? lead.ticket : 0);
+                                dist_span, keep_first, gate, gate_stride, gate_elements, shared_keys, stream, nullptr, lead.late ? lead.ticket : 0, nullptr,
+                                own_pages != 0);
   if (rest < 0) return rest;
   if (lead.unmerged) {
     launch_merge(lead.p, positions, 0, stream);

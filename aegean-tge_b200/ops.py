@@ -236,7 +236,7 @@ def attention_lib(head_dim: int, value_dim: int = 0) -> ctypes.CDLL:
         _declare(lib, "tge_attention_mma", [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr,
                                             _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_int,
                                             _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr,
-                                            _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr])
+                                            _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr])
         _declare(lib, "tge_attention_mma_halves", [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr,
                                                     _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_float,
                                                     _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr])
@@ -910,7 +910,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
               pooled_v: Optional[torch.Tensor] = None, pool_table: Optional[torch.Tensor] = None,
               values_in_keys: int = 0, dist_bias: Optional[torch.Tensor] = None, keep_first: int = 0,
               gate: Optional[torch.Tensor] = None,
-              shared_keys: bool = False, lead_keys: int = 0, lead_longest: int = 0, rest_ctx_len: int = 0) -> torch.Tensor:
+              shared_keys: bool = False, lead_keys: int = 0, lead_longest: int = 0, rest_ctx_len: int = 0, own_pages: bool = False) -> torch.Tensor:
     """Paged causal attention of a flat batch of portions.
 
     q: [T, >= heads*head_dim] (dense rows, any row stride) holding rotated queries;
@@ -938,6 +938,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
     output multiplies it by their logistic function.  [T, heads * value_dim]: one gate per number of the output.
     ``shared_keys`` (single tokens, values inside the keys): the heads go in ``kv_heads`` equal runs that all read the one
     key/value head of the pages, one block per run; for the tensor-core kernels only.
+    ``own_pages``: the pages are this call's own (entries that were read back, say), and nothing is kept of where they lie.
     """
     v_pitch = 0
     if values_in_keys:
@@ -1053,7 +1054,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
                                      max_ctx_len, out.data_ptr(), out_stride, heads, kv_heads, float(scale), window,
                                      split_tokens, _ptr(scratch), status_word().data_ptr(), prefix, prefix_split,
                                      _ptr(sink), int(bool(pool)), v_pitch, _ptr(dist_bias), dist_span,
-                                     keep_first, _ptr(gate), gate_stride, gate_elements, int(shared_keys), rest_ctx, _stream()), lib)
+                                     keep_first, _ptr(gate), gate_stride, gate_elements, int(shared_keys), rest_ctx, int(own_pages), _stream()), lib)
         if pool:
             core_lib = core()
             states = scratch.data_ptr()
@@ -1328,7 +1329,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         if read is not None:
             read.record()
         attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
-                  window=window, out=rows[4], sink=sink)
+                  window=window, out=rows[4], sink=sink, own_pages=True)
 
     def simply(first: int, last: int) -> None:
         """The rows [first, last), a warp each."""

@@ -914,3 +914,21 @@ def test_a_read_back_is_planned_by_a_kernel_of_its_own(ops):
     found = ops._read_8bit((device[0].shape[0], 16, 1), *device, table, q_start, start_pos, [130, 0], torch.bfloat16, 0, 1, starts)
     assert ops.launches - before == 1 and found[0].shape[0] == 0 and starts.tolist() == [0, 0]
     ops.check_status()
+
+
+def test_pages_of_one_call_leave_no_tensor_maps_behind(ops):
+    """Portions that go over bfloat16 pages of the call's own, of other sizes every time."""
+    for heads, kv, dim, odd in ((2, 1, 256, 0), (6, 2, 128, 1)):
+        lib = ops.attention_lib(dim)
+        before = lib.tge_attention_mma_kept_maps()
+        for held in (70, 200, 330, 500):
+            cache = Cache([held, 90], kv, dim, 16, 1)
+            q = torch.randn(100, heads * dim + 2 * odd, generator=torch.Generator().manual_seed(held)).bfloat16()
+            positions, seq, q_start, start_pos = batch_index([40, 60], [held - 40, 30], DEV)
+            rows = q.to(DEV)[:, 2 * odd:]                       # rows that do not lie on 16 bytes
+            out = ops.attention_8bit(rows, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 2, 60, held, heads, kv, dim, 0.09, ctx_lens=[held, 90])
+            want = [plain.attend(q[a:b, 2 * odd:].reshape(b - a, heads, dim), cache.values("k", r), cache.values("v", r), s, 0.09, 0, None)
+                    for r, (a, b, s) in enumerate(((0, 40, held - 40), (40, 100, 30)))]
+            assert rel_error(out, torch.cat(want).flatten(1)) < TOL[torch.bfloat16]
+        assert lib.tge_attention_mma_kept_maps() == before
+    ops.check_status()
