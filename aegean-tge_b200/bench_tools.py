@@ -9,6 +9,7 @@ weights are likewise larger than L2.
 from __future__ import annotations
 
 import random
+import time
 from typing import Dict, List
 
 import torch
@@ -36,7 +37,6 @@ def bench_prefill(engine, prompt_len: int, repeat: int = 3, warmup: int = 2, sus
     more figures are taken, to be read against the two peaks measured the same ways: ``burst_ms`` (the best of
     three runs after a pause of two seconds; the burst peak is a best of ten) and ``sustained_ms`` (the mean over
     a loop of that many seconds; the sustained peak is a loop of four seconds)."""
-    import time
     vocab = engine.spec.vocab_size
     counter = [0]
 
@@ -183,18 +183,27 @@ def step_timeline(engine, batch: int, prompt_len: int, prefill: bool, portion: i
         run()
     torch.cuda.synchronize()
     ops = engine.model.env.ops
-    for _ in range(4):
-        launched = ops.launches
-        with profile(activities=[ProfilerActivity.CUDA]) as prof:
-            run()
-            torch.cuda.synchronize()
-        launched = ops.launches - launched
-        events = [(e.time_range.start, e.time_range.start + e.device_time_total, e.name) for e in prof.events()
-                  if e.device_time_total > 0]
-        if len(events) >= launched:          # the profiler now and then hands over a part of the records only: once more
-            break
-    for n in names:
-        engine.runner.finish(n)
+    try:
+        # the profiler now and then hands over a part of the records only: once more, with a pause on either side of the step within
+        # the profiler's window that gets longer
+        for attempt in range(8):
+            pause = 0.0 if attempt < 2 else 0.02 * 2 ** (attempt - 2)
+            launched = ops.launches
+            with profile(activities=[ProfilerActivity.CUDA]) as prof:
+                time.sleep(pause)
+                run()
+                torch.cuda.synchronize()
+                time.sleep(pause)
+            launched = ops.launches - launched
+            events = [(e.time_range.start, e.time_range.start + e.device_time_total, e.name) for e in prof.events()
+                      if e.device_time_total > 0]
+            if len(events) >= launched:
+                break
+        else:
+            raise RuntimeError(f"the profiler handed over {len(events)} records of a step of {launched} kernels, eight times in a row")
+    finally:
+        for n in names:
+            engine.runner.finish(n)
     events.sort(key=lambda e: e[1])
     first = min(e[0] for e in events)
     by_name: Dict[str, List[float]] = {}
@@ -356,7 +365,6 @@ def compare_designs(configs: Dict[str, dict], prompt_len: int = 2048, batches=(8
     against the copy bandwidth, and where the time of a prefill step and of a decode step of the first batch goes,
     kernel by kernel."""
     import gc
-    import time
     from .engine.engine import Engine
     out: Dict[str, dict] = {}
     for name, config in configs.items():
