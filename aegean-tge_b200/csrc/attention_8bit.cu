@@ -100,18 +100,20 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 //            needs, of positions g and g + 8 (g = lane / 4), a quarter of the row, whole 16-byte chunks, because the order of d is
 //            free as long as the queries come in the same one.  The codes are operands as they are.  A row of queries is rounded to
 //            whole numbers of 15 bits (float32: 22) of its largest and taken as two (three) digits to the base 128, whose products are
-//            added exactly in 32 bits: 2^-15 of the row's largest number is a 64th of what bfloat16 has rounded that number by;
+//            added exactly in 32 bits.  2^-15 of the row's largest number is a 64th of what bfloat16 has rounded that number by; numbers
+//            below 2^-6 of it lose more than bfloat16 had (a third digit: the 64 requests below 87 us where this takes 83);
 //   values   O^T [d x 8 heads] += C'^T [d x 16 positions] P^T [16 x 8]   (m16n8k16 of float16): a lane needs, of positions 2t, 2t + 1,
 //            2t + 8, 2t + 9 (t = lane % 4), the numbers that are rows g and g + 8 of every 16-row tile; which 16 numbers of d make a
 //            tile is free too, so they are those of one 16-byte chunk.  A code becomes a float16 exactly: its byte, the sign bit turned over,
 //            below the exponent of 1,024, less 1,152.  (Whole numbers would need no conversion here either, but a probability's small
-//            numbers matter: a long tail of 2^-16 each must not become zeros.)  p is at most 2^8; with its position's scale over the largest
-//            scale so far it is held times 2^6, at most 2^15, and keeps 11 bits down to 2^-21 of a probability of 1 and some down to
-//            2^-31.  float32 runs add what float16 leaves of it as a second part.
+//            numbers matter: a long tail of 2^-16 each must not become zeros.)  p is at most 2^8; its product with its position's scale
+//            goes over the largest such product that the head had when it was last looked for, times 2^6, is at most 2^15, and keeps
+//            11 bits down to 2^-20 of that product and some down to 2^-30: a large value that the head hardly weighs takes nothing from
+//            the others.  float32 runs add what float16 leaves of it as a second part.
 // Every load of the codes is 16 bytes a lane and whole 128-byte lines a warp.  Probabilities turn from S^T's accumulators into P^T's
 // operand by two 8x8 transposes.  With heads as the narrow side of 8, a group of up to 8 heads wastes no more than its rest.
-// The running maximum is raised only when a score passes it by 2^8, the scales' one when a scale is twice it (one vote a slice); the
-// sums of probabilities stay in their lanes until the end.
+// The running maximum is raised only when a score passes it by 2^8, the products' one looked for again when a scale is twice it (one vote a
+// slice); the sums of probabilities stay in their lanes until the end.
 //
 // Work: the slices of all (request, kv head, tile of heads) units in one row, cut into equal runs, one per block, whatever the
 // requests' lengths; the blocks work that out from the lengths on the device, so a captured graph stays right as they grow.  A unit
@@ -130,7 +132,10 @@ constexpr int DWARPS = 4;
 constexpr int BEGIN = 12;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float HELD = 64.0f;                   // probabilities are held times this
+// Probabilities times their values' scales are held over the largest such product of their head when it was last looked for, times HELD; it is
+// looked for again where a value's scale alone is twice that.  LEAST, MOST: that product is taken as this where it is smaller or larger, so that
+// it, the factor and their reciprocals are ordinary numbers for the fast division.
+constexpr float HELD = 64.0f, LEAST = 1e-36f, MOST = 8e37f;
 
 struct Decode8 {
   Attn8 a;
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
   constexpr int HEADS = 8 * NT, MTILES = HD / 16, PITCH = HD + 4;
   using C = Codes<HD>;
   extern __shared__ float merge_o[];                              // [warps][HEADS][PITCH], a head's numbers in the order of the accumulators
-  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS], factors[HEADS];
+  __shared__ float merge_m[DWARPS][HEADS], merge_l[DWARPS][HEADS], merge_v[DWARPS][HEADS], factors[HEADS];
   __shared__ __align__(16) uint32_t queries[NT][C::KC][DIGITS][32][4];
   __shared__ int start_of[5];
   __shared__ float2 part_state[CLUSTER ? HEADS : 1];              // what merge_o's first place is over: (maximum, sum)
@@ -483,7 +488,8 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       factor[nt][0] = factors[8 * nt + 2 * t];
       factor[nt][1] = factors[8 * nt + 2 * t + 1];
     }
-    float o[NT][MTILES][4], m[NT][2], l[NT][2];
+    // a head's running maximum, its sum of probabilities, and what products of a probability and a value's scale are multiplied with
+    float o[NT][MTILES][4], m[NT][2], l[NT][2], over[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -492,9 +498,8 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
       m[nt][0] = m[nt][1] = NONE;
       l[nt][0] = l[nt][1] = 0.0f;
+      over[nt][0] = over[nt][1] = HELD / LEAST;
     }
-    // the largest scale of the values so far, from the smallest whose factor float32 has, and what scales are multiplied with
-    float v_most = 3e-37f, v_over = HELD / 3e-37f;
 
     for (int slice = first; slice < last; ++slice) {
       const bool here = page >= 0 && page < p.a.num_pages;         // `asked` is this slice still
@@ -527,6 +532,16 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       }
       const float f0 = c.ks[0], f1 = c.ks[1];
       float v0 = c.vs[0], v1 = c.vs[1];
+      float e[NT][4], held[NT][4];                                   // probabilities; with their values' scales, as the tensor core gets them
+      bool raise = false;                                            // (an unseen position's scale costs a look, no more)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          held[nt][i] = v0 * over[nt][i];
+          held[nt][2 + i] = v1 * over[nt][i];
+          raise |= fmaxf(fabsf(held[nt][i]), fabsf(held[nt][2 + i])) > 2.0f * HELD;
+        }
       if (slice + 1 < last) load_keys<HD>(p, c, row, g, t);
 
 #pragma unroll
@@ -547,33 +562,34 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
           for (int e = 0; e < 2; ++e) {
             sc[nt][e] = see0 ? sc[nt][e] : -INFINITY;
             sc[nt][2 + e] = see1 ? sc[nt][2 + e] : -INFINITY;
+            held[nt][e] = see0 ? held[nt][e] : 0.0f;
+            held[nt][2 + e] = see1 ? held[nt][2 + e] : 0.0f;
           }
       }
-      bool raise = fmaxf(v0, v1) > 2.0f * v_most;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + 8.0f;
+        for (int i = 0; i < 2; ++i) raise |= fmaxf(sc[nt][i], sc[nt][2 + i]) > m[nt][i] + 8.0f;
       if (__any_sync(0xffffffffu, raise)) {
-        float v_now = fmaxf(fmaxf(v0, v1), v_most);
-#pragma unroll
-        for (int offset = 4; offset < 32; offset <<= 1) v_now = fmaxf(v_now, __shfl_xor_sync(0xffffffffu, v_now, offset));
-        const float v_down = v_most / v_now;
-        v_most = v_now;
-        v_over = HELD / v_now;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float down[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float most = fmaxf(sc[nt][e], sc[nt][2 + e]);
+          for (int i = 0; i < 2; ++i) {
+            float most = fmaxf(sc[nt][i], sc[nt][2 + i]);
 #pragma unroll
             for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
-            most = fmaxf(most, m[nt][e]);
-            down[e] = exp2_fast(m[nt][e] - most);
-            m[nt][e] = most;
-            l[nt][e] *= down[e];
-            down[e] *= v_down;
+            most = fmaxf(most, m[nt][i]);
+            const float fall = exp2_fast(m[nt][i] - most);
+            m[nt][i] = most;
+            l[nt][i] *= fall;
+            // the largest product here; what the largest so far comes to under the new maximum
+            float seen = fmaxf(fabsf(exp2_fast(sc[nt][i] - most) * v0), fabsf(exp2_fast(sc[nt][2 + i] - most) * v1));
+#pragma unroll
+            for (int offset = 4; offset < 32; offset <<= 1) seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, offset));
+            const float so_far = __fdividef(HELD, over[nt][i]) * fall, now = fminf(fmaxf(fmaxf(so_far, seen), LEAST), MOST);
+            over[nt][i] = __fdividef(HELD, now);
+            down[i] = __fdividef(so_far, now);
           }
 #pragma unroll
           for (int i = 0; i < MTILES; ++i) {
@@ -581,24 +597,36 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
             o[nt][i][2] *= down[0]; o[nt][i][3] *= down[1];
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[nt][i] = exp2_fast(sc[nt][i] - m[nt][i & 1]);
+            held[nt][i] = e[nt][i] * (i < 2 ? v0 : v1) * over[nt][i & 1];        // (in this order: a large value may have no probability)
+          }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[nt][i] = exp2_fast(sc[nt][i] - m[nt][i & 1]);
+            held[nt][i] *= e[nt][i];
+          }
       }
       uint32_t pr[NT][PARTS][2];
-      const float w0 = v0 * v_over, w1 = v1 * v_over;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float e0 = exp2_fast(sc[nt][0] - m[nt][0]), e1 = exp2_fast(sc[nt][1] - m[nt][1]);
-        float e2 = exp2_fast(sc[nt][2] - m[nt][0]), e3 = exp2_fast(sc[nt][3] - m[nt][1]);
-        l[nt][0] += e0 + e2;
-        l[nt][1] += e1 + e3;
-        e0 *= w0; e1 *= w0; e2 *= w1; e3 *= w1;
+        l[nt][0] += e[nt][0] + e[nt][2];
+        l[nt][1] += e[nt][1] + e[nt][3];
+        float (&h)[4] = held[nt];
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const uint32_t x = two_halves(e0, e1), y = two_halves(e2, e3);
+          const uint32_t x = two_halves(h[0], h[1]), y = two_halves(h[2], h[3]);
           pr[nt][part][0] = transposed(x);
           pr[nt][part][1] = transposed(y);
           if (part + 1 < PARTS) {
-            leave(x, e0, e1);
-            leave(y, e2, e3);
+            leave(x, h[0], h[1]);
+            leave(y, h[2], h[3]);
           }
         }
       }
@@ -624,7 +652,6 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
 
     // the warps' states meet in shared memory: the two numbers of a lane and a tile side by side, then the lanes g, then the tiles
     __syncthreads();                                              // whoever still reads the unit before
-    if (lane == 0) merge_v[warp] = v_most * (1.0f / (127.0f * HELD));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -636,6 +663,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
         if (g == 0) {
           merge_m[warp][head] = m[nt][e];
           merge_l[warp][head] = sum;
+          merge_v[warp][head] = __fdividef(1.0f / 127.0f, over[nt][e]);
         }
         float* dst = merge_o + (warp * HEADS + head) * PITCH + 2 * g;
 #pragma unroll
@@ -654,7 +682,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT)) dec
       float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < DWARPS; ++w) {
-        const float f = exp2_fast(merge_m[w][head] - most), fv = f * merge_v[w];
+        const float f = exp2_fast(merge_m[w][head] - most), fv = f * merge_v[w][head];
         const float2 x = *reinterpret_cast<const float2*>(merge_o + (w * HEADS + head) * PITCH + 2 * pair);
         sum = fmaf(f, merge_l[w][head], sum);
         acc.x = fmaf(fv, x.x, acc.x);

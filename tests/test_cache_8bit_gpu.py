@@ -932,3 +932,48 @@ def test_pages_of_one_call_leave_no_tensor_maps_behind(ops):
             assert rel_error(out, torch.cat(want).flatten(1)) < TOL[torch.bfloat16]
         assert lib.tge_attention_mma_kept_maps() == before
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [128, 64, 256, 80])
+@pytest.mark.parametrize("small", [-10, -25, -40, -100])
+@pytest.mark.parametrize("columns", [5, 130])
+def test_single_tokens_that_look_at_a_small_value(ops, dtype, dim, small, columns):
+    """Nearly all of a token's weight is on one position whose value is far smaller than what else it sees, early, late or alone in its slice."""
+    heads, kv, held, looks = 4, 2, [300, 300, 40, 17], (3, 280, 20, 16)
+    cache = Cache(held, kv, dim, 64, 1)
+    wide = torch.full((4, columns), -1, dtype=torch.int32)
+    wide[:, :cache.table.shape[1]] = cache.table
+    cache.table = wide
+    q = torch.stack([cache.values("k", r)[pos].float().repeat_interleave(heads // kv, 0) for r, pos in enumerate(looks)])
+    for r, pos in enumerate(looks):
+        cache.scales["v"][cache.table[r, pos // 64].item(), :, pos % 64] *= 2.0 ** small
+    scale = 100.0 / float(q.pow(2).sum(-1).min())
+    q = q.flatten(1).to(dtype)
+    positions, seq, q_start, start_pos = batch_index([1] * 4, [h - 1 for h in held], DEV)
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 4, 1, 300, heads, kv, dim, scale)
+    ops.check_status()
+    # float32: a score of some hundreds is known to 2^-22 of it
+    assert row_errors(out, q, cache, [1] * 4, heads, scale) < (2 ** -7 if dtype == torch.bfloat16 else 2 ** -12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("far", [60, 100, 400])
+@pytest.mark.parametrize("base,power", [(0, 20), (0, 60), (0, 120), (-110, 230)])
+@pytest.mark.parametrize("order", [(0, 1, 2), (1, 0, 2), (2, 1, 0), (1, 2, 0)])
+def test_single_tokens_that_hardly_weigh_large_values(ops, dtype, far, base, power, order):
+    """Pages whose values are 2^120 the others' size and more, and whose scores lie far below theirs, in front of them and behind them."""
+    heads, kv, dim, held = 4, 2, 128, [192]
+    cache = Cache(held, kv, dim, 64, 1)
+    codes = torch.randint(-127, 128, (dim,), generator=torch.Generator().manual_seed(3)).to(torch.int8)
+    near, away, middle = (cache.table[0, i].item() for i in order)
+    cache.codes["k"][near], cache.codes["k"][away], cache.codes["k"][middle] = codes, -codes, 0
+    cache.scales["k"].fill_(1.0)
+    cache.scales["v"][[near, middle]] *= 2.0 ** base
+    cache.scales["v"][away] *= 2.0 ** (base + power)
+    q = (codes.float() / 127).repeat(1, heads, 1).flatten(1).to(dtype)
+    scale = far / 2 * math.log(2) / float((codes.float() / 127).pow(2).sum())            # scores of far / 2, its negative and 0, in powers of two
+    positions, seq, q_start, start_pos = batch_index([1], [191], DEV)
+    out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 1, 1, 192, heads, kv, dim, scale)
+    ops.check_status()
+    assert row_errors(out, q, cache, [1], heads, scale) < (2 ** -7 if dtype == torch.bfloat16 else 2 ** -12)
