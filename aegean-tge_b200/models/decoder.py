@@ -47,6 +47,8 @@ class DecoderModel:
             else:
                 self.blocks.append(block_class(mixer, ffn, norm1, norm2, env))
         if env.cache_block is not None:
+            if env.cache_block <= 0 or env.cache_block & (env.cache_block - 1) or env.page_size % env.cache_block:
+                raise ValueError(f"cache_block {env.cache_block} must be a power of two that divides the page of {env.page_size}")
             for index, block in enumerate(self.blocks):
                 if (block.mixer.cache_spec() is not None or block.mixer.extra_cache_specs()) and not block.mixer.holds_8bit:
                     raise ValueError(f"layers[{index}]: {spec.layers[index].mixer.kind} as this model has it keeps its cache in the run "

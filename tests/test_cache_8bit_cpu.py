@@ -109,3 +109,16 @@ def test_command_line(tmp_path):
                   ["score", "--config", str(path), "--tokens", "1 2", "--compare"], ["score", "--config", str(path), "--tokens", "1 2", "--top", "33"],
                   ["score", "--config", str(path), "--tokens", "1 2", "--cache-dtype", "int4"]):
         assert tge(*wrong).returncode == 2, wrong
+
+
+@pytest.mark.parametrize("block", [0, -4, 3, 128])
+def test_a_block_that_no_page_holds_is_refused_wherever_a_model_is_put_together(block, tmp_path):
+    """By `tge plan` as by an engine."""
+    import json
+    arch = architecture_of(CONFIG)
+    with pytest.raises(ValueError, match="cache_block"):
+        DecoderModel(arch.build_spec(arch.parse_config(CONFIG)), env(block))
+    (tmp_path / "config.json").write_text(json.dumps(CONFIG))
+    done = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "tge"), "plan", "--model", str(tmp_path), "--cache-dtype", "int8", "--cache-block", str(block)],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode != 0 and "cache_block" in done.stderr
