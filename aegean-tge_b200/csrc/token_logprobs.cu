@@ -289,6 +289,9 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Logpro
   const uint32_t bits = __float_as_uint(own + 0.0f);
   const float above = own != own ? own : __uint_as_float(bits & 0x80000000u ? bits - 1 : bits + 1);
   const bool token_is_nan = own != own;
+  // the round that looks at indices: the token's; in a cluster, whose chunks end inside a round, the chunk's last one if the token lies behind
+  // it (what take() puts behind a chunk is -inf, and so may the token be)
+  const int near = CLUSTER ? min(token, end - 1) : token;
   Sums mine{LEAST, 0.0f, 0.0f, 0};
   unsigned long long least = 0;                  // the smallest of the best so far (0: not as many yet)
   __syncthreads();
@@ -351,8 +354,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Logpro
       mine.w += w;
     }
     mine.z += z;
-    // (in front of the token's round only where the round is all of this chunk's: what take() puts behind the chunk counts as -inf too)
-    if (!token_is_nan && (token < first || (token >= first + ROUND && first + ROUND <= end))) {
+    if (!token_is_nan && (near < first || near >= first + ROUND)) {
       const float from = first < token ? own : above;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) mine.before += v[i] >= from ? 1 : 0;
