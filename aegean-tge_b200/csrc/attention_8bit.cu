@@ -122,9 +122,9 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
 // most two per block, and a second kernel joins them in the order of the positions.  Few units over short contexts (decode_cluster) go without: a
 // cluster of blocks has a unit, its slices in equal shares, and joins them through its shared memory.
 //
-// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (425 MB with their scales) 80.5 us, 5.3 TB/s or 0.81 of a
-// copy's rate; a kernel that only reads the same pages takes 71.7.  Four of 32,768 45 us, eight of 2,048 at 28 heads over 4 (a cluster each unit)
-// 10.3, of 512 8.2: the trips to memory one behind the other.  Not taken: the codes through rings in shared memory (117 us where this took 83), two slices of
+// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (425 MB with their scales) 76.8 us, 5.5 TB/s or 0.85 of a
+// copy's rate; a kernel that only reads the same pages takes 71.7.  Four of 32,768 41.6 us, eight of 2,048 at 28 heads over 4 (a cluster each unit)
+// 9.9, of 512 7.1: the trips to memory one behind the other.  Not taken: the codes through rings in shared memory (117 us where this took 83), two slices of
 // each warp on their way (94), slices dealt to the warps in turn instead of in runs (91 beside 81), pages asked into L2 a slice ahead (86).
 // ---------------------------------------------------------------------------
 constexpr int DWARPS = 4;

@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 // with.  The first blocks have a token each: its groups take its query heads (and, with blocks of one position, its key and value heads) in
 // turn, three rows on their way at a time, the angles loaded once.  With larger blocks the others have a (block of positions, key or value
 // head) each: its groups take the block's rows in turn, once for the scale and, from cache, once for the codes.
-// With the read-back below: one token 8.4 us; a prompt of 2,048 tokens at 28 heads over 4 15 us (43 MB; 6.6 at a copy's rate); 64 tokens
-// of requests that hold up to 512 (25,109 together) at 40 heads over 8, blocks of 16, 48 us (165 MB, 25 at that rate).  With a warp to a head, as above: 25, 57 and 92 us.
+// With the read-back below: one token 7.2 us; a prompt of 2,048 tokens at 28 heads over 4 13.5 us (43 MB; 6.6 at a copy's rate); 64 tokens
+// of requests that hold up to 512 (25,109 together) at 40 heads over 8, blocks of 16, 46 us (165 MB, 25 at that rate).  With a warp to a head, as above: 25, 57 and 92 us.
 // ---------------------------------------------------------------------------
 constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns
 
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_8b
 // first tokens counted from the first one's.  In float16 with a power of two for each run and head, for the attention kernel that takes these.
 // For attention (starts are wanted): it multiplies every value of a tile with a probability, unseen ones with zero, so values are finite there:
 // a position whose values' scale is not gets a key that is not, which whoever sees it turns into the same and nobody else looks at.
-// Bound by the bytes written, two (four) to a code read: 8,128 positions of 8 heads in float16 50 MB, 15.8 us from cold.
+// Bound by the bytes written, two (four) to a code read: 8,128 positions of 8 heads in float16 50 MB, 12.7 us with the plan.
 // ---------------------------------------------------------------------------
 struct ReadParams {
   const int8_t *k_pages, *v_pages;

@@ -262,9 +262,9 @@ __device__ __forceinline__ void take(const T* x, int first, int end, float (&v)[
 // passes the n-th of those, then whatever passes the n-th of the chunk's first 1, 2, 4, 8, ... rounds: of random rows some hundred logits are
 // ever listed.  A row that lists more than there is room for (rising logits) is looked through again.
 //
-// 1,024 rows of 152,064 float32 logits with the 20 best: 120 us, 5.2 TB/s or 0.79 of a copy's rate (without alternatives 109); 70 % of the issue
-// slots are taken, some 20 instructions a logit.  In bfloat16 155 us, for the same number of instructions and the conversions.  One row
-// with 5 alternatives 10.4 us: the trips of three rounds and of the joining.  Not taken: cuts after rounds 1, 4, 16, ... only (127 us); a bar that
+// 1,024 rows of 152,064 float32 logits with the 20 best: 118 us, 5.3 TB/s or 0.81 of a copy's rate (without alternatives 105); 70 % of the issue
+// slots are taken, some 20 instructions a logit.  In bfloat16 152 us, for the same number of instructions and the conversions.  One row
+// with 5 alternatives 9.0 us: the trips of three rounds and of the joining.  Not taken: cuts after rounds 1, 4, 16, ... only (127 us); a bar that
 // stays where the first round put it, with a barrier every round (365).
 template <typename T, bool VECTOR, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const LogprobParams p) {

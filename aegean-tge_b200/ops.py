@@ -1344,7 +1344,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
         if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
             # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
-            # the read-back, on SMs that its last wave leaves.  63 of 2,048 beside 1,985 after 6,143 (40 heads over 8) 471 -> 422 us, 63 of
+            # the read-back, on SMs that its last wave leaves.  63 of 2,048 beside 1,985 after 6,143 (40 heads over 8) 460 -> 425 us, 63 of
             # 4,096 beside 1,000 after 3,000 225 -> 219, 32 of 1,024 beside 2,016 113 -> 110.  The second stream costs the host 37 us more than
             # the 72 of a call, so smaller steps, of which the device would do 31 of 2,048 beside 1,000 after 1,000 (28 over 4) in 64 instead
             # of 76 us, would wait for it.
