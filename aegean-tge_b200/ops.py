@@ -1340,7 +1340,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     as_portions = max_q_len > 1 and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
                                      else head_dim in (16, 32, 64, 128) and sink is None)
-    if as_portions and need >= 0 and MIN_DECODE_PREFIX <= singles < num_seqs and not torch.cuda.is_current_stream_capturing():
+    if as_portions and need >= 0 and MIN_DECODE_PREFIX <= singles < min(num_seqs, tokens) and not torch.cuda.is_current_stream_capturing():
         reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
         if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
             # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
@@ -1365,7 +1365,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if done < singles and as_portions:
         simply(done, singles)                             # (the portions behind them go the way that they go alone)
         done = singles
-    if done == num_seqs:
+    if done == num_seqs or done == tokens:                # (requests that bring nothing may hold nothing)
         return out
     if as_portions:
         portions(done)

@@ -977,3 +977,23 @@ def test_single_tokens_that_hardly_weigh_large_values(ops, dtype, far, base, pow
     out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 1, 1, 192, heads, kv, dim, scale)
     ops.check_status()
     assert row_errors(out, q, cache, [1], heads, scale) < (2 ** -7 if dtype == torch.bfloat16 else 2 ** -12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [128, 80])
+@pytest.mark.parametrize("lens", [[1, 0], [1, 0, 0], [0, 0]])
+@pytest.mark.parametrize("window", [0, 20])
+def test_requests_behind_single_tokens_that_neither_bring_nor_hold(ops, dtype, dim, lens, window):
+    """Under a bound of their lengths that would let them bring more."""
+    held = [50] * lens[0] + [0] * (len(lens) - lens[0])
+    cache = Cache(held, 2, dim, 16, 1)
+    for prefix in (0, lens[0]):
+        positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+        q = torch.randn(sum(lens), 4 * dim, generator=torch.Generator().manual_seed(1)).to(dtype)
+        out = ops.attention_8bit(q.to(DEV), *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, len(lens), 7, 50, 4, 2, dim, 0.1,
+                                 window=window, decode_prefix=prefix, ctx_lens=held)
+        ops.check_status()
+        assert out.shape == q.shape
+        if lens[0]:
+            want = plain.attend(q.view(1, 4, dim), cache.values("k", 0), cache.values("v", 0), 49, 0.1, window, None)
+            assert rel_error(out, want.flatten(1)) < TOL[dtype]
