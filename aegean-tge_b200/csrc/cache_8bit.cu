@@ -445,20 +445,21 @@ __device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
 // The block table over the runs, and the first tokens if wanted.  A kernel of its own: attention kernels look block tables and first tokens up while
 // the kernel in front of them still runs, so these have to be there before that one lets them start.  One block, a request to a thread at a time:
 // one request after the other took 64 of them 9 us longer.
+// The attention kernels size their memory by the host's numbers: where these leave out what the requests hold, the step is reported, and with first
+// tokens of zero no request brings any.
 constexpr int PLAN_THREADS = 256;
 __global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const ReadParams p) {
   __shared__ int first_run[PLAN_THREADS], count[PLAN_THREADS], runs_upto[PLAN_THREADS], of_warp[PLAN_THREADS / 32];
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += PLAN_THREADS)
-    p.starts[i] = p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
   int total = 0;
+  bool beyond = false;
   for (int base = p.first_seq; base < p.num_seqs; base += PLAN_THREADS) {
     const int here = min(PLAN_THREADS, p.num_seqs - base);
     Span s{0, 0};
     if ((int)threadIdx.x < here) s = span_of(p, base + threadIdx.x);
-    if (s.first + s.count > p.width) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+    beyond |= s.first + s.count > p.width;
     int upto = s.count;
 #pragma unroll
     for (int offset = 1; offset < 32; offset <<= 1) {
@@ -481,7 +482,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const Read
     for (int w = 0; w < PLAN_THREADS / 32; ++w) total += of_warp[w];
     __syncthreads();
   }
-  if (total > p.runs && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+  beyond = __syncthreads_or(beyond || total > p.runs);
+  if (beyond && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
+  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += PLAN_THREADS)
+    p.starts[i] = beyond ? 0 : p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
 }
 
 // float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ.

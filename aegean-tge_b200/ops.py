@@ -1248,7 +1248,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     last token.  ``window``: how many of the latest positions a query sees (0: all); ``sink`` (float32 [heads]): a score per head
     that joins the softmax's denominator once, with no key or value.  ``decode_prefix``: how many requests at the head of the batch
     are known to bring one token each while others bring more.  ``ctx_lens`` (host numbers): what every request holds after the
-    step (None: ``max_ctx_len``, a bound).
+    step (None: ``max_ctx_len``, a bound); portions that hold more are reported through the status word and get no output.
     """
     _want(q, "queries", _FLOAT, contiguous=False)
     q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
@@ -1295,6 +1295,8 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         a query tile of those reads each of them again, so that turning codes into numbers there would be done many times over.
         bfloat16 runs, heads of 64 or 128: in float16 over powers of two, three bits more than bfloat16 has.  Else in the run type."""
         starts, longest = q_start.new_empty(num_seqs - first + 1), max(ctx_lens[first:])
+        if longest <= 0:
+            raise KernelError(f"attention: {tokens - first} tokens of requests that hold nothing")
         rows = (q, start_pos, positions, seq_of_token, out)
         if first:
             rows = (q[first:], start_pos[first:], positions[first:], seq_of_token[first:], out[first:])

@@ -997,3 +997,27 @@ def test_requests_behind_single_tokens_that_neither_bring_nor_hold(ops, dtype, d
         if lens[0]:
             want = plain.attend(q.view(1, 4, dim), cache.values("k", 0), cache.values("v", 0), 49, 0.1, window, None)
             assert rel_error(out, want.flatten(1)) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64), (4, 2, 80), (2, 1, 256), (6, 2, 32)])
+@pytest.mark.parametrize("told", [[90, 200], [3000, 40], [0, 200], [64, 64]])
+def test_contexts_longer_than_the_host_was_told_are_reported(ops, dtype, heads, kv, dim, told):
+    """Memory that is sized by the host's numbers is not run over; the next step is right again."""
+    held, lens = [3000, 200], [40, 70]
+    cache = Cache(held, kv, dim, 16, 1)
+    positions, seq, q_start, start_pos = batch_index(lens, [h - n for h, n in zip(held, lens)], DEV)
+    q = torch.randn(sum(lens), heads * dim, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    args = (q, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 2, 70)
+    want = ops.attention_8bit(*args, 3000, heads, kv, dim, 0.09, ctx_lens=held)
+    ops.check_status()
+    out = ops.attention_8bit(*args, max(told), heads, kv, dim, 0.09, ctx_lens=told)
+    if dtype == torch.float32 and dim in (80, 256):              # the kernel that walks the keys row by row needs no such numbers
+        assert torch.equal(out, want)
+    else:
+        with pytest.raises(ops.DeviceStatusError, match="row"):
+            ops.check_status()
+        with pytest.raises(ops.KernelError):
+            ops.attention_8bit(*args, 0, heads, kv, dim, 0.09, ctx_lens=[0, 0])
+    assert torch.equal(ops.attention_8bit(*args, 3000, heads, kv, dim, 0.09, ctx_lens=held), want)
+    ops.check_status()
