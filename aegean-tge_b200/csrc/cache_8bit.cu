@@ -492,7 +492,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const Read
 // float16's numbers are 2^-24 apart below 2^-14, so a position whose scale is at least 2^-13 of the power keeps 2^-12 of its own largest
 // number, which is what float16 keeps of any.  A run with a smaller scale (its largest one is above 2^-8 of the power: they lie 2^5 apart at
 // least) holds whole codes over 128, which float16 has exactly, and the scales go to the attention as factors: what multiplies a key's scores,
-// and the logarithm to the base 2 of what multiplies a value's probability.
+// and the logarithm to the base 2 of what multiplies a value's probability.  So does a run with values of zero beside others: a row that sees those
+// alone adds nothing, whatever the others' power says.
 __device__ __forceinline__ int exponent_above(float s) {      // of such a power that is no smaller than s > 0
   return min(max(((int)(__float_as_uint(s) >> 23) - 126 + 7) & ~7, -120), 120);
 }
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
         ks = here ? fabsf(p.k_scale[block]) : 0.0f;
         vs = here ? fabsf(p.v_scale[block]) : 0.0f;
         const float k = warp_max(ks < INFINITY ? ks : 0.0f), v = warp_max(vs < INFINITY ? vs : 0.0f);
-        const float k_least = -warp_max(ks > 0.0f ? -ks : -INFINITY), v_least = -warp_max(vs > 0.0f ? -vs : -INFINITY);
+        const float k_least = -warp_max(ks > 0.0f ? -ks : -INFINITY), v_least = -warp_max(here && vs >= 0.0f ? -vs : -INFINITY);
         if ((threadIdx.x & 31) == 0) {
           most[threadIdx.x >> 5][0] = k;
           most[threadIdx.x >> 5][1] = v;
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
       const int e = k > 0.0f ? exponent_above(k) : 0, f = v > 0.0f ? exponent_above(v) : 0;
       k_over = power_of_two(-e);
       v_over = power_of_two(-f);
-      whole_codes = fminf(least[0][0], least[1][0]) < power_of_two(e) * 0x1p-13f || fminf(least[0][1], least[1][1]) < power_of_two(f) * 0x1p-13f;
+      whole_codes = fminf(least[0][0], least[1][0]) < power_of_two(e) * 0x1p-13f || (v > 0.0f && fminf(least[0][1], least[1][1]) < power_of_two(f) * 0x1p-13f);
       if (threadIdx.x == 0) p.exponents[(size_t)run * p.kv_heads + kvh] = (int)((uint32_t)e << 16 | ((uint32_t)f & 0xffffu)) | (whole_codes ? 1 : 0);
       // (no factor is infinite or NaN, whatever the scale: a masked position has one too)
       if (whole_codes && threadIdx.x < 64)

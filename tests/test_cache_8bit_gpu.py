@@ -1021,3 +1021,18 @@ def test_contexts_longer_than_the_host_was_told_are_reported(ops, dtype, heads, 
             ops.attention_8bit(*args, 0, heads, kv, dim, 0.09, ctx_lens=[0, 0])
     assert torch.equal(ops.attention_8bit(*args, 3000, heads, kv, dim, 0.09, ctx_lens=held), want)
     ops.check_status()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("powers", [(-60, 100), (0, 110), (-110, 110)])
+@pytest.mark.parametrize("zeros", [1, 3, 64])
+def test_portions_whose_rows_see_only_zeros_of_a_run_of_large_values(ops, heads, kv, dim, powers, zeros):
+    """Values of zero in front of ones 2^110 the run before's size: the rows that see no more of the run than zeros keep what they have."""
+    held = [160]
+    cache = Cache(held, kv, dim, 64, 1)
+    for run in range(3):
+        cache.scales["v"][cache.table[0, run].item()] *= 2.0 ** powers[min(run, 1)]
+    cache.scales["v"][cache.table[0, 1].item(), :, :zeros] = 0.0
+    q = torch.randn(160, heads * dim, generator=torch.Generator().manual_seed(4)).bfloat16()
+    out = portions_of(ops, cache, held, heads, q, 0.02)
+    assert row_errors(out, q, cache, held, heads, 0.02) < 2 ** -7
