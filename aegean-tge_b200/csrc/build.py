@@ -33,8 +33,9 @@ COMMON_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcomp
 CORE_SOURCES = ["host_util.cu", "elementwise.cu", "gemm_simt.cu", "gemm_tcgen05.cu", "gemm_f32_tcgen05.cu", "attention_simt.cu", "attention_f32.cu", "sampling.cu", "sampling_cuts.cu",
                 "gemm_static_scratch.cu", "random_fill.cu", "sequence_mix.cu", "decay_scan_tc.cu", "stream_norm.cu", "latent_attention.cu",
                 "routed_mlp.cu", "gated_mix.cu", "matrix_lstm.cu", "residual_streams.cu",
-                "cache_8bit.cu", "attention_8bit.cu", "token_logprobs.cu"]
-HEADERS = ["common.cuh", "gemm_static_scratch.h", "random_weights.h", "attention_tc.cuh", "attention_tc2.cuh", "tcgen05_ptx.cuh"]
+                "cache_8bit.cu", "attention_8bit.cu", "cache_4bit.cu", "attention_4bit.cu", "token_logprobs.cu"]
+HEADERS = ["common.cuh", "gemm_static_scratch.h", "random_weights.h", "attention_tc.cuh", "attention_tc2.cuh", "tcgen05_ptx.cuh",
+           "cache_runs.cuh", "decode_units.cuh"]
 RUNTIME_SOURCES = ["runtime.cpp"]
 RUNTIME_HEADERS = ["runtime.h", "random_weights.h"]
 

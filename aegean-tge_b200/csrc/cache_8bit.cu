@@ -12,15 +12,10 @@
 //   lo' = lo cos - hi sin ; hi' = lo sin + hi cos
 // keys are quantised from these float32 numbers, with no rounding to the run's type in between.  127 x is exact for a bfloat16 x and
 // the division is rounded once, so x = s (k + 1/2) / 127 meets its tie exactly and goes to even wherever it is computed.
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <type_traits>
 
-#include "common.cuh"
-
-template <>
-__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+#include "cache_runs.cuh"
 
 namespace {
 
@@ -41,13 +36,6 @@ struct Coder {
     return any ? min(max(__float2int_rn(__fdiv_rn(127.0f * (x * shrink), over)), -127), 127) : 0;
   }
 };
-
-// max that keeps NaN, and turns an infinity into one
-__device__ __forceinline__ float magnitude(float x) {
-  const float a = fabsf(x);
-  return a <= 3.402823466e38f ? a : __int_as_float(0x7fc00000);
-}
-__device__ __forceinline__ float larger(float a, float b) { return a > b || !(a == a) ? a : b; }
 
 __device__ __forceinline__ float warp_larger(float v) {
 #pragma unroll
@@ -165,45 +153,6 @@ __global__ void __launch_bounds__(WARPS * 32) store_8bit_kernel(const StoreParam
 // ---------------------------------------------------------------------------
 constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns
 
-struct Eight { float x[8]; };
-// Eight numbers as they lie in memory.
-template <typename T> struct Raw;
-template <> struct Raw<__nv_bfloat16> { uint4 w; };
-template <> struct Raw<float> { float4 a, b; };
-__device__ __forceinline__ Raw<__nv_bfloat16> raw_eight(const __nv_bfloat16* src) { return {*reinterpret_cast<const uint4*>(src)}; }
-__device__ __forceinline__ Raw<float> raw_eight(const float* src) { return {reinterpret_cast<const float4*>(src)[0], reinterpret_cast<const float4*>(src)[1]}; }
-__device__ __forceinline__ Eight eight(const Raw<__nv_bfloat16>& r) {
-  const uint32_t w[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
-  Eight e;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    e.x[2 * i] = __uint_as_float(w[i] << 16);
-    e.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-  return e;
-}
-__device__ __forceinline__ Eight eight(const Raw<float>& r) { return Eight{{r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w}}; }
-template <typename T>
-__device__ __forceinline__ Eight eight(const T* src) { return eight(raw_eight(src)); }
-
-__device__ __forceinline__ void put_eight(__nv_bfloat16* dst, const Eight& e) {
-  uint4 raw;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(e.x[2 * i], e.x[2 * i + 1]);
-  *reinterpret_cast<uint4*>(dst) = raw;
-}
-__device__ __forceinline__ void put_eight(__half* dst, const Eight& e) {
-  uint4 raw;
-  __half2* h = reinterpret_cast<__half2*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(e.x[2 * i], e.x[2 * i + 1]);
-  *reinterpret_cast<uint4*>(dst) = raw;
-}
-__device__ __forceinline__ void put_eight(float* dst, const Eight& e) {
-  reinterpret_cast<float4*>(dst)[0] = make_float4(e.x[0], e.x[1], e.x[2], e.x[3]);
-  reinterpret_cast<float4*>(dst)[1] = make_float4(e.x[4], e.x[5], e.x[6], e.x[7]);
-}
 __device__ __forceinline__ void turn(Eight& lo, Eight& hi, const Eight& c, const Eight& s) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -416,77 +365,14 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_8b
 // a position whose values' scale is not gets a key that is not, which whoever sees it turns into the same and nobody else looks at.
 // Bound by the bytes written, two (four) to a code read: 8,128 positions of 8 heads in float16 50 MB, 12.7 us with the plan.
 // ---------------------------------------------------------------------------
-struct ReadParams {
+struct ReadParams : RunPlan {
   const int8_t *k_pages, *v_pages;
   const float *k_scale, *v_scale;
-  const int *block_table, *q_start, *start_pos;
-  int max_pages, num_pages, page_size, block, first_seq, num_seqs, kv_heads, head_dim, window;
+  int block, kv_heads, head_dim;
   void *k_out, *v_out;
   float2* factors;                             // [runs, kv_heads, 64], for float16 output: of runs whose scales lie far apart, see below
   int* exponents;                              // [runs, kv_heads], for float16 output: f below, e above; 1: the run has factors
-  int *table, *starts;
-  int runs, width;
-  int* status;
 };
-
-// The first position that a step's queries see, from `start` on.  Pages in front of it are given back, also where they lie in its run of 64:
-// those positions are zeros and nobody's fault.
-__device__ __forceinline__ int first_seen(const ReadParams& p, int start) { return p.window > 0 ? max(start - p.window + 1, 0) : 0; }
-
-struct Span { int first, count; };             // a request's runs: from position 64 first on
-__device__ __forceinline__ Span span_of(const ReadParams& p, int seq) {
-  const int start = p.start_pos[seq], held = start + p.q_start[seq + 1] - p.q_start[seq];
-  Span s;
-  s.first = first_seen(p, start) >> 6;
-  s.count = max((held + 63) / 64 - s.first, 0);
-  return s;
-}
-
-// The block table over the runs, and the first tokens if wanted.  A kernel of its own: attention kernels look block tables and first tokens up while
-// the kernel in front of them still runs, so these have to be there before that one lets them start.  One block, a request to a thread at a time:
-// one request after the other took 64 of them 9 us longer.
-// The attention kernels size their memory by the host's numbers: where these leave out what the requests hold, the step is reported, and with first
-// tokens of zero no request brings any.
-constexpr int PLAN_THREADS = 256;
-__global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const ReadParams p) {
-  __shared__ int first_run[PLAN_THREADS], count[PLAN_THREADS], runs_upto[PLAN_THREADS], of_warp[PLAN_THREADS / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int total = 0;
-  bool beyond = false;
-  for (int base = p.first_seq; base < p.num_seqs; base += PLAN_THREADS) {
-    const int here = min(PLAN_THREADS, p.num_seqs - base);
-    Span s{0, 0};
-    if ((int)threadIdx.x < here) s = span_of(p, base + threadIdx.x);
-    beyond |= s.first + s.count > p.width;
-    int upto = s.count;
-#pragma unroll
-    for (int offset = 1; offset < 32; offset <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, offset);
-      if (lane >= offset) upto += v;
-    }
-    first_run[threadIdx.x] = s.first;
-    count[threadIdx.x] = s.count;
-    runs_upto[threadIdx.x] = upto - s.count;
-    if (lane == 31) of_warp[warp] = upto;
-    __syncthreads();
-    for (int r = warp; r < here; r += PLAN_THREADS / 32) {
-      int before = total + runs_upto[r];
-      for (int w = 0; w < r >> 5; ++w) before += of_warp[w];
-      for (int i = lane; i < p.width; i += 32) {
-        const int at = i - first_run[r];
-        p.table[(size_t)(base - p.first_seq + r) * p.width + i] = at >= 0 && at < count[r] ? before + at : -1;
-      }
-    }
-    for (int w = 0; w < PLAN_THREADS / 32; ++w) total += of_warp[w];
-    __syncthreads();
-  }
-  beyond = __syncthreads_or(beyond || total > p.runs);
-  if (beyond && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_ROW);
-  for (int i = threadIdx.x; i <= p.num_seqs - p.first_seq && p.starts != nullptr; i += PLAN_THREADS)
-    p.starts[i] = beyond ? 0 : p.q_start[p.first_seq + i] - p.q_start[p.first_seq];
-}
 
 // float16 pages: keys and values over powers of two of their run and head, so that all of them are at most 1.  Multiples of 8: few runs differ.
 // float16's numbers are 2^-24 apart below 2^-14, so a position whose scale is at least 2^-13 of the power keeps 2^-12 of its own largest
@@ -494,11 +380,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) read_8bit_plan_kernel(const Read
 // least) holds whole codes over 128, which float16 has exactly, and the scales go to the attention as factors: what multiplies a key's scores,
 // and the logarithm to the base 2 of what multiplies a value's probability.  So does a run with values of zero beside others: a row that sees those
 // alone adds nothing, whatever the others' power says.
-__device__ __forceinline__ int exponent_above(float s) {      // of such a power that is no smaller than s > 0
-  return min(max(((int)(__float_as_uint(s) >> 23) - 126 + 7) & ~7, -120), 120);
-}
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-
 template <typename T, bool UNITS>
 __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   constexpr bool HALVES = std::is_same<T, __half>::value;
@@ -506,31 +387,8 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const ReadParams p) {
   __shared__ float most[2][2], least[2][2];    // float16: the largest and smallest scales of the run's first and second 32 positions, keys' and values'
   const int run = blockIdx.x;
   pdl_wait();
-  pdl_trigger();                               // behind the wait: see the kernel above
-  if (threadIdx.x < 32) {                      // whose run is this?  32 requests at a time
-    int before = 0, seq_found = -1, first_run = 0, index = 0;
-    for (int base = p.first_seq; base < p.num_seqs && seq_found < 0; base += 32) {
-      const int seq = base + threadIdx.x;
-      Span s{0, 0};
-      if (seq < p.num_seqs) s = span_of(p, seq);
-      int upto = s.count;
-#pragma unroll
-      for (int offset = 1; offset < 32; offset <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, offset);
-        if ((int)threadIdx.x >= offset) upto += v;
-      }
-      const unsigned mine = __ballot_sync(0xffffffffu, run < before + upto);
-      if (mine != 0) {
-        const int who = __ffs(mine) - 1;
-        seq_found = base + who;
-        index = run - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, s.count, who));
-        first_run = __shfl_sync(0xffffffffu, s.first, who);
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (threadIdx.x == 0) { found[0] = seq_found; found[1] = first_run + index; }
-  }
-  __syncthreads();
+  pdl_trigger();                               // behind the wait: see read_plan_kernel
+  find_owner(p, run, found);
   const int seq = found[0], tile = found[1];
   for (int kvh = blockIdx.y; kvh < p.kv_heads; kvh += gridDim.y) {
   T* k_dst = static_cast<T*>(p.k_out) + ((size_t)run * p.kv_heads + kvh) * 64 * p.head_dim;
@@ -718,13 +576,13 @@ TGE_API int tge_read_8bit(const void* k_pages, const void* v_pages, const float*
   if (rc != 0) return rc;
   TGE_REQUIRE(first_seq >= 0 && num_seqs >= first_seq && runs >= 0 && width >= 0 && window >= 0 && kv_heads <= 65535, "read_8bit: bad sizes");
   if (num_seqs == first_seq) return 0;
-  const ReadParams p{(const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block_table, q_start, start_pos, max_pages, num_pages,
-                     page_size, block, first_seq, num_seqs, kv_heads, head_dim, window, k_out, v_out, static_cast<float2*>(factors),
-                     factors == nullptr ? nullptr : static_cast<int*>(factors) + (size_t)runs * kv_heads * 128, table, starts, runs, width, status};
+  const ReadParams p{{block_table, q_start, start_pos, max_pages, num_pages, page_size, first_seq, num_seqs, window, table, starts, runs, width, status},
+                     (const int8_t*)k_pages, (const int8_t*)v_pages, k_scale, v_scale, block, kv_heads, head_dim, k_out, v_out, static_cast<float2*>(factors),
+                     factors == nullptr ? nullptr : static_cast<int*>(factors) + (size_t)runs * kv_heads * 128};
   const bool units = head_dim >= 16 && (head_dim & (head_dim - 1)) == 0 && (page_size & (page_size - 1)) == 0 &&
                      (long long)num_pages * kv_heads <= 0x7fffffffll && ((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
   if (type == 2 && (!units || factors == nullptr || (uintptr_t)factors % 16 != 0)) return TGE_UNSUPPORTED;
-  tge_launch(read_8bit_plan_kernel, 1, PLAN_THREADS, 0, stream, p);
+  tge_launch(read_plan_kernel, 1, PLAN_THREADS, 0, stream, p);
   if (runs == 0) return tge_launched("read_8bit", 1);
   // a block takes several heads of its run where there are many runs: finding whose it is costs as much as a head
   const int at_once = 10 * tge_sm_count();

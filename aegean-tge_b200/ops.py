@@ -216,6 +216,19 @@ def core() -> ctypes.CDLL:
         _declare(lib, "tge_attention_8bit_simple", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
                                                     _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ll, _c_int, _c_int,
                                                     _c_int, _c_float, _c_int, _c_ptr, _c_ptr, _c_ptr])
+        _declare(lib, "tge_store_4bit", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr,
+                                         ctypes.c_double, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr])
+        _declare(lib, "tge_read_4bit", [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int,
+                                        _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr])
+        lib.tge_attention_4bit_decode_floats.argtypes = [_c_int] * 7
+        lib.tge_attention_4bit_decode_floats.restype = _c_ll
+        _declare(lib, "tge_attention_4bit_decode", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int,
+                                                    _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr,
+                                                    _c_ptr, _c_ll, _c_ptr, _c_ptr])
+        _declare(lib, "tge_attention_4bit_simple", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int,
+                                                    _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ll, _c_int, _c_int, _c_int, _c_float, _c_int,
+                                                    _c_ptr, _c_ptr, _c_ptr])
         _declare(lib, "tge_token_logprobs", [_c_ptr, _c_int, _c_ll, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                              _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr])
         lib.tge_token_logprobs_floats.argtypes = [_c_int] * 3
@@ -1224,7 +1237,7 @@ def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, 
     return (k, v, table) if factors is None else (k, v, table, factors)
 
 
-_decode_8bit_floats: Dict[tuple, int] = {}      # scratch numbers by sizes: asking the library costs a microsecond a call
+_codes_floats: Dict[tuple, int] = {}            # scratch numbers by sizes: asking the library costs a microsecond a call
 BESIDE_8BIT_FLOPS = 1e11                         # bound of the portions' work from which single tokens run beside them (some 130 us of it)
 _side_streams: Dict[int, "torch.cuda.Stream"] = {}
 
@@ -1272,23 +1285,47 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     singles = num_seqs if max_q_len <= 1 else decode_prefix
     if singles < num_seqs and ctx_lens is None:
         ctx_lens = [max_ctx_len] * num_seqs
-
     need = -1                                           # scratch numbers of the single tokens' kernel; -1: sizes that it does not take
     if singles:
-        sizes = (is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
-        need = _decode_8bit_floats.get(sizes)
-        if need is None:
-            if len(_decode_8bit_floats) >= 1024:
-                _decode_8bit_floats.clear()
-            need = _decode_8bit_floats[sizes] = lib.tge_attention_8bit_decode_floats(*sizes)
+        need = _decode_floats(lib.tge_attention_8bit_decode_floats, is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
 
     def single_tokens() -> int:
-        """Serves the requests that bring one token each, if the kernel takes them; returns how many."""
         parts = k_scale.new_empty(need) if need else None
         rc = lib.tge_attention_8bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
                                            out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
                                            _ptr(parts), need, status_word().data_ptr(), _stream())
         return singles if _check(rc, lib) != UNSUPPORTED else 0
+
+    def simply(rows, tokens: int) -> None:
+        _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
+                                             tokens, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
+                                             _ptr(sink), status_word().data_ptr(), _stream()), lib)
+
+    def read_as(dtype: torch.dtype, first: int, starts: torch.Tensor):
+        return _read_8bit((num_pages, page_size, block), k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens,
+                          dtype, window, first, starts)
+
+    return _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, seq_of_token, num_seqs, max_q_len, heads, kv_heads, head_dim, scale,
+                         window, sink, ctx_lens, singles, need >= 0, single_tokens, simply, read_as)
+
+
+def _decode_floats(ask, *sizes) -> int:
+    """Scratch numbers of a single tokens' kernel (-1: sizes that it does not take)."""
+    key = (ask.__name__, *sizes)
+    need = _codes_floats.get(key)
+    if need is None:
+        if len(_codes_floats) >= 1024:
+            _codes_floats.clear()
+        need = _codes_floats[key] = ask(*sizes)
+    return need
+
+
+def _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, seq_of_token, num_seqs, max_q_len, heads, kv_heads, head_dim, scale, window,
+                  sink, ctx_lens, singles, takes_singles, single_tokens, simply, read_as) -> torch.Tensor:
+    """Attention over a cache of codes, of arguments that were looked over.  ``single_tokens()`` serves the ``singles`` requests at the head of the batch that
+    bring one token each, if the kernel takes them, and returns how many; ``simply((q, out, positions, seq_of_token) rows, count)`` a warp each;
+    ``read_as(dtype, first, starts)`` reads the requests from ``first`` on back into pages of 64 (see :func:`_read_8bit`)."""
+    is_bf16, tokens, lib = q.dtype == torch.bfloat16, q.shape[0], core()
 
     def portions(first: int, read=None) -> None:
         """The requests from ``first`` on.  Their keys and values are read once into run-type pages of 64, which the prefill kernels take:
@@ -1300,11 +1337,6 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         rows = (q, start_pos, positions, seq_of_token, out)
         if first:
             rows = (q[first:], start_pos[first:], positions[first:], seq_of_token[first:], out[first:])
-
-        def read_as(dtype):
-            return _read_8bit((num_pages, page_size, block), k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens,
-                              dtype, window, first, starts)
-
         aligned = q_stride % 8 == 0 and out_stride % 8 == 0 and (rows[0].data_ptr() | rows[4].data_ptr()) % 16 == 0
         if is_bf16 and head_dim in (64, 128) and scale > 0 and aligned:
             span = longest if window == 0 else min(longest, (-(-window // 64) + 1) * 64)
@@ -1312,14 +1344,14 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             prefill = attention_lib(head_dim)
             held = None
             if prefill.tge_attention_mma_halves_fit(longest, split):
-                held = read_as(torch.float16)
+                held = read_as(torch.float16, first, starts)
             if held is not None:
                 if read is not None:
                     read.record()
                 k, v, table, factors = held
                 splits = 1 if split == 0 or longest <= split else -(-longest // split)
                 states = prefill.tge_attention_mma_scratch_floats(tokens - first, heads, splits)
-                scratch = k_scale.new_empty(states) if states > 0 else None
+                scratch = q.new_empty(states, dtype=torch.float32) if states > 0 else None
                 rc = _check(prefill.tge_attention_mma_halves(rows[0].data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), factors.data_ptr(),
                                                              table.data_ptr(), table.shape[1], k.shape[0], starts.data_ptr(), rows[1].data_ptr(),
                                                              rows[2].data_ptr(), num_seqs - first, tokens - first, max_q_len, longest,
@@ -1327,22 +1359,19 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                                              _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
                 if rc != UNSUPPORTED:
                     return
-        k, v, table = read_as(q.dtype)
+        k, v, table = read_as(q.dtype, first, starts)
         if read is not None:
             read.record()
         attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
                   window=window, out=rows[4], sink=sink, own_pages=True)
 
-    def simply(first: int, last: int) -> None:
+    def each(first: int, last: int) -> None:
         """The rows [first, last), a warp each."""
-        rows = (q, out, positions, seq_of_token) if first == 0 else (q[first:], out[first:], positions[first:], seq_of_token[first:])
-        _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
-                                             last - first, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
-                                             _ptr(sink), status_word().data_ptr(), _stream()), lib)
+        simply((q, out, positions, seq_of_token) if first == 0 else (q[first:], out[first:], positions[first:], seq_of_token[first:]), last - first)
 
     as_portions = max_q_len > 1 and (mma_attention_supports(head_dim, heads, kv_heads, 64) and USE_MMA_ATTENTION if is_bf16
                                      else head_dim in (16, 32, 64, 128) and sink is None)
-    if as_portions and need >= 0 and MIN_DECODE_PREFIX <= singles < min(num_seqs, tokens) and not torch.cuda.is_current_stream_capturing():
+    if as_portions and takes_singles and MIN_DECODE_PREFIX <= singles < min(num_seqs, tokens) and not torch.cuda.is_current_stream_capturing():
         reach = max(ctx_lens[singles:]) if window == 0 else min(window, max(ctx_lens[singles:]))
         if 4.0 * heads * head_dim * (tokens - singles) * reach >= BESIDE_8BIT_FLOPS:
             # Side by side: the portions' kernel, whose blocks fill an SM each, on a stream of higher priority, the single tokens' blocks behind
@@ -1361,19 +1390,181 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             finally:
                 main.wait_stream(side)       # also when a part raises: what the side stream uses is the main one's again afterwards
             if served < singles:
-                simply(served, singles)                   # (a cache that the single tokens' kernel does not take)
+                each(served, singles)                     # (a cache that the single tokens' kernel does not take)
             return out
-    done = single_tokens() if need >= 0 else 0            # requests, and so tokens, that are served
+    done = single_tokens() if takes_singles else 0        # requests, and so tokens, that are served
     if done < singles and as_portions:
-        simply(done, singles)                             # (the portions behind them go the way that they go alone)
+        each(done, singles)                               # (the portions behind them go the way that they go alone)
         done = singles
     if done == num_seqs or done == tokens:                # (requests that bring nothing may hold nothing)
         return out
     if as_portions:
         portions(done)
     else:
-        simply(done, tokens)
+        each(done, tokens)
     return out
+
+
+# ----------------------------------------------------------------------------
+# a cache held in 4 bits
+# ----------------------------------------------------------------------------
+def _cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torch.Tensor, v_groups: torch.Tensor, block_table: torch.Tensor,
+                num_seqs: int, kv_heads: int, head_dim: int) -> Tuple[int, int]:
+    """(pages, positions in a page) of a cache held in 4 bits."""
+    _want(k_pages, "k pages", torch.uint8)
+    _want(v_pages, "v pages", torch.uint8)
+    _want(k_groups, "k groups", torch.bfloat16)
+    _want(v_groups, "v groups", torch.bfloat16)
+    _want(block_table, "block table", torch.int32)
+    shape, pairs, table, groups = k_pages.shape, k_groups.shape, block_table.shape, -(-head_dim // 32)
+    if len(shape) != 4 or shape[1] != kv_heads or shape[3] != 16 * groups or v_pages.shape != shape:
+        raise KernelError(f"4-bit pages must be [pages, {kv_heads}, page_size, {16 * groups}], got {tuple(shape)} and {tuple(v_pages.shape)}")
+    if tuple(pairs) != (shape[0], kv_heads, shape[2], 2 * groups) or v_groups.shape != pairs:
+        raise KernelError(f"steps and bases must be [{shape[0]}, {kv_heads}, {shape[2]}, {2 * groups}], got {tuple(pairs)} and {tuple(v_groups.shape)}")
+    if len(table) != 2 or table[0] < num_seqs or table[1] == 0:
+        raise KernelError(f"the block table must be [{num_seqs}, pages], got {tuple(table)}")
+    here = _current_device()
+    for t in (k_pages, v_pages, k_groups, v_groups, block_table):
+        if t.get_device() != here:
+            raise KernelError(f"a cache on device {t.get_device()}, while device {here} is the current one")
+    return shape[0], shape[2]
+
+
+def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary: int, positions: torch.Tensor,
+                            seq_of_token: torch.Tensor, num_seqs: int, block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                            k_groups: torch.Tensor, v_groups: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                            q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, pairs: bool = False,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Normalises (if wanted) and rotates q and k and appends k and v to a paged cache of 4-bit codes; returns the queries [T, heads * head_dim].
+
+    qkv: [T, >= (heads + 2*kv_heads) * head_dim], unchanged.  ``q_norm`` / ``k_norm`` (float32 [head_dim]): every head of the queries / keys goes
+    over the root of its mean square plus ``eps`` and times these weights, before the rotation.  cos/sin as for :func:`rope_kv_store`;
+    ``pairs``: numbers 2d and 2d + 1 of a head are turned together instead of d and d + rotary / 2.
+    Pages: uint8 [num_pages, kv_heads, page_size, 16 * groups], groups = ceil(head_dim / 32); steps and bases: bfloat16 [num_pages, kv_heads,
+    page_size, 2 * groups], a (step, base) for each 32 numbers of an entry: a code c of 0..15 stands for base + (c - 8) * step.  The codes of
+    numbers 32 j + 4 g .. 32 j + 4 g + 3 share 16 bits, the first in the lowest four, which are the (g * groups + j)-th of the entry's.  A position's entry
+    does not depend on how its request was cut into steps.  An entry with a number that is not finite, or 2^96 or more, reads as NaN.
+    """
+    _want(qkv, "qkv", _FLOAT, contiguous=False)
+    stride = _rows_2d(qkv, "qkv")
+    tokens = qkv.shape[0]
+    if heads <= 0 or kv_heads <= 0 or qkv.shape[1] < (heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"qkv rows of {qkv.shape[1]} numbers for {heads} + 2 * {kv_heads} heads of {head_dim}")
+    if rotary > 0:
+        _want(cos, "cos table", torch.float32)
+        _want(sin, "sin table", torch.float32)
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rotary // 2:
+            raise KernelError(f"rotary tables must be [positions, {rotary // 2}], got {tuple(cos.shape)}")
+    for name, t in (("q norm weight", q_norm), ("k norm weight", k_norm)):
+        if t is not None:
+            _want(t, name, torch.float32)
+            if t.numel() != head_dim:
+                raise KernelError(f"{name} has {t.numel()} elements for heads of {head_dim}")
+    if (q_norm is not None or k_norm is not None) and not eps >= 0.0:
+        raise KernelError(f"a norm with an eps of {eps}")
+    _per_token(positions, seq_of_token, tokens)
+    num_pages, page_size = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, num_seqs, kv_heads, head_dim)
+    out, out_stride = _rows_like(qkv, heads * head_dim, out, "rotated queries")
+    lib = core()
+    _check(lib.tge_store_4bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), out_stride, _ptr(cos), _ptr(sin),
+                              0 if cos is None else cos.shape[0], rotary, int(pairs), _ptr(q_norm), _ptr(k_norm), float(eps), positions.data_ptr(),
+                              seq_of_token.data_ptr(), num_seqs, block_table.data_ptr(), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(),
+                              k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size, tokens, heads, kv_heads, head_dim,
+                              status_word().data_ptr(), _stream()), lib)
+    return out
+
+
+def read_cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torch.Tensor, v_groups: torch.Tensor, block_table: torch.Tensor,
+                    q_start: torch.Tensor, start_pos: torch.Tensor, ctx_lens, head_dim: int, dtype: torch.dtype, window: int = 0, first_seq: int = 0,
+                    q_lens=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """What the requests of a step hold in a cache of 4-bit codes, as values: (k, v, table), as :func:`read_cache_8bit` returns them.
+
+    ``q_lens`` (host numbers): what every request brings; with a ``window`` k and v then have no more runs than there are (without: as
+    many as there were without one, the last of them zeros)."""
+    if k_pages.dim() != 4:
+        raise KernelError(f"4-bit pages must be [pages, kv_heads, page_size, 16 * groups], got {tuple(k_pages.shape)}")
+    if dtype not in _FLOAT:
+        raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
+    if window < 0 or not 0 <= first_seq <= len(ctx_lens) or (q_lens is not None and len(q_lens) != len(ctx_lens)):
+        raise KernelError(f"a read-back of {len(ctx_lens)} requests from {first_seq} on, a window of {window}, {None if q_lens is None else len(q_lens)} portions")
+    sizes = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, len(ctx_lens), k_pages.shape[1], head_dim)
+    _portions(q_start, start_pos, len(ctx_lens))
+    return _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, None, q_lens)
+
+
+def _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, starts, q_lens=None):
+    """What :func:`read_cache_4bit` does, of arguments that were looked over; ``starts`` and ``dtype`` float16 as for :func:`_read_8bit`."""
+    kv_heads = k_pages.shape[1]
+    num_pages, page_size = sizes
+    mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
+    width = max(mine, default=0)
+    if window and q_lens is not None:
+        mine = [n - min(n, max(int(held) - int(new) - window + 1, 0) // 64) for n, held, new in zip(mine, ctx_lens[first_seq:], q_lens[first_seq:])]
+    runs = sum(mine)
+    k = k_groups.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    table = block_table.new_empty((len(mine), width))
+    factors = block_table.new_empty(runs * kv_heads * (128 + 1)) if dtype == torch.float16 else None
+    lib = core()
+    rc = lib.tge_read_4bit(k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size, block_table.data_ptr(),
+                           block_table.shape[1], q_start.data_ptr(), start_pos.data_ptr(), first_seq, len(ctx_lens), kv_heads, head_dim, int(window),
+                           k.data_ptr(), v.data_ptr(), 2 if factors is not None else int(dtype == torch.bfloat16), _ptr(factors), table.data_ptr(),
+                           _ptr(starts), runs, width, status_word().data_ptr(), _stream())
+    if _check(rc, lib) == UNSUPPORTED:
+        return None
+    return (k, v, table) if factors is None else (k, v, table, factors)
+
+
+def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torch.Tensor, v_groups: torch.Tensor,
+                   block_table: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, positions: torch.Tensor,
+                   seq_of_token: torch.Tensor, num_seqs: int, max_q_len: int, max_ctx_len: int, heads: int, kv_heads: int, head_dim: int,
+                   scale: float, window: int = 0, out: Optional[torch.Tensor] = None, decode_prefix: int = 0,
+                   sink: Optional[torch.Tensor] = None, ctx_lens=None) -> torch.Tensor:
+    """:func:`attention` over a cache of 4-bit codes (see :func:`norm_rope_kv_store_4bit`): [T, heads * head_dim].  Arguments as for :func:`attention_8bit`."""
+    _want(q, "queries", _FLOAT, contiguous=False)
+    q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or q.shape[1] < heads * head_dim:
+        raise KernelError(f"attention: rows of {q.shape[1]} numbers for {heads} heads of {head_dim} over {kv_heads}")
+    num_pages, page_size = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, num_seqs, kv_heads, head_dim)
+    _portions(q_start, start_pos, num_seqs)
+    _per_token(positions, seq_of_token, tokens)
+    if ctx_lens is not None and len(ctx_lens) != num_seqs:
+        raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
+    if not 0 <= decode_prefix <= num_seqs or window < 0:
+        raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
+    if sink is not None:
+        _want(sink, "attention sinks", torch.float32)
+        if sink.numel() != heads:
+            raise KernelError(f"attention: {sink.numel()} sinks for {heads} heads")
+    out, out_stride = _rows_like(q, heads * head_dim, out, "attention output")
+    is_bf16 = int(q.dtype == torch.bfloat16)
+    lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size,
+                          block_table.data_ptr(), block_table.shape[1])
+    singles = num_seqs if max_q_len <= 1 else decode_prefix
+    if singles < num_seqs and ctx_lens is None:
+        ctx_lens = [max_ctx_len] * num_seqs
+    need = -1                                           # scratch numbers of the single tokens' kernel; -1: sizes that it does not take
+    if singles:
+        need = _decode_floats(lib.tge_attention_4bit_decode_floats, is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
+
+    def single_tokens() -> int:
+        parts = q.new_empty(need, dtype=torch.float32) if need else None
+        rc = lib.tge_attention_4bit_decode(q.data_ptr(), is_bf16, q_stride, *cache, q_start.data_ptr(), start_pos.data_ptr(), singles,
+                                           out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
+                                           _ptr(parts), need, status_word().data_ptr(), _stream())
+        return singles if _check(rc, lib) != UNSUPPORTED else 0
+
+    def simply(rows, tokens: int) -> None:
+        _check(lib.tge_attention_4bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
+                                             tokens, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
+                                             _ptr(sink), status_word().data_ptr(), _stream()), lib)
+
+    def read_as(dtype: torch.dtype, first: int, starts: torch.Tensor):
+        return _read_4bit((num_pages, page_size), k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim,
+                          dtype, window, first, starts)
+
+    return _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, seq_of_token, num_seqs, max_q_len, heads, kv_heads, head_dim, scale,
+                         window, sink, ctx_lens, singles, need >= 0, single_tokens, simply, read_as)
 
 
 def to_run_dtype(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
