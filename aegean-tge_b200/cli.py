@@ -7,7 +7,7 @@
     tge bench prefill|decode --model DIR [--prompt-len N] [--batch B] [--n N] [--repeat R]
     tge bench mixed --model DIR [--batch B] [--prompt-len N] [--portion P]      (B single tokens beside a prompt portion)
     tge fidelity --model DIR [--context N] [--tokens N] [--corpus FILE]
-    tge score --model DIR --tokens "a b c" | --corpus FILE | --prompt-len N [--top N] [--cache-dtype int8 [--compare]]
+    tge score --model DIR --tokens "a b c" | --corpus FILE | --prompt-len N [--top N] [--cache-dtype int8|uint4 [--compare]]
     tge bench continuous --model DIR [--requests N] [--tokens N] [--sequences N] [--prompt-tokens N] [--prompt-max N]
     tge make-random --config FILE --out DIR [--seed S] [--dtype float32|bfloat16]
     tge replay --model DIR --dtype D --out DIR --max-tokens N          (same as bin/trace_run)
@@ -60,7 +60,7 @@ def _model_args(parser: argparse.ArgumentParser) -> None:
 
 
 def _cache_args(parser: argparse.ArgumentParser) -> None:
-    parser.add_argument("--cache-dtype", choices=["int8"], help="hold keys and values in 8 bits (default: in --dtype)")
+    parser.add_argument("--cache-dtype", choices=["int8", "uint4"], help="hold keys and values in 8 or 4 bits (default: in --dtype)")
     parser.add_argument("--cache-block", type=int, default=1, help="positions that share a scale of an 8-bit cache (default 1)")
 
 
@@ -186,12 +186,14 @@ def command_plan(args) -> int:
     from .peaks import hbm_gbs
     from .registry import architecture_of
     from .weights.random_init import parse_dtype
+    if args.cache_dtype == "uint4" and args.cache_block != 1:
+        raise UsageError("plan: --cache-block is for --cache-dtype int8")
     raw = read_config_json(args.model)
     arch = architecture_of(raw)
     spec = arch.build_spec(arch.parse_config(raw))
     env = BuildEnv(dtype=parse_dtype(args.dtype), device=torch.device("cpu"), hidden_size=spec.hidden_size,
                    max_positions=min(spec.max_positions, args.context), page_size=PAGE_SIZE, ops=None,
-                   cache_block=None if args.cache_dtype is None else args.cache_block)
+                   cache_block=args.cache_block if args.cache_dtype == "int8" else None, cache_4bit=args.cache_dtype == "uint4")
     model = DecoderModel(spec, env)
     weights = model.weight_bytes()
     decode_bytes = model.step_param_bytes()                 # everything but the embedding rows (plan.cpp:42-46)
@@ -299,7 +301,7 @@ def command_fidelity(args) -> int:
     candidate_cache = args.cache_dtype
     for dtype in ("float32", "bfloat16"):
         args.dtype = dtype
-        args.cache_dtype = candidate_cache if dtype == "bfloat16" else None      # the oracle's cache is never of 8 bits
+        args.cache_dtype = candidate_cache if dtype == "bfloat16" else None      # the oracle's cache is never of codes
         args.max_requests = 1
         t0 = time.time()
         engine = _engine_from(args)
@@ -346,7 +348,7 @@ def command_fidelity(args) -> int:
 
 def command_score(args) -> int:
     """What the model thinks of given tokens: one line per token (id, log probability, entropy, rank, best alternatives) and the mean.  With
-    ``--cache-dtype int8 --compare`` also how far that cache moves the answers from those with the cache in the run's dtype."""
+    ``--cache-dtype int8|uint4 --compare`` also how far that cache moves the answers from those with the cache in the run's dtype."""
     import gc
     import math
     import random
@@ -354,7 +356,7 @@ def command_score(args) -> int:
     if sum(option is not None for option in (args.tokens, args.corpus, args.prompt_len)) != 1:
         raise UsageError("score: give one of --tokens, --corpus and --prompt-len")
     if args.compare and not args.cache_dtype:
-        raise UsageError("score: --compare is for --cache-dtype int8")
+        raise UsageError("score: --compare is for --cache-dtype int8 or uint4")
     if not 0 <= args.top <= 32:
         raise UsageError("score: --top is at most 32")
     args.max_requests = 1

@@ -3,7 +3,7 @@
     engine = Engine("path/to/model", dtype="bfloat16")
     ids = engine.generate([5, 17, 3], n=32)                      # greedy
     ids = engine.generate([[1, 2], [3]], n=8, sampling=SamplingParams(temperature=0.8, seed=7))
-    engine = Engine("path/to/model", cache_dtype="int8")          # keys and values in 8 bits
+    engine = Engine("path/to/model", cache_dtype="int8")          # keys and values in 8 bits; "uint4": in 4
     scores = engine.score([5, 17, 3, 9], top=5)                   # log probabilities of 17, 3, 9, with the five best beside each
 
 Options carry the reference's names and meanings where it has them
@@ -75,7 +75,8 @@ class Engine:
         single-token steps (both on; off for A/B comparisons).
         ``cache_dtype``: None keeps keys and values in ``dtype``; "int8" as 8-bit codes with a float32 scale per head and ``cache_block``
         positions (a power of two that divides the page).  With blocks of one, the default, what a position's entry is does not
-        depend on the steps that brought it; larger blocks save up to 4 bytes a position and head.
+        depend on the steps that brought it; larger blocks save up to 4 bytes a position and head.  "uint4": as 4-bit codes with a step and a
+        base, bfloat16 both, for each 32 numbers of an entry: 5 bits a number, and an entry never depends on the steps.
         """
         if not torch.cuda.is_available():
             raise RuntimeError("this engine runs on a CUDA device only; none is available")
@@ -83,8 +84,10 @@ class Engine:
             raise ValueError("give either model_dir or random_config")
         if page_size <= 0 or 64 % page_size != 0:
             raise ValueError(f"page_size {page_size} must divide 64, the attention kernels' tile of key positions")
-        if cache_dtype not in (None, "int8"):
-            raise ValueError(f"cache_dtype {cache_dtype!r} is neither None (the run's dtype) nor 'int8'")
+        if cache_dtype not in (None, "int8", "uint4"):
+            raise ValueError(f"cache_dtype {cache_dtype!r} is neither None (the run's dtype) nor 'int8' or 'uint4'")
+        if cache_dtype == "uint4" and cache_block != 1:
+            raise ValueError(f"cache_block {cache_block}: blocks of positions are for a cache of int8")
         if cache_dtype is not None and (cache_block <= 0 or cache_block & (cache_block - 1) or page_size % cache_block):
             raise ValueError(f"cache_block {cache_block} must be a power of two that divides the page of {page_size}")
         self.cache_dtype = cache_dtype
@@ -103,7 +106,7 @@ class Engine:
         started = time.time()
         env = BuildEnv(dtype=self.dtype, device=self.device, hidden_size=self.spec.hidden_size,
                        max_positions=self.max_model_len, page_size=page_size, ops=_ops,
-                       cache_block=None if cache_dtype is None else int(cache_block))
+                       cache_block=int(cache_block) if cache_dtype == "int8" else None, cache_4bit=cache_dtype == "uint4")
         _ops.core()     # builds and loads the kernels now, or fails loudly
         self.model = DecoderModel(self.spec, env)
         if model_dir is not None:

@@ -53,6 +53,13 @@ class DecoderModel:
                 if (block.mixer.cache_spec() is not None or block.mixer.extra_cache_specs()) and not block.mixer.holds_8bit:
                     raise ValueError(f"layers[{index}]: {spec.layers[index].mixer.kind} as this model has it keeps its cache in the run "
                                      f"dtype; one of 8 bits is for rotated keys and values without norms, biases or gates")
+        if env.cache_4bit:
+            if env.cache_block is not None:
+                raise ValueError("a cache is held in 8 bits or in 4")
+            for index, block in enumerate(self.blocks):
+                if (block.mixer.cache_spec() is not None or block.mixer.extra_cache_specs()) and not block.mixer.holds_4bit:
+                    raise ValueError(f"layers[{index}]: {spec.layers[index].mixer.kind} as this model has it keeps its cache in the run "
+                                     f"dtype; one of 4 bits is for rotated keys and values, with norms of each head or none, without biases or gates")
         self.layer_caches: List[LayerCache] = [LayerCache() for _ in spec.layers]
         # single-token steps may be replayed from a CUDA graph only if every part says so
         self.graph_safe = all(part.graph_safe for _where, part, _spec in self.named_parts())

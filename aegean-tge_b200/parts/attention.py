@@ -51,6 +51,8 @@ product; one kernel normalises and stores, and the attention adds the bias and a
 
 The plain layer (rotation, values of the keys' size, window, sinks) can hold its cache in 8 bits (``BuildEnv.cache_block``): codes of
 keys and values, and a scale per block of positions and head.  Product, one kernel that rotates, quantises and stores, attention over codes.
+It and the layer with a q/k norm per head (rotated by halves or by neighbouring pairs) can hold it in 4 bits (``BuildEnv.cache_4bit``) in the same
+way, the norm in the kernel that stores: codes, and a step and a base per 32 numbers.
 
 On the general path, too: the norm of q and k after their rotation, with or without weights (``qk_norm`` with
 ``"after_rotation": True``); a sink whose score is a constant and not learned (``sink_score``); and one gate per number of
@@ -203,6 +205,11 @@ class GQAttention(Mixer):
         # a cache of 8-bit codes: the plain layer, with a rotation that the kernels know
         self.cache_block = env.cache_block
         self.holds_8bit = self.plain and not self.general and not self.separate and tables is not None and self.head_dim <= 256
+        # one of 4-bit codes: with norms per head as well, and rotations of neighbouring pairs
+        self.cache_4bit = env.cache_4bit
+        self.holds_4bit = (not (self.general or self.separate or self.values_are_keys) and self.value_mix is None and self.value_dim == self.head_dim
+                           and (self.qk_norm is None or self.qk_norm[0] == "head") and self.head_dim <= 256
+                           and (tables is not None or hasattr(self.position, "pair_tables")))
         self.conv_w: Optional[torch.Tensor] = None
         self.q_norm_w: Optional[torch.Tensor] = None
         self.k_norm_w: Optional[torch.Tensor] = None
@@ -381,6 +388,11 @@ class GQAttention(Mixer):
                                            ("k_scale", (self.kv_heads, 1)), ("v_scale", (self.kv_heads, 1))), window=window,
                                   formats=(("k", torch.int8, 1), ("v", torch.int8, 1), ("k_scale", torch.float32, block),
                                            ("v_scale", torch.float32, block)))
+        if self.cache_4bit and self.holds_4bit:
+            groups = -(-self.head_dim // 32)
+            codes, pairs = (self.kv_heads, 16 * groups), (self.kv_heads, 2 * groups)
+            return PagedCacheSpec(entries=(("k", codes), ("v", codes), ("k_groups", pairs), ("v_groups", pairs)), window=window,
+                                  formats=(("k", torch.uint8, 1), ("v", torch.uint8, 1), ("k_groups", torch.bfloat16, 1), ("v_groups", torch.bfloat16, 1)))
         return PagedCacheSpec(entries=(("k", (self.kv_heads, self.head_dim)), ("v", (self.kv_heads, self.value_dim))),
                               window=window, keep_first=self.keep_first)
 
@@ -443,6 +455,35 @@ class GQAttention(Mixer):
                                   ctx.max_ctx_len, self.heads, self.kv_heads, self.head_dim, self.scale, window=int(self.window or 0), out=out,
                                   decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"))
 
+    def attend_4bit(self, h, ctx: StepContext, cache: LayerCache, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Product with its biases; norm, rotation, codes, steps and bases of k and v stored; attention over the codes."""
+        ops = self.ops
+        held = (cache.paged["k"], cache.paged["v"], cache.paged["k_groups"], cache.paged["v_groups"])
+        table = ctx.block_tables[cache.group]
+        tables = self.position.rotary_tables()
+        pairs = tables is None
+        cos, sin, rotary = self.position.pair_tables() if pairs else tables
+        eps = self.qk_norm[1] if self.qk_norm is not None else 1.0
+        qkv = ops.linear(h, self.w_qkv, self.b_qkv, ops.GEMM_STORE, settled=True)
+        if cache.owner:
+            q = ops.norm_rope_kv_store_4bit(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, ctx.num_seqs, table, *held, self.heads, self.kv_heads,
+                                            self.head_dim, q_norm=self.q_norm_w, k_norm=self.k_norm_w, eps=eps, pairs=pairs)
+        else:
+            if self.qk_norm is not None:
+                ops.qk_norm_kv_store(qkv, self.q_norm_w, self.k_norm_w, eps, True, ctx.positions, ctx.seq_of_token, None, None, None, self.heads,
+                                     self.kv_heads, self.head_dim, self.value_dim)
+            q = qkv[:, :self.q_dim]
+            if pairs:
+                heads = q.view(-1, self.heads, self.head_dim)
+                self.position.apply(heads, qkv[:, self.q_dim:self.q_dim + self.kv_dim].view(-1, self.kv_heads, self.head_dim), ctx.positions)
+            else:
+                ops.rope_kv_store(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, table, None, None, self.heads, self.kv_heads, self.head_dim)
+        if ctx.max_q_len > 1 and "ctx_lens" not in ctx.scratch:
+            ctx.scratch["ctx_lens"] = [start + count for start, count in zip(ctx.host_start_pos, ctx.host_q_lens)]
+        return ops.attention_4bit(q, *held, table, ctx.q_start, ctx.start_pos, ctx.positions, ctx.seq_of_token, ctx.num_seqs, ctx.max_q_len,
+                                  ctx.max_ctx_len, self.heads, self.kv_heads, self.head_dim, self.scale, window=int(self.window or 0), out=out,
+                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"))
+
     def share_input_projection(self, rows: torch.Tensor) -> Optional[torch.Tensor]:
         """A block offers the rows of another product over the same input (a feed-forward's up weight) to be
         multiplied together with q, k and v.  A mixer whose small-batch kernel can carry them (whole-projection
@@ -468,8 +509,8 @@ class GQAttention(Mixer):
             attend = self.attend_keyed if self.values_are_keys else self.attend_separate if self.separate else self.attend_general
             a = attend(h, ctx, cache, out=out)
             return a if beside is None else (a, False)
-        if self.cache_block is not None:
-            a = self.attend_8bit(h, ctx, cache, out=out)
+        if self.cache_block is not None or self.cache_4bit:
+            a = (self.attend_4bit if self.cache_4bit else self.attend_8bit)(h, ctx, cache, out=out)
             return a if beside is None else (a, False)
         ops = self.ops
         k_pages, v_pages = cache.paged["k"], cache.paged["v"]

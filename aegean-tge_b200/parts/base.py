@@ -119,6 +119,7 @@ class BuildEnv:
     page_size: int
     ops: Any                           # the kernel bindings (aegean_tge_b200.ops)
     cache_block: Optional[int] = None  # keys and values held in 8 bits, a scale per so many positions and head (None: in the run dtype)
+    cache_4bit: bool = False           # keys and values held in 4 bits, a step and a base per 32 numbers of an entry
 
 
 @dataclass
@@ -252,6 +253,8 @@ class Mixer(Part):
     """Mixes information between the tokens of a request."""
     # A mixer with a paged cache that can hold it in 8 bits (``BuildEnv.cache_block``) says so; a model with one that cannot refuses.
     holds_8bit = False
+    # The same of one held in 4 bits (``BuildEnv.cache_4bit``).
+    holds_4bit = False
 
     def cache_spec(self) -> Optional[PagedCacheSpec]:
         return None
