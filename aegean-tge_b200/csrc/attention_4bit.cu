@@ -95,20 +95,26 @@ __global__ void __launch_bounds__(128) attention_4bit_simple_kernel(const Attn4 
 // ---------------------------------------------------------------------------
 // Single tokens on the tensor cores: head sizes 64, 128 and 256, pages of 16, 32, 64, ... positions.
 //
-// What bounds it: the cache's bytes, 5/4 head_dim of them a position and kv head for key and value, and close behind them the conversions of the codes.
-// A warp takes slices of 16 positions, nothing of them passes through shared memory.  Everything is bfloat16 into float32: codes and steps and bases
-// are exact in it, and its range is float32's, so nothing has to be held over powers of two.
-//   scores   S^T [16 positions x 8 heads] = sum_j step_j (C_j [16 x 32] Q_j^T [32 x 8]) (m16n8k16, two to a group): a lane needs, of positions g and
-//            g + 8 (g = lane / 4), its quarter (t = lane % 4) of every group, which is how they lie.  A code becomes a bfloat16 by its four bits
-//            below the exponent of 128; the 136 that it is too large, and the bases, are one more product,
-//            [step_j, base_j] [16 x 2 groups] times [-136 sum q, sum q], the sums of a group's queries in three parts of eight bits.
-//   values   O_j^T [32 x 8 heads] += (C'_j - 8)^T [32 x 16 positions] (P step_j)^T [16 x 8], and for the bases one more product,
+// What bounds it: turning codes into operands, some 430 instructions a slice of 16 positions and warp (DRAM would take 39 of the 75 us below).
+// A warp takes slices of 16 positions, nothing of them passes through shared memory.
+//   scores   S^T [16 positions x 8 heads] = sum_j step_j (C_j [16 x 32] Q_j^T [32 x 8]) (m16n8k16 of float16, two to a group): a lane needs, of positions
+//            g and g + 8 (g = lane / 4), its quarter (t = lane % 4) of every group, which is how they lie.  Four bits under a mask are a float16 already,
+//            one of its smallest numbers, c 2^-24 or c 2^-20, which the tensor core multiplies exactly.  What they are too large by, and the bases, are one
+//            more product (bfloat16, as they are held): [step_j, base_j] [16 x 2 groups] times [-8 sum q, sum q], the sums of a group's queries in three parts of eight bits.
+//   values   O_j^T [32 x 8 heads] += (C'_j - 8)^T [32 x 16 positions] (P step_j)^T [16 x 8] in bfloat16, and for the bases one more product,
 //            B^T [2 groups x 16 positions] P^T: a lane needs, of positions 2t, 2t + 1, 2t + 8, 2t + 9, four neighbours of every group (g).
-//            Here 136 is taken off the codes: a sum over a long context must not be the difference of two large ones.
+//            bfloat16 has float32's range, so that no value's size, however far from the others', has to be held over a power of two; a code becomes one
+//            by its bits below the exponent of 128, and 136 is taken off: a sum over a long context must not be the difference of two large ones.
 // Queries are over a power of two above their row's largest number, so that a product with the largest step stays finite.  p is at most 2^8 and is
 // rounded with its step to bfloat16, as a bfloat16 cache's probabilities are; float32 runs take queries and probabilities in three such parts.
 // Probabilities turn from S^T's accumulators into P^T's operand by two 8x8 transposes a group.  The running maximum is raised only when a score
 // passes it by 2^8; the sums of probabilities stay in their lanes until the end.
+//
+// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (258 MB with their pairs) 75.1 us; four of 32,768 to 65,536 69.2; eight of
+// 2,048 at 28 heads over 4 (a cluster each unit) 10.3, one 7.8.  Keys in bfloat16, their codes raised by 128 and the sums lowered after: 76.8.  Not
+// taken: entries through rings in shared memory, bulk copies asked for by each warp or by each block, 77 and 79 (fewer waits, more instructions); pages
+// asked into L2 ahead 90; one slice at a time with four blocks on an SM 79, three 90; values with 136 taken off by a product with a constant 82.
+// Without any conversion or scaling at all it would take 56, without products too 50.
 //
 // Work: see decode_units.cuh; few units over short contexts go to a cluster each (decode_cluster).
 // ---------------------------------------------------------------------------
@@ -127,22 +133,31 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t two_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Codes n of the units in both halves of x, as 128 + c.
-__device__ __forceinline__ uint32_t raised_codes(uint32_t x, int n) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;\n" : "=r"(r) : "r"(x >> (4 * n)));      // (x & mask) | pattern
-  return r;
-}
-// As c - 8.
+// Codes n of the units in both halves of x as c - 8 in bfloat16: 128 + c, less 136.
 __device__ __forceinline__ uint32_t centred_codes(uint32_t x, int n) {
   uint32_t r;
-  asm("add.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(raised_codes(x, n)), "r"(0xc308c308u));   // - 136
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;\n" : "=r"(r) : "r"(x >> (4 * n)));      // (x & mask) | pattern
+  asm("add.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(r), "r"(0xc308c308u));
   return r;
+}
+// Codes n and n + 1 (n even) in float16, as they lie: c 2^-24 and c 2^-20.
+__device__ __forceinline__ void tiny_codes(uint32_t x, int n, uint32_t& even, uint32_t& odd) {
+  even = (x >> (4 * n)) & 0x000f000fu;
+  odd = (x >> (4 * n)) & 0x00f000f0u;
 }
 // Halves `which` (0: lower) of two words, the first one's below.
 __device__ __forceinline__ uint32_t halves_of(uint32_t a, uint32_t b, int which) { return __byte_perm(a, b, which ? 0x7632 : 0x5410); }
@@ -202,15 +217,16 @@ __device__ __forceinline__ uint32_t word_of(const uint32_t (&w)[G], int t, int f
   }
 }
 
-// A tile's queries as operands: numbers (2b, 4 + 2b) and (2b + 1, 5 + 2b) of the lane's eight of group j, and sums of groups t and t + 4 in three parts.
+// A tile's queries as operands: numbers (2b, 4 + 2b) and (2b + 1, 5 + 2b) of the lane's eight of group j (bfloat16 runs: in float16, times 2^15 and 2^11, so
+// that their products with codes are all over 2^9; else in PARTS parts), and what multiplies the pairs of groups t and t + 4, in three parts.
 template <int HD, int PARTS>
 struct Queries {
   static constexpr int G = HD / 32, SUMS = G > 4 ? 2 : 1;
+  static constexpr float OVER = PARTS == 1 ? 0x1p-9f : 1.0f;               // what scores come out times
   uint32_t x[G][2][2][PARTS], sums[SUMS][3];
 
-  // `head`: the head's row, of which the lane takes numbers 32 j + 8 t ..; returns what scores are to be multiplied with (NaN if a number is not finite).
-  // CENTRED: what the codes are too large by has been taken off them.
-  template <typename T, bool CENTRED>
+  // `head`: the head's row, of which the lane takes numbers 32 j + 8 t ..; returns the power of two that they are over (NaN if a number is not finite).
+  template <typename T>
   __device__ __forceinline__ float take(const T* head, bool valid, bool whole, int t) {
     float v[G][8], most = 0.0f;
     bool fine = true;
@@ -254,14 +270,19 @@ struct Queries {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) in_parts<PARTS>(v[j][2 * b + n], v[j][4 + 2 * b + n], x[j][b][n]);
+        for (int n = 0; n < 2; ++n) {
+          const float lo = v[j][2 * b + n], hi = v[j][4 + 2 * b + n], by = n ? 0x1p11f : 0x1p15f;
+          if constexpr (PARTS == 1) x[j][b][n][0] = two_f16(lo * by, hi * by);
+          else in_parts<PARTS>(lo, hi, x[j][b][n]);
+        }
     }
 #pragma unroll
     for (int half = 0; half < SUMS; ++half) {
       float mine = 0.0f;
 #pragma unroll
       for (int j = 4 * half; j < (G < 4 * half + 4 ? G : 4 * half + 4); ++j) mine = t == (j & 3) ? sum[j] : mine;
-      in_parts<3>(CENTRED ? 0.0f : -136.0f * mine, mine, sums[half]);
+      mine *= OVER;
+      in_parts<3>(PARTS == 1 ? -8.0f * mine : 0.0f, mine, sums[half]);               // (codes of bfloat16 runs are 8 too large)
     }
     const unsigned rest = __ballot_sync(0xffffffffu, !fine) >> (threadIdx.x & 28);
     return (rest & 15u) == 0u ? __uint_as_float((uint32_t)(127 + up) << 23) : __int_as_float(0x7fc00000);
@@ -280,7 +301,6 @@ __host__ __device__ constexpr int decode_blocks_per_sm(int head_dim, int tiles, 
 template <typename T, int HD, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, sizeof(T) == 2 ? 1 : 3)) decode_4bit_kernel(const Decode4 p) {
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 3, HEADS = 8 * NT, MTILES = HD / 16, G = HD / 32, AHEAD = decode_ahead(HD, NT, PARTS);
-  constexpr bool CENTRED = PARTS > 1;
   extern __shared__ float merge_o[];                              // see leave_part
   __shared__ Meeting<HD, NT> meet;
   __shared__ int start_of[5];
@@ -372,7 +392,7 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, size
     for (int nt = 0; nt < NT; ++nt) {
       const bool valid = token >= 0 && 8 * nt + g < heads_here;
       const T* src = static_cast<const T*>(p.q) + (size_t)max(token, 0) * p.q_stride + (size_t)(head0 + (valid ? 8 * nt + g : 0)) * HD;
-      const float unit_of = q[nt].template take<T, CENTRED>(src, valid, p.q_whole != 0, t) * (p.scale * LOG2E);
+      const float unit_of = q[nt].template take<T>(src, valid, p.q_whole != 0, t) * (p.scale * (LOG2E / Queries<HD, PARTS>::OVER));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         factor[nt][e] = __shfl_sync(0xffffffffu, unit_of, 4 * (2 * t + e));
@@ -419,12 +439,19 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, size
             for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            auto codes = [&](uint32_t w, int n) { return CENTRED ? centred_codes(w, n) : raised_codes(w, n); };
-            const uint32_t a0 = codes(x0, 2 * b), a1 = codes(x1, 2 * b), a2 = codes(x0, 2 * b + 1), a3 = codes(x1, 2 * b + 1);
+            uint32_t a0, a1, a2, a3;
+            if constexpr (PARTS == 1) {
+              tiny_codes(x0, 2 * b, a0, a2);
+              tiny_codes(x1, 2 * b, a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+              for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt], a0, a1, a2, a3, q[nt].x[j][b][0][0], q[nt].x[j][b][1][0]);
+            } else {
+              a0 = centred_codes(x0, 2 * b); a1 = centred_codes(x1, 2 * b); a2 = centred_codes(x0, 2 * b + 1); a3 = centred_codes(x1, 2 * b + 1);
 #pragma unroll
-              for (int part = 0; part < PARTS; ++part) mma_bf16(acc[nt], a0, a1, a2, a3, q[nt].x[j][b][0][part], q[nt].x[j][b][1][part]);
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) mma_bf16(acc[nt], a0, a1, a2, a3, q[nt].x[j][b][0][part], q[nt].x[j][b][1][part]);
+            }
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)

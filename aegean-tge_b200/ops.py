@@ -1411,22 +1411,23 @@ def _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, s
 def _cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torch.Tensor, v_groups: torch.Tensor, block_table: torch.Tensor,
                 num_seqs: int, kv_heads: int, head_dim: int) -> Tuple[int, int]:
     """(pages, positions in a page) of a cache held in 4 bits."""
-    _want(k_pages, "k pages", torch.uint8)
-    _want(v_pages, "v pages", torch.uint8)
-    _want(k_groups, "k groups", torch.bfloat16)
-    _want(v_groups, "v groups", torch.bfloat16)
-    _want(block_table, "block table", torch.int32)
-    shape, pairs, table, groups = k_pages.shape, k_groups.shape, block_table.shape, -(-head_dim // 32)
+    here, groups = k_pages.get_device(), (head_dim + 31) // 32
+    shape, pairs, table = k_pages.shape, k_groups.shape, block_table.shape
+    # (one look at all of it where nothing is wrong: asked one by one it is a microsecond longer, in a call that the host's time decides)
+    if not (k_pages.dtype is v_pages.dtype is torch.uint8 and k_groups.dtype is v_groups.dtype is torch.bfloat16 and block_table.dtype is torch.int32
+            and v_pages.get_device() == k_groups.get_device() == v_groups.get_device() == block_table.get_device() == here and k_pages.is_cuda and here == _current_device()
+            and k_pages.is_contiguous() and v_pages.is_contiguous() and k_groups.is_contiguous() and v_groups.is_contiguous() and block_table.is_contiguous()):
+        for name, t, dtype in (("k pages", k_pages, torch.uint8), ("v pages", v_pages, torch.uint8), ("k groups", k_groups, torch.bfloat16),
+                               ("v groups", v_groups, torch.bfloat16), ("block table", block_table, torch.int32)):
+            _want(t, name, dtype)
+            if t.get_device() != _current_device():
+                raise KernelError(f"{name} on device {t.get_device()}, while device {_current_device()} is the current one")
     if len(shape) != 4 or shape[1] != kv_heads or shape[3] != 16 * groups or v_pages.shape != shape:
         raise KernelError(f"4-bit pages must be [pages, {kv_heads}, page_size, {16 * groups}], got {tuple(shape)} and {tuple(v_pages.shape)}")
-    if tuple(pairs) != (shape[0], kv_heads, shape[2], 2 * groups) or v_groups.shape != pairs:
+    if len(pairs) != 4 or pairs[:3] != shape[:3] or pairs[3] != 2 * groups or v_groups.shape != pairs:
         raise KernelError(f"steps and bases must be [{shape[0]}, {kv_heads}, {shape[2]}, {2 * groups}], got {tuple(pairs)} and {tuple(v_groups.shape)}")
     if len(table) != 2 or table[0] < num_seqs or table[1] == 0:
         raise KernelError(f"the block table must be [{num_seqs}, pages], got {tuple(table)}")
-    here = _current_device()
-    for t in (k_pages, v_pages, k_groups, v_groups, block_table):
-        if t.get_device() != here:
-            raise KernelError(f"a cache on device {t.get_device()}, while device {here} is the current one")
     return shape[0], shape[2]
 
 
@@ -1496,14 +1497,15 @@ def _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start
     """What :func:`read_cache_4bit` does, of arguments that were looked over; ``starts`` and ``dtype`` float16 as for :func:`_read_8bit`."""
     kv_heads = k_pages.shape[1]
     num_pages, page_size = sizes
-    mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
-    width = max(mine, default=0)
+    told = ctx_lens[first_seq:] if first_seq else ctx_lens
+    width = (max(told, default=0) + 63) // 64
+    runs = sum([(n + 63) // 64 for n in told])
     if window and q_lens is not None:
-        mine = [n - min(n, max(int(held) - int(new) - window + 1, 0) // 64) for n, held, new in zip(mine, ctx_lens[first_seq:], q_lens[first_seq:])]
-    runs = sum(mine)
+        behind = window - 1                    # (positions that a query sees in front of itself)
+        runs -= sum([(n - new - behind) // 64 for n, new in zip(told, q_lens[first_seq:] if first_seq else q_lens) if n - new > behind])
     k = k_groups.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    table = block_table.new_empty((len(mine), width))
+    table = block_table.new_empty((len(told), width))
     factors = block_table.new_empty(runs * kv_heads * (128 + 1)) if dtype == torch.float16 else None
     lib = core()
     rc = lib.tge_read_4bit(k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size, block_table.data_ptr(),
@@ -1537,15 +1539,13 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         if sink.numel() != heads:
             raise KernelError(f"attention: {sink.numel()} sinks for {heads} heads")
     out, out_stride = _rows_like(q, heads * head_dim, out, "attention output")
-    is_bf16 = int(q.dtype == torch.bfloat16)
+    is_bf16 = int(q.dtype is torch.bfloat16)
     lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size,
                           block_table.data_ptr(), block_table.shape[1])
     singles = num_seqs if max_q_len <= 1 else decode_prefix
-    if singles < num_seqs and ctx_lens is None:
-        ctx_lens = [max_ctx_len] * num_seqs
     need = -1                                           # scratch numbers of the single tokens' kernel; -1: sizes that it does not take
     if singles:
-        need = _decode_floats(lib.tge_attention_4bit_decode_floats, is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
+        need = _decode_floats(lib.tge_attention_4bit_decode_floats, is_bf16, singles, heads, kv_heads, head_dim, page_size, cache[7])
 
     def single_tokens() -> int:
         parts = q.new_empty(need, dtype=torch.float32) if need else None
@@ -1553,6 +1553,11 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                            out.data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window), _ptr(sink),
                                            _ptr(parts), need, status_word().data_ptr(), _stream())
         return singles if _check(rc, lib) != UNSUPPORTED else 0
+
+    if need >= 0 and singles == num_seqs and single_tokens() == num_seqs:      # (a decode step: nothing else to set up)
+        return out
+    if singles < num_seqs and ctx_lens is None:
+        ctx_lens = [max_ctx_len] * num_seqs
 
     def simply(rows, tokens: int) -> None:
         _check(lib.tge_attention_4bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
