@@ -629,10 +629,14 @@ int decode_blocks(int head_dim, int tile_heads, int is_bf16) { return tge_sm_cou
 static int decode_tile(int group, int head_dim) { return group <= 8 || head_dim > 128 ? 8 : 16; }
 
 // Blocks of a cluster per unit, which joins its parts itself; 0: runs of slices and a second kernel.  A rule on what the host knows, the units and the
-// bound of their lengths.
+// bound of their lengths, while all clusters are on the device at a time.  us at 28 heads over 4 (four units a request) with 4 / 8 / 16 / none: 1 request of 512
+// 5.9 / 6.3 / 6.9 / 6.8, 16 of them 7.9 / 14.3 / 27.6 / 9.5; 1 of 2,048 10.0 / 7.8 / 7.2 / 7.7, 8 of them 13.0 / 10.3 / 16.6 / 11.0; 4 of 4,096 17.1 /
+// 12.2 / 11.0 / 11.2, 8 of them 21.0 / 14.9 / 21.3 / 13.9; 1 of 8,192 26 / 16 / 11.5 / 12.0, of 16,384 53 / 30 / 18.6 / 15.8.
 static int decode_cluster(long long units, int head_dim, int tile, int is_bf16, long long positions) {
-  if (units <= 16 && positions > 2048 && positions <= 8192) return 16;
-  return 8 * units <= decode_blocks(head_dim, tile, is_bf16) && positions <= 4096 ? 8 : 0;
+  const int blocks = decode_blocks(head_dim, tile, is_bf16);
+  if (positions <= 512 && 4 * units <= blocks) return 4;
+  if (positions > 1024 && positions <= 8192 && units <= 16) return 16;
+  return positions <= 2048 && 8 * units <= blocks ? 8 : 0;
 }
 
 // float32 scratch numbers of tge_attention_4bit_decode; -1: sizes that it does not take.

@@ -43,6 +43,31 @@ __device__ __forceinline__ uint32_t code_of(const Group& g, float x) {
   if (!(g.step > 0.0f)) return 8u;
   return (uint32_t)min(max(__float2int_rn(__fdiv_rn(__fsub_rn(x, g.base), g.step)) + 8, 0), 15);
 }
+// The same where a group's numbers go through one after the other.  The quotient is rounded as the division rounds it: q = fl(y r), r the step's rounded
+// reciprocal, and then fl(q + fl(y - q step) r), which is the nearest number of y / step (P. Markstein, Computation of elementary functions on
+// the IBM RISC System/6000 processor, 1990) while nothing underflows; smaller steps are divided by.  With 1.5 2^23 + 8 added the sum's last four
+// bits are the code (ties to even: 8 is), which lies within 0..15 without a clamp: the step has been rounded up.
+struct Coder4 {
+  float base, step, over;
+  bool by_parts;
+  __device__ __forceinline__ explicit Coder4(const Group& g) {
+    base = g.base;
+    step = g.step;
+    over = __frcp_rn(g.step);
+    by_parts = g.step > 1e-25f;
+  }
+  __device__ __forceinline__ uint32_t four(float a, float b, float c, float d) const {
+    if (!by_parts) {
+      const Group g{step, base};
+      return code_of(g, a) | code_of(g, b) << 4 | code_of(g, c) << 8 | code_of(g, d) << 12;
+    }
+    auto sum = [&](float x) {
+      const float y = __fsub_rn(x, base), q = __fmul_rn(y, over);
+      return __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, step, y), over, q), 12582920.0f));
+    };
+    return (sum(a) & 15u) | (sum(b) & 15u) << 4 | (sum(c) & 15u) << 8 | (sum(d) & 15u) << 12;
+  }
+};
 __device__ __forceinline__ uint32_t packed(const Group& g) { return (__float_as_uint(g.step) >> 16) | (__float_as_uint(g.base) & 0xffff0000u); }
 __device__ __forceinline__ Group unpacked(uint32_t w) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
 __device__ __forceinline__ float value_of(const Group& g, uint32_t code) { return fmaf((float)((int)code - 8), g.step, g.base); }
@@ -69,6 +94,13 @@ __device__ __forceinline__ float over_root(double sum, int count, double eps) { 
 __device__ __forceinline__ double lanes_sum(double v, int lanes) {
   for (int offset = lanes / 2; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
   return v;
+}
+
+// A positive normal float32 as a double by its bits: the conversion does 16 numbers a clock and SM, this and the sum some 60 (a store of 8,192 tokens at 40 heads
+// over 8 with norms 99 us with the one, 87 with the other, before the codes' quotients were found by parts).  0 becomes 2^-127, which no sum with an eps shows.
+__device__ __forceinline__ double widened(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  return __hiloint2double((int)((bits >> 3) + 0x38000000u), (int)(bits << 29));
 }
 
 // Any head size up to 256, any strides: one warp per (token, head), a lane per number of a group.
@@ -148,14 +180,17 @@ __global__ void __launch_bounds__(WARPS * 32) store_4bit_kernel(const StoreParam
 }
 
 // ---------------------------------------------------------------------------
-// The same by units of eight numbers, for head sizes 32, 64, 128 and 256 that are rotated whole or not at all and rows on 16 bytes.  Bound by the rows'
-// bytes; for a token or few, by the trips to memory one behind the other.  A block has a token; HEAD / 16 lanes have a head's row, eight numbers of
-// its first half and eight of its second, and take the token's heads in turn, three rows on their way at a time, the angles loaded once.
+// The same by units of eight numbers, for head sizes 32, 64, 128 and 256 that are rotated whole or not at all and rows on 16 bytes.  A block has a token; HEAD / 16
+// lanes have a head's row, eight numbers of its first half and eight of its second, and take the token's heads in turn, three rows on their way at
+// a time, the angles loaded once.  Bound by the trips to memory one behind the other where there are few tokens, by instructions where there are many (a key's row
+// some 260 a warp and four rows, a query's 90, a norm 170 more).  us: one token 2.5; 2,048 at 28 heads over 4 9.8, with norms 14.9 (34 MB, 5.5 at a
+// copy's rate); 8,192 at 40 over 8 51 and 78 (33).  With a division for every code 3.4, 11.8, 18, 62 and 99; two rows or four blocks to an SM 12 and 11
+// where this takes 9.7; rows asked into L2 ahead no faster.
 // ---------------------------------------------------------------------------
 constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns
 
 template <typename T, int HEAD, bool NORM>
-__global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 && !NORM ? 3 : 2) store_4bit_units_kernel(const StoreParams4 p) {
+__global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_4bit_units_kernel(const StoreParams4 p) {
   constexpr int LANES = HEAD / 16, HALF = HEAD / 2, GROUPS = HEAD / GROUP;
   pdl_trigger();
   const int rows_at_once = blockDim.x / LANES, mine = threadIdx.x / LANES, j = threadIdx.x % LANES;
@@ -207,17 +242,38 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 && !NORM ? 3 : 2)
       Eight lo = eight(lo_raw[i]), hi = eight(hi_raw[i]);
       const bool valid = h < heads, to_cache = h >= p.heads, turns = h < p.heads + p.kv_heads;
       if constexpr (NORM) {
-        double sum = 0.0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum += (double)lo.x[k] * (double)lo.x[k] + (double)hi.x[k] * (double)hi.x[k];
-        const float over = over_root(lanes_sum(sum, LANES), HEAD, p.eps);
         const float* weight = to_cache ? p.k_norm : p.q_norm;
-        if (turns && weight != nullptr) {
-          const Eight a = eight(weight + 8 * j), b = eight(weight + HALF + 8 * j);
+        const bool normed = turns && weight != nullptr;
+        if (__any_sync(0xffffffffu, normed)) {
+          double sum = 0.0;
+          float rough = 0.0f;
+          auto add = [&](float x) {
+            const float square = x * x;                             // (of a bfloat16 exactly)
+            rough += square;
+            if constexpr (sizeof(T) == 2) sum += widened(square);
+            else {
+              const double wide = widened(fabsf(x));
+              sum = fma(wide, wide, sum);
+            }
+          };
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            lo.x[k] = __fmul_rn(__fmul_rn(lo.x[k], over), a.x[k]);
-            hi.x[k] = __fmul_rn(__fmul_rn(hi.x[k], over), b.x[k]);
+            add(lo.x[k]);
+            add(hi.x[k]);
+          }
+          if (!(rough <= 1e38f) || p.eps < 1e-30) {                 // squares that float32 has no room for, numbers that are not finite
+            sum = 0.0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += (double)lo.x[k] * (double)lo.x[k] + (double)hi.x[k] * (double)hi.x[k];
+          }
+          const float over = over_root(lanes_sum(sum, LANES), HEAD, p.eps);
+          if (normed) {
+            const Eight a = eight(weight + 8 * j), b = eight(weight + HALF + 8 * j);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              lo.x[k] = __fmul_rn(__fmul_rn(lo.x[k], over), a.x[k]);
+              hi.x[k] = __fmul_rn(__fmul_rn(hi.x[k], over), b.x[k]);
+            }
           }
         }
       }
@@ -244,10 +300,10 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 && !NORM ? 3 : 2)
         put_eight(dst + HALF, hi);
       }
       if (!__any_sync(0xffffffffu, valid && to_cache)) continue;
-      float most = 0.0f, low[2] = {lo.x[0], hi.x[0]}, high[2] = {lo.x[0], hi.x[0]};
+      float low[2] = {lo.x[0], hi.x[0]}, high[2] = {lo.x[0], hi.x[0]}, nothing = 0.0f;       // NaN where a number is not finite
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        most = larger(larger(most, magnitude(lo.x[k])), magnitude(hi.x[k]));
+        nothing = __fmaf_rn(lo.x[k], 0.0f, __fmaf_rn(hi.x[k], 0.0f, nothing));
         low[0] = fminf(low[0], lo.x[k]);
         low[1] = fminf(low[1], hi.x[k]);
         high[0] = fmaxf(high[0], lo.x[k]);
@@ -264,20 +320,18 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 && !NORM ? 3 : 2)
           low[half] = fminf(low[half], __shfl_xor_sync(0xffffffffu, low[half], offset));
           high[half] = fmaxf(high[half], __shfl_xor_sync(0xffffffffu, high[half], offset));
         }
-#pragma unroll
-      for (int offset = LANES / 2; offset > 0; offset >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, offset));
-      const bool fine = most < LIMIT;
+      const bool mine_fine = nothing == 0.0f && fmaxf(fmaxf(-low[0], high[0]), fmaxf(-low[1], high[1])) < LIMIT;
+      constexpr uint32_t OF_HEAD = LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1u;
+      const bool fine = (__ballot_sync(0xffffffffu, !mine_fine) >> (threadIdx.x & 31 & ~(LANES - 1)) & OF_HEAD) == 0u;
       const Group of[2] = {group_of(low[0], high[0]), group_of(low[1], high[1])};
       uint32_t unit[2][2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half) {
+        const Coder4 coder(of[half]);
+        const Eight& x = half ? hi : lo;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t w = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w |= code_of(of[half], (half ? hi : lo).x[4 * u + k]) << (4 * k);
-          unit[half][u] = fine ? w : 0u;
-        }
+        for (int u = 0; u < 2; ++u) unit[half][u] = fine ? coder.four(x.x[4 * u], x.x[4 * u + 1], x.x[4 * u + 2], x.x[4 * u + 3]) : 0u;
+      }
       // what the lane four away has of the groups beside this one's (a head of 128 numbers)
       [[maybe_unused]] const bool odd = (j & 4) != 0;
       [[maybe_unused]] uint32_t other = 0;

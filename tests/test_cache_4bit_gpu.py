@@ -203,6 +203,52 @@ def test_store_rows_of_an_inner_buffer(ops):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1.0, 1e-35, 1e-24, 1e25])
+def test_codes_of_both_kernels(ops, dtype, size):
+    """A million numbers, many of them halfway between two codes, by the kernel that divides (rows on odd elements) and the one that has the quotients
+    by parts: the same bits."""
+    tokens, heads, kv, dim = 512, 1, 8, 128
+    gen = torch.Generator().manual_seed(4)
+    rows = torch.randn(tokens, (heads + 2 * kv) * dim, generator=gen)
+    grid = torch.randint(-60, 60, rows.shape, generator=gen) / 16.0                 # sums and halves of few bits: ties are common
+    rows[::2] = grid[::2]
+    rows = (rows.double() * size).to(dtype).to(DEV)
+    wide = torch.zeros(tokens, rows.shape[1] + 1, dtype=dtype, device=DEV)
+    wide[:, 1:] = rows
+    cache = Cache([tokens], kv, dim, 64)
+    positions, seq, _, _ = batch_index([tokens], [0], DEV)
+    weight = (1.0 + 0.3 * torch.randn(dim, generator=gen)).to(DEV)
+    for norm in (None, weight):
+        found = []
+        for x in (rows, wide[:, 1:]):
+            device = cache.device()
+            found.append([ops.norm_rope_kv_store_4bit(x, None, None, 0, positions, seq, 1, cache.table.to(DEV), *device, heads, kv, dim, q_norm=norm, k_norm=norm), *device])
+        assert all(torch.equal(a.nan_to_num(0.0) if a.is_floating_point() else a, b.nan_to_num(0.0) if b.is_floating_point() else b) for a, b in zip(*found))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norms_of_rows_that_are_not_finite(ops, dtype):
+    """A number that is not finite makes its row's queries and its entry what the formula makes of them, in both kernels; nobody else's."""
+    heads, kv, dim = 2, 2, 64
+    weight = torch.ones(dim, device=DEV)
+    for bad in (math.nan, math.inf):
+        rows = torch.randn(3, 6 * dim, generator=torch.Generator().manual_seed(2))
+        rows[1, 5] = rows[1, (heads + 1) * dim + 7] = bad
+        rows[2, :dim] = 0.0
+        wide = torch.zeros(3, 6 * dim + 1, dtype=dtype, device=DEV)
+        wide[:, 1:] = rows.to(dtype)
+        positions, seq, _, _ = batch_index([3], [0], DEV)
+        for x in (rows.to(dtype).to(DEV), wide[:, 1:]):
+            cache = Cache([3], kv, dim, 16)
+            device = cache.device()
+            q = ops.norm_rope_kv_store_4bit(x, None, None, 0, positions, seq, 1, cache.table.to(DEV), *device, heads, kv, dim, q_norm=weight, k_norm=weight).cpu().float()
+            want = plain.normalised(rows.to(dtype).float()[:, :2 * dim].reshape(3, 2, dim), torch.ones(dim), 1e-6).flatten(1).to(dtype).float()
+            assert torch.equal(torch.isnan(q), torch.isnan(want)) and torch.equal(q.nan_to_num(9.0), want.nan_to_num(9.0))
+            nan = torch.isnan(device[2][cache.table[0, 0].item(), :, :3].float()).all(-1).cpu()
+            assert nan.tolist() == [[False, False, False], [False, True, False]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_entries_do_not_depend_on_the_cut(ops, dtype):
     heads, kv, dim, n = 4, 2, 128, 150
     cos, sin = (t.to(DEV) for t in tables(n, dim))
@@ -823,7 +869,7 @@ def test_refusals(ops):
         lambda: stored(rotary=66, **angles(33)), lambda: stored(rotary=-2, **angles(1)), lambda: stored(kp=kp.to(torch.int8)), lambda: stored(positions=positions[:0]),
         lambda: stored(out=torch.zeros(1, 5, dtype=torch.bfloat16, device=DEV)), lambda: stored(kg=kg.transpose(1, 2)), lambda: stored(seqs=2),
         lambda: stored(q_norm=torch.ones(32, device=DEV)), lambda: stored(k_norm=torch.ones(64, device=DEV).double()), lambda: stored(heads=0),
-        lambda: stored(k_norm=torch.ones(64, device=DEV), eps=-1.0), lambda: stored(k_norm=torch.ones(64, device=DEV), eps=math.nan),
+        lambda: stored(k_norm=torch.ones(64, device=DEV), eps=-1.0), lambda: stored(q_norm=torch.ones(64, device=DEV), eps=0.0), lambda: stored(k_norm=torch.ones(64, device=DEV), eps=math.nan),
         lambda: read(dtype=torch.float16), lambda: read(ctx=(20, 20)), lambda: read(dim=128), lambda: read(window=-1), lambda: read(first_seq=2), lambda: read(q_lens=[1, 1]),
     ]
     for i, call in enumerate(wrong):
