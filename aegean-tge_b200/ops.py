@@ -1431,6 +1431,13 @@ def _cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torch.Te
     return shape[0], shape[2]
 
 
+def _all_here(*tensors: Optional[torch.Tensor]) -> None:
+    here = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"a tensor on device {t.get_device()}, while device {here} is the current one")
+
+
 def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary: int, positions: torch.Tensor,
                             seq_of_token: torch.Tensor, num_seqs: int, block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                             k_groups: torch.Tensor, v_groups: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
@@ -1445,6 +1452,7 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
     page_size, 2 * groups], a (step, base) for each 32 numbers of an entry: a code c of 0..15 stands for base + (c - 8) * step.  The codes of
     numbers 32 j + 4 g .. 32 j + 4 g + 3 share 16 bits, the first in the lowest four, which are the (g * groups + j)-th of the entry's.  A position's entry
     does not depend on how its request was cut into steps.  An entry with a number that is not finite, or 2^96 or more, reads as NaN.
+    Rows of one call must not name the same position of a request twice: its entry may then be parts of both.
     """
     _want(qkv, "qkv", _FLOAT, contiguous=False)
     stride = _rows_2d(qkv, "qkv")
@@ -1465,6 +1473,7 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
         raise KernelError(f"a norm with an eps of {eps}")
     _per_token(positions, seq_of_token, tokens)
     num_pages, page_size = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, num_seqs, kv_heads, head_dim)
+    _all_here(qkv, cos, sin, q_norm, k_norm, positions, seq_of_token, out)
     out, out_stride = _rows_like(qkv, heads * head_dim, out, "rotated queries")
     lib = core()
     _check(lib.tge_store_4bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), out_stride, _ptr(cos), _ptr(sin),
@@ -1488,8 +1497,11 @@ def read_cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torc
         raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
     if window < 0 or not 0 <= first_seq <= len(ctx_lens) or (q_lens is not None and len(q_lens) != len(ctx_lens)):
         raise KernelError(f"a read-back of {len(ctx_lens)} requests from {first_seq} on, a window of {window}, {None if q_lens is None else len(q_lens)} portions")
+    if min(ctx_lens, default=0) < 0 or (q_lens is not None and min(q_lens, default=0) < 0):
+        raise KernelError("a read-back of requests that hold or bring fewer than no positions")
     sizes = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, len(ctx_lens), k_pages.shape[1], head_dim)
     _portions(q_start, start_pos, len(ctx_lens))
+    _all_here(q_start, start_pos)
     return _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, None, q_lens)
 
 
@@ -1538,6 +1550,7 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         _want(sink, "attention sinks", torch.float32)
         if sink.numel() != heads:
             raise KernelError(f"attention: {sink.numel()} sinks for {heads} heads")
+    _all_here(q, q_start, start_pos, positions, seq_of_token, sink, out)
     out, out_stride = _rows_like(q, heads * head_dim, out, "attention output")
     is_bf16 = int(q.dtype is torch.bfloat16)
     lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size,

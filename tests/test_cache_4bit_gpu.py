@@ -880,3 +880,33 @@ def test_refusals(ops):
     with pytest.raises(ops.KernelError):
         attention(q=torch.zeros(1, 4 * 320, device=DEV), kp=wide[0], vp=wide[0], kg=wide[1], vg=wide[1], dim=320)
     ops.check_status()
+
+
+class Elsewhere(torch.Tensor):
+    """A tensor that says that it is on the device behind its own."""
+
+    def get_device(self):
+        return super().get_device() + 1
+
+
+@pytest.mark.parametrize("which", range(8))
+def test_tensors_of_another_device_are_refused(ops, which):
+    cache = Cache([20], 2, 64, 16)
+    held, table = cache.device(), cache.table.to(DEV)
+    positions, seq, q_start, start_pos = batch_index([1], [19], DEV)
+    q, qkv = torch.zeros(1, 256, dtype=torch.bfloat16, device=DEV), torch.zeros(1, 512, dtype=torch.bfloat16, device=DEV)
+    weight, sink, angles = torch.ones(64, device=DEV), torch.zeros(4, device=DEV), torch.zeros(30, 32, device=DEV)
+
+    def at(place, tensor):
+        return tensor.as_subclass(Elsewhere) if place == which else tensor
+
+    with pytest.raises(ops.KernelError):
+        ops.attention_4bit(at(0, q), *held, table, at(1, q_start), at(2, start_pos), at(3, positions), at(4, seq), 1, 1, 20, 4, 2, 64, 0.1,
+                           sink=at(5, sink), out=at(6, torch.empty_like(q)), **({"ctx_lens": [20, 20]} if which == 7 else {}))
+    with pytest.raises(ops.KernelError):
+        ops.norm_rope_kv_store_4bit(at(0, qkv), at(1, angles), at(2, angles), 64, at(3, positions), at(4, seq), 1, table, *held, 4, 2, 64,
+                                    q_norm=at(5, weight), k_norm=weight, out=at(6, torch.empty_like(q)), eps=0.0 if which == 7 else 1e-6)
+    with pytest.raises(ops.KernelError):
+        ops.read_cache_4bit(*held, table, at(0, q_start), at(1, start_pos), [-64] if which in (2, 4, 6) else [20], 64, torch.float32,
+                            window=8, q_lens=[-300] if which in (3, 5, 7) else [1])
+    ops.check_status()
