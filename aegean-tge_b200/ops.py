@@ -1212,20 +1212,28 @@ def read_cache_8bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch
     return _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, None)
 
 
-def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts):
-    """What :func:`read_cache_8bit` does, of arguments that were looked over (``sizes``: pages, positions in a page and in a block).  With
-    ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a position whose values' scale is not
-    finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a fourth result, what their numbers
-    stand for (int32: two factors a position, and behind them a word a run and head with their exponents, f in the lower half and e in
+def _most_runs(told, window: int, brought) -> int:
+    """At most how many runs of 64 positions requests' queries see that hold no more than ``told`` positions and bring no more than ``brought`` of them: a
+    request's last n positions lie in (n + 126) // 64 runs at most, wherever in a run the first of them is."""
+    if not window or brought is None:
+        return sum([max((n + 63) // 64, 0) for n in told])
+    return sum([max(min((n + 63) // 64, (new + window + 125) // 64), 0) for n, new in zip(told, brought)])
+
+
+def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts, brought=None):
+    """What :func:`read_cache_8bit` does, of arguments that were looked over (``sizes``: pages, positions in a page and in a block; ``brought``: what
+    every request brings at most, if known).  With ``starts`` for attention: the requests' q_start counted from ``first_seq``'s go there, and a
+    position whose values' scale is not finite has a key that is not instead.  ``dtype`` float16: for the attention over such pages, with a
+    fourth result, what their numbers stand for (int32: two factors a position, and behind them a word a run and head with their exponents, f in the lower half and e in
     the upper: keys are over 2^e, values over 2^f, at most 1; 1 in it where the factors count); None for a cache that this is not built for."""
     num_seqs, kv_heads, head_dim = len(ctx_lens), k_pages.shape[1], k_pages.shape[3]
     num_pages, page_size, block = sizes
-    # a window may leave out runs in front: the sum is then a bound
-    mine = [-(-int(n) // 64) for n in ctx_lens[first_seq:]]
-    runs, width = sum(mine), max(mine, default=0)
+    told = [int(n) for n in ctx_lens[first_seq:]]
+    width = (max(told, default=0) + 63) // 64
+    runs = _most_runs(told, window, brought and brought[first_seq:])
     k = k_scale.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    table = block_table.new_empty((len(mine), width))
+    table = block_table.new_empty((len(told), width))
     factors = block_table.new_empty(runs * kv_heads * (128 + 1)) if dtype == torch.float16 else None
     lib = core()
     rc = lib.tge_read_8bit(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
@@ -1254,7 +1262,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    block_table: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, positions: torch.Tensor,
                    seq_of_token: torch.Tensor, num_seqs: int, max_q_len: int, max_ctx_len: int, heads: int, kv_heads: int, head_dim: int,
                    scale: float, window: int = 0, out: Optional[torch.Tensor] = None, decode_prefix: int = 0,
-                   sink: Optional[torch.Tensor] = None, ctx_lens=None) -> torch.Tensor:
+                   sink: Optional[torch.Tensor] = None, ctx_lens=None, q_lens=None) -> torch.Tensor:
     """:func:`attention` over a cache of 8-bit codes (see :func:`rope_kv_store_8bit`): [T, heads * head_dim].
 
     q: [T, >= heads*head_dim] (dense rows, any row stride), rotated; the cache already holds every position up to each portion's
@@ -1262,6 +1270,8 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     that joins the softmax's denominator once, with no key or value.  ``decode_prefix``: how many requests at the head of the batch
     are known to bring one token each while others bring more.  ``ctx_lens`` (host numbers): what every request holds after the
     step (None: ``max_ctx_len``, a bound); portions that hold more are reported through the status word and get no output.
+    ``q_lens`` (host numbers): what every request brings (None: ``max_q_len``, a bound); with a ``window`` portions make room for what their
+    queries see and no more, and more than was said is reported in the same way.
     """
     _want(q, "queries", _FLOAT, contiguous=False)
     q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
@@ -1272,6 +1282,8 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     _per_token(positions, seq_of_token, tokens)
     if ctx_lens is not None and len(ctx_lens) != num_seqs:
         raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
+    if q_lens is not None and len(q_lens) != num_seqs:
+        raise KernelError(f"attention: {len(q_lens)} portions for {num_seqs} requests")
     if not 0 <= decode_prefix <= num_seqs or window < 0:
         raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
     if sink is not None:
@@ -1283,8 +1295,9 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     lib, cache = core(), (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), num_pages, page_size, block,
                           block_table.data_ptr(), block_table.shape[1])
     singles = num_seqs if max_q_len <= 1 else decode_prefix
-    if singles < num_seqs and ctx_lens is None:
-        ctx_lens = [max_ctx_len] * num_seqs
+    if singles < num_seqs:
+        ctx_lens = [max_ctx_len] * num_seqs if ctx_lens is None else ctx_lens
+        q_lens = [max_q_len] * num_seqs if q_lens is None else q_lens
     need = -1                                           # scratch numbers of the single tokens' kernel; -1: sizes that it does not take
     if singles:
         need = _decode_floats(lib.tge_attention_8bit_decode_floats, is_bf16, singles, heads, kv_heads, head_dim, page_size, block_table.shape[1])
@@ -1303,7 +1316,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     def read_as(dtype: torch.dtype, first: int, starts: torch.Tensor):
         return _read_8bit((num_pages, page_size, block), k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens,
-                          dtype, window, first, starts)
+                          dtype, window, first, starts, q_lens)
 
     return _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, seq_of_token, num_seqs, max_q_len, heads, kv_heads, head_dim, scale,
                          window, sink, ctx_lens, singles, need >= 0, single_tokens, simply, read_as)
@@ -1502,19 +1515,20 @@ def read_cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torc
     sizes = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, len(ctx_lens), k_pages.shape[1], head_dim)
     _portions(q_start, start_pos, len(ctx_lens))
     _all_here(q_start, start_pos)
-    return _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, None, q_lens)
+    runs = _most_runs(ctx_lens[first_seq:], 0, None)
+    if window and q_lens is not None:
+        behind = window - 1                    # (positions that a query sees in front of itself)
+        runs -= sum([(n - new - behind) // 64 for n, new in zip(ctx_lens[first_seq:], q_lens[first_seq:]) if n - new > behind])
+    return _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, None, runs)
 
 
-def _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, starts, q_lens=None):
-    """What :func:`read_cache_4bit` does, of arguments that were looked over; ``starts`` and ``dtype`` float16 as for :func:`_read_8bit`."""
+def _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, starts, runs):
+    """What :func:`read_cache_4bit` does, of arguments that were looked over, into so many ``runs`` of 64 positions; ``starts`` and ``dtype`` float16 as for
+    :func:`_read_8bit`."""
     kv_heads = k_pages.shape[1]
     num_pages, page_size = sizes
     told = ctx_lens[first_seq:] if first_seq else ctx_lens
     width = (max(told, default=0) + 63) // 64
-    runs = sum([(n + 63) // 64 for n in told])
-    if window and q_lens is not None:
-        behind = window - 1                    # (positions that a query sees in front of itself)
-        runs -= sum([(n - new - behind) // 64 for n, new in zip(told, q_lens[first_seq:] if first_seq else q_lens) if n - new > behind])
     k = k_groups.new_empty((runs, kv_heads, 64, head_dim), dtype=dtype)
     v = torch.empty_like(k)
     table = block_table.new_empty((len(told), width))
@@ -1533,7 +1547,7 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    block_table: torch.Tensor, q_start: torch.Tensor, start_pos: torch.Tensor, positions: torch.Tensor,
                    seq_of_token: torch.Tensor, num_seqs: int, max_q_len: int, max_ctx_len: int, heads: int, kv_heads: int, head_dim: int,
                    scale: float, window: int = 0, out: Optional[torch.Tensor] = None, decode_prefix: int = 0,
-                   sink: Optional[torch.Tensor] = None, ctx_lens=None) -> torch.Tensor:
+                   sink: Optional[torch.Tensor] = None, ctx_lens=None, q_lens=None) -> torch.Tensor:
     """:func:`attention` over a cache of 4-bit codes (see :func:`norm_rope_kv_store_4bit`): [T, heads * head_dim].  Arguments as for :func:`attention_8bit`."""
     _want(q, "queries", _FLOAT, contiguous=False)
     q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
@@ -1544,6 +1558,8 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     _per_token(positions, seq_of_token, tokens)
     if ctx_lens is not None and len(ctx_lens) != num_seqs:
         raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
+    if q_lens is not None and len(q_lens) != num_seqs:
+        raise KernelError(f"attention: {len(q_lens)} portions for {num_seqs} requests")
     if not 0 <= decode_prefix <= num_seqs or window < 0:
         raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
     if sink is not None:
@@ -1569,8 +1585,9 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     if need >= 0 and singles == num_seqs and single_tokens() == num_seqs:      # (a decode step: nothing else to set up)
         return out
-    if singles < num_seqs and ctx_lens is None:
-        ctx_lens = [max_ctx_len] * num_seqs
+    if singles < num_seqs:
+        ctx_lens = [max_ctx_len] * num_seqs if ctx_lens is None else ctx_lens
+        q_lens = [max_q_len] * num_seqs if q_lens is None else q_lens
 
     def simply(rows, tokens: int) -> None:
         _check(lib.tge_attention_4bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
@@ -1579,7 +1596,7 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     def read_as(dtype: torch.dtype, first: int, starts: torch.Tensor):
         return _read_4bit((num_pages, page_size), k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim,
-                          dtype, window, first, starts)
+                          dtype, window, first, starts, _most_runs(ctx_lens[first:], window, q_lens[first:]))
 
     return _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, seq_of_token, num_seqs, max_q_len, heads, kv_heads, head_dim, scale,
                          window, sink, ctx_lens, singles, need >= 0, single_tokens, simply, read_as)

@@ -453,7 +453,8 @@ class GQAttention(Mixer):
             ctx.scratch["ctx_lens"] = [start + count for start, count in zip(ctx.host_start_pos, ctx.host_q_lens)]
         return ops.attention_8bit(q, *held, table, ctx.q_start, ctx.start_pos, ctx.positions, ctx.seq_of_token, ctx.num_seqs, ctx.max_q_len,
                                   ctx.max_ctx_len, self.heads, self.kv_heads, self.head_dim, self.scale, window=int(self.window or 0), out=out,
-                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"))
+                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"),
+                                  q_lens=ctx.host_q_lens if ctx.max_q_len > 1 else None)
 
     def attend_4bit(self, h, ctx: StepContext, cache: LayerCache, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Product with its biases; norm, rotation, codes, steps and bases of k and v stored; attention over the codes."""
@@ -482,7 +483,8 @@ class GQAttention(Mixer):
             ctx.scratch["ctx_lens"] = [start + count for start, count in zip(ctx.host_start_pos, ctx.host_q_lens)]
         return ops.attention_4bit(q, *held, table, ctx.q_start, ctx.start_pos, ctx.positions, ctx.seq_of_token, ctx.num_seqs, ctx.max_q_len,
                                   ctx.max_ctx_len, self.heads, self.kv_heads, self.head_dim, self.scale, window=int(self.window or 0), out=out,
-                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"))
+                                  decode_prefix=ctx.decode_prefix, sink=self.sink, ctx_lens=ctx.scratch.get("ctx_lens"),
+                                  q_lens=ctx.host_q_lens if ctx.max_q_len > 1 else None)
 
     def share_input_projection(self, rows: torch.Tensor) -> Optional[torch.Tensor]:
         """A block offers the rows of another product over the same input (a feed-forward's up weight) to be
