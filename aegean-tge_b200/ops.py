@@ -1216,8 +1216,8 @@ def _most_runs(told, window: int, brought) -> int:
     """At most how many runs of 64 positions requests' queries see that hold no more than ``told`` positions and bring no more than ``brought`` of them: a
     request's last n positions lie in (n + 126) // 64 runs at most, wherever in a run the first of them is."""
     if not window or brought is None:
-        return sum([max((n + 63) // 64, 0) for n in told])
-    return sum([max(min((n + 63) // 64, (new + window + 125) // 64), 0) for n, new in zip(told, brought)])
+        return sum([(n + 63) // 64 for n in told])
+    return sum([min((n + 63) // 64, (new + window + 125) // 64) for n, new in zip(told, brought)])
 
 
 def _read_8bit(sizes, k_pages, v_pages, k_scale, v_scale, block_table, q_start, start_pos, ctx_lens, dtype, window, first_seq, starts, brought=None):
@@ -1515,10 +1515,11 @@ def read_cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torc
     sizes = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, len(ctx_lens), k_pages.shape[1], head_dim)
     _portions(q_start, start_pos, len(ctx_lens))
     _all_here(q_start, start_pos)
-    runs = _most_runs(ctx_lens[first_seq:], 0, None)
+    told = ctx_lens[first_seq:] if first_seq else ctx_lens
+    runs = _most_runs(told, 0, None)
     if window and q_lens is not None:
         behind = window - 1                    # (positions that a query sees in front of itself)
-        runs -= sum([(n - new - behind) // 64 for n, new in zip(ctx_lens[first_seq:], q_lens[first_seq:]) if n - new > behind])
+        runs -= sum([(n - new - behind) // 64 for n, new in zip(told, q_lens[first_seq:] if first_seq else q_lens) if n - new > behind])
     return _read_4bit(sizes, k_pages, v_pages, k_groups, v_groups, block_table, q_start, start_pos, ctx_lens, head_dim, dtype, window, first_seq, None, runs)
 
 
