@@ -103,6 +103,8 @@ __device__ __forceinline__ double widened(float x) {
   return __hiloint2double((int)((bits >> 3) + 0x38000000u), (int)(bits << 29));
 }
 
+// Queries alone have no kv heads and no pages.
+
 // Any head size up to 256, any strides: one warp per (token, head), a lane per number of a group.
 constexpr int WARPS = 8;
 template <typename T>
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(UNIT_THREADS, sizeof(T) == 2 ? 3 : 2) store_4b
   const int page_index = pos / p.page_size, slot = pos - page_index * p.page_size;
   const int page = page_index < p.max_pages ? p.block_table[(size_t)seq * p.max_pages + page_index] : -1;
   const bool here = page >= 0 && page < p.num_pages;
-  if (!here && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
+  if (!here && p.kv_heads > 0 && threadIdx.x == 0) atomicOr(p.status, TGE_STATUS_BAD_PAGE);
   for (int h0 = mine; h0 < heads + mine; h0 += UNIT_AHEAD * rows_at_once) {       // the same number of rounds for every lane of a warp
     if (h0 != mine) load(h0);
 #pragma unroll
@@ -615,12 +617,19 @@ bool whole_groups(int head_dim) { return head_dim == 32 || head_dim == 64 || hea
 
 }  // namespace
 
+// Without a block table and pages (null): the queries alone, of rows that hold nothing else.
 TGE_API int tge_store_4bit(const void* qkv, int is_bf16, long long row_stride, void* q_out, long long q_stride, const float* cos_table,
                            const float* sin_table, int table_rows, int rotary, int pairs, const float* q_norm, const float* k_norm, double eps,
                            const int* positions, const int* seq_of_token, int num_seqs, const int* block_table, int max_pages, void* k_pages,
                            void* v_pages, void* k_groups, void* v_groups, int num_pages, int page_size, int tokens, int heads, int kv_heads, int head_dim,
                            int* status, cudaStream_t stream) {
-  const int rc = cache_shape("store_4bit", num_pages, page_size, kv_heads, head_dim, max_pages);
+  const bool alone = k_pages == nullptr && block_table == nullptr;
+  TGE_REQUIRE(!alone || (v_pages == nullptr && k_groups == nullptr && v_groups == nullptr), "store_4bit: pages of keys or of values only");
+  if (alone) {
+    kv_heads = num_pages = max_pages = 0;
+    page_size = 1;
+  }
+  const int rc = alone ? cache_shape("store_4bit", 1, 1, 1, head_dim, 1) : cache_shape("store_4bit", num_pages, page_size, kv_heads, head_dim, max_pages);
   if (rc != 0) return rc;
   TGE_REQUIRE(tokens >= 0 && heads > 0 && num_seqs >= 0, "store_4bit: bad sizes");
   TGE_REQUIRE(rotary >= 0 && rotary <= head_dim && rotary % 2 == 0, "store_4bit: rotary width %d must be even and at most head_dim %d", rotary, head_dim);

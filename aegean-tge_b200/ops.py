@@ -1452,10 +1452,10 @@ def _all_here(*tensors: Optional[torch.Tensor]) -> None:
 
 
 def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary: int, positions: torch.Tensor,
-                            seq_of_token: torch.Tensor, num_seqs: int, block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                            k_groups: torch.Tensor, v_groups: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
-                            q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, pairs: bool = False,
-                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                            seq_of_token: torch.Tensor, num_seqs: int, block_table: Optional[torch.Tensor], k_pages: Optional[torch.Tensor],
+                            v_pages: Optional[torch.Tensor], k_groups: Optional[torch.Tensor], v_groups: Optional[torch.Tensor], heads: int, kv_heads: int,
+                            head_dim: int, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                            pairs: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Normalises (if wanted) and rotates q and k and appends k and v to a paged cache of 4-bit codes; returns the queries [T, heads * head_dim].
 
     qkv: [T, >= (heads + 2*kv_heads) * head_dim], unchanged.  ``q_norm`` / ``k_norm`` (float32 [head_dim]): every head of the queries / keys goes
@@ -1466,12 +1466,15 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
     numbers 32 j + 4 g .. 32 j + 4 g + 3 share 16 bits, the first in the lowest four, which are the (g * groups + j)-th of the entry's.  A position's entry
     does not depend on how its request was cut into steps.  An entry with a number that is not finite, or 2^96 or more, reads as NaN.
     Rows of one call must not name the same position of a request twice: its entry may then be parts of both.
+    With None for the block table and all four of the cache's tensors (a layer that reads an earlier layer's cache) nothing is stored: the queries
+    alone, by the same roundings, of rows that need hold no more than them.
     """
     _want(qkv, "qkv", _FLOAT, contiguous=False)
     stride = _rows_2d(qkv, "qkv")
     tokens = qkv.shape[0]
-    if heads <= 0 or kv_heads <= 0 or qkv.shape[1] < (heads + 2 * kv_heads) * head_dim:
-        raise KernelError(f"qkv rows of {qkv.shape[1]} numbers for {heads} + 2 * {kv_heads} heads of {head_dim}")
+    alone = block_table is None and all(t is None for t in (k_pages, v_pages, k_groups, v_groups))
+    if heads <= 0 or kv_heads <= 0 or qkv.shape[1] < (heads if alone else heads + 2 * kv_heads) * head_dim:
+        raise KernelError(f"qkv rows of {qkv.shape[1]} numbers for {heads} + 2 * {0 if alone else kv_heads} heads of {head_dim}")
     if rotary > 0:
         _want(cos, "cos table", torch.float32)
         _want(sin, "sin table", torch.float32)
@@ -1485,15 +1488,17 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
     if (q_norm is not None or k_norm is not None) and not 0.0 < eps < math.inf:
         raise KernelError(f"a norm with an eps of {eps}")
     _per_token(positions, seq_of_token, tokens)
-    num_pages, page_size = _cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, num_seqs, kv_heads, head_dim)
+    if alone:
+        held = (None, 0, None, None, None, None, 0, 0)
+    else:
+        held = (block_table.data_ptr(), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(), k_groups.data_ptr(), v_groups.data_ptr(),
+                *_cache_4bit(k_pages, v_pages, k_groups, v_groups, block_table, num_seqs, kv_heads, head_dim))
     _all_here(qkv, cos, sin, q_norm, k_norm, positions, seq_of_token, out)
     out, out_stride = _rows_like(qkv, heads * head_dim, out, "rotated queries")
     lib = core()
     _check(lib.tge_store_4bit(qkv.data_ptr(), int(qkv.dtype == torch.bfloat16), stride, out.data_ptr(), out_stride, _ptr(cos), _ptr(sin),
                               0 if cos is None else cos.shape[0], rotary, int(pairs), _ptr(q_norm), _ptr(k_norm), float(eps), positions.data_ptr(),
-                              seq_of_token.data_ptr(), num_seqs, block_table.data_ptr(), block_table.shape[1], k_pages.data_ptr(), v_pages.data_ptr(),
-                              k_groups.data_ptr(), v_groups.data_ptr(), num_pages, page_size, tokens, heads, kv_heads, head_dim,
-                              status_word().data_ptr(), _stream()), lib)
+                              seq_of_token.data_ptr(), num_seqs, *held, tokens, heads, kv_heads, head_dim, status_word().data_ptr(), _stream()), lib)
     return out
 
 

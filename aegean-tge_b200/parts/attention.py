@@ -466,19 +466,9 @@ class GQAttention(Mixer):
         cos, sin, rotary = self.position.pair_tables() if pairs else tables
         eps = self.qk_norm[1] if self.qk_norm is not None else 1.0
         qkv = ops.linear(h, self.w_qkv, self.b_qkv, ops.GEMM_STORE, settled=True)
-        if cache.owner:
-            q = ops.norm_rope_kv_store_4bit(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, ctx.num_seqs, table, *held, self.heads, self.kv_heads,
-                                            self.head_dim, q_norm=self.q_norm_w, k_norm=self.k_norm_w, eps=eps, pairs=pairs)
-        else:
-            if self.qk_norm is not None:
-                ops.qk_norm_kv_store(qkv, self.q_norm_w, self.k_norm_w, eps, True, ctx.positions, ctx.seq_of_token, None, None, None, self.heads,
-                                     self.kv_heads, self.head_dim, self.value_dim)
-            q = qkv[:, :self.q_dim]
-            if pairs:
-                heads = q.view(-1, self.heads, self.head_dim)
-                self.position.apply(heads, qkv[:, self.q_dim:self.q_dim + self.kv_dim].view(-1, self.kv_heads, self.head_dim), ctx.positions)
-            else:
-                ops.rope_kv_store(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, table, None, None, self.heads, self.kv_heads, self.head_dim)
+        into = (table, *held) if cache.owner else (None,) * 5          # (a layer that reads an earlier layer's cache: its queries alone)
+        q = ops.norm_rope_kv_store_4bit(qkv, cos, sin, rotary, ctx.positions, ctx.seq_of_token, ctx.num_seqs, *into, self.heads, self.kv_heads, self.head_dim,
+                                        q_norm=self.q_norm_w, k_norm=self.k_norm_w, eps=eps, pairs=pairs)
         if ctx.max_q_len > 1 and "ctx_lens" not in ctx.scratch:
             ctx.scratch["ctx_lens"] = [start + count for start, count in zip(ctx.host_start_pos, ctx.host_q_lens)]
         return ops.attention_4bit(q, *held, table, ctx.q_start, ctx.start_pos, ctx.positions, ctx.seq_of_token, ctx.num_seqs, ctx.max_q_len,
