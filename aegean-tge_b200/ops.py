@@ -1323,8 +1323,8 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
 
 def _decode_floats(ask, *sizes) -> int:
-    """Scratch numbers of a single tokens' kernel (-1: sizes that it does not take)."""
-    key = (ask.__name__, *sizes)
+    """Scratch numbers of a single tokens' kernel on the current device, whose number of SMs decides them (-1: sizes that it does not take)."""
+    key = (_current_device(), ask.__name__, *sizes)
     need = _codes_floats.get(key)
     if need is None:
         if len(_codes_floats) >= 1024:
