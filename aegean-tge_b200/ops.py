@@ -1309,6 +1309,9 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                                            _ptr(parts), need, status_word().data_ptr(), _stream())
         return singles if _check(rc, lib) != UNSUPPORTED else 0
 
+    if need >= 0 and singles == num_seqs and single_tokens() == num_seqs:      # (a decode step: nothing else to set up)
+        return out
+
     def simply(rows, tokens: int) -> None:
         _check(lib.tge_attention_8bit_simple(rows[0].data_ptr(), is_bf16, q_stride, *cache, rows[2].data_ptr(), rows[3].data_ptr(), num_seqs,
                                              tokens, rows[1].data_ptr(), out_stride, heads, kv_heads, head_dim, float(scale), int(window),
