@@ -78,9 +78,9 @@ __global__ void __launch_bounds__(128) attention_8bit_simple_kernel(const Attn8 
       m = m_new;
     }
   }
-  if (p.sink != nullptr) {
-    const float m_new = fmaxf(m, p.sink[h]), corr = m == -INFINITY ? 0.0f : expf(m - m_new);
-    l = l * corr + expf(p.sink[h] - m_new);
+  if (p.sink != nullptr) {                     // minus infinity is none, however large a one leaves zeros
+    const float sink = p.sink[h] > 3.4e38f ? 3.4e38f : p.sink[h], m_new = fmaxf(m, sink), corr = m == -INFINITY ? 0.0f : expf(m - m_new);
+    l = l * corr + (sink == -INFINITY ? 0.0f : expf(sink - m_new));
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) acc[i] *= corr;
   }

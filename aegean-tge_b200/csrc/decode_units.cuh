@@ -63,6 +63,12 @@ __device__ __forceinline__ int slices_before(const DecodeUnits& p, int upto, int
 }
 __device__ __forceinline__ int run_length(const DecodeUnits& p, int total, int blocks) { return max((total + blocks - 1) / blocks, p.least); }
 
+// A head's sink in base-2 units (a finite one however large: it leaves zeros, not NaN).
+__device__ __forceinline__ float sink_of(const DecodeUnits& p, int head) {
+  const float sink = p.sink[head] * LOG2E;
+  return sink > 3.4e38f ? 3.4e38f : sink;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -194,7 +200,7 @@ __device__ __forceinline__ void leave_part(const DecodeUnits& p, Meeting<HD, NT>
     if (whole) {
       if (token < 0) continue;
       if (p.sink != nullptr) {
-        const float sink = p.sink[head0 + head] * LOG2E, top = fmaxf(most, sink), down = exp2_fast(most - top);
+        const float sink = sink_of(p, head0 + head), top = fmaxf(most, sink), down = exp2_fast(most - top);
         sum = fmaf(sum, down, exp2_fast(sink - top));
         acc.x *= down;
         acc.y *= down;
@@ -215,7 +221,7 @@ __device__ __forceinline__ void leave_part(const DecodeUnits& p, Meeting<HD, NT>
     cluster_sync();
     for (int i = rank * DWARPS * 32 + threadIdx.x; token >= 0 && i < heads_here * (HD / 2); i += ranks * DWARPS * 32) {
       const int head = i / (HD / 2), pair = i - head * (HD / 2);
-      const float sink = p.sink != nullptr ? p.sink[head0 + head] * LOG2E : NONE;
+      const float sink = p.sink != nullptr ? sink_of(p, head0 + head) : NONE;
       float top = sink, all = 0.0f;
       for (int r = 0; r < ranks; ++r) top = fmaxf(top, of_rank(&part_state[head], r).x);
       float2 acc = make_float2(0.0f, 0.0f);
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) decode_join_kernel(const Deco
     }
     __syncthreads();
     if (!second && valid) {
-      const float sink = p.sink != nullptr ? p.sink[head0 + head] * LOG2E : NONE;
+      const float sink = p.sink != nullptr ? sink_of(p, head0 + head) : NONE;
       const float top = fmaxf(fmaxf(most, half_m[head & 7]), sink);
       const float f0 = exp2_fast(most - top), f1 = exp2_fast(half_m[head & 7] - top);
       const float all = fmaf(sum, f0, f1 * half_l[head & 7]) + (p.sink != nullptr ? exp2_fast(sink - top) : 0.0f);

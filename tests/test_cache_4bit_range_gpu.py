@@ -1,0 +1,42 @@
+"""The 4-bit cache at the ends of float32's range: norms, queries, sinks."""
+import math
+
+import pytest
+import torch
+
+import test_cache_8bit_gpu as eight
+from helpers import TOL, batch_index, rel_error
+from test_cache_4bit_gpu import DEV, Cache, attend, attention_of, ops, tables  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim,columns", [(64, 16), (64, 300), (128, 16), (128, 300), (80, 16)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sinks_at_the_ends_of_the_range(ops, dtype, dim, columns, bits):
+    """A sink of minus infinity is none, one far above every score leaves zeros; a row that sees nothing (its page is outside the pool, and
+    reported) is zero under any."""
+    heads, kv = 6, 2
+    cache = Cache([100, 20, 5], kv, dim, 16) if bits == 4 else eight.Cache([100, 20, 5], kv, dim, 16, 1)
+    table = torch.full((3, columns), -1, dtype=torch.int32)
+    table[:, :cache.table.shape[1]] = cache.table
+    table[2] = -1
+    positions, seq, q_start, start_pos = batch_index([1] * 3, [99, 19, 4], DEV)
+    q = (torch.randn(3, heads * dim, generator=torch.Generator().manual_seed(7)) * (1.0 if bits == 4 else 0.05)).to(dtype).to(DEV)
+    call = ops.attention_4bit if bits == 4 else ops.attention_8bit
+
+    def rows(sink):
+        out = call(q, *cache.device(), table.to(DEV), q_start, start_pos, positions, seq, 3, 1, 100, heads, kv, dim, 0.1,
+                   sink=None if sink is None else torch.tensor(sink, device=DEV))
+        with pytest.raises(ops.DeviceStatusError):
+            ops.check_status()
+        return out.view(3, heads, dim)
+
+    none = rows(None)
+    assert (none[2] == 0).all() and torch.isfinite(none.float()).all()
+    for sinks in ([-math.inf] * 6, [-3.4e38] * 6):
+        assert torch.equal(rows(sinks), none)
+    some = rows([math.inf, 3.4e38, 2.5e38, -math.inf, math.nan, 0.0])
+    assert (some[:, :3] == 0).all() and torch.equal(some[:, 3], none[:, 3]) and torch.isnan(some[:, 4]).all()
+    assert torch.isfinite(some[:, 5].float()).all() and (some[2, 5] == 0).all()
