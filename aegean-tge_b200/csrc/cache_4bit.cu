@@ -90,7 +90,12 @@ struct StoreParams4 {
 
 __device__ __forceinline__ float turned_first(float lo, float hi, float c, float s) { return __fsub_rn(__fmul_rn(lo, c), __fmul_rn(hi, s)); }
 __device__ __forceinline__ float turned_second(float lo, float hi, float c, float s) { return __fadd_rn(__fmul_rn(lo, s), __fmul_rn(hi, c)); }
-__device__ __forceinline__ float over_root(double sum, int count, double eps) { return __fdiv_rn(1.0f, __fsqrt_rn((float)(sum / count + eps))); }
+// (A mean that float32 has no room for goes over an even power of two first: the same bits times its root.)
+__device__ __forceinline__ float over_root(double sum, int count, double eps) {
+  const double mean = sum / count + eps;
+  if (mean > 1e38) return __fmul_rn(__fdiv_rn(1.0f, __fsqrt_rn((float)(mean * 0x1p-140))), 0x1p-70f);
+  return __fdiv_rn(1.0f, __fsqrt_rn((float)mean));
+}
 __device__ __forceinline__ double lanes_sum(double v, int lanes) {
   for (int offset = lanes / 2; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
   return v;

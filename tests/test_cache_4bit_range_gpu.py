@@ -12,6 +12,42 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256, 48])
+def test_norms_of_large_rows(ops, dtype, dim):
+    """A row times a power of two has the norm of the row, also where its squares are beyond float32: the same bits, in both kernels."""
+    heads, kv, tokens = 2, 2, 9
+    gen = torch.Generator().manual_seed(3)
+    rows = torch.randn(tokens, 6 * dim, generator=gen).to(dtype).float().clamp(-4.0, 4.0)
+    weight = (1.0 + 0.3 * torch.randn(dim, generator=gen)).to(DEV)
+    positions, seq, _, _ = batch_index([tokens], [0], DEV)
+    cache = Cache([tokens], kv, dim, 16)
+    cos, sin = (t.to(DEV) for t in tables(64, dim))
+
+    def stored(up, wide):
+        x = rows.clone()
+        x[:, :4 * dim] *= 2.0 ** up
+        assert torch.isfinite(x).all()
+        place = torch.zeros(tokens, 6 * dim + wide, dtype=dtype, device=DEV)
+        place[:, wide:] = x.to(dtype)
+        device = cache.device()
+        q = ops.norm_rope_kv_store_4bit(place[:, wide:], cos, sin, dim, positions, seq, 1, cache.table.to(DEV), *device, heads, kv, dim,
+                                        q_norm=weight, k_norm=weight, eps=2.0 ** -125)
+        return [q, device[0], device[1], device[2].nan_to_num(0.0), device[3].nan_to_num(0.0)]
+
+    want = stored(0, 0)
+    x = rows[:, :2 * dim].double().view(tokens, 2, dim)
+    norm = x / x.square().mean(-1, keepdim=True).sqrt() * weight.cpu().double()
+    c, s = (t.cpu().double()[:tokens, None] for t in (cos, sin))
+    lo, hi = norm[..., :dim // 2], norm[..., dim // 2:]
+    turned = torch.cat([lo * c - hi * s, lo * s + hi * c], -1).flatten(1)
+    assert rel_error(want[0], turned) < 2 * torch.finfo(dtype).eps + 2.0 ** -20
+    for up in (-20, 40, 63, 64, 65, 100, 125):
+        for wide in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(stored(up, wide), want)), (up, wide)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim,columns", [(64, 16), (64, 300), (128, 16), (128, 300), (80, 16)])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_sinks_at_the_ends_of_the_range(ops, dtype, dim, columns, bits):
