@@ -1462,7 +1462,7 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
     """Normalises (if wanted) and rotates q and k and appends k and v to a paged cache of 4-bit codes; returns the queries [T, heads * head_dim].
 
     qkv: [T, >= (heads + 2*kv_heads) * head_dim], unchanged.  ``q_norm`` / ``k_norm`` (float32 [head_dim]): every head of the queries / keys goes
-    over the root of its mean square plus ``eps`` (positive) and times these weights, before the rotation.  cos/sin as for :func:`rope_kv_store`;
+    over the root of its mean square plus ``eps`` (2^-126 at least) and times these weights, before the rotation.  cos/sin as for :func:`rope_kv_store`;
     ``pairs``: numbers 2d and 2d + 1 of a head are turned together instead of d and d + rotary / 2.
     Pages: uint8 [num_pages, kv_heads, page_size, 16 * groups], groups = ceil(head_dim / 32); steps and bases: bfloat16 [num_pages, kv_heads,
     page_size, 2 * groups], a (step, base) for each 32 numbers of an entry: a code c of 0..15 stands for base + (c - 8) * step.  The codes of
@@ -1488,8 +1488,8 @@ def norm_rope_kv_store_4bit(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin:
             _want(t, name, torch.float32)
             if t.numel() != head_dim:
                 raise KernelError(f"{name} has {t.numel()} elements for heads of {head_dim}")
-    if (q_norm is not None or k_norm is not None) and not 0.0 < eps < math.inf:
-        raise KernelError(f"a norm with an eps of {eps}")
+    if (q_norm is not None or k_norm is not None) and not 2.0 ** -126 <= eps < math.inf:
+        raise KernelError(f"a norm with an eps of {eps}: none that float32 holds as a normal number")
     _per_token(positions, seq_of_token, tokens)
     if alone:
         held = (None, 0, None, None, None, None, 0, 0)

@@ -47,6 +47,17 @@ def test_norms_of_large_rows(ops, dtype, dim):
     ops.check_status()
 
 
+def test_an_eps_that_float32_does_not_hold_is_refused(ops):
+    cache = Cache([1], 1, 64, 16)
+    positions, seq, _, _ = batch_index([1], [0], DEV)
+    qkv, weight = torch.zeros(1, 3 * 64, device=DEV), torch.ones(64, device=DEV)
+    store = lambda eps: ops.norm_rope_kv_store_4bit(qkv, None, None, 0, positions, seq, 1, cache.table.to(DEV), *cache.device(), 1, 1, 64, q_norm=weight, k_norm=weight, eps=eps)  # noqa: E731
+    assert (store(1.2e-38) == 0).all()                       # a row of zeros
+    for eps in (1e-39, 1e-50, 1e-300):
+        with pytest.raises(ops.KernelError):
+            store(eps)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim,columns", [(64, 16), (64, 300), (128, 16), (128, 300), (80, 16)])
 @pytest.mark.parametrize("bits", [4, 8])
