@@ -1284,7 +1284,7 @@ def attention_8bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
     if q_lens is not None and len(q_lens) != num_seqs:
         raise KernelError(f"attention: {len(q_lens)} portions for {num_seqs} requests")
-    if not 0 <= decode_prefix <= num_seqs or window < 0:
+    if not 0 <= decode_prefix <= num_seqs or not 0 <= window < 1 << 31:
         raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
     if sink is not None:
         _want(sink, "attention sinks", torch.float32)
@@ -1516,7 +1516,7 @@ def read_cache_4bit(k_pages: torch.Tensor, v_pages: torch.Tensor, k_groups: torc
         raise KernelError(f"4-bit pages must be [pages, kv_heads, page_size, 16 * groups], got {tuple(k_pages.shape)}")
     if dtype not in _FLOAT:
         raise KernelError(f"cache entries are read as float32 or bfloat16, not {dtype}")
-    if window < 0 or not 0 <= first_seq <= len(ctx_lens) or (q_lens is not None and len(q_lens) != len(ctx_lens)):
+    if not 0 <= window < 1 << 31 or not 0 <= first_seq <= len(ctx_lens) or (q_lens is not None and len(q_lens) != len(ctx_lens)):
         raise KernelError(f"a read-back of {len(ctx_lens)} requests from {first_seq} on, a window of {window}, {None if q_lens is None else len(q_lens)} portions")
     if min(ctx_lens, default=0) < 0 or (q_lens is not None and min(q_lens, default=0) < 0):
         raise KernelError("a read-back of requests that hold or bring fewer than no positions")
@@ -1569,7 +1569,7 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise KernelError(f"attention: {len(ctx_lens)} contexts for {num_seqs} requests")
     if q_lens is not None and len(q_lens) != num_seqs:
         raise KernelError(f"attention: {len(q_lens)} portions for {num_seqs} requests")
-    if not 0 <= decode_prefix <= num_seqs or window < 0:
+    if not 0 <= decode_prefix <= num_seqs or not 0 <= window < 1 << 31:
         raise KernelError(f"attention: {decode_prefix} single tokens of {num_seqs} requests, a window of {window}")
     if sink is not None:
         _want(sink, "attention sinks", torch.float32)

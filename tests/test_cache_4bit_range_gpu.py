@@ -87,3 +87,16 @@ def test_sinks_at_the_ends_of_the_range(ops, dtype, dim, columns, bits):
     some = rows([math.inf, 3.4e38, 2.5e38, -math.inf, math.nan, 0.0])
     assert (some[:, :3] == 0).all() and torch.equal(some[:, 3], none[:, 3]) and torch.isnan(some[:, 4]).all()
     assert torch.isfinite(some[:, 5].float()).all() and (some[2, 5] == 0).all()
+
+
+def test_a_window_beyond_whole_numbers_of_32_bits_is_refused(ops):
+    cache = Cache([20], 2, 64, 16)
+    positions, seq, q_start, start_pos = batch_index([1], [19], DEV)
+    q = torch.zeros(1, 256, device=DEV)
+    for window in (2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ops.KernelError):
+            ops.attention_4bit(q, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 1, 1, 20, 4, 2, 64, 0.1, window=window)
+        with pytest.raises(ops.KernelError):
+            ops.read_cache_4bit(*cache.device(), cache.table.to(DEV), q_start, start_pos, [20], 64, torch.float32, window=window)
+    assert ops.attention_4bit(q, *cache.device(), cache.table.to(DEV), q_start, start_pos, positions, seq, 1, 1, 20, 4, 2, 64, 0.1, window=2 ** 31 - 1).shape == (1, 256)
+    ops.check_status()
