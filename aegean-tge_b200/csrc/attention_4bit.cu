@@ -257,8 +257,9 @@ struct Queries {
     }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int up = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 126, -120), 120) : 0;      // most < 2^up
-    const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+    // most < 2^up; a bfloat16 of 2^127 and more is at most 2 - 2^-7 over 2^127, and that times 2^15 is a float16 still
+    const int up = most > 0.0f ? min(max((int)(__float_as_uint(most) >> 23) - 126, -120), PARTS == 1 ? 127 : 120) : 0;
+    const float down = up < 127 ? __uint_as_float((uint32_t)(127 - up) << 23) : 0x1p-127f;
     float sum[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -388,14 +389,16 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, size
     Queries<HD, PARTS> q[NT];
     float factor[NT][2];                                          // of the scores of heads 2t, 2t + 1
     float o[NT][MTILES][4], o_base[NT][4], m[NT][2], l[NT][2];
+    bool far = false;                                             // a power that has no room for OVER beside it: scores are raised by that first
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool valid = token >= 0 && 8 * nt + g < heads_here;
       const T* src = static_cast<const T*>(p.q) + (size_t)max(token, 0) * p.q_stride + (size_t)(head0 + (valid ? 8 * nt + g : 0)) * HD;
-      const float unit_of = q[nt].template take<T>(src, valid, p.q_whole != 0, t) * (p.scale * (LOG2E / Queries<HD, PARTS>::OVER));
+      const float power = q[nt].template take<T>(src, valid, p.q_whole != 0, t);
+      far |= PARTS == 1 && power > 0x1p110f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        factor[nt][e] = __shfl_sync(0xffffffffu, unit_of, 4 * (2 * t + e));
+        factor[nt][e] = __shfl_sync(0xffffffffu, power, 4 * (2 * t + e));
         m[nt][e] = NONE;
         l[nt][e] = 0.0f;
       }
@@ -406,6 +409,11 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, size
 #pragma unroll
       for (int e = 0; e < 4; ++e) o_base[nt][e] = 0.0f;
     }
+    far = __any_sync(0xffffffffu, far);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) factor[nt][e] *= p.scale * (far ? LOG2E : LOG2E / Queries<HD, PARTS>::OVER);
 
     for (int slice = first; slice < last; slice += AHEAD) {
       bool here[AHEAD];
@@ -466,6 +474,16 @@ __global__ void __launch_bounds__(DWARPS * 32, decode_blocks_per_sm(HD, NT, size
         for (int i = 0; i < AHEAD; ++i) c[i].load_keys(p, rows[i], g, t);
       }
 
+      if (far)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sc[i][nt][e] *= 1.0f / Queries<HD, PARTS>::OVER;
+              sc[i][nt][e] = fmaf(sc[i][nt][e] * factor[nt][e & 1], 0.0f, sc[i][nt][e]);       // NaN where float32 has no room for the score
+            }
       bool raise = false;
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {

@@ -1557,7 +1557,8 @@ def attention_4bit(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    seq_of_token: torch.Tensor, num_seqs: int, max_q_len: int, max_ctx_len: int, heads: int, kv_heads: int, head_dim: int,
                    scale: float, window: int = 0, out: Optional[torch.Tensor] = None, decode_prefix: int = 0,
                    sink: Optional[torch.Tensor] = None, ctx_lens=None, q_lens=None) -> torch.Tensor:
-    """:func:`attention` over a cache of 4-bit codes (see :func:`norm_rope_kv_store_4bit`): [T, heads * head_dim].  Arguments as for :func:`attention_8bit`."""
+    """:func:`attention` over a cache of 4-bit codes (see :func:`norm_rope_kv_store_4bit`): [T, heads * head_dim].  Arguments as for :func:`attention_8bit`.
+    Queries and keys whose scores float32 has no room for are not served: such rows are NaN, or zeros."""
     _want(q, "queries", _FLOAT, contiguous=False)
     q_stride, tokens = _rows_2d(q, "queries"), q.shape[0]
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads or q.shape[1] < heads * head_dim:

@@ -59,6 +59,52 @@ def test_an_eps_that_float32_does_not_hold_is_refused(ops):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 256, 48])
+@pytest.mark.parametrize("up", [112, 118, 120, 121, 122, 124])
+def test_large_queries_over_small_keys(ops, dtype, dim, up):
+    """Rows of queries up to the end of the range, over keys that make scores of ordinary size of them."""
+    cache = Cache([300, 1, 90], 2, dim, 16)
+    cache.pairs["k"] = (cache.pairs["k"].double() * 2.0 ** -up).bfloat16()
+    out, want = attend(ops, cache, [1, 1, 1], 6, dtype, size=2.0 ** up, scale=0.09)
+    assert rel_error(out, want) < TOL[dtype]
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(6, 2, 64), (8, 1, 128), (5, 1, 256), (24, 2, 128)])
+@pytest.mark.parametrize("columns", [16, 130])
+@pytest.mark.parametrize("size", [3.2e38, 2e36])
+def test_large_queries_over_keys_of_ordinary_size(ops, heads, kv, dim, columns, size):
+    """One head's queries near the end of bfloat16's range: its row is its best key's value, or NaN where float32 has no room for a score
+    (in base-2 units); the others' rows are as they were."""
+    cache = Cache([100, 1, 30], kv, dim, 64)
+    wide = torch.full((3, columns), -1, dtype=torch.int32)
+    wide[:, :cache.table.shape[1]] = cache.table
+    positions, seq, q_start, start_pos = batch_index([1] * 3, [h - 1 for h in cache.held], DEV)
+    q = torch.randn(3, heads, dim, generator=torch.Generator().manual_seed(5)).bfloat16()
+    q[:, 1] = (q[:, 1].float() / q[:, 1].float().abs().amax(-1, keepdim=True) * size).bfloat16()
+    assert torch.isfinite(q).all()
+    scale = dim ** -0.5
+    want = torch.cat([attention_of(q[r:r + 1], cache.values("k", r), cache.values("v", r), cache.held[r] - 1, scale, 0, None) for r in range(3)])
+    room = []
+    for r in range(3):
+        scores = cache.values("k", r)[:, 0] @ q[r, 1].double()
+        most = float(scores.abs().max()) * scale / math.log(2)
+        assert not 3.4e38 < most < 3.41e38                  # (float32 ends between the two)
+        room.append(most < 3.4e38)
+        if r != 1:                  # the best key is best by far more than float32's sums are off
+            best = scores.topk(2).values
+            assert float(best[0] - best[1]) > 1e-3 * float(q[r, 1].double().abs().sum()) * 0.2
+    assert all(room) or size > 1e38
+    out = ops.attention_4bit(q.flatten(1).to(DEV), *cache.device(), wide.to(DEV), q_start, start_pos, positions, seq, 3, 1, 100, heads, kv, dim, scale)
+    ops.check_status()
+    out = out.view(3, heads, dim).cpu()
+    for r in range(3):
+        if not room[r]:
+            assert torch.isnan(out[r, 1]).all()
+            out[r, 1] = want[r, 1].to(out.dtype)
+    assert rel_error(out, want) < TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim,columns", [(64, 16), (64, 300), (128, 16), (128, 300), (80, 16)])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_sinks_at_the_ends_of_the_range(ops, dtype, dim, columns, bits):
