@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(128) attention_4bit_simple_kernel(const Attn4 
 // ---------------------------------------------------------------------------
 // Single tokens on the tensor cores: head sizes 64, 128 and 256, pages of 16, 32, 64, ... positions.
 //
-// What bounds it: turning codes into operands, some 390 instructions a slice of 16 positions and warp, and waits for loads (DRAM would take 39 of the 75 us below).
+// What bounds it: instructions (some 390 a slice of 16 positions and warp, over everything that a launch does: no counter splits them by part) and waits for
+// loads; DRAM would take 39 of the 75 us below.
 // A warp takes slices of 16 positions, nothing of them passes through shared memory.
 //   scores   S^T [16 positions x 8 heads] = sum_j step_j (C_j [16 x 32] Q_j^T [32 x 8]) (m16n8k16 of float16, two to a group): a lane needs, of positions
 //            g and g + 8 (g = lane / 4), its quarter (t = lane % 4) of every group, which is how they lie.  Four bits under a mask are a float16 already,
@@ -110,11 +111,11 @@ __global__ void __launch_bounds__(128) attention_4bit_simple_kernel(const Attn4 
 // Probabilities turn from S^T's accumulators into P^T's operand by two 8x8 transposes a group.  The running maximum is raised only when a score
 // passes it by 2^8; the sums of probabilities stay in their lanes until the end.
 //
-// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (258 MB with their pairs) 74.7 us; four of 32,768 to 65,536 69.0; eight of
-// 2,048 at 28 heads over 4 (a cluster each unit) 10.3, one 7.3.  Keys in bfloat16, their codes raised by 128 and the sums lowered after: 76.8, the
-// base of what follows.  Not taken: entries through rings in shared memory, bulk copies asked for by each warp or by each block, 77 and 79 (fewer waits, more instructions); pages
+// Measured, with the joining: 64 requests of 2,048 to 4,096 positions at 40 heads over 8 (258 MB with their pairs) 75.2 us; four of 32,768 to 65,536 69.4; eight of
+// 2,048 at 28 heads over 4 (a cluster each unit) 10.3, one 7.3.  Without raising the scores of rows beyond 2^110, which float32 would have no room for,
+// 74.6 and 68.8.  Keys in bfloat16, their codes raised by 128 and the sums lowered after: 76.8, the base of what follows.  Not taken: entries through rings in shared memory, bulk copies asked for by each warp or by each block, 77 and 79 (fewer waits, more instructions); pages
 // asked into L2 ahead 90; one slice at a time with four blocks on an SM 79, three 90; values with 136 taken off by a product with a constant 82, queries in shared memory 78.
-// Without any conversion or scaling at all it would take 56, without products too 50.
+// Without any conversion or scaling at all that kernel of 76.8 would have taken 56, without products too 50.
 //
 // Work: see decode_units.cuh; few units over short contexts go to a cluster each (decode_cluster).
 // ---------------------------------------------------------------------------
@@ -647,7 +648,8 @@ int decode_blocks(int head_dim, int tile_heads, int is_bf16) { return tge_sm_cou
 static int decode_tile(int group, int head_dim) { return group <= 8 || head_dim > 128 ? 8 : 16; }
 
 // Blocks of a cluster per unit, which joins its parts itself; 0: runs of slices and a second kernel.  A rule on what the host knows, the units and the
-// bound of their lengths, while all clusters are on the device at a time.  us at 28 heads over 4 (four units a request) with 4 / 8 / 16 / none: 1 request of 512
+// bound of their lengths (the block table's, also under a window), while all clusters are on the device at a time.  Measured with bfloat16 and heads of 128
+// alone; it decides for the other sizes and for float32 too.  us at 28 heads over 4 (four units a request) with 4 / 8 / 16 / none: 1 request of 512
 // 5.9 / 6.3 / 6.9 / 6.8, 16 of them 7.9 / 14.3 / 27.6 / 9.5; 1 of 2,048 10.0 / 7.8 / 7.2 / 7.7, 8 of them 13.0 / 10.3 / 16.6 / 11.0; 4 of 4,096 17.1 /
 // 12.2 / 11.0 / 11.2, 8 of them 21.0 / 14.9 / 21.3 / 13.9; 1 of 8,192 26 / 16 / 11.5 / 12.0, of 16,384 53 / 30 / 18.6 / 15.8.
 static int decode_cluster(long long units, int head_dim, int tile, int is_bf16, long long positions) {

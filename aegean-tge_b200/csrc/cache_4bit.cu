@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(WARPS * 32) store_4bit_kernel(const StoreParam
 // ---------------------------------------------------------------------------
 // The same by units of eight numbers, for head sizes 32, 64, 128 and 256 that are rotated whole or not at all and rows on 16 bytes.  A block has a token; HEAD / 16
 // lanes have a head's row, eight numbers of its first half and eight of its second, and take the token's heads in turn, three rows on their way at
-// a time, the angles loaded once.  Bound by the trips to memory one behind the other where there are few tokens, by instructions where there are many (a key's row
-// some 260 a warp and four rows, a query's 90, a norm 170 more).  us: one token 2.5; 2,048 at 28 heads over 4 9.8, with norms 14.9 (34 MB, 5.5 at a
-// copy's rate); 8,192 at 40 over 8 51 and 78 (33).  With a division for every code 3.4, 11.8, 18, 62 and 99; two rows or four blocks to an SM 12 and 11
+// a time, the angles loaded once.  Bound by the trips to memory one behind the other where there are few tokens; what bounds it where
+// there are many was not profiled.  us: one token 2.5; 2,048 at 28 heads over 4 9.8, with norms 14.9 (34 MB, 5.5 at a copy's rate); 8,192 at 40 over 8
+// 51 and 75 (33).  With a division for every code 3.4, 11.8, 18, 62 and 99; two rows or four blocks to an SM 12 and 11
 // where this takes 9.7; rows asked into L2 ahead no faster.
 // ---------------------------------------------------------------------------
 constexpr int UNIT_THREADS = 256, UNIT_AHEAD = 3;         // at most; as many as it takes for a token's heads in UNIT_AHEAD turns

@@ -14,8 +14,8 @@
 namespace {
 
 constexpr int DWARPS = 4;
-// 8-bit codes, 64 requests of 2,048 to 4,096 at 40 heads over 8 at 0 / 12 / 24: 80.9 / 80.2 / 82.5 us, four of 32,768 47.8 / 45.6 / 45.9, eight of
-// 2,048 16.5 / 14.4 / 14.4
+// Measured with the 8-bit kernel as it was, and not with the 4-bit one: 64 requests of 2,048 to 4,096 at 40 heads over 8 at 0 / 12 / 24: 80.9 / 80.2 /
+// 82.5 us (77.4 now), four of 32,768 47.8 / 45.6 / 45.9 (41.7), eight of 2,048 16.5 / 14.4 / 14.4 (10.9)
 constexpr int BEGIN = 12;
 constexpr float NONE = -3.0e38f;                // a running maximum before the first score (finite: -inf less this is still -inf)
 constexpr float LOG2E = 1.4426950408889634f;
