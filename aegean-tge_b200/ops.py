@@ -1375,10 +1375,11 @@ def _attend_codes(q, out, q_stride, out_stride, q_start, start_pos, positions, s
                                                              _ptr(scratch), status_word().data_ptr(), _ptr(sink), _stream()), prefill)
                 if rc != UNSUPPORTED:
                     return
+        mine = rows[3] - first if first else rows[3]      # (the table's requests: the kernel for rows on odd elements goes by them)
         k, v, table = read_as(q.dtype, first, starts)
         if read is not None:
             read.record()
-        attention(rows[0], k, v, table, starts, *rows[1:4], num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
+        attention(rows[0], k, v, table, starts, rows[1], rows[2], mine, num_seqs - first, max_q_len, longest, heads, kv_heads, head_dim, scale,
                   window=window, out=rows[4], sink=sink, own_pages=True)
 
     def each(first: int, last: int) -> None:
