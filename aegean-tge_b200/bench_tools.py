@@ -184,19 +184,26 @@ def step_timeline(engine, batch: int, prompt_len: int, prefill: bool, portion: i
     torch.cuda.synchronize()
     ops = engine.model.env.ops
     try:
-        # the profiler now and then hands over a part of the records only: once more, with a pause on either side of the step within
-        # the profiler's window that gets longer
+        # The profiler now and then hands over a part of the records only, time after time: the first kernels of its window are missing then.  Once
+        # more, with a pause on either side of the step that gets longer, and from the third time on a step in front of it, which is left out.
         for attempt in range(8):
             pause = 0.0 if attempt < 2 else 0.02 * 2 ** (attempt - 2)
-            launched = ops.launches
             with profile(activities=[ProfilerActivity.CUDA]) as prof:
                 time.sleep(pause)
+                if pause > 0.0:
+                    run()
+                    torch.cuda.synchronize()
+                    time.sleep(pause)
+                launched = ops.launches
                 run()
                 torch.cuda.synchronize()
                 time.sleep(pause)
             launched = ops.launches - launched
-            events = [(e.time_range.start, e.time_range.start + e.device_time_total, e.name) for e in prof.events()
-                      if e.device_time_total > 0]
+            events = sorted((e.time_range.start, e.time_range.start + e.device_time_total, e.name) for e in prof.events() if e.device_time_total > 0)
+            for i in range(len(events) - 1, 0, -1):
+                if pause > 0.0 and events[i][0] - events[i - 1][1] > 0.5e6 * pause:
+                    events = events[i:]
+                    break
             if len(events) >= launched:
                 break
         else:

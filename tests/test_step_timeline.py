@@ -72,3 +72,38 @@ def test_a_part_is_never_listed(handed, monkeypatch):
         with pytest.raises(RuntimeError, match="profiler"):
             bench_tools.step_timeline(engine, 2, 20, prefill=prefill)
         assert not engine.live
+
+
+def test_a_step_in_front_takes_what_the_profiler_drops_first(handed, monkeypatch):
+    """A profiler that never has the first kernels of its window: the step in front is what it drops, and what is left of that is not listed."""
+    engine, clock, dropped = Engine(), SimpleNamespace(now=0.0, kernels=[]), 3
+
+    class Profile:
+        def __init__(self, activities):
+            clock.kernels = []
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *what):
+            return False
+
+        def events(self):
+            return [SimpleNamespace(time_range=SimpleNamespace(start=at), device_time_total=4.0, name=f"kernel_{i % KERNELS}(int)")
+                    for i, at in enumerate(clock.kernels) if i >= dropped]
+
+    def step(portions):
+        engine.ops.launches += KERNELS
+        for _ in range(KERNELS):
+            clock.kernels.append(clock.now)
+            clock.now += 5.0
+
+    def sleep(seconds):
+        clock.now += 1e6 * seconds
+
+    monkeypatch.setattr(engine, "step", step, raising=False)
+    monkeypatch.setattr(torch.profiler, "profile", Profile)
+    monkeypatch.setattr(bench_tools.time, "sleep", sleep)
+    rows = bench_tools.step_timeline(engine, 1, 20, prefill=True)
+    assert sorted(r["kernel"] for r in rows[:-1]) == [f"kernel_{i}" for i in range(KERNELS)] and rows[-1]["launches"] == KERNELS
+    assert all(r["launches"] == 1 for r in rows[:-1]) and rows[-1]["us"] == 24.0
